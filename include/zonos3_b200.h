@@ -318,6 +318,50 @@ int zb_gqa_prologue_decode(const uint16_t* proj, int64_t proj_stride, const uint
                            int64_t slot_stride, int64_t num_slots, const int32_t* out_loc, int N, int Hq, int Hkv,
                            int hd, cudaStream_t stream);
 
+/* The new tokens of a ragged batch over a paged KV cache. Both entry points below describe the batch the same way (all
+ * device pointers; nothing is read on the host, so captured graphs follow the lengths):
+ *   cu_seqlens_q [B + 1] int32, non-decreasing: request b's new tokens are rows cu[b] .. cu[b + 1] of the N rows; rows
+ *                outside [cu[0], cu[B]) belong to no request
+ *   cache_seqlens [B] int32: request b's keys, its new tokens included as the last ones: row t is key position
+ *                cache_seqlens[b] - (cu[b + 1] - t)
+ *   page_table   [B, table_stride] int32 with max_pages columns: position j lives in row j % page_size of page
+ *                page_table[b, j / page_size]; a page outside [0, num_pages) or past the columns holds no keys
+ *   k_cache, v_cache bf16: page p, row r, KV head g at p * page_stride + r * slot_stride + g * head_stride elements, hd
+ *                contiguous elements each; strides multiples of 8, bases 16-byte aligned. page_size * max_pages < 2^31.
+ *   hd a multiple of 8, 8 .. 128 (else status 3).
+ *
+ * zb_gqa_append: from projection rows proj [N, Hq*hd | Hkv*hd | Hkv*hd | ...] bf16 (q | k | v, any row stride): q and k rows
+ * divided by sqrt(mean(x^2) + eps) when normalize, q multiplied by |temp[h]| (NULL: not), the first rotary_dim elements
+ * turned by position * rope_theta^(-2j / rotary_dim) in pairs (2j, 2j + 1) when interleaved (rotary_dim a multiple of 8)
+ * or (j, j + rotary_dim / 2) (a multiple of 16); position = positions[t], or the key position when positions is NULL.
+ * fp32 with one rounding (angles in fp64). q to q_out [N, Hq, hd] (row stride q_stride, a multiple of 8; 16-byte
+ * aligned; zero for a row of no request), k and v to the token's cache row (a token without a page is not stored). The
+ * q/k norm, temperature, rotary and store_kv steps of Attention.forward for any batch
+ * (servers/sgl/src/zonos3_sgl/models/zonos3.py:340-375). */
+int zb_gqa_append(const uint16_t* proj, int64_t proj_stride, const uint16_t* temp, const int32_t* positions, float eps,
+                  int normalize, double rope_theta, int rotary_dim, int interleaved, uint16_t* q_out, int64_t q_stride,
+                  uint16_t* k_cache, uint16_t* v_cache, int64_t page_stride, int64_t slot_stride, int64_t head_stride,
+                  int64_t num_pages, int page_size, const int32_t* page_table, int64_t table_stride, int max_pages,
+                  const int32_t* cache_seqlens, const int32_t* cu_seqlens_q, int B, int N, int Hq, int Hkv, int hd,
+                  cudaStream_t stream);
+
+/* zb_gqa_chunk: attention of the N new tokens over the pages of their requests (the FA backend's
+ * flash_attn_with_kvcache for prefill, chunked prefill, decode and mixed batches,
+ * servers/sgl/src/zonos3_sgl/attention/fa.py:64-81, :171-212). The token at key position p sees keys j <= p (causal; else
+ * every key of its request), j > p - window when window > 0 (causal only), in pages of the cache. out[t, h] = softmax(q[t,
+ * h] . K^T * softmax_scale) V, query head h reading KV head h / (Hq / Hkv), times sigmoid(gate[t, h]) when gate is given
+ * ([N, Hq] bf16, row stride gate_stride), rounded once; lse (NULL: not written) [N, Hq] fp32 = the natural logarithm of
+ * the softmax denominator. A row that sees no key or belongs to no request: zeros, lse -inf. q / out [N, Hq, hd] bf16 with
+ * row strides (multiples of 8), 16-byte aligned; softmax_scale > 0; Hq a multiple of Hkv. workspace: 16-byte aligned, at
+ * least zb_gqa_chunk_workspace_bytes(B, N, Hq, Hkv, hd, page_size * max_pages) bytes, not shared by overlapping calls. */
+int64_t zb_gqa_chunk_workspace_bytes(int B, int N, int Hq, int Hkv, int hd, int64_t max_keys);
+int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache,
+                 int64_t page_stride, int64_t slot_stride, int64_t head_stride, int64_t num_pages, int page_size,
+                 const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* cache_seqlens,
+                 const int32_t* cu_seqlens_q, int B, int N, int Hq, int Hkv, int hd, float softmax_scale, int causal,
+                 int window, const uint16_t* gate, int64_t gate_stride, uint16_t* out, int64_t out_stride, float* lse,
+                 void* workspace, int64_t workspace_bytes, cudaStream_t stream);
+
 /* ---------------------------------------------------------------------------------------------- TTS sampler */
 
 /* Next audio codes from per-codebook logits [B, C, V] (row (b, c) of V at b * batch_stride + c * row_stride elements,

@@ -99,6 +99,18 @@ SIGNATURES: dict[str, list] = {
     "zb_gqa_prologue_decode": [_p, _i64, _p, _p, _f32, _f32, _p, _p, _p, _i64, _i64, _p, _i32, _i32, _i32, _i32, _p],
     "zb_gqa_decode": [_p, _i64, _p, _p, _i64, _i64, _p, _i64, _p, _i32, _i32, _i32, _i32, _i32, _f32, _i32, _i32, _p,
                       _i64, _p, _i64, _p, _i64, _p],
+    # proj, proj_stride, temp, positions, eps, normalize, theta, rotary_dim, interleaved, q_out, q_stride, k_cache, v_cache,
+    # page_stride, slot_stride, head_stride, num_pages, page_size, page_table, table_stride, max_pages, cache_seqlens,
+    # cu_seqlens_q, B, N, Hq, Hkv, hd, stream
+    "zb_gqa_append": [_p, _i64, _p, _p, _f32, _i32, ctypes.c_double, _i32, _i32, _p, _i64, _p, _p, _i64, _i64, _i64, _i64,
+                      _i32, _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _p],
+    # q, q_stride, k_cache, v_cache, page_stride, slot_stride, head_stride, num_pages, page_size, page_table,
+    # table_stride, max_pages, cache_seqlens, cu_seqlens_q, B, N, Hq, Hkv, hd, scale, causal, window, gate, gate_stride,
+    # out, out_stride, lse, workspace, workspace_bytes, stream
+    "zb_gqa_chunk": [_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i32, _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32,
+                     _f32, _i32, _i32, _p, _i64, _p, _i64, _p, _p, _i64, _p],
+    # B, N, Hq, Hkv, hd, max_keys -> bytes (int64)
+    "zb_gqa_chunk_workspace_bytes": [_i32, _i32, _i32, _i32, _i32, _i64],
     # n, out (complex float64 [n]), stream
     "zb_istft_twiddles": [_i32, _p, _p],
     # y0, y0_stride, y1, y1_stride, y_is_f64, streams, cols, n0, n1, hop, window0, window1, twiddle0, twiddle1,
@@ -112,7 +124,8 @@ SIGNATURES: dict[str, list] = {
                          _i64, _p],
 }
 _RESTYPES = {"zb_last_error": ctypes.c_char_p, "zb_clear_error": None, "zb_launch_count": ctypes.c_uint64,
-             "zb_gdn_chunk_prefill_workspace_bytes": ctypes.c_int64, "zb_proj_gemm_workspace_bytes": ctypes.c_int64}
+             "zb_gdn_chunk_prefill_workspace_bytes": ctypes.c_int64, "zb_proj_gemm_workspace_bytes": ctypes.c_int64,
+             "zb_gqa_chunk_workspace_bytes": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

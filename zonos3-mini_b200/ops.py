@@ -1027,3 +1027,147 @@ def decode_advance(codes, ids, positions, cache_seqlens, out_loc, page_table, co
     _lib.call("zb_decode_advance", codes.data_ptr(), codes.shape[1], ids.data_ptr(), ids.shape[1], ptr(history), C, W,
               ptr(ring), counter.data_ptr(), positions.data_ptr(), cache_seqlens.data_ptr(), out_loc.data_ptr(),
               page_table.data_ptr(), page_table.stride(0), page_table.shape[1], B, _stream(dev))
+
+
+# ------------------------------------------------------------- ragged batches of new tokens over a paged KV cache
+
+
+def _paged(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, kv_heads):
+    """The checks and the C arguments that the operators over a paged KV cache share (``q``: their query-side input)."""
+    dev = q.device
+    if not q.is_cuda:
+        raise ValueError("the paged KV operators take CUDA tensors (the B200 kernels have no CPU path)")
+    for name, t, dtype in (("k_cache", k_cache, torch.bfloat16), ("v_cache", v_cache, torch.bfloat16),
+                           ("page_table", page_table, torch.int32), ("cache_seqlens", cache_seqlens, torch.int32),
+                           ("cu_seqlens_q", cu_seqlens_q, torch.int32)):
+        if t.dtype != dtype or t.device != dev:
+            raise ValueError(f"{name} must be a {dtype} tensor on {dev}, got {t.dtype} on {t.device}")
+    shape, strides = k_cache.shape, k_cache.stride()
+    if len(shape) == 3:  # [slots, Hkv, hd]: one token a page
+        page_size, slot_stride, head_stride = 1, 0, strides[1]
+    elif len(shape) == 4:
+        page_size, slot_stride, head_stride = shape[1], strides[1], strides[2]
+    else:
+        raise ValueError(f"k_cache must be [pages, page_size, Hkv, hd] or [slots, Hkv, hd], got {tuple(shape)}")
+    if v_cache.shape != shape or v_cache.stride() != strides or strides[-1] != 1:
+        raise ValueError("k_cache and v_cache must have the same shape and strides, their last dimension contiguous")
+    if kv_heads is not None and shape[-2] != kv_heads:
+        raise ValueError(f"the caches hold {shape[-2]} KV heads, expected {kv_heads}")
+    B = cache_seqlens.shape[0]
+    if (page_table.dim() != 2 or page_table.shape[0] != B or cache_seqlens.dim() != 1
+            or cu_seqlens_q.shape != (B + 1,)):
+        raise ValueError(f"page_table, cache_seqlens and cu_seqlens_q must be [B, pages], [B] and [B + 1], got "
+                         f"{tuple(page_table.shape)}, {tuple(cache_seqlens.shape)}, {tuple(cu_seqlens_q.shape)}")
+    columns = page_table.shape[1]
+    if (columns > 1 and page_table.stride(1) != 1) or (B > 1 and cache_seqlens.stride(0) != 1) or cu_seqlens_q.stride(0) != 1:
+        raise ValueError("page_table rows, cache_seqlens and cu_seqlens_q must be contiguous")
+    return (k_cache.data_ptr(), v_cache.data_ptr(), strides[0], slot_stride, head_stride, shape[0], page_size,
+            page_table.data_ptr(), page_table.stride(0) if B > 1 else columns, columns, cache_seqlens.data_ptr(),
+            cu_seqlens_q.data_ptr(), B), shape[-2], shape[-1]
+
+
+def _token_rows(name: str, t: torch.Tensor, heads: int, hd: int) -> int:
+    """Row stride of a [N, heads, hd] bf16 tensor whose rows are contiguous."""
+    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd:
+        raise ValueError(f"{name} must be a bfloat16 [N, {heads}, {hd}] tensor, got {t.dtype} {tuple(t.shape)}")
+    if (hd > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != hd):
+        raise ValueError(f"{name}'s rows must be contiguous")
+    return t.stride(0) if t.shape[0] > 1 else heads * hd
+
+
+def gqa_append(proj, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, heads, kv_heads, temp=None,
+               eps=1e-6, rope_theta=10000.0, rotary_dim=None, interleaved=True, positions=None, q_out=None):
+    """The new tokens' keys and values into a paged KV cache, with the attention layer's q / k norm and rotary embedding
+    on the way, for a ragged batch (prompts, chunks of prompts, single tokens, or nothing, mixed as they come): the
+    q / k norm, ``temp``, rotary and store_kv steps of Attention.forward
+    (servers/sgl/src/zonos3_sgl/models/zonos3.py:340-375) with the FA backend's batch description
+    (servers/sgl/src/zonos3_sgl/attention/fa.py).
+
+    proj [N, >= (heads + 2 kv_heads) * hd] bf16 holds q | k | v (rows contiguous, any row stride). Request b's new tokens
+    are rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] ([B + 1] int32, on the device); cache_seqlens [B] int32 counts its
+    keys, the new ones included, so its last new token is key position cache_seqlens[b] - 1. k_cache, v_cache [pages,
+    page_size, kv_heads, hd] bf16, or [slots, kv_heads, hd] for one token a page (strides allowed, multiples of 8, the last
+    dimension contiguous); position j lives in row j % page_size of page page_table[b, j // page_size] ([B, columns]
+    int32). A token whose page is outside [0, pages) or past the table is not stored; a row of no request stores
+    nothing and gets a zero q.
+
+    q and k are divided by sqrt(mean(x^2) + eps) (``eps=None``: not), q is multiplied by |temp| ([heads] bf16, None:
+    not), and the first ``rotary_dim`` elements (default: all) turn by position * rope_theta^(-2j / rotary_dim), as
+    pairs (2j, 2j + 1) when ``interleaved`` (rotary_dim a multiple of 8), else (j, j + rotary_dim / 2) (a multiple of
+    16). The position is the key position unless ``positions`` ([N] int32) gives it. fp32 with one rounding at the end.
+    hd: a multiple of 8 up to 128. Returns q [N, heads, hd] bf16 (``q_out`` when given; a row stride is allowed)."""
+    paged, Hkv, hd = _paged(proj, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, kv_heads)
+    dev = proj.device
+    if proj.dtype != torch.bfloat16 or proj.dim() != 2 or proj.shape[1] < (heads + 2 * Hkv) * hd or (
+            proj.shape[1] > 1 and proj.stride(1) != 1):
+        raise ValueError(f"proj must be a bfloat16 [N, >= {(heads + 2 * Hkv) * hd}] tensor with contiguous rows")
+    N = proj.shape[0]
+    if temp is not None:
+        _check_cuda("temp", temp, torch.bfloat16, dev)
+        _require(temp.numel() == heads and temp.is_contiguous(), f"temp must hold {heads} values")
+    if positions is not None:
+        _check_cuda("positions", positions, torch.int32, dev)
+        _require(positions.shape == (N,) and positions.is_contiguous(), f"positions must be a contiguous [{N}] tensor")
+    if q_out is None:
+        q_out = torch.empty((N, heads, hd), device=dev, dtype=torch.bfloat16)
+    elif q_out.device != dev or q_out.shape[0] != N:
+        raise ValueError(f"q_out must be a [{N}, {heads}, {hd}] tensor on {dev}")
+    _lib.call("zb_gqa_append", proj.data_ptr(), proj.stride(0) if N > 1 else proj.shape[1],
+              None if temp is None else temp.data_ptr(), None if positions is None else positions.data_ptr(),
+              0.0 if eps is None else eps, eps is not None, rope_theta, hd if rotary_dim is None else rotary_dim,
+              bool(interleaved), q_out.data_ptr(), _token_rows("q_out", q_out, heads, hd), *paged, N, heads, Hkv, hd,
+              _stream(dev))
+    return q_out
+
+
+def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, softmax_scale=None, causal=True, window=0,
+              gate=None, out=None, lse=None, workspace=None):
+    """Attention of every request's new tokens over its pages of a KV cache (which hold the new tokens' keys already:
+    :func:`gqa_append`): the FA backend's flash_attn_with_kvcache for prefill, chunked prefill, decode and batches that
+    mix them (servers/sgl/src/zonos3_sgl/attention/fa.py:64-81, :171-212).
+
+    q [N, Hq, hd] bf16 (row stride allowed); the caches, page_table, cache_seqlens and cu_seqlens_q as for
+    :func:`gqa_append`. Query head h reads KV head h // (Hq / Hkv). A token at key position p sees keys 0 .. p (with
+    ``window`` > 0 the last ``window`` of them; with ``causal=False`` every key of its request); a page outside
+    [0, pages) masks its keys. softmax_scale (> 0) defaults to hd ** -0.5. gate: optional [N, Hq] bf16 logits (row
+    stride allowed); head h's output is multiplied by sigmoid(gate[t, h]) before its one rounding. lse: optional
+    contiguous [N, Hq] fp32 tensor that receives the natural logarithm of the softmax denominators. A token that sees
+    no key, or belongs to no request, gets zeros and an lse of -inf. The lengths are read on the device: a captured
+    graph follows them. workspace: optional uint8 tensor of at least :func:`gqa_chunk_workspace_bytes` bytes
+    (allocated when absent). hd: a multiple of 8 up to 128. Returns out [N, Hq, hd] bf16."""
+    paged, Hkv, hd = _paged(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, None)
+    dev = q.device
+    N, Hq = q.shape[0], q.shape[1]
+    qs = _token_rows("q", q, Hq, hd)
+    if out is None:
+        out = torch.empty((N, Hq, hd), device=dev, dtype=torch.bfloat16)
+    elif out.device != dev or out.shape[0] != N:
+        raise ValueError(f"out must be a [{N}, {Hq}, {hd}] tensor on {dev}")
+    gate_ptr, gate_stride = None, 0
+    if gate is not None:
+        _check_cuda("gate", gate, torch.bfloat16, dev)
+        _require(gate.shape == (N, Hq) and (Hq == 1 or gate.stride(1) == 1), f"gate must be [{N}, {Hq}] with contiguous rows")
+        gate_ptr, gate_stride = gate.data_ptr(), gate.stride(0) if N > 1 else Hq
+    if lse is not None:
+        _check_cuda("lse", lse, torch.float32, dev)
+        _require(lse.shape == (N, Hq) and lse.is_contiguous(), f"lse must be a contiguous [{N}, {Hq}] tensor")
+    need = gqa_chunk_workspace_bytes(N, Hq, page_table, k_cache)
+    if workspace is None:
+        workspace = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+    else:
+        _check_cuda("workspace", workspace, torch.uint8, dev)
+        _require(workspace.is_contiguous() and workspace.numel() >= need,
+                 f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
+    _lib.call("zb_gqa_chunk", q.data_ptr(), qs, *paged, N, Hq, Hkv, hd,
+              hd ** -0.5 if softmax_scale is None else softmax_scale, bool(causal), window, gate_ptr, gate_stride,
+              out.data_ptr(), _token_rows("out", out, Hq, hd), None if lse is None else lse.data_ptr(),
+              None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(),
+              _stream(dev))
+    return out
+
+
+def gqa_chunk_workspace_bytes(tokens: int, heads: int, page_table, k_cache) -> int:
+    """Bytes of workspace :func:`gqa_chunk` needs for ``tokens`` rows of ``heads`` query heads over these tables."""
+    page_size = k_cache.shape[1] if k_cache.dim() == 4 else 1
+    return _lib.load().zb_gqa_chunk_workspace_bytes(page_table.shape[0], tokens, heads, k_cache.shape[-2],
+                                                    k_cache.shape[-1], page_table.shape[1] * page_size)
