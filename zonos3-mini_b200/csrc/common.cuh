@@ -47,6 +47,8 @@ enum DeviceStatusBits : unsigned {
   kStatusAttnresExchangeTimeout = 1u << 3,
   kStatusAttnDecodeTimeout = 1u << 4,
   kStatusEmbedIndex = 1u << 5,  // an embedding id outside its table (read as a zero row)
+  kStatusAttnChunkTimeout = 1u << 6,
+  kStatusAttnChunkBatch = 1u << 7,  // a chunk attention call whose cu_seqlens_q decreases (no output written)
 };
 
 }  // namespace zb

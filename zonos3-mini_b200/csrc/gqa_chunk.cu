@@ -2,23 +2,56 @@
 //
 // Token t of request b at key position p (paged.cuh) sees the keys j <= p (causal; every key of the request otherwise)
 // with j > p - window when there is a window, and whose page is in the cache. With s_j = scale q . k_j over them,
-//   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  m = max_j s_j,  lse = m + log sum_j e^(s_j - m);
+//   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  lse = m + log sum_j e^(s_j - m),  m = max_j s_j;
 // a token that sees no key, or belongs to no request, gives 0 (lse -inf). Query head h reads KV head h / (Hq / Hkv).
 // The layer's output gate multiplies head h's row by sigmoid(gate[t, h]) before the one rounding to bf16.
 //
-// A warp per (token, query head): groups of lanes, 8 elements each, take the keys in turn with their own running
-// maximum, sum and accumulator, joined at the end. All in fp32.
+// Both products run on the tensor cores. The G = Hq / Hkv heads of a KV head share its keys, so the rows of a
+// request's score matrix are its (token, head of the group) pairs, token-major; a unit of work is 256 such rows of one
+// (request, KV head), as two streams of 128 rows (the lanes of tensor memory), against a range of 128-key tiles. Per
+// stream and tile: S = Q K^T (tcgen05, fp32 in tensor memory); a thread takes a row, finds its maximum, forms p = 2^(s
+// scale log2 e - m), adds up its sum in fp32 and writes p back over S as bf16; O += P V with P read from tensor memory.
+// The two streams share each tile's K and V in shared memory and take turns: one's exponentials run while the tensor
+// cores work for the other. The subtracted maximum m only follows the true one when that has grown by more than 8 (in
+// log2): the stale one keeps p <= 2^8 and cancels in the final division, so the accumulator is hardly ever rescaled.
+// p is rounded to bf16 because the tensor cores multiply bf16; its sum is kept from before the rounding.
+//
+// The lengths live on the device, so the split of the work does too: every CTA adds up the tiles of all units (a scan
+// over the requests) and takes an equal run of them. A unit that spans CTAs leaves partial results (accumulator,
+// maximum, sum) in the workspace, and a second kernel joins them in order; so one token over a long cache uses the whole
+// GPU, a ragged batch is balanced whatever its lengths, and the result does not depend on timing.
+//
+// Warps: 0-3 and 4-7 the rows of stream 0 and 1; 8 issues the tensor-core work; 9-11 look up pages and copy K, V and Q
+// rows (any page size, any strides) into shared memory, several tiles ahead and across units.
+//
+// A key hidden from some rows of a tile must not reach them even when its value is not finite, and 0 x inf is NaN in a
+// matrix product. So where a tile's keys are visible to some of its rows only, warp 8 looks through the V tile while the
+// scores are being worked on; values that are not finite are added to the rows that see them one by one, then zeroed.
+#include <algorithm>
+
 #include "paged.cuh"
+#include "tc.cuh"
 
 namespace {
 
-constexpr int kWarps = 4;
+namespace tc = zb::tc;
+
+constexpr int kTile = 128;       // keys of a tile
+constexpr int kStreamRows = 128;  // rows of a stream
+constexpr int kUnitRows = 2 * kStreamRows;
+constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
+constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
+constexpr uint32_t kBlk = kTile * 128;  // 64 dims of 128 rows, 128-byte swizzled
+constexpr int kMaxSlots = 10, kDescs = 4;
+constexpr int kMasks = 8;  // the loaders run at most 5 tiles ahead of the rows
+constexpr float kRescale = 8.f;  // log2 growth of a row's maximum that the accumulator is rescaled for
+constexpr int kMaxRequests = 16384;
 
 struct ChunkParams {
   zb::PagedBatch kv;
   const __nv_bfloat16* q;  // [N, Hq, hd], row stride q_stride
   int64_t q_stride;
-  int Hq;
+  int Hq, G;
   float scale_log2;  // softmax scale * log2(e)
   int causal, window;
   const __nv_bfloat16* gate;  // [N, Hq] or null
@@ -26,82 +59,869 @@ struct ChunkParams {
   __nv_bfloat16* out;  // [N, Hq, hd]
   int64_t out_stride;
   float* lse;  // [N, Hq] or null
+  // workspace: per CTA a header and two slots of partial results, rows_max rows each
+  struct Header* headers;
+  float* acc;  // [CTA][2][HD / 4][rows_max][4]
+  float* ml;   // [CTA][2][2][rows_max]: maximum, sum
+  int rows_max;
+  int pairs_max;  // units of a KV head, at most
+  unsigned* status;
 };
 
-template <int GL>
-__global__ void __launch_bounds__(kWarps * 32) gqa_chunk_kernel(const __grid_constant__ ChunkParams p) {
+// A unit that starts in this CTA and ends in another one (parts = 0: there is none).
+struct Header {
+  int parts;  // CTAs that hold a part of it, this one the first
+  int row0;   // first token row of its request
+  int pr0;    // its first (token, head) row within the request
+  int rows;
+  int kvh;
+  int pad[3];
+};
+
+// What a CTA does with one unit.
+struct Desc {
+  int row0, tokens, keys;  // the request: first token row, new tokens, keys (not negative)
+  int pr0, rows;           // (token, head) rows [pr0, pr0 + rows) of the request
+  int kvh;
+  int tile0, tiles;  // tiles of keys; 0: no row sees a key
+  int mode;          // kFinal, kPart0, kPart1, kStop
+  int parts;
+  int all_lo, all_hi;  // no key of [all_lo, all_hi) is hidden from some row (a key the request does not have is a zero)
+};
+enum Mode { kFinal = 0, kPart0 = 1, kPart1 = 2, kStop = 3 };
+
+struct Tail {
+  uint64_t full[kMaxSlots], empty[kMaxSlots];
+  uint64_t q_full[2], q_empty[2];
+  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t scanned, drained;
+  uint64_t desc_full[kDescs], desc_empty[kDescs];
+  unsigned mask[kMasks][4];  // keys of a tile that exist
+  Desc desc[kDescs];
+  int64_t sums[16];
+  int start[4];  // this CTA's first unit: request, pair, steps of the unit, KV head and tile
+  int64_t start_off;
+  uint32_t tmem;
+  int abort;
+  int found;  // the scanned V tile holds values that are not finite
+};
+
+template <int HD>
+struct Shape {
+  static constexpr uint32_t kItem = HD / 64 * kBlk;
+  static constexpr int kSlots = HD == 128 ? 5 : 10;
+  static constexpr uint32_t kOffQ = kSlots * kItem;
+  static constexpr uint32_t kOffTail = kOffQ + 2 * kItem;
+  static constexpr size_t kSmem = kOffTail + sizeof(Tail) + 1024;
+  static_assert(kSlots * kItem >= kMaxRequests * 4, "the requests' prefix fits the ring");
+  static_assert(kSmem <= 232448, "shared memory");
+  static constexpr uint32_t kColS = 0, kColO = 2 * kTile;  // stream s: S at s * 128, O at 256 + s * HD
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+// Arrives on `bar` once every cp.async this thread issued before has completed (counts as one expected arrival).
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void ld32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ uint32_t ld1(uint32_t taddr) {
+  uint32_t r;
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+  return r;
+}
+__device__ __forceinline__ void st1(uint32_t taddr, uint32_t r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r) : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t to_bf16x2(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Whether any of the 8 bf16 values is not finite (all exponent bits set).
+__device__ __forceinline__ bool not_finite(const uint4& v) {
+  const unsigned a = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                              __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+  return (a & 0xffffu) >= 0x7f80u || (a >> 16) >= 0x7f80u;
+}
+
+// A wait that gives up after a second, and at once after any earlier one of the CTA did.
+__device__ __forceinline__ void wait(const uint64_t& bar, uint32_t parity, int* abort, unsigned* status) {
+  const uint32_t at = zb::smem_addr(&bar);
+  if (zb::mbar_try_wait(at, parity)) return;
+  if (*reinterpret_cast<volatile int*>(abort) != 0) return;
+  if (!zb::mbar_wait_bounded(at, parity, status, zb::kStatusAttnChunkTimeout))
+    *reinterpret_cast<volatile int*>(abort) = 1;
+}
+// The same answer for every lane of the warp.
+__device__ __forceinline__ bool gave_up(int* abort) {
+  return __any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(abort) != 0);
+}
+__device__ __forceinline__ void arrive(const uint64_t& bar) { zb::mbar_arrive(zb::smem_addr(&bar)); }
+
+struct Request {
+  int row0, tokens, keys;
+};
+__device__ __forceinline__ Request request(const ChunkParams& p, int b) {
+  Request r;
+  r.row0 = min(max(p.kv.cu[b], 0), p.kv.N);
+  r.tokens = min(max(p.kv.cu[b + 1], r.row0), p.kv.N) - r.row0;
+  r.keys = max(p.kv.keys[b], 0);
+  return r;
+}
+
+// Keys [lo, hi) that token i of a request sees.
+__device__ __forceinline__ void visible(const ChunkParams& p, const Request& r, int i, int& lo, int& hi) {
+  const int pos = r.keys - r.tokens + i, held = min(r.keys, p.kv.max_pages * p.kv.page_size);
+  hi = p.causal ? min(held, pos + 1) : held;
+  hi = max(hi, 0);
+  lo = p.window > 0 ? max(0, (int)((int64_t)pos + 1 - p.window)) : 0;
+}
+
+// The unit of rows [pair * 256, ..) of a request: its rows and key tiles.
+__device__ __forceinline__ void unit_tiles(const ChunkParams& p, const Request& r, int pair, Desc& d) {
+  d.row0 = r.row0;
+  d.tokens = r.tokens;
+  d.keys = r.keys;
+  d.pr0 = pair * kUnitRows;
+  d.rows = min(r.tokens * p.G - d.pr0, kUnitRows);
+  int lo0, hi0, lo1, hi1;
+  visible(p, r, d.pr0 / p.G, lo0, hi0);
+  visible(p, r, (d.pr0 + d.rows - 1) / p.G, lo1, hi1);
+  d.all_lo = lo1;
+  d.all_hi = hi0 == min(r.keys, p.kv.max_pages * p.kv.page_size) ? INT32_MAX : hi0;
+  d.tile0 = lo0 / kTile;
+  d.tiles = hi1 > lo0 ? (hi1 + kTile - 1) / kTile - d.tile0 : 0;
+}
+
+__device__ __forceinline__ int64_t warp_scan(int64_t v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+
+// Exclusive prefix of v over the block's threads; `total` the sum.
+__device__ __forceinline__ int64_t block_scan(int64_t v, Tail& tl, int64_t& total) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int64_t in = warp_scan(v, lane);
+  if (lane == 31) tl.sums[warp] = in;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    const int64_t s = tl.sums[w];
+    if (w < warp) before += s;
+    total += s;
+  }
+  __syncthreads();
+  return before + in - v;
+}
+
+// One row's output: acc[8] of dims d .. d + 7, scaled and rounded once.
+__device__ __forceinline__ void store8(__nv_bfloat16* dst, const float* x, float f) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = x[i] * f;
+  *reinterpret_cast<uint4*>(dst) = zb::pack_bf16x8(y);
+}
+
+// What a row's accumulator is multiplied by: 1 / sum (0 for a row that saw no key, NaN stays NaN) times the gate.
+__device__ __forceinline__ float row_factor(const ChunkParams& p, int64_t t, int h, float l) {
+  float f = l == 0.f ? 0.f : 1.f / l;
+  if (p.gate) f *= 1.f / (1.f + expf(-__bfloat162float(p.gate[t * p.gate_stride + h])));
+  return f;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_constant__ ChunkParams p) {
+  using L = Shape<HD>;
   zb::pdl_enter();
-  constexpr int kKeys = 32 / GL;
-  const int64_t unit = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
-  const int lane = threadIdx.x % 32, gl = lane % GL, kl = lane / GL;
-  if (unit >= (int64_t)p.kv.N * p.Hq) return;
-  const int t = (int)(unit / p.Hq), h = (int)(unit % p.Hq), kvh = h / (p.Hq / p.kv.Hkv);
-  const int hd = p.kv.hd;
-  const bool carries = gl * 8 < hd;
-  const int b = zb::request_of(p.kv.cu, p.kv.B, t, lane);
-  float m = -INFINITY, l = 0.f, acc[8] = {};
-  if (b >= 0) {
-    const int64_t keys = p.kv.keys[b], pos = keys - ((int64_t)p.kv.cu[b + 1] - t);
-    const int64_t capacity = (int64_t)p.kv.max_pages * p.kv.page_size;
-    int64_t end = p.causal ? pos + 1 : keys, begin = p.window > 0 ? pos + 1 - p.window : 0;
-    if (end > keys) end = keys;
-    if (end > capacity) end = capacity;
-    if (begin < 0) begin = 0;
-    float q[8] = {};
-    if (carries) zb::ld_bf16x8(p.q + (int64_t)t * p.q_stride + (int64_t)h * hd + gl * 8, q);
-    for (int64_t j0 = begin; j0 < end; j0 += kKeys) {
-      const int64_t j = j0 + kl;
-      bool sees = j < end;
-      int page = -1;
-      if (sees) page = p.kv.table[(int64_t)b * p.kv.table_stride + j / p.kv.page_size];
-      sees = page >= 0 && page < p.kv.num_pages;
-      float k[8] = {}, v[8] = {};
-      if (sees && carries) {
-        const int64_t at = (int64_t)page * p.kv.page_stride + (int64_t)(j % p.kv.page_size) * p.kv.slot_stride +
-                           (int64_t)kvh * p.kv.head_stride + gl * 8;
-        zb::ld_bf16x8(p.kv.k + at, k);
-        zb::ld_bf16x8(p.kv.v + at, v);
-      }
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s = fmaf(q[i], k[i], s);
-#pragma unroll
-      for (int o = GL / 2; o > 0; o /= 2) s += __shfl_xor_sync(0xffffffffu, s, o);
-      if (!sees) continue;
-      s *= p.scale_log2;
-      const float m_new = fmaxf(m, s), corr = exp2f(m - m_new), e = exp2f(s - m_new);
-      l = l * corr + e;
-      m = m_new;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] = acc[i] * corr + e * v[i];
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  const uint32_t raw = zb::smem_addr(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  unsigned char* gbase = smem_raw + (base - raw);
+  Tail& tl = *reinterpret_cast<Tail*>(gbase + L::kOffTail);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int B = p.kv.B, Hkv = p.kv.Hkv, hd = p.kv.hd, G = p.G;
+  const int cta = blockIdx.x, ctas = gridDim.x;
+
+  if (tid == 0) {
+    for (int s = 0; s < L::kSlots; ++s) {
+      zb::mbar_init(zb::smem_addr(&tl.full[s]), kLoadWarps * 32 + 1);
+      zb::mbar_init(zb::smem_addr(&tl.empty[s]), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      zb::mbar_init(zb::smem_addr(&tl.q_full[s]), kLoadWarps * 32);
+      zb::mbar_init(zb::smem_addr(&tl.q_empty[s]), 1);
+      zb::mbar_init(zb::smem_addr(&tl.s_full[s]), 2);
+      zb::mbar_init(zb::smem_addr(&tl.p_full[s]), kStreamRows);
+      zb::mbar_init(zb::smem_addr(&tl.o_full[s]), 1);
+    }
+    zb::mbar_init(zb::smem_addr(&tl.scanned), 1);
+    zb::mbar_init(zb::smem_addr(&tl.drained), 1);
+    for (int s = 0; s < kDescs; ++s) {
+      zb::mbar_init(zb::smem_addr(&tl.desc_full[s]), 1);
+      zb::mbar_init(zb::smem_addr(&tl.desc_empty[s]), kSoftWarps + 1);
+    }
+    zb::fence_mbar_init();
+    tl.abort = 0;
+    tl.found = 0;
+    if (p.headers) p.headers[cta].parts = 0;
+  }
+  if (warp == kMmaWarp) tc::alloc(zb::smem_addr(&tl.tmem), 512);
+
+  // ---- rows of no request
+  {
+    const int first = min(max(p.kv.cu[0], 0), p.kv.N), last = min(max(p.kv.cu[B], first), p.kv.N);
+    const int idle = first + p.kv.N - last;
+    for (int i = cta * (kThreads / 32) + warp; i < idle; i += ctas * (kThreads / 32)) {
+      const int64_t t = i < first ? i : last + i - first;
+      for (int c = lane; c < p.Hq * hd / 8; c += 32)
+        *reinterpret_cast<uint4*>(p.out + t * p.out_stride + c * 8) = make_uint4(0, 0, 0, 0);
+      if (p.lse)
+        for (int h = lane; h < p.Hq; h += 32) p.lse[t * p.Hq + h] = -INFINITY;
     }
   }
-#pragma unroll
-  for (int o = GL; o < 32; o *= 2) {  // join the key groups
-    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
-    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
-    const float c1 = exp2f(m - base), c2 = exp2f(m2 - base);
-    l = l * c1 + l2 * c2;
-    m = top;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = acc[i] * c1 + __shfl_xor_sync(0xffffffffu, acc[i], o) * c2;
+
+  // ---- the plan: steps (tiles, at least one a unit) of all units, and this CTA's first one
+  int* pairs_before = reinterpret_cast<int*>(gbase);  // [B], over the ring
+  int64_t all_pairs = 0;
+  for (int b0 = 0; b0 < B; b0 += kThreads) {
+    const int b = b0 + tid;
+    const int n = b < B ? (request(p, b).tokens * G + kUnitRows - 1) / kUnitRows : 0;
+    int64_t total;
+    const int64_t before = block_scan(n, tl, total);
+    if (b < B) pairs_before[b] = (int)(all_pairs + before);
+    all_pairs += total;
   }
-  float f = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // a NaN sum stays one
-  if (p.gate) f *= 1.f / (1.f + expf(-__bfloat162float(p.gate[(int64_t)t * p.gate_stride + h])));
-  if (kl == 0 && carries) {
-    float y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = acc[i] * f;
-    *reinterpret_cast<uint4*>(p.out + (int64_t)t * p.out_stride + (int64_t)h * hd + gl * 8) = zb::pack_bf16x8(y);
+  __syncthreads();
+  // more than the tokens can make: cu decreases somewhere, nothing is done
+  const int pairs = all_pairs <= p.pairs_max ? (int)all_pairs : 0;
+  if (all_pairs > p.pairs_max && cta == 0 && tid == 0 && p.status) atomicOr(p.status, zb::kStatusAttnChunkBatch);
+  auto pair_steps = [&](int j, int& b, int& pair) {  // steps of pair j for one KV head
+    int lo = 0, hi = B;  // the last b with pairs_before[b] <= j
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (pairs_before[mid] <= j) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+    pair = j - pairs_before[lo];
+    Desc d;
+    unit_tiles(p, request(p, b), pair, d);
+    return max(d.tiles, 1);
+  };
+  int64_t work = 0;
+  for (int j0 = 0; j0 < pairs; j0 += kThreads) {
+    int b, pair;
+    int64_t total;
+    block_scan(j0 + tid < pairs ? pair_steps(j0 + tid, b, pair) : 0, tl, total);
+    work += total;
   }
-  if (p.lse && lane == 0)
-    p.lse[(int64_t)t * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  work *= Hkv;
+  const int64_t share = (work + ctas - 1) / ctas;
+  const int64_t begin = share * cta, end = min(work, begin + share);
+  if (begin < end) {
+    int64_t seen = 0;
+    for (int j0 = 0; j0 < pairs; j0 += kThreads) {
+      int b = 0, pair = 0;
+      int64_t total;
+      const int n = j0 + tid < pairs ? pair_steps(j0 + tid, b, pair) : 0;
+      const int64_t at = (seen + block_scan(n, tl, total)) * Hkv;
+      if (n > 0 && begin >= at && begin < at + (int64_t)n * Hkv) {
+        tl.start[0] = b;
+        tl.start[1] = pair;
+        tl.start_off = begin - at;
+      }
+      seen += total;
+      if (begin < seen * Hkv) break;
+    }
+  }
+  if (hd < HD) {  // the padding dims of every tile stay zero
+    __syncthreads();
+    for (uint32_t i = tid; i < L::kOffTail / 16; i += kThreads) reinterpret_cast<uint4*>(gbase)[i] = make_uint4(0, 0, 0, 0);
+    tc::fence_proxy_async();
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  const uint32_t tmem = tl.tmem;
+  int* abort = &tl.abort;
+
+  if (begin >= end) {
+    // nothing for this CTA
+  } else if (warp >= kLoadWarp) {
+    // =============================================================================================== loaders
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    const int lw = warp - kLoadWarp;
+    constexpr int kChunks = HD / 8;          // 16-byte pieces of a row
+    constexpr int kPass = 32 / kChunks;      // rows of a warp's copy instruction
+    constexpr int kGroup = 32 / kPass;       // instructions of 32 rows
+    const int chunk = lane % kChunks, sub = lane / kChunks;
+    const bool carries = chunk * 8 < hd;
+    // rows 32 k + l of a tile are at element offset off[k] of lane l (negative: absent, zeros)
+    auto copy_tile = [&](uint32_t dst, const __nv_bfloat16* src, const int64_t (&off)[4]) {
+      const uint32_t col = (uint32_t)(chunk / 8) * kBlk;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll 2
+        for (int g = (lw + k) % kLoadWarps; g < kGroup; g += kLoadWarps) {
+          const int r = g * kPass + sub;
+          const int64_t o = __shfl_sync(0xffffffffu, off[k], r);
+          if (carries) cp_async16(dst + col + tc::sw128(32 * k + r, chunk % 8), src + (o < 0 ? 0 : o) + chunk * 8, o >= 0);
+        }
+      }
+    };
+    // this lane's request of the window of 32 requests around the current one
+    int window0 = -1;
+    Request mine{};
+    auto fetch_window = [&](int b) {
+      if (b / 32 != window0) {
+        window0 = b / 32;
+        const int i = window0 * 32 + lane;
+        mine = i < B ? request(p, i) : Request{0, 0, 0};
+      }
+    };
+    int b = tl.start[0], pair = tl.start[1];
+    fetch_window(b);
+    Request req;
+    auto take = [&](int i) {
+      req.row0 = __shfl_sync(0xffffffffu, mine.row0, i % 32);
+      req.tokens = __shfl_sync(0xffffffffu, mine.tokens, i % 32);
+      req.keys = __shfl_sync(0xffffffffu, mine.keys, i % 32);
+    };
+    take(b);
+    Desc d;
+    unit_tiles(p, req, pair, d);
+    int64_t done = begin;
+    int kvh = (int)(tl.start_off / max(d.tiles, 1)), skip = (int)(tl.start_off % max(d.tiles, 1));
+    int item = 0, tile_no = 0, uses[2] = {0, 0};
+    for (int n = 0;; ++n) {
+      // ---- the unit's descriptor
+      const int steps = max(d.tiles, 1);
+      const int64_t left = end - done;
+      const int take_steps = (int)min((int64_t)(steps - skip), left);
+      Desc u = d;
+      u.kvh = kvh;
+      if (d.tiles > 0) {
+        u.tile0 = d.tile0 + skip;
+        u.tiles = take_steps;
+      }
+      const bool starts = skip == 0, ends = skip + take_steps == steps;
+      u.mode = left <= 0 ? kStop : starts && ends ? kFinal : starts ? kPart1 : kPart0;
+      u.parts = (int)((done - skip + steps - 1) / share) - cta + 1;
+      if (warp == kLoadWarp && lane == 0) {
+        const int slot = n % kDescs;
+        if (n >= kDescs) wait(tl.desc_empty[slot], (n / kDescs - 1) & 1, abort, p.status);
+        tl.desc[slot] = u;
+        arrive(tl.desc_full[slot]);
+      }
+      __syncwarp();
+      if (u.mode == kStop) break;
+      if (u.tiles > 0) {
+        const int held = min(req.keys, p.kv.max_pages * p.kv.page_size);
+        const int32_t* table = p.kv.table + (int64_t)b * p.kv.table_stride;
+        int pages[4];
+        auto look = [&](int t) {  // pages of the lane's rows of tile t
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int pos = t * kTile + 32 * k + lane;
+            pages[k] = pos < held ? table[pos / p.kv.page_size] : -1;
+          }
+        };
+        look(u.tile0);
+        for (int t = 0; t < u.tiles; ++t) {
+          int64_t off[4];
+          unsigned bits[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int pos = (u.tile0 + t) * kTile + 32 * k + lane;
+            const bool there = pages[k] >= 0 && pages[k] < p.kv.num_pages;
+            off[k] = there ? (int64_t)pages[k] * p.kv.page_stride + (int64_t)(pos % p.kv.page_size) * p.kv.slot_stride +
+                                 (int64_t)kvh * p.kv.head_stride
+                           : -1;
+            bits[k] = __ballot_sync(0xffffffffu, there);
+          }
+          if (t + 1 < u.tiles) look(u.tile0 + t + 1);
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv, ++item) {
+            const int slot = item % L::kSlots;
+            if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort, p.status);
+            copy_tile(base + slot * L::kItem, kv ? p.kv.v : p.kv.k, off);
+            cp_async_arrive(zb::smem_addr(&tl.full[slot]));
+            if (warp == kLoadWarp && lane == 0) {
+              if (kv == 0) *reinterpret_cast<uint4*>(tl.mask[tile_no % kMasks]) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+              arrive(tl.full[slot]);
+            }
+          }
+          ++tile_no;
+          if (t == 0) {  // the unit's queries, behind its first tile so that the ring keeps filling meanwhile
+            for (int s = 0; s < (u.rows > kStreamRows ? 2 : 1); ++s) {
+              int64_t qoff[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int r = s * kStreamRows + 32 * k + lane, pr = u.pr0 + r;
+                qoff[k] = r < u.rows ? (int64_t)(u.row0 + pr / G) * p.q_stride + (int64_t)(kvh * G + pr % G) * hd : -1;
+              }
+              if (uses[s] > 0) wait(tl.q_empty[s], (uses[s] - 1) & 1, abort, p.status);
+              ++uses[s];
+              copy_tile(base + L::kOffQ + s * L::kItem, p.q, qoff);
+              cp_async_arrive(zb::smem_addr(&tl.q_full[s]));
+            }
+          }
+        }
+      }
+      // ---- the next unit: KV head, then pair, then request
+      done += take_steps;
+      skip = 0;
+      if (done >= end) {
+        d.tiles = 0;
+        continue;  // the stop descriptor
+      }
+      if (++kvh == Hkv) {
+        kvh = 0;
+        if ((pair + 1) * kUnitRows < req.tokens * G) {
+          ++pair;
+        } else {
+          pair = 0;
+          do {
+            ++b;
+            fetch_window(min(b, B - 1));
+            take(min(b, B - 1));
+          } while (b < B && req.tokens == 0);
+        }
+        unit_tiles(p, req, pair, d);
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+  } else if (warp == kMmaWarp) {
+    // =============================================================================================== tensor cores
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    constexpr uint32_t kIdS = tc::idesc_bf16(kStreamRows, kTile);
+    constexpr uint32_t kIdO = tc::idesc_bf16(kStreamRows, HD, false, /*b_mn=*/true);
+    int item = 0, tiles_done[2] = {0, 0}, q_uses[2] = {0, 0};
+    auto full = [&](int i) { wait(tl.full[i % L::kSlots], (i / L::kSlots) & 1, abort, p.status); };
+    auto issue_s = [&](int s, int i) {  // S_s = Q_s K^T of ring item i
+      if (lane != 0) return;
+      const uint32_t kb = base + (uint32_t)(i % L::kSlots) * L::kItem, qb = base + L::kOffQ + s * L::kItem;
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        const uint32_t o = (ks / 4) * kBlk + (ks % 4) * 32;
+        tc::mma(tmem + L::kColS + s * kTile, tc::desc_kmajor(qb + o), tc::desc_kmajor(kb + o), kIdS, ks > 0);
+      }
+      tc::commit(zb::smem_addr(&tl.s_full[s]));
+      arrive(tl.s_full[s]);  // passes on the tile's key mask, which this thread got with the tile
+    };
+    auto issue_o = [&](int s, int i, bool accumulate) {  // O_s (+)= P_s V of ring item i
+      if (lane != 0) return;
+      const uint32_t vb = base + (uint32_t)(i % L::kSlots) * L::kItem;
+#pragma unroll
+      for (int ks = 0; ks < kTile / 16; ++ks)
+        mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, tc::desc_mnmajor(vb + ks * 2048, kBlk, 1024),
+               kIdO, accumulate || ks > 0);
+    };
+    auto commit = [&](const uint64_t& bar) {
+      if (lane == 0) tc::commit(zb::smem_addr(&bar));
+    };
+    for (int n = 0;; ++n) {
+      const int slot = n % kDescs;
+      wait(tl.desc_full[slot], (n / kDescs) & 1, abort, p.status);
+      const Desc u = tl.desc[slot];
+      __syncwarp();
+      if (lane == 0) arrive(tl.desc_empty[slot]);
+      if (u.mode == kStop || gave_up(abort)) break;
+      if (u.tiles == 0) continue;
+      const int streams = u.rows > kStreamRows ? 2 : 1;
+      for (int t = -1; t < u.tiles; ++t) {
+        // O_s += P_s(t) V(t) as soon as P_s(t) is there, then S_s(t + 1)
+        const int v_item = item + 1, k_next = t < 0 ? item : item + 2;
+        const bool more = t + 1 < u.tiles;
+        bool found = false;
+        if (t >= 0) {
+          full(v_item);
+          const int first = (u.tile0 + t) * kTile;
+          if (first + kTile > u.all_hi || first < u.all_lo) {  // keys that some rows see and others do not
+            bool bad = false;
+            const uint4* v = reinterpret_cast<const uint4*>(gbase + (v_item % L::kSlots) * L::kItem);
+#pragma unroll 8
+            for (uint32_t i = lane; i < L::kItem / 16; i += 32) bad |= not_finite(v[i]);
+            found = __any_sync(0xffffffffu, bad);
+            if (lane == 0) {
+              tl.found = found;
+              arrive(tl.scanned);
+            }
+            if (found) {  // every stream adds what it sees before it hands over P; then the values are zeroed
+              for (int s = 0; s < streams; ++s) wait(tl.p_full[s], tiles_done[s] & 1, abort, p.status);
+              uint16_t* e = reinterpret_cast<uint16_t*>(gbase + (v_item % L::kSlots) * L::kItem);
+              for (uint32_t i = lane; i < L::kItem / 2; i += 32)
+                if ((e[i] & 0x7f80u) == 0x7f80u) e[i] = 0;
+              tc::fence_proxy_async();
+              __syncwarp();
+            }
+          }
+          tc::fence_proxy_async();  // the loaders' copies -> the tensor cores
+        }
+        for (int s = 0; s < streams; ++s) {
+          if (t >= 0) {
+            wait(tl.p_full[s], tiles_done[s] & 1, abort, p.status);
+            ++tiles_done[s];
+            tc::fence_after();
+            issue_o(s, v_item, t > 0 || found);
+            if (!more) commit(tl.o_full[s]);
+            if (s == streams - 1) commit(tl.empty[v_item % L::kSlots]);
+          } else {
+            wait(tl.q_full[s], q_uses[s] & 1, abort, p.status);
+            ++q_uses[s];
+          }
+          if (more) {
+            if (s == 0 || t < 0) {
+              full(k_next);
+              tc::fence_proxy_async();
+            }
+            issue_s(s, k_next);
+            if (t + 2 >= u.tiles) commit(tl.q_empty[s]);
+            if (s == streams - 1) commit(tl.empty[k_next % L::kSlots]);
+          }
+        }
+        if (t >= 0) item += 2;
+      }
+    }
+    commit(tl.drained);  // nothing is in flight when the tensor memory is given back, also after a wait that gave up
+    if (lane == 0) zb::mbar_wait_bounded(zb::smem_addr(&tl.drained), 0, p.status, zb::kStatusAttnChunkTimeout);
+    __syncwarp();
+  } else {
+    // =============================================================================================== rows
+    // 8 x 32 x 208 + 4 x 32 x 88 registers are the 384 x 168 that the CTA was launched with
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int s = warp / 4;  // stream
+    const uint32_t tlane = tmem + ((uint32_t)(32 * (warp % 4)) << 16);
+    const uint32_t col_s = tlane + L::kColS + s * kTile, col_o = tlane + L::kColO + s * HD;
+    int tile_no = 0, k_item = 0, mine = 0, units = 0, scans = 0;  // counters of what this CTA / this stream has done
+    for (int n = 0;; ++n) {
+      const int slot = n % kDescs;
+      wait(tl.desc_full[slot], (n / kDescs) & 1, abort, p.status);
+      const Desc u = tl.desc[slot];
+      __syncwarp();
+      if (lane == 0) arrive(tl.desc_empty[slot]);
+      if (u.mode == kStop || gave_up(abort)) break;
+      const int r = s * kStreamRows + 32 * (warp % 4) + lane;
+      const bool live = r < u.rows;
+      const int pr = u.pr0 + r, i = live ? pr / G : 0, h = u.kvh * G + (live ? pr % G : 0);
+      const int64_t token = u.row0 + i;
+      const Request req{u.row0, u.tokens, u.keys};
+      float m = -INFINITY, l = 0.f;
+      if (u.tiles > 0 && s * kStreamRows < u.rows) {
+        int lo = 0, hi = INT32_MAX;  // a row past the unit's last sees everything; it is not stored
+        if (live) visible(p, req, i, lo, hi);
+        for (int t = 0; t < u.tiles; ++t, ++mine) {
+          const int first = (u.tile0 + t) * kTile;
+          const bool scan = first + kTile > u.all_hi || first < u.all_lo;
+          wait(tl.s_full[s], mine & 1, abort, p.status);
+          tc::fence_after();
+          uint32_t x[kTile];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) ld32(col_s + 32 * c, x + 32 * c);
+          const uint4 there = *reinterpret_cast<const uint4*>(tl.mask[(tile_no + t) % kMasks]);
+          const unsigned words[4] = {there.x, there.y, there.z, there.w};
+          tc::ld_wait();
+          unsigned seen[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+          const bool partly = first < lo || first + kTile > hi || (there.x & there.y & there.z & there.w) != 0xffffffffu;
+          if (__any_sync(0xffffffffu, partly)) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int a = min(max(lo - first - 32 * c, 0), 32), z = min(max(hi - first - 32 * c, 0), 32);
+              const unsigned below = z >= 32 ? 0xffffffffu : (1u << z) - 1u;
+              const unsigned under = a >= 32 ? 0xffffffffu : (1u << a) - 1u;
+              seen[c] = words[c] & below & ~under;
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (!((seen[c] >> j) & 1u)) x[32 * c + j] = __float_as_uint(-INFINITY);
+            }
+          }
+          float top = -INFINITY;
+          {
+            float part[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              part[c] = __uint_as_float(x[c]);
+#pragma unroll
+              for (int j = 1; j < 32; ++j) part[c] = fmaxf(part[c], __uint_as_float(x[4 * j + c]));
+            }
+            top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * p.scale_log2;
+          }
+          const bool grow = top > m + kRescale;
+          if (__any_sync(0xffffffffu, grow)) {
+            const float corr = grow ? ex2(m - top) : 1.f;  // 0 for the row's first key
+            if (grow) m = top;
+            l *= corr;
+            if (t > 0) {
+#pragma unroll
+              for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                ld32(col_o + 32 * c, o);
+                tc::ld_wait();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                st32(col_o + 32 * c, o);
+              }
+            }
+          }
+          const float mb = m == -INFINITY ? 0.f : m;
+          const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), minus = pack2(-mb, -mb);
+          uint64_t sum2[2] = {0, 0};
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t packed[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const int e = 64 * c + 2 * j;
+              float a, z;
+              unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), scale2, minus), a, z);
+              a = ex2(a);
+              z = ex2(z);
+              sum2[j % 2] = add2(sum2[j % 2], pack2(a, z));
+              packed[j] = to_bf16x2(a, z);
+            }
+            st32(col_s + 32 * c, packed);
+          }
+          {
+            float a, z;
+            unpack2(add2(sum2[0], sum2[1]), a, z);
+            l += a + z;
+          }
+          if (scan) {
+            wait(tl.scanned, scans & 1, abort, p.status);
+            ++scans;
+            if (*reinterpret_cast<volatile int*>(&tl.found)) {  // values that are not finite, one by one
+              if (t == 0) {  // the tile's product adds to the accumulator then
+                uint32_t zero[32] = {};
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) st32(col_o + 32 * c, zero);
+              }
+              tc::st_wait();
+              const unsigned char* v = gbase + (size_t)((k_item + 2 * t + 1) % L::kSlots) * L::kItem;
+              for (int j = 0; j < kTile; ++j) {
+                const unsigned word = j < 32 ? seen[0] : j < 64 ? seen[1] : j < 96 ? seen[2] : seen[3];
+                const bool sees = (word >> (j % 32)) & 1u;
+                for (int c = 0; c < HD / 8; ++c) {
+                  const uint4 w = *reinterpret_cast<const uint4*>(v + (c / 8) * kBlk + tc::sw128(j, c % 8));
+                  if (!not_finite(w)) continue;  // the same for every lane
+                  const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) {
+                    const float val = __uint_as_float(e % 2 ? q[e / 2] & 0xffff0000u : q[e / 2] << 16);
+                    if ((__float_as_uint(val) & 0x7f800000u) != 0x7f800000u) continue;
+                    const float o = __uint_as_float(ld1(col_o + c * 8 + e));
+                    tc::ld_wait();
+                    st1(col_o + c * 8 + e, __float_as_uint(sees ? o + val : o));
+                    tc::st_wait();
+                  }
+                }
+              }
+            }
+          }
+          tc::st_wait();
+          tc::fence_before();
+          arrive(tl.p_full[s]);
+        }
+        wait(tl.o_full[s], units & 1, abort, p.status);
+        ++units;
+        tc::fence_after();
+      }
+      // the scans of tiles this stream had no rows in
+      if (u.tiles > 0 && s * kStreamRows >= u.rows)
+        for (int t = 0; t < u.tiles; ++t)
+          if ((u.tile0 + t) * kTile + kTile > u.all_hi || (u.tile0 + t) * kTile < u.all_lo) ++scans;
+      tile_no += u.tiles;
+      k_item += 2 * u.tiles;
+      if (s * kStreamRows >= u.rows || gave_up(abort)) continue;
+      if (u.mode == kFinal) {
+        const float f = live ? row_factor(p, token, h, l) : 0.f;
+        __nv_bfloat16* dst = p.out + token * p.out_stride + (int64_t)h * hd;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32] = {};
+          if (u.tiles > 0) {
+            ld32(col_o + 32 * c, o);
+            tc::ld_wait();
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = l == 0.f ? 0.f : __uint_as_float(o[8 * j + e]);
+            if (live && 32 * c + 8 * j < hd) store8(dst + 32 * c + 8 * j, y, f);
+          }
+        }
+        if (p.lse && live) p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      } else {
+        const int64_t part = (int64_t)cta * 2 + (u.mode == kPart1);
+        float* acc = p.acc + part * HD * p.rows_max;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+          uint32_t o[32];
+          ld32(col_o + 32 * c, o);
+          tc::ld_wait();
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (live)
+              *reinterpret_cast<uint4*>(acc + ((int64_t)(8 * c + j) * p.rows_max + r) * 4) =
+                  make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+        }
+        if (live) {
+          p.ml[part * 2 * p.rows_max + r] = m;
+          p.ml[(part * 2 + 1) * p.rows_max + r] = l;
+        }
+        if (u.mode == kPart1 && tid == 0) p.headers[cta] = Header{u.parts, u.row0, u.pr0, u.rows, u.kvh, {0, 0, 0}};
+      }
+      tc::fence_before();  // the accumulator's reads come before the next unit's products
+    }
+  }
+  tc::fence_before();
+  __syncthreads();
+  tc::fence_after();
+  if (warp == kMmaWarp) tc::dealloc(tmem, 512);
+}
+
+// Joins the parts of the units that span CTAs, in the order of their keys: a thread takes 4 dims of a row.
+template <int HD>
+__global__ void __launch_bounds__(256) gqa_chunk_join_kernel(const __grid_constant__ ChunkParams p) {
+  zb::pdl_enter();
+  const Header u = p.headers[blockIdx.x];
+  const int at = blockIdx.y * 256 + threadIdx.x, d4 = at / p.rows_max, r = at % p.rows_max;
+  if (u.parts == 0 || r >= u.rows || d4 >= HD / 4) return;
+  float top = -INFINITY;
+  for (int i = 0; i < u.parts; ++i) {
+    const int64_t part = (int64_t)(blockIdx.x + i) * 2 + (i == 0);
+    top = fmaxf(top, p.ml[part * 2 * p.rows_max + r]);
+  }
+  const float mb = top == -INFINITY ? 0.f : top;
+  float l = 0.f, y[4] = {};
+  for (int i = 0; i < u.parts; ++i) {
+    const int64_t part = (int64_t)(blockIdx.x + i) * 2 + (i == 0);
+    const float sum = p.ml[(part * 2 + 1) * p.rows_max + r];
+    const float4 a = *reinterpret_cast<const float4*>(p.acc + (part * (HD / 4) + d4) * p.rows_max * 4 + r * 4);
+    const float f = ex2(p.ml[part * 2 * p.rows_max + r] - mb);
+    if (sum == 0.f) continue;  // no key of this part is visible to the row
+    l += sum * f;
+    y[0] += a.x * f;
+    y[1] += a.y * f;
+    y[2] += a.z * f;
+    y[3] += a.w * f;
+  }
+  const int pr = u.pr0 + r, h = u.kvh * p.G + pr % p.G;
+  const int64_t token = u.row0 + pr / p.G;
+  const float f = row_factor(p, token, h, l);
+  if (d4 * 4 < p.kv.hd) {
+    const uint2 packed = make_uint2(to_bf16x2(y[0] * f, y[1] * f), to_bf16x2(y[2] * f, y[3] * f));
+    *reinterpret_cast<uint2*>(p.out + token * p.out_stride + (int64_t)h * p.kv.hd + d4 * 4) = packed;
+  }
+  if (p.lse && d4 == 0) p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+}
+
+// The launch: CTAs, and whether a unit can span several of them.
+struct Launch {
+  int ctas, rows_max;
+  bool splits;
+  int64_t pairs, header_bytes, acc_bytes, ml_bytes;
+};
+Launch plan(int B, int64_t N, int Hq, int Hkv, int hd, int64_t max_keys) {
+  Launch l{};
+  if (Hkv < 1 || B < 1 || N < 1) return l;
+  const int64_t rows = N * (Hq / Hkv), tiles = std::max<int64_t>((max_keys + kTile - 1) / kTile, 1);
+  l.pairs = rows / kUnitRows + std::min<int64_t>(B, N);
+  l.ctas = (int)std::min<int64_t>(zb::sm_count(), l.pairs * Hkv * tiles);
+  l.splits = tiles > 1 && l.ctas > 1;
+  l.rows_max = (int)std::min<int64_t>(rows, kUnitRows);
+  if (l.splits) {
+    const int64_t width = hd <= 64 ? 64 : 128;
+    l.header_bytes = ((int64_t)l.ctas * (int64_t)sizeof(Header) + 255) / 256 * 256;
+    l.acc_bytes = (int64_t)l.ctas * 2 * l.rows_max * width * 4;
+    l.ml_bytes = (int64_t)l.ctas * 4 * l.rows_max * 4;
+  }
+  return l;
+}
+
+template <int HD>
+int launch_chunk(const ChunkParams& p, const Launch& l, cudaStream_t stream) {
+  auto kernel = gqa_chunk_kernel<HD>;
+  static bool configured[64] = {false};  // the shared-memory attribute, set once per device
+  int dev = 0;
+  ZB_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64 || !configured[dev]) {
+    ZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD>::kSmem));
+    if (dev >= 0 && dev < 64) configured[dev] = true;
+  }
+  ZB_CUDA(zb::launch(kernel, dim3((unsigned)l.ctas), dim3(kThreads), Shape<HD>::kSmem, stream, 1, p));
+  if (int rc = zb::check_launch("gqa_chunk")) return rc;
+  if (l.splits) {
+    const dim3 grid((unsigned)l.ctas, (unsigned)((l.rows_max * (HD / 4) + 255) / 256));
+    ZB_CUDA(zb::launch(gqa_chunk_join_kernel<HD>, grid, dim3(256), 0, stream, 1, p));
+    return zb::check_launch("gqa_chunk(join)");
+  }
+  return zb::kOk;
 }
 
 }  // namespace
 
 ZB_API int64_t zb_gqa_chunk_workspace_bytes(int B, int N, int Hq, int Hkv, int hd, int64_t max_keys) {
-  return 0;
+  const Launch l = plan(B, N, Hq, Hkv, hd, max_keys);
+  return l.header_bytes + l.acc_bytes + l.ml_bytes;
 }
 
 ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache,
@@ -124,14 +944,22 @@ ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_c
                  (!gate || gate_stride >= Hq),
              "gqa_chunk: strides (q %lld, out %lld, gate %lld)", (long long)q_stride, (long long)out_stride,
              (long long)gate_stride);
+  ZB_REQUIRE((int64_t)N * Hq < (int64_t)1 << 31, "gqa_chunk: %d tokens x %d heads", N, Hq);
+  if (B > kMaxRequests) return zb::fail(zb::kUnsupported, "gqa_chunk: %d requests (at most %d)", B, kMaxRequests);
   if (N == 0) return zb::kOk;
   ZB_REQUIRE(B > 0, "gqa_chunk: %d tokens of no request", N);
   ZB_REQUIRE(q && out, "gqa_chunk: null pointer");
   ZB_REQUIRE_ALIGNED(q, 16, "gqa_chunk q");
   ZB_REQUIRE_ALIGNED(out, 16, "gqa_chunk out");
+  const Launch l = plan(B, N, Hq, Hkv, hd, (int64_t)page_size * max_pages);
+  const int64_t need = l.header_bytes + l.acc_bytes + l.ml_bytes;
+  ZB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "gqa_chunk: a workspace of %lld bytes, got %lld",
+             (long long)need, (long long)workspace_bytes);
+  ZB_REQUIRE_ALIGNED(workspace, 16, "gqa_chunk workspace");
   p.q = reinterpret_cast<const __nv_bfloat16*>(q);
   p.q_stride = q_stride;
   p.Hq = Hq;
+  p.G = Hq / Hkv;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.causal = causal;
   p.window = window;
@@ -140,11 +968,12 @@ ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_c
   p.out = reinterpret_cast<__nv_bfloat16*>(out);
   p.out_stride = out_stride;
   p.lse = lse;
-  const dim3 grid((unsigned)(((int64_t)N * Hq + kWarps - 1) / kWarps)), block(kWarps * 32);
-  const int lanes = hd / 8;
-  cudaError_t err = lanes <= 4   ? zb::launch(gqa_chunk_kernel<4>, grid, block, 0, stream, 1, p)
-                    : lanes <= 8 ? zb::launch(gqa_chunk_kernel<8>, grid, block, 0, stream, 1, p)
-                                 : zb::launch(gqa_chunk_kernel<16>, grid, block, 0, stream, 1, p);
-  ZB_CUDA(err);
-  return zb::check_launch("gqa_chunk");
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  p.headers = l.splits ? reinterpret_cast<Header*>(ws) : nullptr;
+  p.acc = reinterpret_cast<float*>(ws + l.header_bytes);
+  p.ml = reinterpret_cast<float*>(ws + l.header_bytes + l.acc_bytes);
+  p.rows_max = l.rows_max;
+  p.pairs_max = (int)l.pairs;
+  p.status = zb::device_status_ptr();
+  return hd <= 64 ? launch_chunk<64>(p, l, stream) : launch_chunk<128>(p, l, stream);
 }
