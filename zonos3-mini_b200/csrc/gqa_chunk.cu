@@ -31,6 +31,7 @@
 
 #include "paged.cuh"
 #include "tc.cuh"
+#include "tc_pair.cuh"
 
 namespace {
 
@@ -41,7 +42,6 @@ constexpr int kStreamRows = 128;  // rows of a stream
 constexpr int kUnitRows = 2 * kStreamRows;
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
-constexpr uint32_t kBlk = kTile * 128;  // 64 dims of 128 rows, 128-byte swizzled
 constexpr int kMaxSlots = 10, kDescs = 4;
 constexpr int kMasks = 8;  // the loaders run at most 5 tiles ahead of the rows
 constexpr float kRescale = 8.f;  // log2 growth of a row's maximum that the accumulator is rescaled for
@@ -66,6 +66,11 @@ struct ChunkParams {
   int rows_max;
   int pairs_max;  // units of a KV head, at most
   unsigned* status;
+  int box;  // rows of a page that one tensor copy brings; 0: K and V rows come by 16-byte copies
+  int head_atoms, page_heads;  // a KV head's atom offset, and a page's index step, in the tensor maps
+};
+struct Maps {
+  CUtensorMap k, v;
 };
 
 // A unit that starts in this CTA and ends in another one (parts = 0: there is none).
@@ -108,7 +113,10 @@ struct Tail {
 
 template <int HD>
 struct Shape {
-  static constexpr uint32_t kItem = HD / 64 * kBlk;
+  // A tile of 128 rows: 8 rows x 64 dims (128 swizzled bytes each) are an atom; an 8-row group's atoms lie together, so
+  // that one tensor copy of whole rows of a page, of any multiple of 8, lands in place.
+  static constexpr uint32_t kGroup = HD / 64 * 1024;
+  static constexpr uint32_t kItem = kTile / 8 * kGroup;
   static constexpr int kSlots = HD == 128 ? 5 : 10;
   static constexpr uint32_t kOffQ = kSlots * kItem;
   static constexpr uint32_t kOffTail = kOffQ + 2 * kItem;
@@ -117,6 +125,21 @@ struct Shape {
   static_assert(kSmem <= 232448, "shared memory");
   static constexpr uint32_t kColS = 0, kColO = 2 * kTile;  // stream s: S at s * 128, O at 256 + s * HD
 };
+
+// Byte offset of 16-byte piece c of row r in a tile.
+template <int HD>
+__device__ __forceinline__ uint32_t piece(int r, int c) {
+  return (uint32_t)(r / 8) * Shape<HD>::kGroup + (uint32_t)(c / 8) * 1024 + tc::sw128(r % 8, c % 8);
+}
+
+// Rows of a page, of one KV head: a box of 64 dims x 8 rows x atoms x row groups.
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, int atom, int group, int page, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
+      "[%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(0), "r"(atom), "r"(group), "r"(page), "r"(bar)
+      : "memory");
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -288,7 +311,8 @@ __device__ __forceinline__ float row_factor(const ChunkParams& p, int64_t t, int
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_constant__ ChunkParams p) {
+__global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_constant__ ChunkParams p,
+                                                                const __grid_constant__ Maps maps) {
   using L = Shape<HD>;
   zb::pdl_enter();
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -302,11 +326,11 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 
   if (tid == 0) {
     for (int s = 0; s < L::kSlots; ++s) {
-      zb::mbar_init(zb::smem_addr(&tl.full[s]), kLoadWarps * 32 + 1);
+      zb::mbar_init(zb::smem_addr(&tl.full[s]), p.box ? 1 : kLoadWarps * 32 + 1);
       zb::mbar_init(zb::smem_addr(&tl.empty[s]), 1);
     }
     for (int s = 0; s < 2; ++s) {
-      zb::mbar_init(zb::smem_addr(&tl.q_full[s]), kLoadWarps * 32);
+      zb::mbar_init(zb::smem_addr(&tl.q_full[s]), (kLoadWarps - 1) * 32);
       zb::mbar_init(zb::smem_addr(&tl.q_empty[s]), 1);
       zb::mbar_init(zb::smem_addr(&tl.s_full[s]), 2);
       zb::mbar_init(zb::smem_addr(&tl.p_full[s]), kStreamRows);
@@ -411,19 +435,26 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     const int lw = warp - kLoadWarp;
     constexpr int kChunks = HD / 8;          // 16-byte pieces of a row
     constexpr int kPass = 32 / kChunks;      // rows of a warp's copy instruction
-    constexpr int kGroup = 32 / kPass;       // instructions of 32 rows
+    constexpr int kCopies = kTile / kPass;   // instructions of a tile
     const int chunk = lane % kChunks, sub = lane / kChunks;
     const bool carries = chunk * 8 < hd;
-    // rows 32 k + l of a tile are at element offset off[k] of lane l (negative: absent, zeros)
-    auto copy_tile = [&](uint32_t dst, const __nv_bfloat16* src, const int64_t (&off)[4]) {
-      const uint32_t col = (uint32_t)(chunk / 8) * kBlk;
+    // Rows 32 k + l of a tile are at element offset off[k] of lane l (negative: absent, zeros). `warps` warps share the
+    // tile, this one the `which`-th; the addresses of 4 copies are formed before they are issued, as each copy takes
+    // its row's offset from another lane.
+    auto copy_tile = [&](uint32_t dst, const __nv_bfloat16* src, const int64_t (&off)[4], int which, int warps) {
+      constexpr int kAhead = 4;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-#pragma unroll 2
-        for (int g = (lw + k) % kLoadWarps; g < kGroup; g += kLoadWarps) {
-          const int r = g * kPass + sub;
-          const int64_t o = __shfl_sync(0xffffffffu, off[k], r);
-          if (carries) cp_async16(dst + col + tc::sw128(32 * k + r, chunk % 8), src + (o < 0 ? 0 : o) + chunk * 8, o >= 0);
+        constexpr int kPart = kCopies / 4;
+        for (int g = 0; g < kPart; g += kAhead) {
+          if ((k * (kPart / kAhead) + g / kAhead) % warps != which) continue;
+          int64_t o[kAhead];
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i) o[i] = __shfl_sync(0xffffffffu, off[k], (g + i) * kPass + sub);
+          if (!carries) continue;
+#pragma unroll
+          for (int i = 0; i < kAhead; ++i)
+            cp_async16(dst + piece<HD>(32 * k + (g + i) * kPass + sub, chunk), src + (o[i] < 0 ? 0 : o[i]) + chunk * 8, o[i] >= 0);
         }
       }
     };
@@ -476,53 +507,96 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       if (u.tiles > 0) {
         const int held = min(req.keys, p.kv.max_pages * p.kv.page_size);
         const int32_t* table = p.kv.table + (int64_t)b * p.kv.table_stride;
-        int pages[4];
-        auto look = [&](int t) {  // pages of the lane's rows of tile t
+        // the unit's queries: the warps that bring no keys, or behind the first tile so that the ring keeps filling
+        auto load_q = [&]() {
+          if (warp == kLoadWarp) return;
+          for (int s = 0; s < (u.rows > kStreamRows ? 2 : 1); ++s) {
+            int64_t off[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int pos = t * kTile + 32 * k + lane;
-            pages[k] = pos < held ? table[pos / p.kv.page_size] : -1;
+            for (int k = 0; k < 4; ++k) {
+              const int r = s * kStreamRows + 32 * k + lane, pr = u.pr0 + r;
+              off[k] = r < u.rows ? (int64_t)(u.row0 + pr / G) * p.q_stride + (int64_t)(kvh * G + pr % G) * hd : -1;
+            }
+            if (uses[s] > 0) wait(tl.q_empty[s], (uses[s] - 1) & 1, abort, p.status);
+            ++uses[s];
+            copy_tile(base + L::kOffQ + s * L::kItem, p.q, off, lw - 1, kLoadWarps - 1);
+            cp_async_arrive(zb::smem_addr(&tl.q_full[s]));
           }
         };
-        look(u.tile0);
-        for (int t = 0; t < u.tiles; ++t) {
-          int64_t off[4];
-          unsigned bits[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int pos = (u.tile0 + t) * kTile + 32 * k + lane;
-            const bool there = pages[k] >= 0 && pages[k] < p.kv.num_pages;
-            off[k] = there ? (int64_t)pages[k] * p.kv.page_stride + (int64_t)(pos % p.kv.page_size) * p.kv.slot_stride +
-                                 (int64_t)kvh * p.kv.head_stride
-                           : -1;
-            bits[k] = __ballot_sync(0xffffffffu, there);
-          }
-          if (t + 1 < u.tiles) look(u.tile0 + t + 1);
-#pragma unroll
-          for (int kv = 0; kv < 2; ++kv, ++item) {
-            const int slot = item % L::kSlots;
-            if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort, p.status);
-            copy_tile(base + slot * L::kItem, kv ? p.kv.v : p.kv.k, off);
-            cp_async_arrive(zb::smem_addr(&tl.full[slot]));
-            if (warp == kLoadWarp && lane == 0) {
-              if (kv == 0) *reinterpret_cast<uint4*>(tl.mask[tile_no % kMasks]) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
-              arrive(tl.full[slot]);
-            }
-          }
-          ++tile_no;
-          if (t == 0) {  // the unit's queries, behind its first tile so that the ring keeps filling meanwhile
-            for (int s = 0; s < (u.rows > kStreamRows ? 2 : 1); ++s) {
-              int64_t qoff[4];
+        if (p.box) {
+          if (warp == kLoadWarp) {
+            const int boxes = kTile / p.box;  // of a tile; lane i brings box i
+            auto look = [&](int t) {
+              const int pos = t * kTile + lane * p.box;
+              return lane < boxes && pos < held ? table[pos / p.kv.page_size] : -1;
+            };
+            int next = look(u.tile0);
+            for (int t = 0; t < u.tiles; ++t, ++tile_no) {
+              const int first = (u.tile0 + t) * kTile, pos = first + lane * p.box;
+              const bool there = next >= 0 && next < p.kv.num_pages;
+              const int page = there ? next * p.page_heads + (p.page_heads > 1 ? kvh : 0)
+                                     : (int)(p.kv.num_pages * p.page_heads);  // past the end: zeros
+              const int group = there ? pos % p.kv.page_size / 8 : 0;
+              const unsigned live = __ballot_sync(0xffffffffu, there);
+              unsigned bits[4];
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                const int r = s * kStreamRows + 32 * k + lane, pr = u.pr0 + r;
-                qoff[k] = r < u.rows ? (int64_t)(u.row0 + pr / G) * p.q_stride + (int64_t)(kvh * G + pr % G) * hd : -1;
+                const int r = 32 * k + lane;
+                bits[k] = __ballot_sync(0xffffffffu, first + r < held && (live >> (r / p.box) & 1u));
               }
-              if (uses[s] > 0) wait(tl.q_empty[s], (uses[s] - 1) & 1, abort, p.status);
-              ++uses[s];
-              copy_tile(base + L::kOffQ + s * L::kItem, p.q, qoff);
-              cp_async_arrive(zb::smem_addr(&tl.q_full[s]));
+              if (t + 1 < u.tiles) next = look(u.tile0 + t + 1);
+#pragma unroll
+              for (int kv = 0; kv < 2; ++kv, ++item) {
+                const int slot = item % L::kSlots;
+                if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort, p.status);
+                if (lane == 0) {
+                  if (kv == 0) *reinterpret_cast<uint4*>(tl.mask[tile_no % kMasks]) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+                  zb::mbar_arrive_expect_tx(zb::smem_addr(&tl.full[slot]), L::kItem);
+                }
+                __syncwarp();
+                if (lane < boxes)
+                  load_rows(base + slot * L::kItem + lane * (p.box / 8) * L::kGroup, kv ? &maps.v : &maps.k,
+                            kvh * p.head_atoms, group, page, zb::smem_addr(&tl.full[slot]));
+              }
             }
+          } else {
+            load_q();
+          }
+        } else {
+          int pages[4];
+          auto look = [&](int t) {  // pages of the lane's rows of tile t
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int pos = t * kTile + 32 * k + lane;
+              pages[k] = pos < held ? table[pos / p.kv.page_size] : -1;
+            }
+          };
+          look(u.tile0);
+          for (int t = 0; t < u.tiles; ++t, ++tile_no) {
+            int64_t off[4];
+            unsigned bits[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int pos = (u.tile0 + t) * kTile + 32 * k + lane;
+              const bool there = pages[k] >= 0 && pages[k] < p.kv.num_pages;
+              off[k] = there ? (int64_t)pages[k] * p.kv.page_stride + (int64_t)(pos % p.kv.page_size) * p.kv.slot_stride +
+                                   (int64_t)kvh * p.kv.head_stride
+                             : -1;
+              bits[k] = __ballot_sync(0xffffffffu, there);
+            }
+            if (t + 1 < u.tiles) look(u.tile0 + t + 1);
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv, ++item) {
+              const int slot = item % L::kSlots;
+              if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort, p.status);
+              copy_tile(base + slot * L::kItem, kv ? p.kv.v : p.kv.k, off, lw, kLoadWarps);
+              cp_async_arrive(zb::smem_addr(&tl.full[slot]));
+              if (warp == kLoadWarp && lane == 0) {
+                if (kv == 0) *reinterpret_cast<uint4*>(tl.mask[tile_no % kMasks]) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+                arrive(tl.full[slot]);
+              }
+            }
+            if (t == 0) load_q();
           }
         }
       }
@@ -561,8 +635,9 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const uint32_t kb = base + (uint32_t)(i % L::kSlots) * L::kItem, qb = base + L::kOffQ + s * L::kItem;
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks) {
-        const uint32_t o = (ks / 4) * kBlk + (ks % 4) * 32;
-        tc::mma(tmem + L::kColS + s * kTile, tc::desc_kmajor(qb + o), tc::desc_kmajor(kb + o), kIdS, ks > 0);
+        const uint32_t o = (ks / 4) * 1024 + (ks % 4) * 32;
+        tc::mma(tmem + L::kColS + s * kTile, tc::desc_mnmajor(qb + o, 16, L::kGroup), tc::desc_mnmajor(kb + o, 16, L::kGroup),
+                kIdS, ks > 0);
       }
       tc::commit(zb::smem_addr(&tl.s_full[s]));
       arrive(tl.s_full[s]);  // passes on the tile's key mask, which this thread got with the tile
@@ -572,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const uint32_t vb = base + (uint32_t)(i % L::kSlots) * L::kItem;
 #pragma unroll
       for (int ks = 0; ks < kTile / 16; ++ks)
-        mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, tc::desc_mnmajor(vb + ks * 2048, kBlk, 1024),
+        mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, tc::desc_mnmajor(vb + ks * 2 * L::kGroup, 1024, L::kGroup),
                kIdO, accumulate || ks > 0);
     };
     auto commit = [&](const uint64_t& bar) {
@@ -594,6 +669,16 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         bool found = false;
         if (t >= 0) {
           full(v_item);
+          const int held = min(u.keys, p.kv.max_pages * p.kv.page_size);
+          // rows of the last page past the request's keys came along with a tensor copy: no key, so no value either
+          if (p.box && (u.tile0 + t + 1) * kTile > held && held % p.box != 0) {
+            const int r0 = held - (u.tile0 + t) * kTile, r1 = (r0 + p.box - 1) / p.box * p.box;
+            for (int i = r0 * (HD / 8) + lane; i < r1 * (HD / 8); i += 32)
+              *reinterpret_cast<uint4*>(gbase + (v_item % L::kSlots) * L::kItem + piece<HD>(i / (HD / 8), i % (HD / 8))) =
+                  make_uint4(0, 0, 0, 0);
+            tc::fence_proxy_async();
+            __syncwarp();
+          }
           const int first = (u.tile0 + t) * kTile;
           if (first + kTile > u.all_hi || first < u.all_lo) {  // keys that some rows see and others do not
             bool bad = false;
@@ -759,7 +844,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                 const unsigned word = j < 32 ? seen[0] : j < 64 ? seen[1] : j < 96 ? seen[2] : seen[3];
                 const bool sees = (word >> (j % 32)) & 1u;
                 for (int c = 0; c < HD / 8; ++c) {
-                  const uint4 w = *reinterpret_cast<const uint4*>(v + (c / 8) * kBlk + tc::sw128(j, c % 8));
+                  const uint4 w = *reinterpret_cast<const uint4*>(v + piece<HD>(j, c));
                   if (!not_finite(w)) continue;  // the same for every lane
                   const uint32_t q[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -897,8 +982,43 @@ Launch plan(int B, int64_t N, int Hq, int Hkv, int hd, int64_t max_keys) {
   return l;
 }
 
+// Tensor maps over the caches for copies of whole page rows: [64 dims, 8 rows, atoms, row groups, pages], with the KV
+// heads folded into the atoms (a row's heads side by side) or the pages (a page's heads one after the other). p.box
+// stays 0 where the layout, the page size or the head dim does not allow them.
 template <int HD>
-int launch_chunk(const ChunkParams& p, const Launch& l, cudaStream_t stream) {
+int make_maps(ChunkParams& p, Maps& maps) {
+  const zb::PagedBatch& c = p.kv;
+  p.box = 0;
+  int box = 1;
+  while (box < kTile && c.page_size % (2 * box) == 0) box *= 2;
+  const bool beside = c.head_stride == c.hd || c.Hkv == 1;
+  const bool behind = c.page_stride == c.Hkv * c.head_stride && c.num_pages * c.Hkv < INT32_MAX;
+  if (box < 8 || c.hd != HD || !(beside || behind) || c.num_pages < 1 || c.num_pages >= INT32_MAX || c.slot_stride < HD ||
+      c.page_stride < HD || c.page_stride >= (int64_t)1 << 38 || c.slot_stride >= (int64_t)1 << 34)
+    return zb::kOk;
+  auto fn = zb::tcp::encode_fn();
+  if (fn == nullptr) return zb::fail(zb::kCudaError, "gqa_chunk: cuTensorMapEncodeTiled unavailable");
+  const int64_t page = beside ? c.page_stride : c.head_stride;
+  cuuint64_t dims[5] = {64, 8, (cuuint64_t)(HD / 64 * (beside ? c.Hkv : 1)), (cuuint64_t)(c.page_size / 8),
+                        (cuuint64_t)(c.num_pages * (beside ? 1 : c.Hkv))};
+  cuuint64_t strides[4] = {(cuuint64_t)c.slot_stride * 2, 128, (cuuint64_t)c.slot_stride * 16, (cuuint64_t)page * 2};
+  cuuint32_t boxes[5] = {64, 8, HD / 64, (cuuint32_t)(box / 8), 1}, step[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < 2; ++i) {
+    const CUresult r = fn(i ? &maps.v : &maps.k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, i ? c.v : c.k, dims, strides, boxes,
+                          step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return zb::fail(zb::kCudaError, "gqa_chunk: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  }
+  p.box = box;
+  p.head_atoms = beside ? HD / 64 : 0;
+  p.page_heads = beside ? 1 : c.Hkv;
+  return zb::kOk;
+}
+
+template <int HD>
+int launch_chunk(ChunkParams& p, const Launch& l, cudaStream_t stream) {
+  Maps maps = {};
+  if (int rc = make_maps<HD>(p, maps)) return rc;
   auto kernel = gqa_chunk_kernel<HD>;
   static bool configured[64] = {false};  // the shared-memory attribute, set once per device
   int dev = 0;
@@ -907,7 +1027,7 @@ int launch_chunk(const ChunkParams& p, const Launch& l, cudaStream_t stream) {
     ZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD>::kSmem));
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  ZB_CUDA(zb::launch(kernel, dim3((unsigned)l.ctas), dim3(kThreads), Shape<HD>::kSmem, stream, 1, p));
+  ZB_CUDA(zb::launch(kernel, dim3((unsigned)l.ctas), dim3(kThreads), Shape<HD>::kSmem, stream, 1, p, maps));
   if (int rc = zb::check_launch("gqa_chunk")) return rc;
   if (l.splits) {
     const dim3 grid((unsigned)l.ctas, (unsigned)((l.rows_max * (HD / 4) + 255) / 256));
