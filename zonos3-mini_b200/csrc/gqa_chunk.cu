@@ -39,7 +39,7 @@ namespace tc = zb::tc;
 
 constexpr int kTile = 128;       // keys of a tile
 constexpr int kStreamRows = 128;  // rows of a stream
-constexpr int kUnitRows = 2 * kStreamRows;
+constexpr int kUnitCost = 2;  // what a unit costs besides its tiles, in tiles
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
 constexpr int kMaxSlots = 10, kDescs = 4;
@@ -52,6 +52,7 @@ struct ChunkParams {
   const __nv_bfloat16* q;  // [N, Hq, hd], row stride q_stride
   int64_t q_stride;
   int Hq, G;
+  int tokens;  // of a stream: kStreamRows / G
   float scale_log2;  // softmax scale * log2(e)
   int causal, window;
   const __nv_bfloat16* gate;  // [N, Hq] or null
@@ -70,23 +71,23 @@ struct ChunkParams {
   int head_atoms, page_heads;  // a KV head's atom offset, and a page's index step, in the tensor maps
 };
 struct Maps {
-  CUtensorMap k, v;
+  CUtensorMap q, k, v;
 };
 
 // A unit that starts in this CTA and ends in another one (parts = 0: there is none).
 struct Header {
-  int parts;  // CTAs that hold a part of it, this one the first
-  int row0;   // first token row of its request
-  int pr0;    // its first (token, head) row within the request
+  int parts;   // CTAs that hold a part of it, this one the first
+  int token0;  // its first token row
   int rows;
   int kvh;
-  int pad[3];
 };
 
 // What a CTA does with one unit.
 struct Desc {
-  int row0, tokens, keys;  // the request: first token row, new tokens, keys (not negative)
-  int pr0, rows;           // (token, head) rows [pr0, pr0 + rows) of the request
+  int token0;     // the unit's first token row
+  int pos0;       // and its key position
+  int keys;       // of the request (not negative)
+  int rows;       // (token, head) rows
   int kvh;
   int tile0, tiles;  // tiles of keys; 0: no row sees a key
   int mode;          // kFinal, kPart0, kPart1, kStop
@@ -99,13 +100,14 @@ struct Tail {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t q_full[2], q_empty[2];
   uint64_t s_full[2], p_full[2], o_full[2];
-  uint64_t scanned, drained;
+  uint64_t scanned, drained, halves;
   uint64_t desc_full[kDescs], desc_empty[kDescs];
-  unsigned mask[kMasks][4];  // keys of a tile that exist
+  alignas(16) unsigned mask[kMasks][4];  // keys of a tile that exist
   Desc desc[kDescs];
   int64_t sums[16];
-  int start[4];  // this CTA's first unit: request, pair, steps of the unit, KV head and tile
-  int64_t start_off;
+  int start[2];       // this CTA's first unit: request and pair of streams
+  int64_t start_off;  // how far into the pair's work, all KV heads, the CTA begins
+  float ml[2][kStreamRows][2];  // maximum and sum of the rows' two halves, when the streams share rows
   uint32_t tmem;
   int abort;
   int found;  // the scanned V tile holds values that are not finite
@@ -117,10 +119,11 @@ struct Shape {
   // that one tensor copy of whole rows of a page, of any multiple of 8, lands in place.
   static constexpr uint32_t kGroup = HD / 64 * 1024;
   static constexpr uint32_t kItem = kTile / 8 * kGroup;
+  static constexpr uint32_t kQAtom = kStreamRows * 128;  // the queries lie dims apart: 64 dims of all rows, then the next
   static constexpr int kSlots = HD == 128 ? 5 : 10;
   static constexpr uint32_t kOffQ = kSlots * kItem;
   static constexpr uint32_t kOffTail = kOffQ + 2 * kItem;
-  static constexpr size_t kSmem = kOffTail + sizeof(Tail) + 1024;
+  static constexpr size_t kSmem = kOffTail + sizeof(Tail);
   static_assert(kSlots * kItem >= kMaxRequests * 4, "the requests' prefix fits the ring");
   static_assert(kSmem <= 232448, "shared memory");
   static constexpr uint32_t kColS = 0, kColO = 2 * kTile;  // stream s: S at s * 128, O at 256 + s * HD
@@ -138,6 +141,15 @@ __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, 
       "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], "
       "[%7];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(0), "r"(0), "r"(atom), "r"(group), "r"(page), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void load_queries(uint32_t dst, const CUtensorMap* map, int dim, int head, int token,
+                                             uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(dim), "r"(head), "r"(token), "r"(bar)
       : "memory");
 }
 
@@ -244,26 +256,31 @@ __device__ __forceinline__ Request request(const ChunkParams& p, int b) {
   return r;
 }
 
-// Keys [lo, hi) that token i of a request sees.
-__device__ __forceinline__ void visible(const ChunkParams& p, const Request& r, int i, int& lo, int& hi) {
-  const int pos = r.keys - r.tokens + i, held = min(r.keys, p.kv.max_pages * p.kv.page_size);
-  hi = p.causal ? min(held, pos + 1) : held;
-  hi = max(hi, 0);
-  lo = p.window > 0 ? max(0, (int)((int64_t)pos + 1 - p.window)) : 0;
+// Keys [lo, hi) that the token at position pos of a request with `keys` keys sees.
+__device__ __forceinline__ int held_keys(const ChunkParams& p, int keys) {
+  return min(keys, p.kv.max_pages * p.kv.page_size);
+}
+__device__ __forceinline__ void visible(const ChunkParams& p, int keys, int pos, int& lo, int& hi) {
+  const int held = held_keys(p, keys);
+  hi = max(p.causal ? min(held, pos + 1) : held, 0);
+  lo = p.window > 0 ? (int)max((int64_t)0, (int64_t)pos + 1 - p.window) : 0;
 }
 
-// The unit of rows [pair * 256, ..) of a request: its rows and key tiles.
+// Streams of a request's rows come in pairs; a pair's unit of work for one KV head: its rows and key tiles.
+__device__ __forceinline__ int stream_pairs(const ChunkParams& p, int tokens) {
+  return (tokens + 2 * p.tokens - 1) / (2 * p.tokens);
+}
 __device__ __forceinline__ void unit_tiles(const ChunkParams& p, const Request& r, int pair, Desc& d) {
-  d.row0 = r.row0;
-  d.tokens = r.tokens;
+  const int first = pair * 2 * p.tokens, tokens = min(r.tokens - first, 2 * p.tokens);
+  d.token0 = r.row0 + first;
+  d.pos0 = r.keys - r.tokens + first;
   d.keys = r.keys;
-  d.pr0 = pair * kUnitRows;
-  d.rows = min(r.tokens * p.G - d.pr0, kUnitRows);
+  d.rows = tokens * p.G;
   int lo0, hi0, lo1, hi1;
-  visible(p, r, d.pr0 / p.G, lo0, hi0);
-  visible(p, r, (d.pr0 + d.rows - 1) / p.G, lo1, hi1);
+  visible(p, r.keys, d.pos0, lo0, hi0);
+  visible(p, r.keys, d.pos0 + tokens - 1, lo1, hi1);
   d.all_lo = lo1;
-  d.all_hi = hi0 == min(r.keys, p.kv.max_pages * p.kv.page_size) ? INT32_MAX : hi0;
+  d.all_hi = hi0 == held_keys(p, r.keys) ? INT32_MAX : hi0;
   d.tile0 = lo0 / kTile;
   d.tiles = hi1 > lo0 ? (hi1 + kTile - 1) / kTile - d.tile0 : 0;
 }
@@ -315,10 +332,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                                                                 const __grid_constant__ Maps maps) {
   using L = Shape<HD>;
   zb::pdl_enter();
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  const uint32_t raw = zb::smem_addr(smem_raw);
-  const uint32_t base = (raw + 1023u) & ~1023u;
-  unsigned char* gbase = smem_raw + (base - raw);
+  extern __shared__ __align__(1024) unsigned char gbase[];
+  const uint32_t base = zb::smem_addr(gbase);
+  if (base % 1024 != 0) {  // the swizzled tiles ask for it; there is no static shared memory before them
+    if (p.status) atomicOr(p.status, zb::kStatusAttnChunkTimeout);
+    return;
+  }
   Tail& tl = *reinterpret_cast<Tail*>(gbase + L::kOffTail);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int B = p.kv.B, Hkv = p.kv.Hkv, hd = p.kv.hd, G = p.G;
@@ -330,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       zb::mbar_init(zb::smem_addr(&tl.empty[s]), 1);
     }
     for (int s = 0; s < 2; ++s) {
-      zb::mbar_init(zb::smem_addr(&tl.q_full[s]), (kLoadWarps - 1) * 32);
+      zb::mbar_init(zb::smem_addr(&tl.q_full[s]), 1);
       zb::mbar_init(zb::smem_addr(&tl.q_empty[s]), 1);
       zb::mbar_init(zb::smem_addr(&tl.s_full[s]), 2);
       zb::mbar_init(zb::smem_addr(&tl.p_full[s]), kStreamRows);
@@ -338,6 +357,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     }
     zb::mbar_init(zb::smem_addr(&tl.scanned), 1);
     zb::mbar_init(zb::smem_addr(&tl.drained), 1);
+    zb::mbar_init(zb::smem_addr(&tl.halves), 32 * kSoftWarps);
     for (int s = 0; s < kDescs; ++s) {
       zb::mbar_init(zb::smem_addr(&tl.desc_full[s]), 1);
       zb::mbar_init(zb::smem_addr(&tl.desc_empty[s]), kSoftWarps + 1);
@@ -362,12 +382,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     }
   }
 
-  // ---- the plan: steps (tiles, at least one a unit) of all units, and this CTA's first one
+  // ---- the plan: the work of all units, and this CTA's first one
   int* pairs_before = reinterpret_cast<int*>(gbase);  // [B], over the ring
   int64_t all_pairs = 0;
   for (int b0 = 0; b0 < B; b0 += kThreads) {
     const int b = b0 + tid;
-    const int n = b < B ? (request(p, b).tokens * G + kUnitRows - 1) / kUnitRows : 0;
+    const int n = b < B ? stream_pairs(p, request(p, b).tokens) : 0;
     int64_t total;
     const int64_t before = block_scan(n, tl, total);
     if (b < B) pairs_before[b] = (int)(all_pairs + before);
@@ -377,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   // more than the tokens can make: cu decreases somewhere, nothing is done
   const int pairs = all_pairs <= p.pairs_max ? (int)all_pairs : 0;
   if (all_pairs > p.pairs_max && cta == 0 && tid == 0 && p.status) atomicOr(p.status, zb::kStatusAttnChunkBatch);
-  auto pair_steps = [&](int j, int& b, int& pair) {  // steps of pair j for one KV head
+  auto pair_work = [&](int j, int& b, int& pair) {  // work of pair j for one KV head
     int lo = 0, hi = B;  // the last b with pairs_before[b] <= j
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
@@ -388,13 +408,13 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     pair = j - pairs_before[lo];
     Desc d;
     unit_tiles(p, request(p, b), pair, d);
-    return max(d.tiles, 1);
+    return d.tiles + kUnitCost;
   };
   int64_t work = 0;
   for (int j0 = 0; j0 < pairs; j0 += kThreads) {
     int b, pair;
     int64_t total;
-    block_scan(j0 + tid < pairs ? pair_steps(j0 + tid, b, pair) : 0, tl, total);
+    block_scan(j0 + tid < pairs ? pair_work(j0 + tid, b, pair) : 0, tl, total);
     work += total;
   }
   work *= Hkv;
@@ -405,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     for (int j0 = 0; j0 < pairs; j0 += kThreads) {
       int b = 0, pair = 0;
       int64_t total;
-      const int n = j0 + tid < pairs ? pair_steps(j0 + tid, b, pair) : 0;
+      const int n = j0 + tid < pairs ? pair_work(j0 + tid, b, pair) : 0;
       const int64_t at = (seen + block_scan(n, tl, total)) * Hkv;
       if (n > 0 && begin >= at && begin < at + (int64_t)n * Hkv) {
         tl.start[0] = b;
@@ -479,50 +499,51 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     take(b);
     Desc d;
     unit_tiles(p, req, pair, d);
-    int64_t done = begin;
-    int kvh = (int)(tl.start_off / max(d.tiles, 1)), skip = (int)(tl.start_off % max(d.tiles, 1));
-    int item = 0, tile_no = 0, uses[2] = {0, 0};
-    for (int n = 0;; ++n) {
-      // ---- the unit's descriptor
-      const int steps = max(d.tiles, 1);
-      const int64_t left = end - done;
-      const int take_steps = (int)min((int64_t)(steps - skip), left);
+    int64_t at = begin;
+    const int unit0 = d.tiles + kUnitCost;
+    int kvh = (int)(tl.start_off / unit0), off = (int)(tl.start_off % unit0);
+    int item = 0, tile_no = 0, q_item = 0, n = 0;
+    for (;;) {
+      // ---- the unit's tiles here: its work is kUnitCost, then a step a tile
+      const int unit = d.tiles + kUnitCost, to = (int)min((int64_t)unit, off + (end - at));
+      const int from_tile = max(off - kUnitCost, 0), to_tile = max(to - kUnitCost, 0);
+      const bool here = d.tiles > 0 ? to_tile > from_tile : off == 0;
       Desc u = d;
       u.kvh = kvh;
-      if (d.tiles > 0) {
-        u.tile0 = d.tile0 + skip;
-        u.tiles = take_steps;
+      if (here || at >= end) {
+        u.tile0 = d.tile0 + from_tile;
+        u.tiles = to_tile - from_tile;
+        const bool starts = from_tile == 0, ends = to_tile == d.tiles;
+        u.mode = at >= end ? kStop : starts && ends ? kFinal : starts ? kPart1 : kPart0;
+        u.parts = (int)((at - off + unit - 1) / share) - cta + 1;
+        if (warp == kLoadWarp && lane == 0) {
+          const int slot = n % kDescs;
+          if (n >= kDescs) wait(tl.desc_empty[slot], (n / kDescs - 1) & 1, abort, p.status);
+          tl.desc[slot] = u;
+          arrive(tl.desc_full[slot]);
+        }
+        __syncwarp();
+        ++n;
+        if (u.mode == kStop) break;
+      } else {
+        u.tiles = 0;
       }
-      const bool starts = skip == 0, ends = skip + take_steps == steps;
-      u.mode = left <= 0 ? kStop : starts && ends ? kFinal : starts ? kPart1 : kPart0;
-      u.parts = (int)((done - skip + steps - 1) / share) - cta + 1;
-      if (warp == kLoadWarp && lane == 0) {
-        const int slot = n % kDescs;
-        if (n >= kDescs) wait(tl.desc_empty[slot], (n / kDescs - 1) & 1, abort, p.status);
-        tl.desc[slot] = u;
-        arrive(tl.desc_full[slot]);
-      }
-      __syncwarp();
-      if (u.mode == kStop) break;
       if (u.tiles > 0) {
         const int held = min(req.keys, p.kv.max_pages * p.kv.page_size);
         const int32_t* table = p.kv.table + (int64_t)b * p.kv.table_stride;
-        // the unit's queries: the warps that bring no keys, or behind the first tile so that the ring keeps filling
-        auto load_q = [&]() {
-          if (warp == kLoadWarp) return;
-          for (int s = 0; s < (u.rows > kStreamRows ? 2 : 1); ++s) {
-            int64_t off[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int r = s * kStreamRows + 32 * k + lane, pr = u.pr0 + r;
-              off[k] = r < u.rows ? (int64_t)(u.row0 + pr / G) * p.q_stride + (int64_t)(kvh * G + pr % G) * hd : -1;
+        if (warp == kLoadWarp + 1) {  // the unit's queries: a stream's tokens, the group's heads of each
+          for (int s = 0; s < (u.rows > p.tokens * G ? 2 : 1); ++s, ++q_item) {
+            const int slot = q_item % 2;
+            if (q_item >= 2) wait(tl.q_empty[slot], (q_item / 2 - 1) & 1, abort, p.status);
+            if (lane == 0) {
+              zb::mbar_arrive_expect_tx(zb::smem_addr(&tl.q_full[slot]), (uint32_t)(p.tokens * G * HD * 2));
+              for (int a = 0; a < HD / 64; ++a)
+                load_queries(base + L::kOffQ + slot * L::kItem + a * L::kQAtom, &maps.q, a * 64, kvh * G,
+                             u.token0 + s * p.tokens, zb::smem_addr(&tl.q_full[slot]));
             }
-            if (uses[s] > 0) wait(tl.q_empty[s], (uses[s] - 1) & 1, abort, p.status);
-            ++uses[s];
-            copy_tile(base + L::kOffQ + s * L::kItem, p.q, off, lw - 1, kLoadWarps - 1);
-            cp_async_arrive(zb::smem_addr(&tl.q_full[s]));
+            __syncwarp();
           }
-        };
+        }
         if (p.box) {
           if (warp == kLoadWarp) {
             const int boxes = kTile / p.box;  // of a tile; lane i brings box i
@@ -559,8 +580,6 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                             kvh * p.head_atoms, group, page, zb::smem_addr(&tl.full[slot]));
               }
             }
-          } else {
-            load_q();
           }
         } else {
           int pages[4];
@@ -596,20 +615,16 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                 arrive(tl.full[slot]);
               }
             }
-            if (t == 0) load_q();
           }
         }
       }
       // ---- the next unit: KV head, then pair, then request
-      done += take_steps;
-      skip = 0;
-      if (done >= end) {
-        d.tiles = 0;
-        continue;  // the stop descriptor
-      }
+      at += to - off;
+      off = 0;
+      if (at >= end) continue;  // the stop descriptor
       if (++kvh == Hkv) {
         kvh = 0;
-        if ((pair + 1) * kUnitRows < req.tokens * G) {
+        if (pair + 1 < stream_pairs(p, req.tokens)) {
           ++pair;
         } else {
           pair = 0;
@@ -628,17 +643,20 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     constexpr uint32_t kIdS = tc::idesc_bf16(kStreamRows, kTile);
     constexpr uint32_t kIdO = tc::idesc_bf16(kStreamRows, HD, false, /*b_mn=*/true);
-    int item = 0, tiles_done[2] = {0, 0}, q_uses[2] = {0, 0};
+    int item = 0, q_item = 0, tiles_done[2] = {0, 0};
     auto full = [&](int i) { wait(tl.full[i % L::kSlots], (i / L::kSlots) & 1, abort, p.status); };
-    auto issue_s = [&](int s, int i) {  // S_s = Q_s K^T of ring item i
+    auto commit = [&](const uint64_t& bar) {
+      if (lane == 0) tc::commit(zb::smem_addr(&bar));
+    };
+    auto issue_s = [&](int s, int i, int q) {  // S_s = Q K^T of ring item i and queries q
+      full(i);
+      tc::fence_proxy_async();  // 16-byte copies -> the tensor cores
       if (lane != 0) return;
-      const uint32_t kb = base + (uint32_t)(i % L::kSlots) * L::kItem, qb = base + L::kOffQ + s * L::kItem;
+      const uint32_t kb = base + (uint32_t)(i % L::kSlots) * L::kItem, qb = base + L::kOffQ + (q % 2) * L::kItem;
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) {
-        const uint32_t o = (ks / 4) * 1024 + (ks % 4) * 32;
-        tc::mma(tmem + L::kColS + s * kTile, tc::desc_mnmajor(qb + o, 16, L::kGroup), tc::desc_mnmajor(kb + o, 16, L::kGroup),
-                kIdS, ks > 0);
-      }
+      for (int ks = 0; ks < HD / 16; ++ks)
+        tc::mma(tmem + L::kColS + s * kTile, tc::desc_kmajor(qb + (ks / 4) * L::kQAtom + (ks % 4) * 32),
+                tc::desc_mnmajor(kb + (ks / 4) * 1024 + (ks % 4) * 32, 16, L::kGroup), kIdS, ks > 0);
       tc::commit(zb::smem_addr(&tl.s_full[s]));
       arrive(tl.s_full[s]);  // passes on the tile's key mask, which this thread got with the tile
     };
@@ -647,11 +665,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const uint32_t vb = base + (uint32_t)(i % L::kSlots) * L::kItem;
 #pragma unroll
       for (int ks = 0; ks < kTile / 16; ++ks)
-        mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, tc::desc_mnmajor(vb + ks * 2 * L::kGroup, 1024, L::kGroup),
-               kIdO, accumulate || ks > 0);
-    };
-    auto commit = [&](const uint64_t& bar) {
-      if (lane == 0) tc::commit(zb::smem_addr(&bar));
+        mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks,
+               tc::desc_mnmajor(vb + ks * 2 * L::kGroup, 1024, L::kGroup), kIdO, accumulate || ks > 0);
     };
     for (int n = 0;; ++n) {
       const int slot = n % kDescs;
@@ -661,70 +676,74 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       if (lane == 0) arrive(tl.desc_empty[slot]);
       if (u.mode == kStop || gave_up(abort)) break;
       if (u.tiles == 0) continue;
-      const int streams = u.rows > kStreamRows ? 2 : 1;
-      for (int t = -1; t < u.tiles; ++t) {
-        // O_s += P_s(t) V(t) as soon as P_s(t) is there, then S_s(t + 1)
-        const int v_item = item + 1, k_next = t < 0 ? item : item + 2;
-        const bool more = t + 1 < u.tiles;
-        bool found = false;
-        if (t >= 0) {
-          full(v_item);
-          const int held = min(u.keys, p.kv.max_pages * p.kv.page_size);
-          // rows of the last page past the request's keys came along with a tensor copy: no key, so no value either
-          if (p.box && (u.tile0 + t + 1) * kTile > held && held % p.box != 0) {
-            const int r0 = held - (u.tile0 + t) * kTile, r1 = (r0 + p.box - 1) / p.box * p.box;
-            for (int i = r0 * (HD / 8) + lane; i < r1 * (HD / 8); i += 32)
-              *reinterpret_cast<uint4*>(gbase + (v_item % L::kSlots) * L::kItem + piece<HD>(i / (HD / 8), i % (HD / 8))) =
-                  make_uint4(0, 0, 0, 0);
-            tc::fence_proxy_async();
-            __syncwarp();
-          }
-          const int first = (u.tile0 + t) * kTile;
-          if (first + kTile > u.all_hi || first < u.all_lo) {  // keys that some rows see and others do not
-            bool bad = false;
-            const uint4* v = reinterpret_cast<const uint4*>(gbase + (v_item % L::kSlots) * L::kItem);
-#pragma unroll 8
-            for (uint32_t i = lane; i < L::kItem / 16; i += 32) bad |= not_finite(v[i]);
-            found = __any_sync(0xffffffffu, bad);
-            if (lane == 0) {
-              tl.found = found;
-              arrive(tl.scanned);
-            }
-            if (found) {  // every stream adds what it sees before it hands over P; then the values are zeroed
-              for (int s = 0; s < streams; ++s) wait(tl.p_full[s], tiles_done[s] & 1, abort, p.status);
-              uint16_t* e = reinterpret_cast<uint16_t*>(gbase + (v_item % L::kSlots) * L::kItem);
-              for (uint32_t i = lane; i < L::kItem / 2; i += 32)
-                if ((e[i] & 0x7f80u) == 0x7f80u) e[i] = 0;
-              tc::fence_proxy_async();
-              __syncwarp();
-            }
-          }
-          tc::fence_proxy_async();  // the loaders' copies -> the tensor cores
-        }
-        for (int s = 0; s < streams; ++s) {
-          if (t >= 0) {
-            wait(tl.p_full[s], tiles_done[s] & 1, abort, p.status);
-            ++tiles_done[s];
-            tc::fence_after();
-            issue_o(s, v_item, t > 0 || found);
-            if (!more) commit(tl.o_full[s]);
-            if (s == streams - 1) commit(tl.empty[v_item % L::kSlots]);
-          } else {
-            wait(tl.q_full[s], q_uses[s] & 1, abort, p.status);
-            ++q_uses[s];
-          }
-          if (more) {
-            if (s == 0 || t < 0) {
-              full(k_next);
-              tc::fence_proxy_async();
-            }
-            issue_s(s, k_next);
-            if (t + 2 >= u.tiles) commit(tl.q_empty[s]);
-            if (s == streams - 1) commit(tl.empty[k_next % L::kSlots]);
-          }
-        }
-        if (t >= 0) item += 2;
+      const bool two = u.rows > p.tokens * G;  // two streams of rows share each tile, or one's two halves take turns
+      const int stride = two ? 1 : 2;          // tiles from one of a stream to its next
+      auto wait_q = [&](int q) { wait(tl.q_full[q % 2], (q / 2) & 1, abort, p.status); };
+      wait_q(q_item);
+      issue_s(0, item, q_item);
+      if (two) {
+        wait_q(q_item + 1);
+        issue_s(1, item, q_item + 1);
       }
+      commit(tl.empty[item % L::kSlots]);
+      if (!two && u.tiles > 1) {
+        issue_s(1, item + 2, q_item);
+        commit(tl.empty[(item + 2) % L::kSlots]);
+      }
+      if (u.tiles <= stride) {
+        commit(tl.q_empty[q_item % 2]);
+        if (two) commit(tl.q_empty[(q_item + 1) % 2]);
+      }
+      for (int t = 0; t < u.tiles; ++t) {
+        // O_s += P_s(t) V(t) as soon as P_s(t) is there, then the stream's next scores
+        const int v_item = item + 2 * t + 1, k_next = item + 2 * (t + stride);
+        const int s0 = two ? 0 : t & 1, s1 = two ? 1 : s0, first = (u.tile0 + t) * kTile;
+        unsigned char* v_tile = gbase + (v_item % L::kSlots) * L::kItem;
+        bool found = false;
+        full(v_item);
+        const int held = held_keys(p, u.keys);
+        // rows of the last page past the request's keys came along with a tensor copy: no key, so no value either
+        if (p.box && first + kTile > held && held % p.box != 0) {
+          const int r0 = held - first, r1 = (r0 + p.box - 1) / p.box * p.box;
+          for (int i = r0 * (HD / 8) + lane; i < r1 * (HD / 8); i += 32)
+            *reinterpret_cast<uint4*>(v_tile + piece<HD>(i / (HD / 8), i % (HD / 8))) = make_uint4(0, 0, 0, 0);
+        }
+        if (first + kTile > u.all_hi || first < u.all_lo) {  // keys that some rows see and others do not
+          __syncwarp();
+          bool bad = false;
+#pragma unroll 8
+          for (uint32_t i = lane; i < L::kItem / 16; i += 32) bad |= not_finite(reinterpret_cast<const uint4*>(v_tile)[i]);
+          found = __any_sync(0xffffffffu, bad);
+          if (lane == 0) {
+            tl.found = found;
+            arrive(tl.scanned);
+          }
+          if (found) {  // every stream adds what it sees before it hands over P; then the values are zeroed
+            for (int s = s0; s <= s1; ++s) wait(tl.p_full[s], tiles_done[s] & 1, abort, p.status);
+            uint16_t* e = reinterpret_cast<uint16_t*>(v_tile);
+            for (uint32_t i = lane; i < L::kItem / 2; i += 32)
+              if ((e[i] & 0x7f80u) == 0x7f80u) e[i] = 0;
+          }
+        }
+        tc::fence_proxy_async();
+        __syncwarp();
+        for (int s = s0; s <= s1; ++s) {
+          wait(tl.p_full[s], tiles_done[s] & 1, abort, p.status);
+          ++tiles_done[s];
+          tc::fence_after();
+          issue_o(s, v_item, t >= stride || found);
+          if (t + stride >= u.tiles) commit(tl.o_full[s]);
+          if (s == s1) commit(tl.empty[v_item % L::kSlots]);
+          if (t + stride < u.tiles) {
+            const int q = q_item + (two ? s : 0);
+            issue_s(s, k_next, q);
+            if (s == s1) commit(tl.empty[k_next % L::kSlots]);
+            if (t + stride == u.tiles - 1) commit(tl.q_empty[q % 2]);
+          }
+        }
+      }
+      item += 2 * u.tiles;
+      q_item += two ? 2 : 1;
     }
     commit(tl.drained);  // nothing is in flight when the tensor memory is given back, also after a wait that gave up
     if (lane == 0) zb::mbar_wait_bounded(zb::smem_addr(&tl.drained), 0, p.status, zb::kStatusAttnChunkTimeout);
@@ -736,7 +755,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     const int s = warp / 4;  // stream
     const uint32_t tlane = tmem + ((uint32_t)(32 * (warp % 4)) << 16);
     const uint32_t col_s = tlane + L::kColS + s * kTile, col_o = tlane + L::kColO + s * HD;
-    int tile_no = 0, k_item = 0, mine = 0, units = 0, scans = 0;  // counters of what this CTA / this stream has done
+    int tile_no = 0, mine = 0, units = 0, scans = 0, meetings = 0;  // counters of what this CTA, or this stream, has done
+    auto meet = [&]() {  // the 8 row warps
+      arrive(tl.halves);
+      wait(tl.halves, meetings & 1, abort, p.status);
+      ++meetings;
+    };
     for (int n = 0;; ++n) {
       const int slot = n % kDescs;
       wait(tl.desc_full[slot], (n / kDescs) & 1, abort, p.status);
@@ -744,19 +768,26 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       __syncwarp();
       if (lane == 0) arrive(tl.desc_empty[slot]);
       if (u.mode == kStop || gave_up(abort)) break;
-      const int r = s * kStreamRows + 32 * (warp % 4) + lane;
-      const bool live = r < u.rows;
-      const int pr = u.pr0 + r, i = live ? pr / G : 0, h = u.kvh * G + (live ? pr % G : 0);
-      const int64_t token = u.row0 + i;
-      const Request req{u.row0, u.tokens, u.keys};
+      const int stream_rows = p.tokens * G;
+      const bool two = u.rows > stream_rows;
+      const int own = 32 * (warp % 4) + lane, r = (two ? s * stream_rows : 0) + own;
+      const bool live = own < stream_rows && r < u.rows;
+      const int i = live ? r / G : 0, h = u.kvh * G + (live ? r % G : 0);
+      const int64_t token = u.token0 + i;
+      const int stride = two ? 1 : 2;
       float m = -INFINITY, l = 0.f;
-      if (u.tiles > 0 && s * kStreamRows < u.rows) {
-        int lo = 0, hi = INT32_MAX;  // a row past the unit's last sees everything; it is not stored
-        if (live) visible(p, req, i, lo, hi);
-        for (int t = 0; t < u.tiles; ++t, ++mine) {
+      {
+        int lo = 0, hi = INT32_MAX;  // a lane without a row sees everything; it is not stored
+        if (live) visible(p, u.keys, u.pos0 + i, lo, hi);
+        for (int t = 0; t < u.tiles; ++t) {
           const int first = (u.tile0 + t) * kTile;
           const bool scan = first + kTile > u.all_hi || first < u.all_lo;
+          if (!two && (t & 1) != s) {  // the other half's tile
+            scans += scan;
+            continue;
+          }
           wait(tl.s_full[s], mine & 1, abort, p.status);
+          ++mine;
           tc::fence_after();
           uint32_t x[kTile];
 #pragma unroll
@@ -794,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             const float corr = grow ? ex2(m - top) : 1.f;  // 0 for the row's first key
             if (grow) m = top;
             l *= corr;
-            if (t > 0) {
+            if (t >= stride) {
 #pragma unroll
               for (int c = 0; c < HD / 32; ++c) {
                 uint32_t o[32];
@@ -833,13 +864,13 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             wait(tl.scanned, scans & 1, abort, p.status);
             ++scans;
             if (*reinterpret_cast<volatile int*>(&tl.found)) {  // values that are not finite, one by one
-              if (t == 0) {  // the tile's product adds to the accumulator then
+              if (t < stride) {  // the tile's product adds to the accumulator then
                 uint32_t zero[32] = {};
 #pragma unroll
                 for (int c = 0; c < HD / 32; ++c) st32(col_o + 32 * c, zero);
               }
               tc::st_wait();
-              const unsigned char* v = gbase + (size_t)((k_item + 2 * t + 1) % L::kSlots) * L::kItem;
+              const unsigned char* v = gbase + (size_t)((2 * (tile_no + t) + 1) % L::kSlots) * L::kItem;
               for (int j = 0; j < kTile; ++j) {
                 const unsigned word = j < 32 ? seen[0] : j < 64 ? seen[1] : j < 96 ? seen[2] : seen[3];
                 const bool sees = (word >> (j % 32)) & 1u;
@@ -864,57 +895,81 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           tc::fence_before();
           arrive(tl.p_full[s]);
         }
-        wait(tl.o_full[s], units & 1, abort, p.status);
-        ++units;
+        if (u.tiles > (two ? 0 : s)) {
+          wait(tl.o_full[s], units & 1, abort, p.status);
+          ++units;
+        }
         tc::fence_after();
       }
-      // the scans of tiles this stream had no rows in
-      if (u.tiles > 0 && s * kStreamRows >= u.rows)
-        for (int t = 0; t < u.tiles; ++t)
-          if ((u.tile0 + t) * kTile + kTile > u.all_hi || (u.tile0 + t) * kTile < u.all_lo) ++scans;
       tile_no += u.tiles;
-      k_item += 2 * u.tiles;
-      if (s * kStreamRows >= u.rows || gave_up(abort)) continue;
-      if (u.mode == kFinal) {
+      // The accumulator of the row: its stream's, or both halves' of it, each half of the dims by one of the streams.
+      float own_c = 1.f, other_c = 0.f;
+      int c0 = 0, c1 = HD / 32;
+      if (!two && u.tiles > 1) {
+        tl.ml[s][own][0] = m;
+        tl.ml[s][own][1] = l;
+        tc::fence_before();
+        meet();
+        tc::fence_after();
+        const float m2 = tl.ml[1 - s][own][0], l2 = tl.ml[1 - s][own][1];
+        const float top = fmaxf(m, m2), mb = top == -INFINITY ? 0.f : top;
+        own_c = ex2(m - mb);
+        other_c = ex2(m2 - mb);
+        l = s == 0 ? l * own_c + l2 * other_c : l2 * other_c + l * own_c;
+        m = top;
+        c0 = s * (HD / 64);
+        c1 = c0 + HD / 64;
+      }
+      const uint32_t col_other = tlane + L::kColO + (1 - s) * HD;
+      if ((two || s == 0 || u.tiles > 1) && !gave_up(abort)) {
         const float f = live ? row_factor(p, token, h, l) : 0.f;
         __nv_bfloat16* dst = p.out + token * p.out_stride + (int64_t)h * hd;
-#pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
+        const int64_t part = (int64_t)cta * 2 + (u.mode == kPart1);
+        float* acc = p.acc + part * HD * p.rows_max;
+        for (int c = c0; c < c1; ++c) {
           uint32_t o[32] = {};
           if (u.tiles > 0) {
             ld32(col_o + 32 * c, o);
+            if (c1 - c0 < HD / 32) {
+              uint32_t o2[32];
+              ld32(col_other + 32 * c, o2);
+              tc::ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                const float a = __uint_as_float(o[j]) * own_c, z = __uint_as_float(o2[j]) * other_c;
+                o[j] = __float_as_uint(s == 0 ? a + z : z + a);
+              }
+            }
             tc::ld_wait();
           }
+          if (!live) continue;
+          if (u.mode == kFinal) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float y[8];
+            for (int j = 0; j < 4; ++j) {
+              float y[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = l == 0.f ? 0.f : __uint_as_float(o[8 * j + e]);
-            if (live && 32 * c + 8 * j < hd) store8(dst + 32 * c + 8 * j, y, f);
-          }
-        }
-        if (p.lse && live) p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-      } else {
-        const int64_t part = (int64_t)cta * 2 + (u.mode == kPart1);
-        float* acc = p.acc + part * HD * p.rows_max;
+              for (int e = 0; e < 8; ++e) y[e] = l == 0.f ? 0.f : __uint_as_float(o[8 * j + e]);
+              if (32 * c + 8 * j < hd) store8(dst + 32 * c + 8 * j, y, f);
+            }
+          } else {
 #pragma unroll
-        for (int c = 0; c < HD / 32; ++c) {
-          uint32_t o[32];
-          ld32(col_o + 32 * c, o);
-          tc::ld_wait();
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (live)
+            for (int j = 0; j < 8; ++j)
               *reinterpret_cast<uint4*>(acc + ((int64_t)(8 * c + j) * p.rows_max + r) * 4) =
                   make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          }
         }
-        if (live) {
-          p.ml[part * 2 * p.rows_max + r] = m;
-          p.ml[(part * 2 + 1) * p.rows_max + r] = l;
+        if (live && c0 == 0) {
+          if (u.mode != kFinal) {
+            p.ml[part * 2 * p.rows_max + r] = m;
+            p.ml[(part * 2 + 1) * p.rows_max + r] = l;
+          } else if (p.lse) {
+            p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+          }
         }
-        if (u.mode == kPart1 && tid == 0) p.headers[cta] = Header{u.parts, u.row0, u.pr0, u.rows, u.kvh, {0, 0, 0}};
+        if (u.mode == kPart1 && tid == 0) p.headers[cta] = Header{u.parts, u.token0, u.rows, u.kvh};
       }
       tc::fence_before();  // the accumulator's reads come before the next unit's products
+      if (!two && u.tiles > 1) meet();
     }
   }
   tc::fence_before();
@@ -949,8 +1004,8 @@ __global__ void __launch_bounds__(256) gqa_chunk_join_kernel(const __grid_consta
     y[2] += a.z * f;
     y[3] += a.w * f;
   }
-  const int pr = u.pr0 + r, h = u.kvh * p.G + pr % p.G;
-  const int64_t token = u.row0 + pr / p.G;
+  const int h = u.kvh * p.G + r % p.G;
+  const int64_t token = u.token0 + r / p.G;
   const float f = row_factor(p, token, h, l);
   if (d4 * 4 < p.kv.hd) {
     const uint2 packed = make_uint2(to_bf16x2(y[0] * f, y[1] * f), to_bf16x2(y[2] * f, y[3] * f));
@@ -967,12 +1022,13 @@ struct Launch {
 };
 Launch plan(int B, int64_t N, int Hq, int Hkv, int hd, int64_t max_keys) {
   Launch l{};
-  if (Hkv < 1 || B < 1 || N < 1) return l;
-  const int64_t rows = N * (Hq / Hkv), tiles = std::max<int64_t>((max_keys + kTile - 1) / kTile, 1);
-  l.pairs = rows / kUnitRows + std::min<int64_t>(B, N);
-  l.ctas = (int)std::min<int64_t>(zb::sm_count(), l.pairs * Hkv * tiles);
+  if (Hkv < 1 || B < 1 || N < 1 || Hq < Hkv || Hq / Hkv > kStreamRows) return l;
+  const int G = Hq / Hkv, pair_tokens = 2 * (kStreamRows / G);
+  const int64_t tiles = std::max<int64_t>((max_keys + kTile - 1) / kTile, 1);
+  l.pairs = N / pair_tokens + std::min<int64_t>(B, N);
+  l.ctas = (int)std::min<int64_t>(zb::sm_count(), l.pairs * Hkv * (tiles + kUnitCost));
   l.splits = tiles > 1 && l.ctas > 1;
-  l.rows_max = (int)std::min<int64_t>(rows, kUnitRows);
+  l.rows_max = (int)std::min<int64_t>(N, pair_tokens) * G;
   if (l.splits) {
     const int64_t width = hd <= 64 ? 64 : 128;
     l.header_bytes = ((int64_t)l.ctas * (int64_t)sizeof(Header) + 255) / 256 * 256;
@@ -982,12 +1038,29 @@ Launch plan(int B, int64_t N, int Hq, int Hkv, int hd, int64_t max_keys) {
   return l;
 }
 
-// Tensor maps over the caches for copies of whole page rows: [64 dims, 8 rows, atoms, row groups, pages], with the KV
+// Tensor maps: the queries, and over the caches for copies of whole page rows: [64 dims, 8 rows, atoms, row groups, pages], with the KV
 // heads folded into the atoms (a row's heads side by side) or the pages (a page's heads one after the other). p.box
 // stays 0 where the layout, the page size or the head dim does not allow them.
 template <int HD>
 int make_maps(ChunkParams& p, Maps& maps) {
   const zb::PagedBatch& c = p.kv;
+  auto fn = zb::tcp::encode_fn();
+  if (fn == nullptr) return zb::fail(zb::kCudaError, "gqa_chunk: cuTensorMapEncodeTiled unavailable");
+  auto encode = [&](CUtensorMap* map, int rank, const void* at, const cuuint64_t* dims, const cuuint64_t* strides,
+                    const cuuint32_t* boxes) {
+    const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(at), dims, strides, boxes, step,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? zb::kOk : zb::fail(zb::kCudaError, "gqa_chunk: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  };
+  {  // the queries: [dims, heads, tokens], a box of 64 dims of the group's heads of a stream's tokens
+    const cuuint64_t dims[3] = {(cuuint64_t)c.hd, (cuuint64_t)p.Hq, (cuuint64_t)c.N};
+    const cuuint64_t strides[2] = {(cuuint64_t)c.hd * 2, (cuuint64_t)p.q_stride * 2};
+    const cuuint32_t boxes[3] = {64, (cuuint32_t)p.G, (cuuint32_t)p.tokens};
+    ZB_REQUIRE(p.q_stride < (int64_t)1 << 38, "gqa_chunk: q_stride %lld", (long long)p.q_stride);
+    if (int rc = encode(&maps.q, 3, p.q, dims, strides, boxes)) return rc;
+  }
   p.box = 0;
   int box = 1;
   while (box < kTile && c.page_size % (2 * box) == 0) box *= 2;
@@ -996,19 +1069,13 @@ int make_maps(ChunkParams& p, Maps& maps) {
   if (box < 8 || c.hd != HD || !(beside || behind) || c.num_pages < 1 || c.num_pages >= INT32_MAX || c.slot_stride < HD ||
       c.page_stride < HD || c.page_stride >= (int64_t)1 << 38 || c.slot_stride >= (int64_t)1 << 34)
     return zb::kOk;
-  auto fn = zb::tcp::encode_fn();
-  if (fn == nullptr) return zb::fail(zb::kCudaError, "gqa_chunk: cuTensorMapEncodeTiled unavailable");
   const int64_t page = beside ? c.page_stride : c.head_stride;
-  cuuint64_t dims[5] = {64, 8, (cuuint64_t)(HD / 64 * (beside ? c.Hkv : 1)), (cuuint64_t)(c.page_size / 8),
-                        (cuuint64_t)(c.num_pages * (beside ? 1 : c.Hkv))};
-  cuuint64_t strides[4] = {(cuuint64_t)c.slot_stride * 2, 128, (cuuint64_t)c.slot_stride * 16, (cuuint64_t)page * 2};
-  cuuint32_t boxes[5] = {64, 8, HD / 64, (cuuint32_t)(box / 8), 1}, step[5] = {1, 1, 1, 1, 1};
-  for (int i = 0; i < 2; ++i) {
-    const CUresult r = fn(i ? &maps.v : &maps.k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, i ? c.v : c.k, dims, strides, boxes,
-                          step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return zb::fail(zb::kCudaError, "gqa_chunk: cuTensorMapEncodeTiled failed (%d)", (int)r);
-  }
+  const cuuint64_t dims[5] = {64, 8, (cuuint64_t)(HD / 64 * (beside ? c.Hkv : 1)), (cuuint64_t)(c.page_size / 8),
+                              (cuuint64_t)(c.num_pages * (beside ? 1 : c.Hkv))};
+  const cuuint64_t strides[4] = {(cuuint64_t)c.slot_stride * 2, 128, (cuuint64_t)c.slot_stride * 16, (cuuint64_t)page * 2};
+  const cuuint32_t boxes[5] = {64, 8, HD / 64, (cuuint32_t)(box / 8), 1};
+  if (int rc = encode(&maps.k, 5, c.k, dims, strides, boxes)) return rc;
+  if (int rc = encode(&maps.v, 5, c.v, dims, strides, boxes)) return rc;
   p.box = box;
   p.head_atoms = beside ? HD / 64 : 0;
   p.page_heads = beside ? 1 : c.Hkv;
@@ -1065,6 +1132,8 @@ ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_c
              "gqa_chunk: strides (q %lld, out %lld, gate %lld)", (long long)q_stride, (long long)out_stride,
              (long long)gate_stride);
   ZB_REQUIRE((int64_t)N * Hq < (int64_t)1 << 31, "gqa_chunk: %d tokens x %d heads", N, Hq);
+  if (Hq / Hkv > kStreamRows)
+    return zb::fail(zb::kUnsupported, "gqa_chunk: %d query heads a KV head (at most %d)", Hq / Hkv, kStreamRows);
   if (B > kMaxRequests) return zb::fail(zb::kUnsupported, "gqa_chunk: %d requests (at most %d)", B, kMaxRequests);
   if (N == 0) return zb::kOk;
   ZB_REQUIRE(B > 0, "gqa_chunk: %d tokens of no request", N);
@@ -1080,6 +1149,7 @@ ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_c
   p.q_stride = q_stride;
   p.Hq = Hq;
   p.G = Hq / Hkv;
+  p.tokens = kStreamRows / p.G;
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.causal = causal;
   p.window = window;
