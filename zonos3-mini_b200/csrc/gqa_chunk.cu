@@ -28,6 +28,7 @@
 // matrix product. So where a tile's keys are visible to some of its rows only, warp 8 looks through the V tile while the
 // scores are being worked on; values that are not finite are added to the rows that see them one by one, then zeroed.
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.cuh"
 #include "tc.cuh"
@@ -44,6 +45,7 @@ constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
 constexpr int kMaxSlots = 10, kDescs = 4;
 constexpr int kMasks = 8;  // the loaders run at most 5 tiles ahead of the rows
+constexpr int kPoly = 2;          // of every 8 pairs of exponentials, those on the multiply-add units
 constexpr float kRescale = 8.f;  // log2 growth of a row's maximum that the accumulator is rescaled for
 constexpr int kMaxRequests = 16384;
 
@@ -99,7 +101,7 @@ enum Mode { kFinal = 0, kPart0 = 1, kPart1 = 2, kStop = 3 };
 struct Tail {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t q_full[2], q_empty[2];
-  uint64_t s_full[2], p_full[2], o_full[2];
+  uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
   uint64_t scanned, drained, halves;
   uint64_t desc_full[kDescs], desc_empty[kDescs];
   alignas(16) unsigned mask[kMasks][4];  // keys of a tile that exist
@@ -189,6 +191,13 @@ __device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+// 16 columns of 16 lanes (of those from taddr's on): thread T gets, for block b of 8 columns, columns 2 (T % 4), + 1 of
+// lane T / 4 in r[4 b], r[4 b + 1] and of lane T / 4 + 8 in the next two.
+__device__ __forceinline__ void ld_across(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr));
+}
 __device__ __forceinline__ uint32_t ld1(uint32_t taddr) {
   uint32_t r;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
@@ -196,6 +205,13 @@ __device__ __forceinline__ uint32_t ld1(uint32_t taddr) {
 }
 __device__ __forceinline__ void st1(uint32_t taddr, uint32_t r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r) : "memory");
+}
+// One lane of a converged warp, always the same. Code under it stays uniform for the compiler, so that the operands of
+// the tensor-core instructions are kept in uniform registers.
+__device__ __forceinline__ bool elect() {
+  uint32_t yes;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
+  return yes != 0;
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -219,6 +235,29 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+// 2^a for two values on the multiply-add units: a = j + f with j the nearest integer, a minimax polynomial of degree 4 in f
+// (fitted by Remez exchange on [-1/2, 1/2], relative error 2.7e-6 in fp32) times 2^j. a <= 8 (kRescale); below -126 it
+// gives 2^-126. NaN stays NaN.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t a) {
+  float x, y;
+  unpack2(a, x, y);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(-126.f));
+  a = pack2(x, y);
+  const float magic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, in the low bits of the sum
+  const uint64_t t = add2(a, pack2(magic, magic));
+  const uint64_t f = fma2(add2(t, pack2(-magic, -magic)), pack2(-1.f, -1.f), a);
+  uint64_t r = fma2(f, pack2(0.009570102207362652f, 0.009570102207362652f), pack2(0.05591785907745361f, 0.05591785907745361f));
+  r = fma2(r, f, pack2(0.240247443318367f, 0.240247443318367f));
+  r = fma2(r, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+  r = fma2(r, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+  unpack2(t, x, y);
+  const uint64_t e = pack2(__uint_as_float((__float_as_uint(x) << 23) + 0x3f800000u),
+                           __uint_as_float((__float_as_uint(y) << 23) + 0x3f800000u));
+  uint64_t out;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(out) : "l"(r), "l"(e));
+  return out;
 }
 __device__ __forceinline__ uint32_t to_bf16x2(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -312,14 +351,6 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, Tail& tl, int64_t& tota
   return before + in - v;
 }
 
-// One row's output: acc[8] of dims d .. d + 7, scaled and rounded once.
-__device__ __forceinline__ void store8(__nv_bfloat16* dst, const float* x, float f) {
-  float y[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = x[i] * f;
-  *reinterpret_cast<uint4*>(dst) = zb::pack_bf16x8(y);
-}
-
 // What a row's accumulator is multiplied by: 1 / sum (0 for a row that saw no key, NaN stays NaN) times the gate.
 __device__ __forceinline__ float row_factor(const ChunkParams& p, int64_t t, int h, float l) {
   float f = l == 0.f ? 0.f : 1.f / l;
@@ -352,6 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       zb::mbar_init(zb::smem_addr(&tl.q_full[s]), 1);
       zb::mbar_init(zb::smem_addr(&tl.q_empty[s]), 1);
       zb::mbar_init(zb::smem_addr(&tl.s_full[s]), 2);
+      zb::mbar_init(zb::smem_addr(&tl.p_half[s]), kStreamRows);
       zb::mbar_init(zb::smem_addr(&tl.p_full[s]), kStreamRows);
       zb::mbar_init(zb::smem_addr(&tl.o_full[s]), 1);
     }
@@ -646,27 +678,36 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     int item = 0, q_item = 0, tiles_done[2] = {0, 0};
     auto full = [&](int i) { wait(tl.full[i % L::kSlots], (i / L::kSlots) & 1, abort, p.status); };
     auto commit = [&](const uint64_t& bar) {
-      if (lane == 0) tc::commit(zb::smem_addr(&bar));
+      if (elect()) tc::commit(zb::smem_addr(&bar));
+      __syncwarp();
     };
     auto issue_s = [&](int s, int i, int q) {  // S_s = Q K^T of ring item i and queries q
       full(i);
       tc::fence_proxy_async();  // 16-byte copies -> the tensor cores
-      if (lane != 0) return;
-      const uint32_t kb = base + (uint32_t)(i % L::kSlots) * L::kItem, qb = base + L::kOffQ + (q % 2) * L::kItem;
+      if (elect()) {
+        const uint32_t kb = base + (uint32_t)(i % L::kSlots) * L::kItem, qb = base + L::kOffQ + (q % 2) * L::kItem;
+        const uint64_t kd = tc::desc_mnmajor(kb, 16, L::kGroup), qd = tc::desc_kmajor(qb);
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks)
-        tc::mma(tmem + L::kColS + s * kTile, tc::desc_kmajor(qb + (ks / 4) * L::kQAtom + (ks % 4) * 32),
-                tc::desc_mnmajor(kb + (ks / 4) * 1024 + (ks % 4) * 32, 16, L::kGroup), kIdS, ks > 0);
-      tc::commit(zb::smem_addr(&tl.s_full[s]));
-      arrive(tl.s_full[s]);  // passes on the tile's key mask, which this thread got with the tile
+        for (int ks = 0; ks < HD / 16; ++ks)
+          tc::mma(tmem + L::kColS + s * kTile, qd + ((ks / 4) * L::kQAtom + (ks % 4) * 32) / 16,
+                  kd + ((ks / 4) * 1024 + (ks % 4) * 32) / 16, kIdS, ks > 0);
+        tc::commit(zb::smem_addr(&tl.s_full[s]));
+        arrive(tl.s_full[s]);  // passes on the tile's key mask, which this thread got with the tile
+      }
+      __syncwarp();
     };
-    auto issue_o = [&](int s, int i, bool accumulate) {  // O_s (+)= P_s V of ring item i
-      if (lane != 0) return;
-      const uint32_t vb = base + (uint32_t)(i % L::kSlots) * L::kItem;
+    auto issue_o = [&](int s, int i, int half, bool accumulate) {  // O_s (+)= P_s V of ring item i, half of its keys
+      if (elect()) {
+        const uint32_t vb = base + (uint32_t)(i % L::kSlots) * L::kItem;
+        const uint64_t vd = tc::desc_mnmajor(vb, 1024, L::kGroup);
 #pragma unroll
-      for (int ks = 0; ks < kTile / 16; ++ks)
-        mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks,
-               tc::desc_mnmajor(vb + ks * 2 * L::kGroup, 1024, L::kGroup), kIdO, accumulate || ks > 0);
+        for (int k0 = 0; k0 < kTile / 32; ++k0) {
+          const int ks = k0 + half * (kTile / 32);
+          mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, vd + ks * 2 * L::kGroup / 16, kIdO,
+                 accumulate || ks > 0);
+        }
+      }
+      __syncwarp();
     };
     for (int n = 0;; ++n) {
       const int slot = n % kDescs;
@@ -728,10 +769,13 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         tc::fence_proxy_async();
         __syncwarp();
         for (int s = s0; s <= s1; ++s) {
+          wait(tl.p_half[s], tiles_done[s] & 1, abort, p.status);
+          tc::fence_after();
+          issue_o(s, v_item, 0, t >= stride || found);
           wait(tl.p_full[s], tiles_done[s] & 1, abort, p.status);
           ++tiles_done[s];
           tc::fence_after();
-          issue_o(s, v_item, t >= stride || found);
+          issue_o(s, v_item, 1, true);
           if (t + stride >= u.tiles) commit(tl.o_full[s]);
           if (s == s1) commit(tl.empty[v_item % L::kSlots]);
           if (t + stride < u.tiles) {
@@ -746,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       q_item += two ? 2 : 1;
     }
     commit(tl.drained);  // nothing is in flight when the tensor memory is given back, also after a wait that gave up
-    if (lane == 0) zb::mbar_wait_bounded(zb::smem_addr(&tl.drained), 0, p.status, zb::kStatusAttnChunkTimeout);
+    zb::mbar_wait_bounded(zb::smem_addr(&tl.drained), 0, p.status, zb::kStatusAttnChunkTimeout);
     __syncwarp();
   } else {
     // =============================================================================================== rows
@@ -796,8 +840,9 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           const unsigned words[4] = {there.x, there.y, there.z, there.w};
           tc::ld_wait();
           unsigned seen[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-          const bool partly = first < lo || first + kTile > hi || (there.x & there.y & there.z & there.w) != 0xffffffffu;
-          if (__any_sync(0xffffffffu, partly)) {
+          const bool partly = __any_sync(0xffffffffu, first < lo || first + kTile > hi ||
+                                                          (there.x & there.y & there.z & there.w) != 0xffffffffu);
+          if (partly) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const int a = min(max(lo - first - 32 * c, 0), 32), z = min(max(hi - first - 32 * c, 0), 32);
@@ -840,20 +885,43 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           const float mb = m == -INFINITY ? 0.f : m;
           const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), minus = pack2(-mb, -mb);
           uint64_t sum2[2] = {0, 0};
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
+          // p of half a tile's keys, to tensor memory. kPoly of every 8 pairs take the polynomial: the exponential unit
+          // does 16 a cycle, as long for a tile's as the tensor cores take for its products, and the multiply-add units
+          // have room. A tile with hidden keys takes the unit alone: its 2^-inf is an exact 0.
+          auto weigh = [&](int c, auto poly) {
             uint32_t packed[32];
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               const int e = 64 * c + 2 * j;
+              uint64_t a2 = fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), scale2, minus);
               float a, z;
-              unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), scale2, minus), a, z);
-              a = ex2(a);
-              z = ex2(z);
-              sum2[j % 2] = add2(sum2[j % 2], pack2(a, z));
+              if (decltype(poly)::value && j % 8 >= 8 - kPoly) {
+                a2 = exp2_poly(a2);
+                unpack2(a2, a, z);
+              } else {
+                unpack2(a2, a, z);
+                a = ex2(a);
+                z = ex2(z);
+                a2 = pack2(a, z);
+              }
+              sum2[j % 2] = add2(sum2[j % 2], a2);
               packed[j] = to_bf16x2(a, z);
             }
             st32(col_s + 32 * c, packed);
+          };
+          auto hand_over = [&](const uint64_t& bar) {
+            tc::st_wait();
+            tc::fence_before();
+            arrive(bar);
+          };
+          if (partly || scan) {
+            weigh(0, std::false_type());
+            if (!scan) hand_over(tl.p_half[s]);
+            weigh(1, std::false_type());
+          } else {
+            weigh(0, std::true_type());
+            hand_over(tl.p_half[s]);
+            weigh(1, std::true_type());
           }
           {
             float a, z;
@@ -891,9 +959,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               }
             }
           }
-          tc::st_wait();
-          tc::fence_before();
-          arrive(tl.p_full[s]);
+          if (scan) hand_over(tl.p_half[s]);
+          hand_over(tl.p_full[s]);
         }
         if (u.tiles > (two ? 0 : s)) {
           wait(tl.o_full[s], units & 1, abort, p.status);
@@ -923,7 +990,6 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const uint32_t col_other = tlane + L::kColO + (1 - s) * HD;
       if ((two || s == 0 || u.tiles > 1) && !gave_up(abort)) {
         const float f = live ? row_factor(p, token, h, l) : 0.f;
-        __nv_bfloat16* dst = p.out + token * p.out_stride + (int64_t)h * hd;
         const int64_t part = (int64_t)cta * 2 + (u.mode == kPart1);
         float* acc = p.acc + part * HD * p.rows_max;
         for (int c = c0; c < c1; ++c) {
@@ -942,20 +1008,40 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             }
             tc::ld_wait();
           }
-          if (!live) continue;
           if (u.mode == kFinal) {
+            // packed over the columns that this chunk was read from, so that 4 lanes then hold 64 bytes of a row
+            uint32_t w[16];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              float y[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = l == 0.f ? 0.f : __uint_as_float(o[8 * j + e]);
-              if (32 * c + 8 * j < hd) store8(dst + 32 * c + 8 * j, y, f);
+            for (int j = 0; j < 16; ++j) {  // column j takes word 4 (j / 2 % 4) + 2 (j / 8) + j % 2 of the chunk
+              const int e = 2 * (4 * (j / 2 % 4) + 2 * (j / 8) + j % 2);
+              w[j] = l == 0.f ? 0u : to_bf16x2(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
             }
-          } else {
+            tc::st16(col_o + 32 * c0 + 16 * (c - c0), w);
+          } else if (live) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               *reinterpret_cast<uint4*>(acc + ((int64_t)(8 * c + j) * p.rows_max + r) * 4) =
                   make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+          }
+        }
+        if (u.mode == kFinal) {
+          tc::st_wait();
+          const int64_t row = live ? token * p.out_stride + (int64_t)h * hd : -1;
+          int64_t rows4[4];  // the rows this lane stores: lane / 4 and every 8th
+#pragma unroll
+          for (int k = 0; k < 4; ++k) rows4[k] = __shfl_sync(0xffffffffu, row, 8 * k + lane / 4);
+          for (int c = c0; c < c1; ++c) {
+            const int dim = 32 * c + 8 * (lane % 4);
+            uint32_t w[2][8];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) ld_across(col_o + 32 * c0 + 16 * (c - c0) + ((uint32_t)(16 * k) << 16), w[k]);
+            tc::ld_wait();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t* q = w[k / 2] + 2 * (k % 2);
+              if (rows4[k] >= 0 && dim < hd)
+                *reinterpret_cast<uint4*>(p.out + rows4[k] + dim) = make_uint4(q[0], q[1], q[4], q[5]);
+            }
           }
         }
         if (live && c0 == 0) {
