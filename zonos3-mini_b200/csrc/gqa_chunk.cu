@@ -28,7 +28,6 @@
 // matrix product. So where a tile's keys are visible to some of its rows only, warp 8 looks through the V tile while the
 // scores are being worked on; values that are not finite are added to the rows that see them one by one, then zeroed.
 #include <algorithm>
-#include <type_traits>
 
 #include "paged.cuh"
 #include "tc.cuh"
@@ -45,7 +44,6 @@ constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
 constexpr int kMaxSlots = 10, kDescs = 4;
 constexpr int kMasks = 8;  // the loaders run at most 5 tiles ahead of the rows
-constexpr int kPoly = 2;          // of every 8 pairs of exponentials, those on the multiply-add units
 constexpr float kRescale = 8.f;  // log2 growth of a row's maximum that the accumulator is rescaled for
 constexpr int kMaxRequests = 16384;
 
@@ -208,6 +206,24 @@ __device__ __forceinline__ void st1(uint32_t taddr, uint32_t r) {
 }
 // One lane of a converged warp, always the same. Code under it stays uniform for the compiler, so that the operands of
 // the tensor-core instructions are kept in uniform registers.
+// A value that is the same on every lane, told to the compiler: it and what follows from it stay in uniform registers,
+// which the tensor-core instructions take their operands from.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ Desc uniform(const Desc& d) {
+  Desc u;
+  u.token0 = uniform(d.token0);
+  u.pos0 = uniform(d.pos0);
+  u.keys = uniform(d.keys);
+  u.rows = uniform(d.rows);
+  u.kvh = uniform(d.kvh);
+  u.tile0 = uniform(d.tile0);
+  u.tiles = uniform(d.tiles);
+  u.mode = uniform(d.mode);
+  u.parts = uniform(d.parts);
+  u.all_lo = uniform(d.all_lo);
+  u.all_hi = uniform(d.all_hi);
+  return u;
+}
 __device__ __forceinline__ bool elect() {
   uint32_t yes;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
@@ -215,7 +231,7 @@ __device__ __forceinline__ bool elect() {
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ uint64_t pack2(float a, float b) {
@@ -228,36 +244,13 @@ __device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) {
 }
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  asm volatile("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  asm volatile("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-// 2^a for two values on the multiply-add units: a = j + f with j the nearest integer, a minimax polynomial of degree 4 in f
-// (fitted by Remez exchange on [-1/2, 1/2], relative error 2.7e-6 in fp32) times 2^j. a <= 8 (kRescale); below -126 it
-// gives 2^-126. NaN stays NaN.
-__device__ __forceinline__ uint64_t exp2_poly(uint64_t a) {
-  float x, y;
-  unpack2(a, x, y);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-126.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(y) : "f"(-126.f));
-  a = pack2(x, y);
-  const float magic = 12582912.f;  // 1.5 * 2^23: adding it rounds to an integer, in the low bits of the sum
-  const uint64_t t = add2(a, pack2(magic, magic));
-  const uint64_t f = fma2(add2(t, pack2(-magic, -magic)), pack2(-1.f, -1.f), a);
-  uint64_t r = fma2(f, pack2(0.009570102207362652f, 0.009570102207362652f), pack2(0.05591785907745361f, 0.05591785907745361f));
-  r = fma2(r, f, pack2(0.240247443318367f, 0.240247443318367f));
-  r = fma2(r, f, pack2(0.6931217908859253f, 0.6931217908859253f));
-  r = fma2(r, f, pack2(0.9999992847442627f, 0.9999992847442627f));
-  unpack2(t, x, y);
-  const uint64_t e = pack2(__uint_as_float((__float_as_uint(x) << 23) + 0x3f800000u),
-                           __uint_as_float((__float_as_uint(y) << 23) + 0x3f800000u));
-  uint64_t out;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(out) : "l"(r), "l"(e));
-  return out;
 }
 __device__ __forceinline__ uint32_t to_bf16x2(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
@@ -370,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     return;
   }
   Tail& tl = *reinterpret_cast<Tail*>(gbase + L::kOffTail);
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const int tid = threadIdx.x, warp = uniform(tid / 32), lane = tid % 32;
   const int B = p.kv.B, Hkv = p.kv.Hkv, hd = p.kv.hd, G = p.G;
   const int cta = blockIdx.x, ctas = gridDim.x;
 
@@ -383,8 +376,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       zb::mbar_init(zb::smem_addr(&tl.q_full[s]), 1);
       zb::mbar_init(zb::smem_addr(&tl.q_empty[s]), 1);
       zb::mbar_init(zb::smem_addr(&tl.s_full[s]), 2);
-      zb::mbar_init(zb::smem_addr(&tl.p_half[s]), kStreamRows);
-      zb::mbar_init(zb::smem_addr(&tl.p_full[s]), kStreamRows);
+      zb::mbar_init(zb::smem_addr(&tl.p_half[s]), kSoftWarps / 2);
+      zb::mbar_init(zb::smem_addr(&tl.p_full[s]), kSoftWarps / 2);
       zb::mbar_init(zb::smem_addr(&tl.o_full[s]), 1);
     }
     zb::mbar_init(zb::smem_addr(&tl.scanned), 1);
@@ -476,14 +469,14 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
-  const uint32_t tmem = tl.tmem;
+  const uint32_t tmem = uniform((int)tl.tmem);
   int* abort = &tl.abort;
 
   if (begin >= end) {
     // nothing for this CTA
   } else if (warp >= kLoadWarp) {
     // =============================================================================================== loaders
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     const int lw = warp - kLoadWarp;
     constexpr int kChunks = HD / 8;          // 16-byte pieces of a row
     constexpr int kPass = 32 / kChunks;      // rows of a warp's copy instruction
@@ -672,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kMmaWarp) {
     // =============================================================================================== tensor cores
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     constexpr uint32_t kIdS = tc::idesc_bf16(kStreamRows, kTile);
     constexpr uint32_t kIdO = tc::idesc_bf16(kStreamRows, HD, false, /*b_mn=*/true);
     int item = 0, q_item = 0, tiles_done[2] = {0, 0};
@@ -683,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     };
     auto issue_s = [&](int s, int i, int q) {  // S_s = Q K^T of ring item i and queries q
       full(i);
-      tc::fence_proxy_async();  // 16-byte copies -> the tensor cores
+      if (p.box == 0) tc::fence_proxy_async();  // 16-byte copies -> the tensor cores
       if (elect()) {
         const uint32_t kb = base + (uint32_t)(i % L::kSlots) * L::kItem, qb = base + L::kOffQ + (q % 2) * L::kItem;
         const uint64_t kd = tc::desc_mnmajor(kb, 16, L::kGroup), qd = tc::desc_kmajor(qb);
@@ -712,8 +705,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     for (int n = 0;; ++n) {
       const int slot = n % kDescs;
       wait(tl.desc_full[slot], (n / kDescs) & 1, abort, p.status);
-      const Desc u = tl.desc[slot];
-      __syncwarp();
+      const Desc u = uniform(tl.desc[slot]);
       if (lane == 0) arrive(tl.desc_empty[slot]);
       if (u.mode == kStop || gave_up(abort)) break;
       if (u.tiles == 0) continue;
@@ -748,9 +740,10 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           const int r0 = held - first, r1 = (r0 + p.box - 1) / p.box * p.box;
           for (int i = r0 * (HD / 8) + lane; i < r1 * (HD / 8); i += 32)
             *reinterpret_cast<uint4*>(v_tile + piece<HD>(i / (HD / 8), i % (HD / 8))) = make_uint4(0, 0, 0, 0);
+          tc::fence_proxy_async();
+          __syncwarp();
         }
         if (first + kTile > u.all_hi || first < u.all_lo) {  // keys that some rows see and others do not
-          __syncwarp();
           bool bad = false;
 #pragma unroll 8
           for (uint32_t i = lane; i < L::kItem / 16; i += 32) bad |= not_finite(reinterpret_cast<const uint4*>(v_tile)[i]);
@@ -764,10 +757,11 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             uint16_t* e = reinterpret_cast<uint16_t*>(v_tile);
             for (uint32_t i = lane; i < L::kItem / 2; i += 32)
               if ((e[i] & 0x7f80u) == 0x7f80u) e[i] = 0;
+            tc::fence_proxy_async();
+            __syncwarp();
           }
         }
-        tc::fence_proxy_async();
-        __syncwarp();
+        if (p.box == 0) tc::fence_proxy_async();
         for (int s = s0; s <= s1; ++s) {
           wait(tl.p_half[s], tiles_done[s] & 1, abort, p.status);
           tc::fence_after();
@@ -794,8 +788,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     __syncwarp();
   } else {
     // =============================================================================================== rows
-    // 8 x 32 x 208 + 4 x 32 x 88 registers are the 384 x 168 that the CTA was launched with
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // 8 x 32 x 192 + 4 x 32 x 120 registers are the 384 x 168 that the CTA was launched with
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int s = warp / 4;  // stream
     const uint32_t tlane = tmem + ((uint32_t)(32 * (warp % 4)) << 16);
     const uint32_t col_s = tlane + L::kColS + s * kTile, col_o = tlane + L::kColO + s * HD;
@@ -808,21 +802,19 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     for (int n = 0;; ++n) {
       const int slot = n % kDescs;
       wait(tl.desc_full[slot], (n / kDescs) & 1, abort, p.status);
-      const Desc u = tl.desc[slot];
-      __syncwarp();
+      const Desc u = uniform(tl.desc[slot]);
       if (lane == 0) arrive(tl.desc_empty[slot]);
       if (u.mode == kStop || gave_up(abort)) break;
       const int stream_rows = p.tokens * G;
       const bool two = u.rows > stream_rows;
-      const int own = 32 * (warp % 4) + lane, r = (two ? s * stream_rows : 0) + own;
-      const bool live = own < stream_rows && r < u.rows;
-      const int i = live ? r / G : 0, h = u.kvh * G + (live ? r % G : 0);
-      const int64_t token = u.token0 + i;
+      const int first_row = two ? s * stream_rows : 0, rows = min(stream_rows, u.rows - first_row);
+      const bool idle = 32 * (warp % 4) >= rows;  // no lane of the warp has a row
       const int stride = two ? 1 : 2;
       float m = -INFINITY, l = 0.f;
       {
         int lo = 0, hi = INT32_MAX;  // a lane without a row sees everything; it is not stored
-        if (live) visible(p, u.keys, u.pos0 + i, lo, hi);
+        if (32 * (warp % 4) + lane < rows)
+          visible(p, u.keys, u.pos0 + (first_row + 32 * (warp % 4) + lane) / G, lo, hi);
         for (int t = 0; t < u.tiles; ++t) {
           const int first = (u.tile0 + t) * kTile;
           const bool scan = first + kTile > u.all_hi || first < u.all_lo;
@@ -832,36 +824,44 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           }
           wait(tl.s_full[s], mine & 1, abort, p.status);
           ++mine;
+          if (idle) {  // whatever the tensor memory holds there, its rows are stored nowhere
+            scans += scan;
+            if (lane == 0) {
+              arrive(tl.p_half[s]);
+              arrive(tl.p_full[s]);
+            }
+            continue;
+          }
           tc::fence_after();
           uint32_t x[kTile];
 #pragma unroll
           for (int c = 0; c < 4; ++c) ld32(col_s + 32 * c, x + 32 * c);
           const uint4 there = *reinterpret_cast<const uint4*>(tl.mask[(tile_no + t) % kMasks]);
-          const unsigned words[4] = {there.x, there.y, there.z, there.w};
-          tc::ld_wait();
-          unsigned seen[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+          unsigned seen[4] = {there.x, there.y, there.z, there.w};
           const bool partly = __any_sync(0xffffffffu, first < lo || first + kTile > hi ||
                                                           (there.x & there.y & there.z & there.w) != 0xffffffffu);
+          tc::ld_wait();
           if (partly) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const int a = min(max(lo - first - 32 * c, 0), 32), z = min(max(hi - first - 32 * c, 0), 32);
               const unsigned below = z >= 32 ? 0xffffffffu : (1u << z) - 1u;
               const unsigned under = a >= 32 ? 0xffffffffu : (1u << a) - 1u;
-              seen[c] = words[c] & below & ~under;
+              seen[c] &= below & ~under;
 #pragma unroll
               for (int j = 0; j < 32; ++j)
                 if (!((seen[c] >> j) & 1u)) x[32 * c + j] = __float_as_uint(-INFINITY);
             }
           }
-          float top = -INFINITY;
+          float top;
           {
             float part[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              part[c] = __uint_as_float(x[c]);
+            for (int j = 0; j < 4; ++j) {
+              part[j] = fmaxf(__uint_as_float(x[j]), __uint_as_float(x[4 + j]));
 #pragma unroll
-              for (int j = 1; j < 32; ++j) part[c] = fmaxf(part[c], __uint_as_float(x[4 * j + c]));
+              for (int i = 8; i < kTile; i += 8)
+                part[j] = fmaxf(fmaxf(part[j], __uint_as_float(x[i + j])), __uint_as_float(x[i + 4 + j]));
             }
             top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * p.scale_log2;
           }
@@ -871,58 +871,63 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             if (grow) m = top;
             l *= corr;
             if (t >= stride) {
-#pragma unroll
-              for (int c = 0; c < HD / 32; ++c) {
-                uint32_t o[32];
-                ld32(col_o + 32 * c, o);
+#pragma unroll 1
+              for (int c = 0; c < HD / 16; ++c) {
+                uint32_t o[16];
+                tc::ld16(col_o + 16 * c, o);
                 tc::ld_wait();
 #pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-                st32(col_o + 32 * c, o);
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                tc::st16(col_o + 16 * c, o);
               }
             }
           }
           const float mb = m == -INFINITY ? 0.f : m;
           const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), minus = pack2(-mb, -mb);
           uint64_t sum2[2] = {0, 0};
-          // p of half a tile's keys, to tensor memory. kPoly of every 8 pairs take the polynomial: the exponential unit
-          // does 16 a cycle, as long for a tile's as the tensor cores take for its products, and the multiply-add units
-          // have room. A tile with hidden keys takes the unit alone: its 2^-inf is an exact 0.
-          auto weigh = [&](int c, auto poly) {
-            uint32_t packed[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const int e = 64 * c + 2 * j;
-              uint64_t a2 = fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), scale2, minus);
-              float a, z;
-              if (decltype(poly)::value && j % 8 >= 8 - kPoly) {
-                a2 = exp2_poly(a2);
-                unpack2(a2, a, z);
-              } else {
-                unpack2(a2, a, z);
-                a = ex2(a);
-                z = ex2(z);
-                a2 = pack2(a, z);
-              }
-              sum2[j % 2] = add2(sum2[j % 2], a2);
-              packed[j] = to_bf16x2(a, z);
-            }
-            st32(col_s + 32 * c, packed);
-          };
           auto hand_over = [&](const uint64_t& bar) {
             tc::st_wait();
             tc::fence_before();
-            arrive(bar);
+            __syncwarp();
+            if (lane == 0) arrive(bar);
           };
-          if (partly || scan) {
-            weigh(0, std::false_type());
-            if (!scan) hand_over(tl.p_half[s]);
-            weigh(1, std::false_type());
-          } else {
-            weigh(0, std::true_type());
-            hand_over(tl.p_half[s]);
-            weigh(1, std::true_type());
-          }
+          // p of a half of the keys. The exponential unit takes 8 cycles an instruction, so everything else has to run in
+          // its shadow: the scaling of the next group, and the sum and the packing of the one before, are written between
+          // a group's exponentials.
+          auto weigh = [&](int half) {
+            constexpr int kPairs = 4, kGroups = kTile / 4 / kPairs;
+            uint32_t packed[32];
+            uint64_t a2[kPairs];
+            float e[2][2 * kPairs];
+            auto scaled = [&](int g, int i) {
+              const int k = 64 * half + 2 * (g * kPairs + i);
+              return fma2(pack2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), scale2, minus);
+            };
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) a2[i] = scaled(0, i);
+#pragma unroll
+            for (int g = 0; g <= kGroups; ++g) {
+#pragma unroll
+              for (int i = 0; i < kPairs; ++i) {
+                if (g < kGroups) {
+                  float a, z;
+                  unpack2(a2[i], a, z);
+                  e[g % 2][2 * i] = ex2(a);
+                  e[g % 2][2 * i + 1] = ex2(z);
+                  if (g + 1 < kGroups) a2[i] = scaled(g + 1, i);
+                }
+                if (g > 0) {
+                  const float a = e[(g + 1) % 2][2 * i], z = e[(g + 1) % 2][2 * i + 1];
+                  sum2[i % 2] = add2(sum2[i % 2], pack2(a, z));
+                  packed[(g - 1) * kPairs + i] = to_bf16x2(a, z);
+                }
+              }
+            }
+            st32(col_s + 32 * half, packed);
+          };
+          weigh(0);
+          if (!scan) hand_over(tl.p_half[s]);
+          weigh(1);
           {
             float a, z;
             unpack2(add2(sum2[0], sum2[1]), a, z);
@@ -969,6 +974,11 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         tc::fence_after();
       }
       tile_no += u.tiles;
+      int own = 32 * (warp % 4) + lane;
+      asm volatile("" : "+r"(own));  // the row is worked out here anew: kept through the tiles it would cost registers
+      const bool live = own < rows;
+      const int r = first_row + own, h = u.kvh * G + (live ? r % G : 0);
+      const int64_t token = u.token0 + (live ? r / G : 0);
       // The accumulator of the row: its stream's, or both halves' of it, each half of the dims by one of the streams.
       float own_c = 1.f, other_c = 0.f;
       int c0 = 0, c1 = HD / 32;
