@@ -327,7 +327,7 @@ int zb_gqa_prologue_decode(const uint16_t* proj, int64_t proj_stride, const uint
  *   page_table   [B, table_stride] int32 with max_pages columns: position j lives in row j % page_size of page
  *                page_table[b, j / page_size]; a page outside [0, num_pages) or past the columns holds no keys
  *   k_cache, v_cache bf16: page p, row r, KV head g at p * page_stride + r * slot_stride + g * head_stride elements, hd
- *                contiguous elements each; strides multiples of 8, bases 16-byte aligned. page_size * max_pages < 2^31.
+ *                contiguous elements each; strides multiples of 8, bases 16-byte aligned. page_size * max_pages at most 2^29.
  *   hd a multiple of 8, 8 .. 128 (else status 3).
  *
  * zb_gqa_append: from projection rows proj [N, Hq*hd | Hkv*hd | Hkv*hd | ...] bf16 (q | k | v, any row stride): q and k rows
@@ -353,7 +353,9 @@ int zb_gqa_append(const uint16_t* proj, int64_t proj_stride, const uint16_t* tem
  * ([N, Hq] bf16, row stride gate_stride), rounded once; lse (NULL: not written) [N, Hq] fp32 = the natural logarithm of
  * the softmax denominator. A row that sees no key or belongs to no request: zeros, lse -inf. q / out [N, Hq, hd] bf16 with
  * row strides (multiples of 8), 16-byte aligned; softmax_scale > 0; Hq a multiple of Hkv. workspace: 16-byte aligned, at
- * least zb_gqa_chunk_workspace_bytes(B, N, Hq, Hkv, hd, page_size * max_pages) bytes, not shared by overlapping calls. */
+ * least zb_gqa_chunk_workspace_bytes(B, N, Hq, Hkv, hd, page_size * max_pages) bytes, not shared by overlapping calls; its
+ * first 4096 bytes (flags) must be zero before the first call and are left zero by each (a wait that gave up, status bit
+ * 64, may leave them non-zero: re-zero them then). Status bit 128: cu_seqlens_q decreases, nothing was written. */
 int64_t zb_gqa_chunk_workspace_bytes(int B, int N, int Hq, int Hkv, int hd, int64_t max_keys);
 int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache,
                  int64_t page_stride, int64_t slot_stride, int64_t head_stride, int64_t num_pages, int page_size,

@@ -18,8 +18,9 @@
 //
 // The lengths live on the device, so the split of the work does too: every CTA adds up the tiles of all units (a scan
 // over the requests) and takes an equal run of them. A unit that spans CTAs leaves partial results (accumulator,
-// maximum, sum) in the workspace, and a second kernel joins them in order; so one token over a long cache uses the whole
-// GPU, a ragged batch is balanced whatever its lengths, and the result does not depend on timing.
+// maximum, sum) in the workspace, and the CTA where it began joins them in order (the others hand theirs over as the
+// first thing they do); so one token over a long cache uses the whole GPU, a ragged batch is balanced whatever its
+// lengths, and the result does not depend on timing.
 //
 // Warps: 0-3 and 4-7 the rows of stream 0 and 1; 8 issues the tensor-core work; 9-11 look up pages and copy K, V and Q
 // rows (any page size, any strides) into shared memory, several tiles ahead and across units.
@@ -60,8 +61,9 @@ struct ChunkParams {
   __nv_bfloat16* out;  // [N, Hq, hd]
   int64_t out_stride;
   float* lse;  // [N, Hq] or null
-  // workspace: per CTA a header and two slots of partial results, rows_max rows each
-  struct Header* headers;
+  // workspace: per CTA a flag (0 between calls) and two slots of partial results, rows_max rows each: of the unit that
+  // began before this CTA, and of the one that goes on after it
+  unsigned* flags;
   float* acc;  // [CTA][2][HD / 4][rows_max][4]
   float* ml;   // [CTA][2][2][rows_max]: maximum, sum
   int rows_max;
@@ -72,14 +74,6 @@ struct ChunkParams {
 };
 struct Maps {
   CUtensorMap q, k, v;
-};
-
-// A unit that starts in this CTA and ends in another one (parts = 0: there is none).
-struct Header {
-  int parts;   // CTAs that hold a part of it, this one the first
-  int token0;  // its first token row
-  int rows;
-  int kvh;
 };
 
 // What a CTA does with one unit.
@@ -104,8 +98,9 @@ struct Tail {
   uint64_t desc_full[kDescs], desc_empty[kDescs];
   alignas(16) unsigned mask[kMasks][4];  // keys of a tile that exist
   Desc desc[kDescs];
-  int64_t sums[16];
-  int start[2];       // this CTA's first unit: request and pair of streams
+  int sums[2][kThreads / 32];
+  int idle[2];        // rows of no request: those before the first, those from the second on
+  int start[5];       // this CTA's first unit: request, its row, tokens and keys, and the pair of streams
   int64_t start_off;  // how far into the pair's work, all KV heads, the CTA begins
   float ml[2][kStreamRows][2];  // maximum and sum of the rows' two halves, when the streams share rows
   uint32_t tmem;
@@ -124,7 +119,7 @@ struct Shape {
   static constexpr uint32_t kOffQ = kSlots * kItem;
   static constexpr uint32_t kOffTail = kOffQ + 2 * kItem;
   static constexpr size_t kSmem = kOffTail + sizeof(Tail);
-  static_assert(kSlots * kItem >= kMaxRequests * 4, "the requests' prefix fits the ring");
+  static_assert(kSlots * kItem >= kMaxRequests * 4 + kThreads * 16, "the plan's tables fit the ring");
   static_assert(kSmem <= 232448, "shared memory");
   static constexpr uint32_t kColS = 0, kColO = 2 * kTile;  // stream s: S at s * 128, O at 256 + s * HD
 };
@@ -317,45 +312,108 @@ __device__ __forceinline__ void unit_tiles(const ChunkParams& p, const Request& 
   d.tiles = hi1 > lo0 ? (hi1 + kTile - 1) / kTile - d.tile0 : 0;
 }
 
-__device__ __forceinline__ int64_t warp_scan(int64_t v, int lane) {
+// Exclusive prefix of v over the block's threads; `total` the sum. `buffer` alternates from call to call.
+__device__ __forceinline__ int block_scan(int v, Tail& tl, int buffer, int& total) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int in = v;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += u;
+    const int u = __shfl_up_sync(0xffffffffu, in, o);
+    if (lane >= o) in += u;
   }
-  return v;
-}
-
-// Exclusive prefix of v over the block's threads; `total` the sum.
-__device__ __forceinline__ int64_t block_scan(int64_t v, Tail& tl, int64_t& total) {
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int64_t in = warp_scan(v, lane);
-  if (lane == 31) tl.sums[warp] = in;
+  if (lane == 31) tl.sums[buffer][warp] = in;
   __syncthreads();
-  int64_t before = 0;
+  int before = 0;
   total = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 32; ++w) {
-    const int64_t s = tl.sums[w];
+    const int s = tl.sums[buffer][w];
     if (w < warp) before += s;
     total += s;
   }
-  __syncthreads();
   return before + in - v;
 }
 
-// What a row's accumulator is multiplied by: 1 / sum (0 for a row that saw no key, NaN stays NaN) times the gate.
-__device__ __forceinline__ float row_factor(const ChunkParams& p, int64_t t, int h, float l) {
+__device__ __forceinline__ float sigmoid(__nv_bfloat16 x) { return 1.f / (1.f + expf(-__bfloat162float(x))); }
+
+__device__ __forceinline__ void raise_flag(unsigned* flag) {
+  asm volatile("st.release.gpu.global.u32 [%0], 1;" ::"l"(flag) : "memory");
+}
+// Whether the flag was raised within a second.
+__device__ __forceinline__ bool wait_flag(const unsigned* flag) {
+  const uint64_t start = zb::globaltimer_ns();
+  for (;;) {
+    unsigned v;
+    asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
+    if (v != 0) return true;
+    if (zb::globaltimer_ns() - start > 1000000000ull) return false;
+  }
+}
+
+// Joins the parts of a unit that began in this CTA, in the order of their keys. A thread of the row warps takes a row, or
+// with few rows one of its pieces of 4 * N dims: the parts' maxima and sums once, then the loads of a piece of several
+// parts together.
+template <int HD, int N>
+__device__ __forceinline__ void join_rows(const ChunkParams& p, const Desc& u, int cta, int tid) {
+  const int sharers = 32 * kSoftWarps / u.rows, r = tid % u.rows;  // of a row; at least one, as a unit has 256 rows at most
+  if (tid / u.rows >= sharers) return;
+  auto part = [&](int i) { return (int64_t)(cta + i) * 2 + (i == 0); };
+  auto maximum = [&](int i) { return __ldcg(p.ml + part(i) * 2 * p.rows_max + r); };
+  float top = -INFINITY, l = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < u.parts; ++i) top = fmaxf(top, maximum(i));
+  const float mb = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+  for (int i = 0; i < u.parts; ++i) l += __ldcg(p.ml + (part(i) * 2 + 1) * p.rows_max + r) * ex2(maximum(i) - mb);
+  const int h = u.kvh * p.G + r % p.G;
+  const int64_t token = u.token0 + r / p.G;
   float f = l == 0.f ? 0.f : 1.f / l;
-  if (p.gate) f *= 1.f / (1.f + expf(-__bfloat162float(p.gate[t * p.gate_stride + h])));
-  return f;
+  if (p.gate) f *= sigmoid(p.gate[token * p.gate_stride + h]);
+  for (int piece = tid / u.rows; piece < HD / 4 / N; piece += sharers) {
+    float y[4 * N] = {};
+#pragma unroll 2
+    for (int i = 0; i < u.parts; ++i) {
+      const float4* a = reinterpret_cast<const float4*>(p.acc + (part(i) * (HD / 4) + piece * N) * p.rows_max * 4 + r * 4);
+      float4 v[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] = __ldcg(a + (int64_t)k * p.rows_max);
+      const float w = ex2(maximum(i) - mb);  // 0 for a part none of whose keys the row sees; its accumulator is 0 too
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        y[4 * k] += v[k].x * w;
+        y[4 * k + 1] += v[k].y * w;
+        y[4 * k + 2] += v[k].z * w;
+        y[4 * k + 3] += v[k].w * w;
+      }
+    }
+    __nv_bfloat16* out = p.out + token * p.out_stride + (int64_t)h * p.kv.hd + piece * 4 * N;
+#pragma unroll
+    for (int k = 0; k < N; k += 2)
+      if (piece * 4 * N + 4 * k < p.kv.hd) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = to_bf16x2(y[4 * k + 2 * e] * f, y[4 * k + 2 * e + 1] * f);
+        *reinterpret_cast<uint4*>(out + 4 * k) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+  }
+  if (p.lse && tid < u.rows) p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+}
+template <int HD>
+__device__ __forceinline__ void join(const ChunkParams& p, const Desc& u, int cta, int tid) {
+  bool there = true;
+  for (int i = 1 + tid % 32; i < u.parts; i += 32) there = wait_flag(p.flags + cta + i) && there;
+  if (!__all_sync(0xffffffffu, there)) {
+    if (p.status && tid % 32 == 0) atomicOr(p.status, zb::kStatusAttnChunkTimeout);
+    return;
+  }
+  if (u.rows <= 32) join_rows<HD, 2>(p, u, cta, tid);
+  else join_rows<HD, 8>(p, u, cta, tid);
 }
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_constant__ ChunkParams p,
                                                                 const __grid_constant__ Maps maps) {
   using L = Shape<HD>;
-  zb::pdl_enter();
   extern __shared__ __align__(1024) unsigned char gbase[];
   const uint32_t base = zb::smem_addr(gbase);
   if (base % 1024 != 0) {  // the swizzled tiles ask for it; there is no static shared memory before them
@@ -365,7 +423,9 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   Tail& tl = *reinterpret_cast<Tail*>(gbase + L::kOffTail);
   const int tid = threadIdx.x, warp = uniform(tid / 32), lane = tid % 32;
   const int B = p.kv.B, Hkv = p.kv.Hkv, hd = p.kv.hd, G = p.G;
-  const int cta = blockIdx.x, ctas = gridDim.x;
+  // The work goes backwards over the blocks: a block that joins a unit's parts waits for blocks with lower indices, which
+  // were started before it, and they have nothing to wait for before they hand their parts over.
+  const int ctas = gridDim.x, cta = ctas - 1 - (int)blockIdx.x;
 
   if (tid == 0) {
     for (int s = 0; s < L::kSlots; ++s) {
@@ -390,71 +450,84 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     zb::fence_mbar_init();
     tl.abort = 0;
     tl.found = 0;
-    if (p.headers) p.headers[cta].parts = 0;
   }
   if (warp == kMmaWarp) tc::alloc(zb::smem_addr(&tl.tmem), 512);
-
-  // ---- rows of no request
-  {
-    const int first = min(max(p.kv.cu[0], 0), p.kv.N), last = min(max(p.kv.cu[B], first), p.kv.N);
-    const int idle = first + p.kv.N - last;
-    for (int i = cta * (kThreads / 32) + warp; i < idle; i += ctas * (kThreads / 32)) {
-      const int64_t t = i < first ? i : last + i - first;
-      for (int c = lane; c < p.Hq * hd / 8; c += 32)
-        *reinterpret_cast<uint4*>(p.out + t * p.out_stride + c * 8) = make_uint4(0, 0, 0, 0);
-      if (p.lse)
-        for (int h = lane; h < p.Hq; h += 32) p.lse[t * p.Hq + h] = -INFINITY;
-    }
-  }
+  if (warp == kLoadWarp && lane < 3)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &maps.q : lane == 1 ? &maps.k : &maps.v))
+                 : "memory");
+  zb::pdl_enter();  // nothing before it touches memory that another kernel may still write
 
   // ---- the plan: the work of all units, and this CTA's first one
-  int* pairs_before = reinterpret_cast<int*>(gbase);  // [B], over the ring
+  // Requests (and below, pairs of streams) go by the block's threads, kThreads at a time; the first ones' stay at hand.
+  const Request mine = tid < B ? request(p, tid) : Request{0, 0, 0};
+  if (tid == 0) {
+    tl.idle[0] = min(max(p.kv.cu[0], 0), p.kv.N);
+    tl.idle[1] = min(max(p.kv.cu[B], tl.idle[0]), p.kv.N);
+  }
+  int* pairs_before = reinterpret_cast<int*>(gbase);                             // [B], over the ring
+  Request* requests = reinterpret_cast<Request*>(gbase + kMaxRequests * 4);  // [kThreads], the first requests
+  if (tid < B) requests[tid] = mine;
   int64_t all_pairs = 0;
-  for (int b0 = 0; b0 < B; b0 += kThreads) {
+  int buffer = 0;
+  for (int b0 = 0; b0 < B; b0 += kThreads, buffer ^= 1) {
     const int b = b0 + tid;
-    const int n = b < B ? stream_pairs(p, request(p, b).tokens) : 0;
-    int64_t total;
-    const int64_t before = block_scan(n, tl, total);
+    const int n = b < B ? stream_pairs(p, b0 == 0 ? mine.tokens : request(p, b).tokens) : 0;
+    int total;
+    const int before = block_scan(n, tl, buffer, total);
     if (b < B) pairs_before[b] = (int)(all_pairs + before);
     all_pairs += total;
   }
   __syncthreads();
   // more than the tokens can make: cu decreases somewhere, nothing is done
   const int pairs = all_pairs <= p.pairs_max ? (int)all_pairs : 0;
-  if (all_pairs > p.pairs_max && cta == 0 && tid == 0 && p.status) atomicOr(p.status, zb::kStatusAttnChunkBatch);
-  auto pair_work = [&](int j, int& b, int& pair) {  // work of pair j for one KV head
+  if (all_pairs > p.pairs_max && blockIdx.x == 0 && tid == 0 && p.status) atomicOr(p.status, zb::kStatusAttnChunkBatch);
+  struct Pair {
+    int b, pair, work;  // work: for one KV head
+  };
+  auto at_hand = [&](int b) { return b < kThreads ? requests[b] : request(p, b); };
+  auto pair_of = [&](int j) {
+    if (j >= pairs) return Pair{0, 0, 0};
     int lo = 0, hi = B;  // the last b with pairs_before[b] <= j
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
       if (pairs_before[mid] <= j) lo = mid;
       else hi = mid;
     }
-    b = lo;
-    pair = j - pairs_before[lo];
     Desc d;
-    unit_tiles(p, request(p, b), pair, d);
-    return d.tiles + kUnitCost;
+    unit_tiles(p, at_hand(lo), j - pairs_before[lo], d);
+    return Pair{lo, j - pairs_before[lo], d.tiles + kUnitCost};
   };
-  int64_t work = 0;
-  for (int j0 = 0; j0 < pairs; j0 += kThreads) {
-    int b, pair;
-    int64_t total;
-    block_scan(j0 + tid < pairs ? pair_work(j0 + tid, b, pair) : 0, tl, total);
+  const Pair first_pair = pair_of(tid);
+  int first_total = 0;
+  const int first_before = block_scan(first_pair.work, tl, buffer, first_total);
+  int64_t work = first_total;
+  for (int j0 = kThreads; j0 < pairs; j0 += kThreads) {
+    int total;
+    buffer ^= 1;
+    block_scan(pair_of(j0 + tid).work, tl, buffer, total);
     work += total;
   }
   work *= Hkv;
-  const int64_t share = (work + ctas - 1) / ctas;
+  const int64_t share = work < INT32_MAX - ctas ? ((int)work + ctas - 1) / ctas : (work + ctas - 1) / ctas;
   const int64_t begin = share * cta, end = min(work, begin + share);
   if (begin < end) {
     int64_t seen = 0;
     for (int j0 = 0; j0 < pairs; j0 += kThreads) {
-      int b = 0, pair = 0;
-      int64_t total;
-      const int n = j0 + tid < pairs ? pair_work(j0 + tid, b, pair) : 0;
-      const int64_t at = (seen + block_scan(n, tl, total)) * Hkv;
-      if (n > 0 && begin >= at && begin < at + (int64_t)n * Hkv) {
-        tl.start[0] = b;
-        tl.start[1] = pair;
+      Pair q = first_pair;
+      int before = first_before, total = first_total;
+      if (j0 > 0) {
+        q = pair_of(j0 + tid);
+        buffer ^= 1;
+        before = block_scan(q.work, tl, buffer, total);
+      }
+      const int64_t at = (seen + before) * Hkv;
+      if (q.work > 0 && begin >= at && begin < at + (int64_t)q.work * Hkv) {
+        const Request r = at_hand(q.b);
+        tl.start[0] = q.b;
+        tl.start[1] = r.row0;
+        tl.start[2] = r.tokens;
+        tl.start[3] = r.keys;
+        tl.start[4] = q.pair;
         tl.start_off = begin - at;
       }
       seen += total;
@@ -505,23 +578,21 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     };
     // this lane's request of the window of 32 requests around the current one
     int window0 = -1;
-    Request mine{};
+    Request window{};
     auto fetch_window = [&](int b) {
       if (b / 32 != window0) {
         window0 = b / 32;
         const int i = window0 * 32 + lane;
-        mine = i < B ? request(p, i) : Request{0, 0, 0};
+        window = i < B ? request(p, i) : Request{0, 0, 0};
       }
     };
-    int b = tl.start[0], pair = tl.start[1];
-    fetch_window(b);
-    Request req;
+    int b = tl.start[0], pair = tl.start[4];
+    Request req{tl.start[1], tl.start[2], tl.start[3]};
     auto take = [&](int i) {
-      req.row0 = __shfl_sync(0xffffffffu, mine.row0, i % 32);
-      req.tokens = __shfl_sync(0xffffffffu, mine.tokens, i % 32);
-      req.keys = __shfl_sync(0xffffffffu, mine.keys, i % 32);
+      req.row0 = __shfl_sync(0xffffffffu, window.row0, i % 32);
+      req.tokens = __shfl_sync(0xffffffffu, window.tokens, i % 32);
+      req.keys = __shfl_sync(0xffffffffu, window.keys, i % 32);
     };
-    take(b);
     Desc d;
     unit_tiles(p, req, pair, d);
     int64_t at = begin;
@@ -540,7 +611,9 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         u.tiles = to_tile - from_tile;
         const bool starts = from_tile == 0, ends = to_tile == d.tiles;
         u.mode = at >= end ? kStop : starts && ends ? kFinal : starts ? kPart1 : kPart0;
-        u.parts = (int)((at - off + unit - 1) / share) - cta + 1;
+        // CTAs that hold a part of it from this one on
+        u.parts = ends ? 1 : at - off + unit < INT32_MAX ? (int)(at - off + unit - 1) / (int)share - cta + 1
+                                                         : (int)((at - off + unit - 1) / share) - cta + 1;
         if (warp == kLoadWarp && lane == 0) {
           const int slot = n % kDescs;
           if (n >= kDescs) wait(tl.desc_empty[slot], (n / kDescs - 1) & 1, abort, p.status);
@@ -810,11 +883,15 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const int first_row = two ? s * stream_rows : 0, rows = min(stream_rows, u.rows - first_row);
       const bool idle = 32 * (warp % 4) >= rows;  // no lane of the warp has a row
       const int stride = two ? 1 : 2;
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f, gate = 1.f;
       {
         int lo = 0, hi = INT32_MAX;  // a lane without a row sees everything; it is not stored
         if (32 * (warp % 4) + lane < rows)
           visible(p, u.keys, u.pos0 + (first_row + 32 * (warp % 4) + lane) / G, lo, hi);
+        if (p.gate && u.mode == kFinal && 32 * (warp % 4) + lane < rows) {
+          const int r = first_row + 32 * (warp % 4) + lane;
+          gate = sigmoid(p.gate[(int64_t)(u.token0 + r / G) * p.gate_stride + u.kvh * G + r % G]);
+        }
         for (int t = 0; t < u.tiles; ++t) {
           const int first = (u.tile0 + t) * kTile;
           const bool scan = first + kTile > u.all_hi || first < u.all_lo;
@@ -999,10 +1076,10 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       }
       const uint32_t col_other = tlane + L::kColO + (1 - s) * HD;
       if ((two || s == 0 || u.tiles > 1) && !gave_up(abort)) {
-        const float f = live ? row_factor(p, token, h, l) : 0.f;
+        const float f = l == 0.f ? 0.f : gate / l;  // 0 for a row that saw no key; a NaN sum stays NaN
         const int64_t part = (int64_t)cta * 2 + (u.mode == kPart1);
         float* acc = p.acc + part * HD * p.rows_max;
-        for (int c = c0; c < c1; ++c) {
+        auto chunk = [&](int c) {  // 32 dims of the row's accumulator
           uint32_t o[32] = {};
           if (u.tiles > 0) {
             ld32(col_o + 32 * c, o);
@@ -1033,18 +1110,21 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               *reinterpret_cast<uint4*>(acc + ((int64_t)(8 * c + j) * p.rows_max + r) * 4) =
                   make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           }
-        }
+        };
+        for (int c = c0; c < c1; ++c) chunk(c);
         if (u.mode == kFinal) {
           tc::st_wait();
           const int64_t row = live ? token * p.out_stride + (int64_t)h * hd : -1;
           int64_t rows4[4];  // the rows this lane stores: lane / 4 and every 8th
 #pragma unroll
           for (int k = 0; k < 4; ++k) rows4[k] = __shfl_sync(0xffffffffu, row, 8 * k + lane / 4);
-          for (int c = c0; c < c1; ++c) {
-            const int dim = 32 * c + 8 * (lane % 4);
+#pragma unroll
+          for (int i = 0; i < HD / 32; ++i) {
+            const int c = c0 + i, dim = 32 * c + 8 * (lane % 4);
+            if (c >= c1) break;
             uint32_t w[2][8];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) ld_across(col_o + 32 * c0 + 16 * (c - c0) + ((uint32_t)(16 * k) << 16), w[k]);
+            for (int k = 0; k < 2; ++k) ld_across(col_o + 32 * c0 + 16 * i + ((uint32_t)(16 * k) << 16), w[k]);
             tc::ld_wait();
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -1062,11 +1142,31 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
           }
         }
-        if (u.mode == kPart1 && tid == 0) p.headers[cta] = Header{u.parts, u.token0, u.rows, u.kvh};
       }
       tc::fence_before();  // the accumulator's reads come before the next unit's products
-      if (!two && u.tiles > 1) meet();
+      if (u.mode != kFinal) {
+        __threadfence();
+        meet();
+        if (u.mode == kPart0) {
+          if (tid == 0) raise_flag(p.flags + cta);
+        } else {
+          join<HD>(p, u, cta, tid);
+          meet();  // every thread is done with the parts
+          if (tid < u.parts - 1) p.flags[cta + 1 + tid] = 0;
+        }
+      } else if (!two && u.tiles > 1) {
+        meet();
+      }
     }
+  }
+  // ---- rows of no request
+  const int idle = tl.idle[0] + p.kv.N - tl.idle[1];
+  for (int i = cta * (kThreads / 32) + warp; i < idle; i += ctas * (kThreads / 32)) {
+    const int64_t t = i < tl.idle[0] ? i : tl.idle[1] + i - tl.idle[0];
+    for (int c = lane; c < p.Hq * hd / 8; c += 32)
+      *reinterpret_cast<uint4*>(p.out + t * p.out_stride + c * 8) = make_uint4(0, 0, 0, 0);
+    if (p.lse)
+      for (int h = lane; h < p.Hq; h += 32) p.lse[t * p.Hq + h] = -INFINITY;
   }
   tc::fence_before();
   __syncthreads();
@@ -1074,47 +1174,11 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   if (warp == kMmaWarp) tc::dealloc(tmem, 512);
 }
 
-// Joins the parts of the units that span CTAs, in the order of their keys: a thread takes 4 dims of a row.
-template <int HD>
-__global__ void __launch_bounds__(256) gqa_chunk_join_kernel(const __grid_constant__ ChunkParams p) {
-  zb::pdl_enter();
-  const Header u = p.headers[blockIdx.x];
-  const int at = blockIdx.y * 256 + threadIdx.x, d4 = at / p.rows_max, r = at % p.rows_max;
-  if (u.parts == 0 || r >= u.rows || d4 >= HD / 4) return;
-  float top = -INFINITY;
-  for (int i = 0; i < u.parts; ++i) {
-    const int64_t part = (int64_t)(blockIdx.x + i) * 2 + (i == 0);
-    top = fmaxf(top, p.ml[part * 2 * p.rows_max + r]);
-  }
-  const float mb = top == -INFINITY ? 0.f : top;
-  float l = 0.f, y[4] = {};
-  for (int i = 0; i < u.parts; ++i) {
-    const int64_t part = (int64_t)(blockIdx.x + i) * 2 + (i == 0);
-    const float sum = p.ml[(part * 2 + 1) * p.rows_max + r];
-    const float4 a = *reinterpret_cast<const float4*>(p.acc + (part * (HD / 4) + d4) * p.rows_max * 4 + r * 4);
-    const float f = ex2(p.ml[part * 2 * p.rows_max + r] - mb);
-    if (sum == 0.f) continue;  // no key of this part is visible to the row
-    l += sum * f;
-    y[0] += a.x * f;
-    y[1] += a.y * f;
-    y[2] += a.z * f;
-    y[3] += a.w * f;
-  }
-  const int h = u.kvh * p.G + r % p.G;
-  const int64_t token = u.token0 + r / p.G;
-  const float f = row_factor(p, token, h, l);
-  if (d4 * 4 < p.kv.hd) {
-    const uint2 packed = make_uint2(to_bf16x2(y[0] * f, y[1] * f), to_bf16x2(y[2] * f, y[3] * f));
-    *reinterpret_cast<uint2*>(p.out + token * p.out_stride + (int64_t)h * p.kv.hd + d4 * 4) = packed;
-  }
-  if (p.lse && d4 == 0) p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
-}
-
 // The launch: CTAs, and whether a unit can span several of them.
 struct Launch {
   int ctas, rows_max;
   bool splits;
-  int64_t pairs, header_bytes, acc_bytes, ml_bytes;
+  int64_t pairs, flag_bytes, acc_bytes, ml_bytes;
 };
 Launch plan(int B, int64_t N, int Hq, int Hkv, int hd, int64_t max_keys) {
   Launch l{};
@@ -1127,7 +1191,7 @@ Launch plan(int B, int64_t N, int Hq, int Hkv, int hd, int64_t max_keys) {
   l.rows_max = (int)std::min<int64_t>(N, pair_tokens) * G;
   if (l.splits) {
     const int64_t width = hd <= 64 ? 64 : 128;
-    l.header_bytes = ((int64_t)l.ctas * (int64_t)sizeof(Header) + 255) / 256 * 256;
+    l.flag_bytes = ((int64_t)l.ctas * 4 + 255) / 256 * 256;
     l.acc_bytes = (int64_t)l.ctas * 2 * l.rows_max * width * 4;
     l.ml_bytes = (int64_t)l.ctas * 4 * l.rows_max * 4;
   }
@@ -1191,20 +1255,14 @@ int launch_chunk(ChunkParams& p, const Launch& l, cudaStream_t stream) {
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   ZB_CUDA(zb::launch(kernel, dim3((unsigned)l.ctas), dim3(kThreads), Shape<HD>::kSmem, stream, 1, p, maps));
-  if (int rc = zb::check_launch("gqa_chunk")) return rc;
-  if (l.splits) {
-    const dim3 grid((unsigned)l.ctas, (unsigned)((l.rows_max * (HD / 4) + 255) / 256));
-    ZB_CUDA(zb::launch(gqa_chunk_join_kernel<HD>, grid, dim3(256), 0, stream, 1, p));
-    return zb::check_launch("gqa_chunk(join)");
-  }
-  return zb::kOk;
+  return zb::check_launch("gqa_chunk");
 }
 
 }  // namespace
 
 ZB_API int64_t zb_gqa_chunk_workspace_bytes(int B, int N, int Hq, int Hkv, int hd, int64_t max_keys) {
   const Launch l = plan(B, N, Hq, Hkv, hd, max_keys);
-  return l.header_bytes + l.acc_bytes + l.ml_bytes;
+  return l.flag_bytes + l.acc_bytes + l.ml_bytes;
 }
 
 ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache,
@@ -1237,7 +1295,7 @@ ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_c
   ZB_REQUIRE_ALIGNED(q, 16, "gqa_chunk q");
   ZB_REQUIRE_ALIGNED(out, 16, "gqa_chunk out");
   const Launch l = plan(B, N, Hq, Hkv, hd, (int64_t)page_size * max_pages);
-  const int64_t need = l.header_bytes + l.acc_bytes + l.ml_bytes;
+  const int64_t need = l.flag_bytes + l.acc_bytes + l.ml_bytes;
   ZB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "gqa_chunk: a workspace of %lld bytes, got %lld",
              (long long)need, (long long)workspace_bytes);
   ZB_REQUIRE_ALIGNED(workspace, 16, "gqa_chunk workspace");
@@ -1255,9 +1313,9 @@ ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_c
   p.out_stride = out_stride;
   p.lse = lse;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  p.headers = l.splits ? reinterpret_cast<Header*>(ws) : nullptr;
-  p.acc = reinterpret_cast<float*>(ws + l.header_bytes);
-  p.ml = reinterpret_cast<float*>(ws + l.header_bytes + l.acc_bytes);
+  p.flags = reinterpret_cast<unsigned*>(ws);
+  p.acc = reinterpret_cast<float*>(ws + l.flag_bytes);
+  p.ml = reinterpret_cast<float*>(ws + l.flag_bytes + l.acc_bytes);
   p.rows_max = l.rows_max;
   p.pairs_max = (int)l.pairs;
   p.status = zb::device_status_ptr();

@@ -1133,8 +1133,9 @@ def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, s
     stride allowed); head h's output is multiplied by sigmoid(gate[t, h]) before its one rounding. lse: optional
     contiguous [N, Hq] fp32 tensor that receives the natural logarithm of the softmax denominators. A token that sees
     no key, or belongs to no request, gets zeros and an lse of -inf. The lengths are read on the device: a captured
-    graph follows them. workspace: optional uint8 tensor of at least :func:`gqa_chunk_workspace_bytes` bytes
-    (allocated when absent). hd: a multiple of 8 up to 128. Returns out [N, Hq, hd] bf16."""
+    graph follows them. workspace: optional uint8 tensor of at least :func:`gqa_chunk_workspace_bytes` bytes, its first
+    4096 zero before the first call (every call leaves them zero) and not shared by calls that may overlap; absent, the
+    stream's own is used. hd: a multiple of 8 up to 128. Returns out [N, Hq, hd] bf16."""
     paged, Hkv, hd = _paged(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, None)
     dev = q.device
     N, Hq = q.shape[0], q.shape[1]
@@ -1152,8 +1153,9 @@ def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, s
         _check_cuda("lse", lse, torch.float32, dev)
         _require(lse.shape == (N, Hq) and lse.is_contiguous(), f"lse must be a contiguous [{N}, {Hq}] tensor")
     need = gqa_chunk_workspace_bytes(N, Hq, page_table, k_cache)
+    stream = _stream(dev)
     if workspace is None:
-        workspace = torch.empty(need, device=dev, dtype=torch.uint8) if need else None
+        workspace = _chunk_workspace(dev, stream, need) if need else None
     else:
         _check_cuda("workspace", workspace, torch.uint8, dev)
         _require(workspace.is_contiguous() and workspace.numel() >= need,
@@ -1162,8 +1164,26 @@ def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, s
               hd ** -0.5 if softmax_scale is None else softmax_scale, bool(causal), window, gate_ptr, gate_stride,
               out.data_ptr(), _token_rows("out", out, Hq, hd), None if lse is None else lse.data_ptr(),
               None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(),
-              _stream(dev))
+              stream)
     return out
+
+
+_CHUNK_WS: dict = {}  # (device, stream) -> the workspace of eager calls on that stream (its flags zero between calls)
+_CHUNK_FLAG_BYTES = 4096  # the flags lie at the workspace's start
+
+
+def _chunk_workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+    """A workspace with its flags zero. Eager calls on a stream share one, in stream order; under capture every call gets
+    its own (from the graph's pool, its flags zeroed by the graph), as a replay may run beside eager calls."""
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        ws[:_CHUNK_FLAG_BYTES].zero_()
+        return ws
+    ws = _CHUNK_WS.get((dev, stream))
+    if ws is None or ws.numel() < nbytes:  # a smaller one goes back to the allocator, which reuses it in stream order
+        ws = _CHUNK_WS[(dev, stream)] = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        ws[:_CHUNK_FLAG_BYTES].zero_()
+    return ws
 
 
 def gqa_chunk_workspace_bytes(tokens: int, heads: int, page_table, k_cache) -> int:
