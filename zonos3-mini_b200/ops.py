@@ -8,6 +8,7 @@ caller-provided tensors when given, so a wrapper allocates nothing inside a CUDA
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -1032,47 +1033,64 @@ def decode_advance(codes, ids, positions, cache_seqlens, out_loc, page_table, co
 # ------------------------------------------------------------- ragged batches of new tokens over a paged KV cache
 
 
+# These calls serve single tokens too, where the host's time is the call's: the checks build their messages only to raise
+# them, and read each attribute once.
+_BF16, _I32 = torch.bfloat16, torch.int32
+
+
+def _raw_stream(device_index: int) -> int:
+    """The current CUDA stream's handle, without the stream object."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
 def _paged(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, kv_heads):
     """The checks and the C arguments that the operators over a paged KV cache share (``q``: their query-side input)."""
-    dev = q.device
-    if not q.is_cuda:
+    index = q.get_device()
+    if index < 0:
         raise ValueError("the paged KV operators take CUDA tensors (the B200 kernels have no CPU path)")
-    for name, t, dtype in (("k_cache", k_cache, torch.bfloat16), ("v_cache", v_cache, torch.bfloat16),
-                           ("page_table", page_table, torch.int32), ("cache_seqlens", cache_seqlens, torch.int32),
-                           ("cu_seqlens_q", cu_seqlens_q, torch.int32)):
-        if t.dtype != dtype or t.device != dev:
-            raise ValueError(f"{name} must be a {dtype} tensor on {dev}, got {t.dtype} on {t.device}")
+    if (k_cache.dtype is not _BF16 or v_cache.dtype is not _BF16 or page_table.dtype is not _I32
+            or cache_seqlens.dtype is not _I32 or cu_seqlens_q.dtype is not _I32 or k_cache.get_device() != index
+            or v_cache.get_device() != index or page_table.get_device() != index or cache_seqlens.get_device() != index
+            or cu_seqlens_q.get_device() != index):
+        raise ValueError("k_cache and v_cache must be bfloat16, page_table, cache_seqlens and cu_seqlens_q int32 tensors "
+                         f"on {q.device}, got " + ", ".join(f"{t.dtype} on {t.device}" for t in (
+                             k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q)))
     shape, strides = k_cache.shape, k_cache.stride()
-    if len(shape) == 3:  # [slots, Hkv, hd]: one token a page
-        page_size, slot_stride, head_stride = 1, 0, strides[1]
-    elif len(shape) == 4:
-        page_size, slot_stride, head_stride = shape[1], strides[1], strides[2]
+    if len(shape) == 4:
+        pages, page_size, Hkv, hd = shape
+        page_stride, slot_stride, head_stride, last = strides
+    elif len(shape) == 3:  # [slots, Hkv, hd]: one token a page
+        pages, Hkv, hd = shape
+        page_size, slot_stride = 1, 0
+        page_stride, head_stride, last = strides
     else:
         raise ValueError(f"k_cache must be [pages, page_size, Hkv, hd] or [slots, Hkv, hd], got {tuple(shape)}")
-    if v_cache.shape != shape or v_cache.stride() != strides or strides[-1] != 1:
+    if v_cache.shape != shape or v_cache.stride() != strides or last != 1:
         raise ValueError("k_cache and v_cache must have the same shape and strides, their last dimension contiguous")
-    if kv_heads is not None and shape[-2] != kv_heads:
-        raise ValueError(f"the caches hold {shape[-2]} KV heads, expected {kv_heads}")
-    B = cache_seqlens.shape[0]
-    if (page_table.dim() != 2 or page_table.shape[0] != B or cache_seqlens.dim() != 1
-            or cu_seqlens_q.shape != (B + 1,)):
+    if kv_heads is not None and Hkv != kv_heads:
+        raise ValueError(f"the caches hold {Hkv} KV heads, expected {kv_heads}")
+    table_shape, table_strides = page_table.shape, page_table.stride()
+    B = cache_seqlens.shape[0] if cache_seqlens.dim() == 1 else -1
+    if len(table_shape) != 2 or table_shape[0] != B or cu_seqlens_q.shape != (B + 1,):
         raise ValueError(f"page_table, cache_seqlens and cu_seqlens_q must be [B, pages], [B] and [B + 1], got "
-                         f"{tuple(page_table.shape)}, {tuple(cache_seqlens.shape)}, {tuple(cu_seqlens_q.shape)}")
-    columns = page_table.shape[1]
-    if (columns > 1 and page_table.stride(1) != 1) or (B > 1 and cache_seqlens.stride(0) != 1) or cu_seqlens_q.stride(0) != 1:
+                         f"{tuple(table_shape)}, {tuple(cache_seqlens.shape)}, {tuple(cu_seqlens_q.shape)}")
+    columns = table_shape[1]
+    if (table_strides[1] != 1 and columns > 1) or not cache_seqlens.is_contiguous() or not cu_seqlens_q.is_contiguous():
         raise ValueError("page_table rows, cache_seqlens and cu_seqlens_q must be contiguous")
-    return (k_cache.data_ptr(), v_cache.data_ptr(), strides[0], slot_stride, head_stride, shape[0], page_size,
-            page_table.data_ptr(), page_table.stride(0) if B > 1 else columns, columns, cache_seqlens.data_ptr(),
-            cu_seqlens_q.data_ptr(), B), shape[-2], shape[-1]
+    return (k_cache.data_ptr(), v_cache.data_ptr(), page_stride, slot_stride, head_stride, pages, page_size,
+            page_table.data_ptr(), table_strides[0] if B > 1 else columns, columns, cache_seqlens.data_ptr(),
+            cu_seqlens_q.data_ptr(), B), index, Hkv, hd
 
 
-def _token_rows(name: str, t: torch.Tensor, heads: int, hd: int) -> int:
-    """Row stride of a [N, heads, hd] bf16 tensor whose rows are contiguous."""
-    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != hd:
-        raise ValueError(f"{name} must be a bfloat16 [N, {heads}, {hd}] tensor, got {t.dtype} {tuple(t.shape)}")
-    if (hd > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != hd):
+def _token_rows(name: str, t: torch.Tensor, index: int, N: int, heads: int, hd: int) -> int:
+    """Row stride of a [N, heads, hd] bf16 tensor on device ``index`` whose rows are contiguous."""
+    if t.dtype is not _BF16 or t.get_device() != index or t.shape != (N, heads, hd):
+        raise ValueError(f"{name} must be a bfloat16 [{N}, {heads}, {hd}] tensor on cuda:{index}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
+    row, head, last = t.stride()
+    if (last != 1 and hd > 1) or (head != hd and heads > 1):
         raise ValueError(f"{name}'s rows must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else heads * hd
+    return row if N > 1 else heads * hd
 
 
 def gqa_append(proj, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, heads, kv_heads, temp=None,
@@ -1096,27 +1114,29 @@ def gqa_append(proj, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, 
     pairs (2j, 2j + 1) when ``interleaved`` (rotary_dim a multiple of 8), else (j, j + rotary_dim / 2) (a multiple of
     16). The position is the key position unless ``positions`` ([N] int32) gives it. fp32 with one rounding at the end.
     hd: a multiple of 8 up to 128. Returns q [N, heads, hd] bf16 (``q_out`` when given; a row stride is allowed)."""
-    paged, Hkv, hd = _paged(proj, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, kv_heads)
-    dev = proj.device
-    if proj.dtype != torch.bfloat16 or proj.dim() != 2 or proj.shape[1] < (heads + 2 * Hkv) * hd or (
-            proj.shape[1] > 1 and proj.stride(1) != 1):
+    paged, index, Hkv, hd = _paged(proj, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, kv_heads)
+    shape = proj.shape
+    if proj.dtype is not _BF16 or len(shape) != 2 or shape[1] < (heads + 2 * Hkv) * hd or (
+            shape[1] > 1 and proj.stride(1) != 1):
         raise ValueError(f"proj must be a bfloat16 [N, >= {(heads + 2 * Hkv) * hd}] tensor with contiguous rows")
-    N = proj.shape[0]
-    if temp is not None:
-        _check_cuda("temp", temp, torch.bfloat16, dev)
-        _require(temp.numel() == heads and temp.is_contiguous(), f"temp must hold {heads} values")
-    if positions is not None:
-        _check_cuda("positions", positions, torch.int32, dev)
-        _require(positions.shape == (N,) and positions.is_contiguous(), f"positions must be a contiguous [{N}] tensor")
+    N = shape[0]
+    if temp is not None and (temp.dtype is not _BF16 or temp.get_device() != index or temp.numel() != heads
+                             or not temp.is_contiguous()):
+        raise ValueError(f"temp must hold {heads} bfloat16 values on {proj.device}")
+    if positions is not None and (positions.dtype is not _I32 or positions.get_device() != index
+                                  or positions.shape != (N,) or not positions.is_contiguous()):
+        raise ValueError(f"positions must be a contiguous int32 [{N}] tensor on {proj.device}")
     if q_out is None:
-        q_out = torch.empty((N, heads, hd), device=dev, dtype=torch.bfloat16)
-    elif q_out.device != dev or q_out.shape[0] != N:
-        raise ValueError(f"q_out must be a [{N}, {heads}, {hd}] tensor on {dev}")
-    _lib.call("zb_gqa_append", proj.data_ptr(), proj.stride(0) if N > 1 else proj.shape[1],
+        if heads < 1:
+            raise ValueError(f"heads must be positive, got {heads}")
+        q_out = proj.new_empty((N, heads, hd))
+        q_stride = heads * hd
+    else:
+        q_stride = _token_rows("q_out", q_out, index, N, heads, hd)
+    _lib.call("zb_gqa_append", proj.data_ptr(), proj.stride(0) if N > 1 else shape[1],
               None if temp is None else temp.data_ptr(), None if positions is None else positions.data_ptr(),
               0.0 if eps is None else eps, eps is not None, rope_theta, hd if rotary_dim is None else rotary_dim,
-              bool(interleaved), q_out.data_ptr(), _token_rows("q_out", q_out, heads, hd), *paged, N, heads, Hkv, hd,
-              _stream(dev))
+              interleaved, q_out.data_ptr(), q_stride, *paged, N, heads, Hkv, hd, _raw_stream(index))
     return q_out
 
 
@@ -1136,58 +1156,62 @@ def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, s
     graph follows them. workspace: optional uint8 tensor of at least :func:`gqa_chunk_workspace_bytes` bytes, its first
     4096 zero before the first call (every call leaves them zero) and not shared by calls that may overlap; absent, the
     stream's own is used. hd: a multiple of 8 up to 128. Returns out [N, Hq, hd] bf16."""
-    paged, Hkv, hd = _paged(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, None)
-    dev = q.device
+    paged, index, Hkv, hd = _paged(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, None)
     N, Hq = q.shape[0], q.shape[1]
-    qs = _token_rows("q", q, Hq, hd)
+    q_stride = _token_rows("q", q, index, N, Hq, hd)
     if out is None:
-        out = torch.empty((N, Hq, hd), device=dev, dtype=torch.bfloat16)
-    elif out.device != dev or out.shape[0] != N:
-        raise ValueError(f"out must be a [{N}, {Hq}, {hd}] tensor on {dev}")
+        out = torch.empty_like(q) if q_stride == Hq * hd else q.new_empty((N, Hq, hd))
+        out_stride = Hq * hd
+    else:
+        out_stride = _token_rows("out", out, index, N, Hq, hd)
     gate_ptr, gate_stride = None, 0
     if gate is not None:
-        _check_cuda("gate", gate, torch.bfloat16, dev)
-        _require(gate.shape == (N, Hq) and (Hq == 1 or gate.stride(1) == 1), f"gate must be [{N}, {Hq}] with contiguous rows")
+        if gate.dtype is not _BF16 or gate.get_device() != index or gate.shape != (N, Hq) or (
+                Hq > 1 and gate.stride(1) != 1):
+            raise ValueError(f"gate must be a bfloat16 [{N}, {Hq}] tensor on {q.device} with contiguous rows")
         gate_ptr, gate_stride = gate.data_ptr(), gate.stride(0) if N > 1 else Hq
-    if lse is not None:
-        _check_cuda("lse", lse, torch.float32, dev)
-        _require(lse.shape == (N, Hq) and lse.is_contiguous(), f"lse must be a contiguous [{N}, {Hq}] tensor")
-    need = gqa_chunk_workspace_bytes(N, Hq, page_table, k_cache)
-    stream = _stream(dev)
+    if lse is not None and (lse.dtype is not torch.float32 or lse.get_device() != index or lse.shape != (N, Hq)
+                            or not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous float32 [{N}, {Hq}] tensor on {q.device}")
+    need = _chunk_workspace_bytes(paged[12], N, Hq, Hkv, hd, paged[9] * paged[6])
+    stream = _raw_stream(index)
     if workspace is None:
-        workspace = _chunk_workspace(dev, stream, need) if need else None
-    else:
-        _check_cuda("workspace", workspace, torch.uint8, dev)
-        _require(workspace.is_contiguous() and workspace.numel() >= need,
-                 f"workspace must be a contiguous uint8 tensor of at least {need} bytes")
-    _lib.call("zb_gqa_chunk", q.data_ptr(), qs, *paged, N, Hq, Hkv, hd,
-              hd ** -0.5 if softmax_scale is None else softmax_scale, bool(causal), window, gate_ptr, gate_stride,
-              out.data_ptr(), _token_rows("out", out, Hq, hd), None if lse is None else lse.data_ptr(),
-              None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(),
-              stream)
+        workspace = _chunk_workspace(q, stream, need) if need else None
+    elif (workspace.dtype is not torch.uint8 or workspace.get_device() != index or not workspace.is_contiguous()
+          or workspace.numel() < need):
+        raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on {q.device}")
+    _lib.call("zb_gqa_chunk", q.data_ptr(), q_stride, *paged, N, Hq, Hkv, hd,
+              hd ** -0.5 if softmax_scale is None else softmax_scale, causal, window, gate_ptr, gate_stride,
+              out.data_ptr(), out_stride, None if lse is None else lse.data_ptr(),
+              None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(), stream)
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _chunk_workspace_bytes(B, N, Hq, Hkv, hd, max_keys) -> int:
+    return _lib.load().zb_gqa_chunk_workspace_bytes(B, N, Hq, Hkv, hd, max_keys)
 
 
 _CHUNK_WS: dict = {}  # (device, stream) -> the workspace of eager calls on that stream (its flags zero between calls)
 _CHUNK_FLAG_BYTES = 4096  # the flags lie at the workspace's start
 
 
-def _chunk_workspace(dev: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+def _chunk_workspace(q: torch.Tensor, stream: int, nbytes: int) -> torch.Tensor:
     """A workspace with its flags zero. Eager calls on a stream share one, in stream order; under capture every call gets
     its own (from the graph's pool, its flags zeroed by the graph), as a replay may run beside eager calls."""
-    if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-        ws[:_CHUNK_FLAG_BYTES].zero_()
-        return ws
-    ws = _CHUNK_WS.get((dev, stream))
+    key = q.get_device(), stream
+    capturing = torch.cuda.is_current_stream_capturing()
+    ws = None if capturing else _CHUNK_WS.get(key)
     if ws is None or ws.numel() < nbytes:  # a smaller one goes back to the allocator, which reuses it in stream order
-        ws = _CHUNK_WS[(dev, stream)] = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+        ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
         ws[:_CHUNK_FLAG_BYTES].zero_()
+        if not capturing:
+            _CHUNK_WS[key] = ws
     return ws
 
 
 def gqa_chunk_workspace_bytes(tokens: int, heads: int, page_table, k_cache) -> int:
     """Bytes of workspace :func:`gqa_chunk` needs for ``tokens`` rows of ``heads`` query heads over these tables."""
     page_size = k_cache.shape[1] if k_cache.dim() == 4 else 1
-    return _lib.load().zb_gqa_chunk_workspace_bytes(page_table.shape[0], tokens, heads, k_cache.shape[-2],
-                                                    k_cache.shape[-1], page_table.shape[1] * page_size)
+    return _chunk_workspace_bytes(page_table.shape[0], tokens, heads, k_cache.shape[-2], k_cache.shape[-1],
+                                  page_table.shape[1] * page_size)
