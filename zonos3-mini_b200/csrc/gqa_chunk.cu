@@ -258,13 +258,19 @@ __device__ __forceinline__ bool not_finite(const uint4& v) {
   return (a & 0xffffu) >= 0x7f80u || (a >> 16) >= 0x7f80u;
 }
 
-// A wait that gives up after a second, and at once after any earlier one of the CTA did.
+// A wait that gives up after about a second (2^31 cycles), and at once after any earlier one of the CTA did. Short, because
+// it stands in many places of loops that already fill the instruction cache.
 __device__ __forceinline__ void wait(const uint64_t& bar, uint32_t parity, int* abort, unsigned* status) {
   const uint32_t at = zb::smem_addr(&bar);
   if (zb::mbar_try_wait(at, parity)) return;
-  if (*reinterpret_cast<volatile int*>(abort) != 0) return;
-  if (!zb::mbar_wait_bounded(at, parity, status, zb::kStatusAttnChunkTimeout))
-    *reinterpret_cast<volatile int*>(abort) = 1;
+  const int start = clock();
+  while (!zb::mbar_try_wait_sleep(at, parity, 20000u)) {
+    if (*reinterpret_cast<volatile int*>(abort) != 0) return;
+    if ((int)clock() - start < 0) {
+      if (status) atomicOr(status, zb::kStatusAttnChunkTimeout);
+      *reinterpret_cast<volatile int*>(abort) = 1;
+    }
+  }
 }
 // The same answer for every lane of the warp.
 __device__ __forceinline__ bool gave_up(int* abort) {
@@ -369,6 +375,7 @@ __device__ __forceinline__ void join_rows(const ChunkParams& p, const Desc& u, i
   const int64_t token = u.token0 + r / p.G;
   float f = l == 0.f ? 0.f : 1.f / l;
   if (p.gate) f *= sigmoid(p.gate[token * p.gate_stride + h]);
+#pragma unroll 1
   for (int piece = tid / u.rows; piece < HD / 4 / N; piece += sharers) {
     float y[4 * N] = {};
 #pragma unroll 2
@@ -401,6 +408,7 @@ __device__ __forceinline__ void join_rows(const ChunkParams& p, const Desc& u, i
 template <int HD>
 __device__ __forceinline__ void join(const ChunkParams& p, const Desc& u, int cta, int tid) {
   bool there = true;
+#pragma unroll 1
   for (int i = 1 + tid % 32; i < u.parts; i += 32) there = wait_flag(p.flags + cta + i) && there;
   if (!__all_sync(0xffffffffu, there)) {
     if (p.status && tid % 32 == 0) atomicOr(p.status, zb::kStatusAttnChunkTimeout);
@@ -469,6 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   if (tid < B) requests[tid] = mine;
   int64_t all_pairs = 0;
   int buffer = 0;
+#pragma unroll 1
   for (int b0 = 0; b0 < B; b0 += kThreads, buffer ^= 1) {
     const int b = b0 + tid;
     const int n = b < B ? stream_pairs(p, b0 == 0 ? mine.tokens : request(p, b).tokens) : 0;
@@ -488,6 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   auto pair_of = [&](int j) {
     if (j >= pairs) return Pair{0, 0, 0};
     int lo = 0, hi = B;  // the last b with pairs_before[b] <= j
+#pragma unroll 1
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
       if (pairs_before[mid] <= j) lo = mid;
@@ -501,6 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   int first_total = 0;
   const int first_before = block_scan(first_pair.work, tl, buffer, first_total);
   int64_t work = first_total;
+#pragma unroll 1
   for (int j0 = kThreads; j0 < pairs; j0 += kThreads) {
     int total;
     buffer ^= 1;
@@ -512,6 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   const int64_t begin = share * cta, end = min(work, begin + share);
   if (begin < end) {
     int64_t seen = 0;
+#pragma unroll 1
     for (int j0 = 0; j0 < pairs; j0 += kThreads) {
       Pair q = first_pair;
       int before = first_before, total = first_total;
@@ -536,6 +548,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   }
   if (hd < HD) {  // the padding dims of every tile stay zero
     __syncthreads();
+#pragma unroll 1
     for (uint32_t i = tid; i < L::kOffTail / 16; i += kThreads) reinterpret_cast<uint4*>(gbase)[i] = make_uint4(0, 0, 0, 0);
     tc::fence_proxy_async();
   }
@@ -564,6 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         constexpr int kPart = kCopies / 4;
+#pragma unroll 1
         for (int g = 0; g < kPart; g += kAhead) {
           if ((k * (kPart / kAhead) + g / kAhead) % warps != which) continue;
           int64_t o[kAhead];
@@ -630,11 +644,13 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         const int held = min(req.keys, p.kv.max_pages * p.kv.page_size);
         const int32_t* table = p.kv.table + (int64_t)b * p.kv.table_stride;
         if (warp == kLoadWarp + 1) {  // the unit's queries: a stream's tokens, the group's heads of each
+#pragma unroll 1
           for (int s = 0; s < (u.rows > p.tokens * G ? 2 : 1); ++s, ++q_item) {
             const int slot = q_item % 2;
             if (q_item >= 2) wait(tl.q_empty[slot], (q_item / 2 - 1) & 1, abort, p.status);
             if (lane == 0) {
               zb::mbar_arrive_expect_tx(zb::smem_addr(&tl.q_full[slot]), (uint32_t)(p.tokens * G * HD * 2));
+  #pragma unroll 1
               for (int a = 0; a < HD / 64; ++a)
                 load_queries(base + L::kOffQ + slot * L::kItem + a * L::kQAtom, &maps.q, a * 64, kvh * G,
                              u.token0 + s * p.tokens, zb::smem_addr(&tl.q_full[slot]));
@@ -650,7 +666,9 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               return lane < boxes && pos < held ? table[pos / p.kv.page_size] : -1;
             };
             int next = look(u.tile0);
-            for (int t = 0; t < u.tiles; ++t, ++tile_no) {
+#pragma unroll 1
+  #pragma unroll 1
+          for (int t = 0; t < u.tiles; ++t, ++tile_no) {
               const int first = (u.tile0 + t) * kTile, pos = first + lane * p.box;
               const bool there = next >= 0 && next < p.kv.num_pages;
               const int page = there ? next * p.page_heads + (p.page_heads > 1 ? kvh : 0)
@@ -664,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                 bits[k] = __ballot_sync(0xffffffffu, first + r < held && (live >> (r / p.box) & 1u));
               }
               if (t + 1 < u.tiles) next = look(u.tile0 + t + 1);
-#pragma unroll
+#pragma unroll 1
               for (int kv = 0; kv < 2; ++kv, ++item) {
                 const int slot = item % L::kSlots;
                 if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort, p.status);
@@ -689,6 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             }
           };
           look(u.tile0);
+#pragma unroll 1
           for (int t = 0; t < u.tiles; ++t, ++tile_no) {
             int64_t off[4];
             unsigned bits[4];
@@ -702,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               bits[k] = __ballot_sync(0xffffffffu, there);
             }
             if (t + 1 < u.tiles) look(u.tile0 + t + 1);
-#pragma unroll
+#pragma unroll 1
             for (int kv = 0; kv < 2; ++kv, ++item) {
               const int slot = item % L::kSlots;
               if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort, p.status);
@@ -800,6 +819,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         commit(tl.q_empty[q_item % 2]);
         if (two) commit(tl.q_empty[(q_item + 1) % 2]);
       }
+#pragma unroll 1
       for (int t = 0; t < u.tiles; ++t) {
         // O_s += P_s(t) V(t) as soon as P_s(t) is there, then the stream's next scores
         const int v_item = item + 2 * t + 1, k_next = item + 2 * (t + stride);
@@ -811,6 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         // rows of the last page past the request's keys came along with a tensor copy: no key, so no value either
         if (p.box && first + kTile > held && held % p.box != 0) {
           const int r0 = held - first, r1 = (r0 + p.box - 1) / p.box * p.box;
+#pragma unroll 1
           for (int i = r0 * (HD / 8) + lane; i < r1 * (HD / 8); i += 32)
             *reinterpret_cast<uint4*>(v_tile + piece<HD>(i / (HD / 8), i % (HD / 8))) = make_uint4(0, 0, 0, 0);
           tc::fence_proxy_async();
@@ -818,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         }
         if (first + kTile > u.all_hi || first < u.all_lo) {  // keys that some rows see and others do not
           bool bad = false;
-#pragma unroll 8
+#pragma unroll 4
           for (uint32_t i = lane; i < L::kItem / 16; i += 32) bad |= not_finite(reinterpret_cast<const uint4*>(v_tile)[i]);
           found = __any_sync(0xffffffffu, bad);
           if (lane == 0) {
@@ -826,8 +847,10 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             arrive(tl.scanned);
           }
           if (found) {  // every stream adds what it sees before it hands over P; then the values are zeroed
+#pragma unroll 1
             for (int s = s0; s <= s1; ++s) wait(tl.p_full[s], tiles_done[s] & 1, abort, p.status);
             uint16_t* e = reinterpret_cast<uint16_t*>(v_tile);
+#pragma unroll 1
             for (uint32_t i = lane; i < L::kItem / 2; i += 32)
               if ((e[i] & 0x7f80u) == 0x7f80u) e[i] = 0;
             tc::fence_proxy_async();
@@ -835,6 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           }
         }
         if (p.box == 0) tc::fence_proxy_async();
+#pragma unroll 1
         for (int s = s0; s <= s1; ++s) {
           wait(tl.p_half[s], tiles_done[s] & 1, abort, p.status);
           tc::fence_after();
@@ -892,6 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           const int r = first_row + 32 * (warp % 4) + lane;
           gate = sigmoid(p.gate[(int64_t)(u.token0 + r / G) * p.gate_stride + u.kvh * G + r % G]);
         }
+#pragma unroll 1
         for (int t = 0; t < u.tiles; ++t) {
           const int first = (u.tile0 + t) * kTile;
           const bool scan = first + kTile > u.all_hi || first < u.all_lo;
@@ -1021,9 +1046,11 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               }
               tc::st_wait();
               const unsigned char* v = gbase + (size_t)((2 * (tile_no + t) + 1) % L::kSlots) * L::kItem;
+#pragma unroll 1
               for (int j = 0; j < kTile; ++j) {
                 const unsigned word = j < 32 ? seen[0] : j < 64 ? seen[1] : j < 96 ? seen[2] : seen[3];
                 const bool sees = (word >> (j % 32)) & 1u;
+#pragma unroll 1
                 for (int c = 0; c < HD / 8; ++c) {
                   const uint4 w = *reinterpret_cast<const uint4*>(v + piece<HD>(j, c));
                   if (!not_finite(w)) continue;  // the same for every lane
@@ -1111,6 +1138,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                   make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           }
         };
+#pragma unroll 1
         for (int c = c0; c < c1; ++c) chunk(c);
         if (u.mode == kFinal) {
           tc::st_wait();
@@ -1161,11 +1189,14 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   }
   // ---- rows of no request
   const int idle = tl.idle[0] + p.kv.N - tl.idle[1];
+#pragma unroll 1
   for (int i = cta * (kThreads / 32) + warp; i < idle; i += ctas * (kThreads / 32)) {
     const int64_t t = i < tl.idle[0] ? i : tl.idle[1] + i - tl.idle[0];
+#pragma unroll 1
     for (int c = lane; c < p.Hq * hd / 8; c += 32)
       *reinterpret_cast<uint4*>(p.out + t * p.out_stride + c * 8) = make_uint4(0, 0, 0, 0);
     if (p.lse)
+#pragma unroll 1
       for (int h = lane; h < p.Hq; h += 32) p.lse[t * p.Hq + h] = -INFINITY;
   }
   tc::fence_before();
