@@ -40,7 +40,8 @@ namespace tc = zb::tc;
 
 constexpr int kTile = 128;       // keys of a tile
 constexpr int kStreamRows = 128;  // rows of a stream
-constexpr int kUnitCost = 2;  // what a unit costs besides its tiles, in tiles
+constexpr int kUnitCost = 4;     // what a unit costs besides its tiles, in tiles: the best of 1, 2, 3, 4, 6 on every batch
+constexpr int kFewRows = 32;     // up to here the row warps share a unit's rows in joining its parts
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
 constexpr int kMaxSlots = 10, kDescs = 4;
@@ -48,8 +49,23 @@ constexpr int kMasks = 8;  // the loaders run at most 5 tiles ahead of the rows
 constexpr float kRescale = 8.f;  // log2 growth of a row's maximum that the accumulator is rescaled for
 constexpr int kMaxRequests = 16384;
 
+// n / d and n % d for 0 <= n < 2^31 by a multiplication: m = ceil(2^(31 + l) / d) with 2^l >= d.
+struct Divisor {
+  unsigned d, m, shift;
+  __host__ void set(int by) {
+    unsigned l = 0;
+    while ((1u << l) < (unsigned)by) ++l;
+    d = (unsigned)by;
+    shift = 31 + l;
+    m = (unsigned)((((uint64_t)1 << shift) + d - 1) / d);
+  }
+  __device__ __forceinline__ int quotient(int n) const { return (int)(((uint64_t)(unsigned)n * m) >> shift); }
+  __device__ __forceinline__ int rest(int n) const { return n - quotient(n) * (int)d; }
+};
+
 struct ChunkParams {
   zb::PagedBatch kv;
+  Divisor by_page, by_group, by_pair;  // page size, G, tokens of a pair of streams
   const __nv_bfloat16* q;  // [N, Hq, hd], row stride q_stride
   int64_t q_stride;
   int Hq, G;
@@ -301,7 +317,7 @@ __device__ __forceinline__ void visible(const ChunkParams& p, int keys, int pos,
 
 // Streams of a request's rows come in pairs; a pair's unit of work for one KV head: its rows and key tiles.
 __device__ __forceinline__ int stream_pairs(const ChunkParams& p, int tokens) {
-  return (tokens + 2 * p.tokens - 1) / (2 * p.tokens);
+  return p.by_pair.quotient(tokens + 2 * p.tokens - 1);
 }
 __device__ __forceinline__ void unit_tiles(const ChunkParams& p, const Request& r, int pair, Desc& d) {
   const int first = pair * 2 * p.tokens, tokens = min(r.tokens - first, 2 * p.tokens);
@@ -356,66 +372,53 @@ __device__ __forceinline__ bool wait_flag(const unsigned* flag) {
   }
 }
 
-// Joins the parts of a unit that began in this CTA, in the order of their keys. A thread of the row warps takes a row, or
-// with few rows one of its pieces of 4 * N dims: the parts' maxima and sums once, then the loads of a piece of several
-// parts together.
-template <int HD, int N>
-__device__ __forceinline__ void join_rows(const ChunkParams& p, const Desc& u, int cta, int tid) {
-  const int sharers = 32 * kSoftWarps / u.rows, r = tid % u.rows;  // of a row; at least one, as a unit has 256 rows at most
-  if (tid / u.rows >= sharers) return;
-  auto part = [&](int i) { return (int64_t)(cta + i) * 2 + (i == 0); };
-  auto maximum = [&](int i) { return __ldcg(p.ml + part(i) * 2 * p.rows_max + r); };
-  float top = -INFINITY, l = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < u.parts; ++i) top = fmaxf(top, maximum(i));
-  const float mb = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
-  for (int i = 0; i < u.parts; ++i) l += __ldcg(p.ml + (part(i) * 2 + 1) * p.rows_max + r) * ex2(maximum(i) - mb);
-  const int h = u.kvh * p.G + r % p.G;
-  const int64_t token = u.token0 + r / p.G;
-  float f = l == 0.f ? 0.f : 1.f / l;
-  if (p.gate) f *= sigmoid(p.gate[token * p.gate_stride + h]);
-#pragma unroll 1
-  for (int piece = tid / u.rows; piece < HD / 4 / N; piece += sharers) {
-    float y[4 * N] = {};
-#pragma unroll 2
-    for (int i = 0; i < u.parts; ++i) {
-      const float4* a = reinterpret_cast<const float4*>(p.acc + (part(i) * (HD / 4) + piece * N) * p.rows_max * 4 + r * 4);
-      float4 v[N];
-#pragma unroll
-      for (int k = 0; k < N; ++k) v[k] = __ldcg(a + (int64_t)k * p.rows_max);
-      const float w = ex2(maximum(i) - mb);  // 0 for a part none of whose keys the row sees; its accumulator is 0 too
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        y[4 * k] += v[k].x * w;
-        y[4 * k + 1] += v[k].y * w;
-        y[4 * k + 2] += v[k].z * w;
-        y[4 * k + 3] += v[k].w * w;
-      }
-    }
-    __nv_bfloat16* out = p.out + token * p.out_stride + (int64_t)h * p.kv.hd + piece * 4 * N;
-#pragma unroll
-    for (int k = 0; k < N; k += 2)
-      if (piece * 4 * N + 4 * k < p.kv.hd) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = to_bf16x2(y[4 * k + 2 * e] * f, y[4 * k + 2 * e + 1] * f);
-        *reinterpret_cast<uint4*>(out + 4 * k) = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-  }
-  if (p.lse && tid < u.rows) p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
-}
-template <int HD>
-__device__ __forceinline__ void join(const ChunkParams& p, const Desc& u, int cta, int tid) {
+// Waits for the parts of a unit that began in this CTA: those of the CTAs after it, every warp for itself.
+__device__ __forceinline__ bool wait_parts(const ChunkParams& p, const Desc& u, int cta, int lane) {
   bool there = true;
 #pragma unroll 1
-  for (int i = 1 + tid % 32; i < u.parts; i += 32) there = wait_flag(p.flags + cta + i) && there;
-  if (!__all_sync(0xffffffffu, there)) {
-    if (p.status && tid % 32 == 0) atomicOr(p.status, zb::kStatusAttnChunkTimeout);
-    return;
+  for (int i = 1 + lane; i < u.parts; i += 32) there = wait_flag(p.flags + cta + i) && there;
+  there = __all_sync(0xffffffffu, there);
+  if (!there && p.status && lane == 0) atomicOr(p.status, zb::kStatusAttnChunkTimeout);
+  return there;
+}
+// Part i of a unit that began in CTA cta: the CTA's own, then those of the CTAs after it.
+__device__ __forceinline__ int64_t part_slot(int cta, int i) { return (int64_t)(cta + i) * 2 + (i == 0); }
+
+// Joins the parts of a unit of few rows, in the order of their keys: a thread of the row warps takes 8 dims of a row, its
+// loads of several parts in flight together.
+template <int HD>
+__device__ __forceinline__ void join_few(const ChunkParams& p, const Desc& u, int cta, int tid) {
+  const int sharers = 32 * kSoftWarps / u.rows, r = tid % u.rows;  // threads of a row
+  if (tid / u.rows >= sharers) return;
+  auto maximum = [&](int i) { return __ldcg(p.ml + part_slot(cta, i) * 2 * p.rows_max + r); };
+  auto sum = [&](int i) { return __ldcg(p.ml + (part_slot(cta, i) * 2 + 1) * p.rows_max + r); };
+  const int h = u.kvh * p.G + p.by_group.rest(r);
+  const int64_t token = u.token0 + p.by_group.quotient(r);
+  const float gate = p.gate ? sigmoid(p.gate[token * p.gate_stride + h]) : 1.f;
+  float top = -INFINITY, l = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < u.parts; ++i) top = fmaxf(top, maximum(i));
+  const float mb = top == -INFINITY ? 0.f : top;
+#pragma unroll 1
+  for (int piece = tid / u.rows; piece < HD / 8; piece += sharers) {
+    float y[8] = {};
+    l = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < u.parts; ++i) {
+      const float4* a = reinterpret_cast<const float4*>(p.acc + (part_slot(cta, i) * (HD / 4) + piece * 2) * p.rows_max * 4 + r * 4);
+      const float4 v0 = __ldcg(a), v1 = __ldcg(a + p.rows_max);
+      const float w = ex2(maximum(i) - mb);  // 0 for a part none of whose keys the row sees; its accumulator is 0 too
+      l += sum(i) * w;
+      y[0] += v0.x * w, y[1] += v0.y * w, y[2] += v0.z * w, y[3] += v0.w * w;
+      y[4] += v1.x * w, y[5] += v1.y * w, y[6] += v1.z * w, y[7] += v1.w * w;
+    }
+    const float f = l == 0.f ? 0.f : gate / l;
+    if (piece * 8 < p.kv.hd)
+      *reinterpret_cast<uint4*>(p.out + token * p.out_stride + (int64_t)h * p.kv.hd + piece * 8) =
+          make_uint4(to_bf16x2(y[0] * f, y[1] * f), to_bf16x2(y[2] * f, y[3] * f), to_bf16x2(y[4] * f, y[5] * f),
+                     to_bf16x2(y[6] * f, y[7] * f));
+    if (p.lse && piece == 0) p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
   }
-  if (u.rows <= 32) join_rows<HD, 2>(p, u, cta, tid);
-  else join_rows<HD, 8>(p, u, cta, tid);
 }
 
 template <int HD>
@@ -620,6 +623,16 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const bool here = d.tiles > 0 ? to_tile > from_tile : off == 0;
       Desc u = d;
       u.kvh = kvh;
+      const int held = held_keys(p, req.keys);
+      const int32_t* table = p.kv.table + (int64_t)min(b, B - 1) * p.kv.table_stride;
+      // Page lookups, a tile ahead of their use and before anything that can wait. A lane's box of a tile:
+      const int boxes = p.box ? kTile / p.box : 0;
+      auto look_box = [&](int t) {
+        const int pos = t * kTile + lane * p.box;
+        return lane < boxes && pos < held ? table[p.by_page.quotient(pos)] : -1;
+      };
+      int next = -1;
+      if (p.box && here && warp == kLoadWarp) next = look_box(d.tile0 + from_tile);
       if (here || at >= end) {
         u.tile0 = d.tile0 + from_tile;
         u.tiles = to_tile - from_tile;
@@ -641,8 +654,6 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         u.tiles = 0;
       }
       if (u.tiles > 0) {
-        const int held = min(req.keys, p.kv.max_pages * p.kv.page_size);
-        const int32_t* table = p.kv.table + (int64_t)b * p.kv.table_stride;
         if (warp == kLoadWarp + 1) {  // the unit's queries: a stream's tokens, the group's heads of each
 #pragma unroll 1
           for (int s = 0; s < (u.rows > p.tokens * G ? 2 : 1); ++s, ++q_item) {
@@ -660,12 +671,6 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         }
         if (p.box) {
           if (warp == kLoadWarp) {
-            const int boxes = kTile / p.box;  // of a tile; lane i brings box i
-            auto look = [&](int t) {
-              const int pos = t * kTile + lane * p.box;
-              return lane < boxes && pos < held ? table[pos / p.kv.page_size] : -1;
-            };
-            int next = look(u.tile0);
 #pragma unroll 1
   #pragma unroll 1
           for (int t = 0; t < u.tiles; ++t, ++tile_no) {
@@ -673,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               const bool there = next >= 0 && next < p.kv.num_pages;
               const int page = there ? next * p.page_heads + (p.page_heads > 1 ? kvh : 0)
                                      : (int)(p.kv.num_pages * p.page_heads);  // past the end: zeros
-              const int group = there ? pos % p.kv.page_size / 8 : 0;
+              const int group = there ? p.by_page.rest(pos) / 8 : 0;
               const unsigned live = __ballot_sync(0xffffffffu, there);
               unsigned bits[4];
 #pragma unroll
@@ -681,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                 const int r = 32 * k + lane;
                 bits[k] = __ballot_sync(0xffffffffu, first + r < held && (live >> (r / p.box) & 1u));
               }
-              if (t + 1 < u.tiles) next = look(u.tile0 + t + 1);
+              if (t + 1 < u.tiles) next = look_box(u.tile0 + t + 1);
 #pragma unroll 1
               for (int kv = 0; kv < 2; ++kv, ++item) {
                 const int slot = item % L::kSlots;
@@ -703,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const int pos = t * kTile + 32 * k + lane;
-              pages[k] = pos < held ? table[pos / p.kv.page_size] : -1;
+              pages[k] = pos < held ? table[p.by_page.quotient(pos)] : -1;
             }
           };
           look(u.tile0);
@@ -715,7 +720,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             for (int k = 0; k < 4; ++k) {
               const int pos = (u.tile0 + t) * kTile + 32 * k + lane;
               const bool there = pages[k] >= 0 && pages[k] < p.kv.num_pages;
-              off[k] = there ? (int64_t)pages[k] * p.kv.page_stride + (int64_t)(pos % p.kv.page_size) * p.kv.slot_stride +
+              off[k] = there ? (int64_t)pages[k] * p.kv.page_stride + (int64_t)p.by_page.rest(pos) * p.kv.slot_stride +
                                    (int64_t)kvh * p.kv.head_stride
                              : -1;
               bits[k] = __ballot_sync(0xffffffffu, there);
@@ -911,10 +916,10 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       {
         int lo = 0, hi = INT32_MAX;  // a lane without a row sees everything; it is not stored
         if (32 * (warp % 4) + lane < rows)
-          visible(p, u.keys, u.pos0 + (first_row + 32 * (warp % 4) + lane) / G, lo, hi);
-        if (p.gate && u.mode == kFinal && 32 * (warp % 4) + lane < rows) {
+          visible(p, u.keys, u.pos0 + p.by_group.quotient(first_row + 32 * (warp % 4) + lane), lo, hi);
+        if (p.gate && u.mode != kPart0 && 32 * (warp % 4) + lane < rows) {
           const int r = first_row + 32 * (warp % 4) + lane;
-          gate = sigmoid(p.gate[(int64_t)(u.token0 + r / G) * p.gate_stride + u.kvh * G + r % G]);
+          gate = sigmoid(p.gate[(int64_t)(u.token0 + p.by_group.quotient(r)) * p.gate_stride + u.kvh * G + p.by_group.rest(r)]);
         }
 #pragma unroll 1
         for (int t = 0; t < u.tiles; ++t) {
@@ -1081,8 +1086,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       int own = 32 * (warp % 4) + lane;
       asm volatile("" : "+r"(own));  // the row is worked out here anew: kept through the tiles it would cost registers
       const bool live = own < rows;
-      const int r = first_row + own, h = u.kvh * G + (live ? r % G : 0);
-      const int64_t token = u.token0 + (live ? r / G : 0);
+      const int r = first_row + own, h = u.kvh * G + p.by_group.rest(r);
+      const int64_t token = u.token0 + p.by_group.quotient(r);
       // The accumulator of the row: its stream's, or both halves' of it, each half of the dims by one of the streams.
       float own_c = 1.f, other_c = 0.f;
       int c0 = 0, c1 = HD / 32;
@@ -1102,6 +1107,26 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         c1 = c0 + HD / 64;
       }
       const uint32_t col_other = tlane + L::kColO + (1 - s) * HD;
+      // A unit that began here and goes on in other CTAs: they handed their parts over as the first thing they did. With
+      // many rows each row adds them to its own accumulator; few rows are joined by all the warps, below.
+      const bool few = u.rows <= kFewRows, adds = u.mode == kPart1 && !few;
+      float own_w = 1.f;
+      if (adds && wait_parts(p, u, cta, lane)) {
+        float top = m;
+#pragma unroll 4
+        for (int i = 1; i < u.parts; ++i) top = fmaxf(top, live ? __ldcg(p.ml + part_slot(cta, i) * 2 * p.rows_max + r) : top);
+        const float mb = top == -INFINITY ? 0.f : top;
+        own_w = ex2(m - mb);
+        l *= own_w;
+#pragma unroll 4
+        for (int i = 1; i < u.parts; ++i)
+          if (live) {
+            const float* ml = p.ml + part_slot(cta, i) * 2 * p.rows_max + r;
+            l += __ldcg(ml + p.rows_max) * ex2(__ldcg(ml) - mb);
+          }
+        m = top;
+      }
+      const bool done = u.mode == kFinal || adds;  // the row's output is formed here
       if ((two || s == 0 || u.tiles > 1) && !gave_up(abort)) {
         const float f = l == 0.f ? 0.f : gate / l;  // 0 for a row that saw no key; a NaN sum stays NaN
         const int64_t part = (int64_t)cta * 2 + (u.mode == kPart1);
@@ -1122,7 +1147,27 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             }
             tc::ld_wait();
           }
-          if (u.mode == kFinal) {
+          if (adds) {
+            const float mb = m == -INFINITY ? 0.f : m;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * own_w);
+#pragma unroll 1
+            for (int i = 1; i < u.parts && live; ++i) {
+              const float4* a = reinterpret_cast<const float4*>(p.acc + (part_slot(cta, i) * (HD / 4) + 8 * c) * p.rows_max * 4 + r * 4);
+              float4 v[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) v[j] = __ldcg(a + (int64_t)j * p.rows_max);
+              const float w = ex2(__ldcg(p.ml + part_slot(cta, i) * 2 * p.rows_max + r) - mb);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                o[4 * j] = __float_as_uint(fmaf(v[j].x, w, __uint_as_float(o[4 * j])));
+                o[4 * j + 1] = __float_as_uint(fmaf(v[j].y, w, __uint_as_float(o[4 * j + 1])));
+                o[4 * j + 2] = __float_as_uint(fmaf(v[j].z, w, __uint_as_float(o[4 * j + 2])));
+                o[4 * j + 3] = __float_as_uint(fmaf(v[j].w, w, __uint_as_float(o[4 * j + 3])));
+              }
+            }
+          }
+          if (done) {
             // packed over the columns that this chunk was read from, so that 4 lanes then hold 64 bytes of a row
             uint32_t w[16];
 #pragma unroll
@@ -1140,7 +1185,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         };
 #pragma unroll 1
         for (int c = c0; c < c1; ++c) chunk(c);
-        if (u.mode == kFinal) {
+        if (done) {
           tc::st_wait();
           const int64_t row = live ? token * p.out_stride + (int64_t)h * hd : -1;
           int64_t rows4[4];  // the rows this lane stores: lane / 4 and every 8th
@@ -1163,7 +1208,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           }
         }
         if (live && c0 == 0) {
-          if (u.mode != kFinal) {
+          if (!done) {
             p.ml[part * 2 * p.rows_max + r] = m;
             p.ml[(part * 2 + 1) * p.rows_max + r] = l;
           } else if (p.lse) {
@@ -1173,12 +1218,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       }
       tc::fence_before();  // the accumulator's reads come before the next unit's products
       if (u.mode != kFinal) {
-        __threadfence();
+        if (!done) __threadfence();
         meet();
         if (u.mode == kPart0) {
           if (tid == 0) raise_flag(p.flags + cta);
         } else {
-          join<HD>(p, u, cta, tid);
+          if (few && wait_parts(p, u, cta, lane)) join_few<HD>(p, u, cta, tid);
           meet();  // every thread is done with the parts
           if (tid < u.parts - 1) p.flags[cta + 1 + tid] = 0;
         }
@@ -1335,6 +1380,9 @@ ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_c
   p.Hq = Hq;
   p.G = Hq / Hkv;
   p.tokens = kStreamRows / p.G;
+  p.by_page.set(page_size);
+  p.by_group.set(p.G);
+  p.by_pair.set(2 * p.tokens);
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.causal = causal;
   p.window = window;
