@@ -26,8 +26,8 @@
 // rows (any page size, any strides) into shared memory, several tiles ahead and across units.
 //
 // A key hidden from some rows of a tile must not reach them even when its value is not finite, and 0 x inf is NaN in a
-// matrix product. So where a tile's keys are visible to some of its rows only, warp 8 looks through the V tile while the
-// scores are being worked on; values that are not finite are added to the rows that see them one by one, then zeroed.
+// matrix product. So where a tile's keys are visible to some of its rows only, warps 10 and 11 look through the V tile while
+// the scores are being worked on; values that are not finite are added to the rows that see them one by one, then zeroed.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -45,7 +45,7 @@ constexpr int kFewRows = 32;     // up to here the row warps share a unit's rows
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
 constexpr int kMaxSlots = 10, kDescs = 4;
-constexpr int kMasks = 8;  // the loaders run at most 5 tiles ahead of the rows
+constexpr int kMasks = 8;  // of key masks and of looked-through tiles: the loaders run at most 5 tiles ahead of the rows
 constexpr float kRescale = 8.f;  // log2 growth of a row's maximum that the accumulator is rescaled for
 constexpr int kMaxRequests = 16384;
 
@@ -85,7 +85,7 @@ struct ChunkParams {
   int rows_max;
   int pairs_max;  // units of a KV head, at most
   unsigned* status;
-  int box;  // rows of a page that one tensor copy brings; 0: K and V rows come by 16-byte copies
+  int box, box_shift;  // rows of a page that one tensor copy brings; 0: K and V rows come by 16-byte copies
   int head_atoms, page_heads;  // a KV head's atom offset, and a page's index step, in the tensor maps
 };
 struct Maps {
@@ -110,7 +110,7 @@ struct Tail {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t q_full[2], q_empty[2];
   uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
-  uint64_t scanned, drained, halves;
+  uint64_t scanned[kMasks], drained, halves;
   uint64_t desc_full[kDescs], desc_empty[kDescs];
   alignas(16) unsigned mask[kMasks][4];  // keys of a tile that exist
   Desc desc[kDescs];
@@ -121,7 +121,7 @@ struct Tail {
   float ml[2][kStreamRows][2];  // maximum and sum of the rows' two halves, when the streams share rows
   uint32_t tmem;
   int abort;
-  int found;  // the scanned V tile holds values that are not finite
+  int found[kMasks][2];  // either half of the tile's values holds some that are not finite
 };
 
 template <int HD>
@@ -267,12 +267,13 @@ __device__ __forceinline__ uint32_t to_bf16x2(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Whether any of the 8 bf16 values is not finite (all exponent bits set).
-__device__ __forceinline__ bool not_finite(const uint4& v) {
-  const unsigned a = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
-                              __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
-  return (a & 0xffffu) >= 0x7f80u || (a >> 16) >= 0x7f80u;
+// Sign bits set where the bf16 values are not finite (all exponent bits set: one more carries into the sign).
+__device__ __forceinline__ unsigned not_finite(unsigned pair) { return (pair & 0x7f807f80u) + 0x00800080u; }
+__device__ __forceinline__ unsigned not_finite(const uint4& v) {
+  return not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w);
 }
+// Whether a tile of keys from `first` on has keys that some of the unit's rows see and others do not.
+__device__ __forceinline__ bool mixed_tile(const Desc& u, int first) { return first + kTile > u.all_hi || first < u.all_lo; }
 
 // A wait that gives up after about a second (2^31 cycles), and at once after any earlier one of the CTA did. Short, because
 // it stands in many places of loops that already fill the instruction cache.
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       zb::mbar_init(zb::smem_addr(&tl.p_full[s]), kSoftWarps / 2);
       zb::mbar_init(zb::smem_addr(&tl.o_full[s]), 1);
     }
-    zb::mbar_init(zb::smem_addr(&tl.scanned), 1);
+    for (int s = 0; s < kMasks; ++s) zb::mbar_init(zb::smem_addr(&tl.scanned[s]), kLoadWarps - 1);
     zb::mbar_init(zb::smem_addr(&tl.drained), 1);
     zb::mbar_init(zb::smem_addr(&tl.halves), 32 * kSoftWarps);
     for (int s = 0; s < kDescs; ++s) {
@@ -460,7 +461,6 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     }
     zb::fence_mbar_init();
     tl.abort = 0;
-    tl.found = 0;
   }
   if (warp == kMmaWarp) tc::alloc(zb::smem_addr(&tl.tmem), 512);
   if (warp == kLoadWarp && lane < 3)
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     int64_t at = begin;
     const int unit0 = d.tiles + kUnitCost;
     int kvh = (int)(tl.start_off / unit0), off = (int)(tl.start_off % unit0);
-    int item = 0, tile_no = 0, q_item = 0, n = 0;
+    int item = 0, tile_no = 0, q_item = 0, scans = 0, n = 0;
     for (;;) {
       // ---- the unit's tiles here: its work is kUnitCost, then a step a tile
       const int unit = d.tiles + kUnitCost, to = (int)min((int64_t)unit, off + (end - at));
@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const int held = held_keys(p, req.keys);
       const int32_t* table = p.kv.table + (int64_t)min(b, B - 1) * p.kv.table_stride;
       // Page lookups, a tile ahead of their use and before anything that can wait. A lane's box of a tile:
-      const int boxes = p.box ? kTile / p.box : 0;
+      const int boxes = p.box ? kTile >> p.box_shift : 0;
       auto look_box = [&](int t) {
         const int pos = t * kTile + lane * p.box;
         return lane < boxes && pos < held ? table[p.by_page.quotient(pos)] : -1;
@@ -669,6 +669,28 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             __syncwarp();
           }
         }
+        // The last two warps look through the values of tiles that hold keys hidden from some rows, half of a tile each.
+        auto look_through = [&](int t, int v_item) {
+          const int first = (u.tile0 + t) * kTile, slot = scans % kMasks;
+          if (warp == kLoadWarp || !mixed_tile(u, first)) return;
+          wait(tl.full[v_item % L::kSlots], (v_item / L::kSlots) & 1, abort, p.status);
+          constexpr uint32_t kHalf = L::kItem / 32;  // 16-byte pieces
+          const uint4* v = reinterpret_cast<const uint4*>(gbase + (v_item % L::kSlots) * L::kItem);
+          unsigned bad = 0;
+          const bool tail = first + kTile > held;  // rows past the request's keys are no values; warp 8 zeroes them
+#pragma unroll 4
+          for (uint32_t i = (lw - 1) * kHalf + lane; i < lw * kHalf; i += 32) {
+            const int row = (int)(i / (L::kGroup / 16) * 8 + i % 64 / 8);
+            const unsigned b = not_finite(v[i]);
+            bad |= tail && first + row >= held ? 0u : b;
+          }
+          const bool found = __any_sync(0xffffffffu, (bad & 0x80008000u) != 0);
+          if (lane == 0) {
+            tl.found[slot][lw - 1] = found;
+            arrive(tl.scanned[slot]);
+          }
+          ++scans;
+        };
         if (p.box) {
           if (warp == kLoadWarp) {
 #pragma unroll 1
@@ -684,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const int r = 32 * k + lane;
-                bits[k] = __ballot_sync(0xffffffffu, first + r < held && (live >> (r / p.box) & 1u));
+                bits[k] = __ballot_sync(0xffffffffu, first + r < held && (live >> (r >> p.box_shift) & 1u));
               }
               if (t + 1 < u.tiles) next = look_box(u.tile0 + t + 1);
 #pragma unroll 1
@@ -701,6 +723,9 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                             kvh * p.head_atoms, group, page, zb::smem_addr(&tl.full[slot]));
               }
             }
+          } else {
+#pragma unroll 1
+            for (int t = 0; t < u.tiles; ++t, item += 2) look_through(t, item + 1);
           }
         } else {
           int pages[4];
@@ -737,6 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                 arrive(tl.full[slot]);
               }
             }
+            look_through(t, item - 1);
           }
         }
       }
@@ -765,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     constexpr uint32_t kIdS = tc::idesc_bf16(kStreamRows, kTile);
     constexpr uint32_t kIdO = tc::idesc_bf16(kStreamRows, HD, false, /*b_mn=*/true);
-    int item = 0, q_item = 0, tiles_done[2] = {0, 0};
+    int item = 0, q_item = 0, scans = 0, tiles_done[2] = {0, 0};
     auto full = [&](int i) { wait(tl.full[i % L::kSlots], (i / L::kSlots) & 1, abort, p.status); };
     auto commit = [&](const uint64_t& bar) {
       if (elect()) tc::commit(zb::smem_addr(&bar));
@@ -842,15 +868,11 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           tc::fence_proxy_async();
           __syncwarp();
         }
-        if (first + kTile > u.all_hi || first < u.all_lo) {  // keys that some rows see and others do not
-          bool bad = false;
-#pragma unroll 4
-          for (uint32_t i = lane; i < L::kItem / 16; i += 32) bad |= not_finite(reinterpret_cast<const uint4*>(v_tile)[i]);
-          found = __any_sync(0xffffffffu, bad);
-          if (lane == 0) {
-            tl.found = found;
-            arrive(tl.scanned);
-          }
+        if (mixed_tile(u, first)) {
+          const int slot = scans % kMasks;
+          wait(tl.scanned[slot], (scans / kMasks) & 1, abort, p.status);
+          ++scans;
+          found = (tl.found[slot][0] | tl.found[slot][1]) != 0;
           if (found) {  // every stream adds what it sees before it hands over P; then the values are zeroed
 #pragma unroll 1
             for (int s = s0; s <= s1; ++s) wait(tl.p_full[s], tiles_done[s] & 1, abort, p.status);
@@ -924,7 +946,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll 1
         for (int t = 0; t < u.tiles; ++t) {
           const int first = (u.tile0 + t) * kTile;
-          const bool scan = first + kTile > u.all_hi || first < u.all_lo;
+          const bool scan = mixed_tile(u, first);
           if (!two && (t & 1) != s) {  // the other half's tile
             scans += scan;
             continue;
@@ -940,110 +962,146 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             continue;
           }
           tc::fence_after();
-          uint32_t x[kTile];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) ld32(col_s + 32 * c, x + 32 * c);
-          const uint4 there = *reinterpret_cast<const uint4*>(tl.mask[(tile_no + t) % kMasks]);
-          unsigned seen[4] = {there.x, there.y, there.z, there.w};
+          const unsigned* there = tl.mask[(tile_no + t) % kMasks];
+          const uint4 all4 = *reinterpret_cast<const uint4*>(there);
           const bool partly = __any_sync(0xffffffffu, first < lo || first + kTile > hi ||
-                                                          (there.x & there.y & there.z & there.w) != 0xffffffffu);
-          tc::ld_wait();
-          if (partly) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int a = min(max(lo - first - 32 * c, 0), 32), z = min(max(hi - first - 32 * c, 0), 32);
-              const unsigned below = z >= 32 ? 0xffffffffu : (1u << z) - 1u;
-              const unsigned under = a >= 32 ? 0xffffffffu : (1u << a) - 1u;
-              seen[c] &= below & ~under;
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                if (!((seen[c] >> j) & 1u)) x[32 * c + j] = __float_as_uint(-INFINITY);
-            }
-          }
-          float top;
-          {
-            float part[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              part[j] = fmaxf(__uint_as_float(x[j]), __uint_as_float(x[4 + j]));
-#pragma unroll
-              for (int i = 8; i < kTile; i += 8)
-                part[j] = fmaxf(fmaxf(part[j], __uint_as_float(x[i + j])), __uint_as_float(x[i + 4 + j]));
-            }
-            top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * p.scale_log2;
-          }
-          const bool grow = top > m + kRescale;
-          if (__any_sync(0xffffffffu, grow)) {
-            const float corr = grow ? ex2(m - top) : 1.f;  // 0 for the row's first key
-            if (grow) m = top;
-            l *= corr;
-            if (t >= stride) {
+                                                          (all4.x & all4.y & all4.z & all4.w) != 0xffffffffu);
+          auto seen = [&](int c) {  // which of keys 32 c .. of the tile the row sees
+            const int a = min(max(lo - first - 32 * c, 0), 32), z = min(max(hi - first - 32 * c, 0), 32);
+            const unsigned below = z >= 32 ? 0xffffffffu : (1u << z) - 1u;
+            const unsigned under = a >= 32 ? 0xffffffffu : (1u << a) - 1u;
+            return there[c] & below & ~under;
+          };
+          const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
+          uint64_t minus, sum2[2] = {0, 0};
+          // Takes the tile's largest score: the maximum follows it, and the sum and the accumulator with it, if it has grown
+          // too far for any row of the warp.
+          auto follow = [&](float top) {
+            top *= p.scale_log2;
+            const bool grow = top > m + kRescale;
+            if (__any_sync(0xffffffffu, grow)) {
+              const float corr = grow ? ex2(m - top) : 1.f;  // 0 for the row's first key
+              if (grow) m = top;
+              l *= corr;
+              if (t >= stride) {
 #pragma unroll 1
-              for (int c = 0; c < HD / 16; ++c) {
-                uint32_t o[16];
-                tc::ld16(col_o + 16 * c, o);
-                tc::ld_wait();
+                for (int c = 0; c < HD / 16; ++c) {
+                  uint32_t o[16];
+                  tc::ld16(col_o + 16 * c, o);
+                  tc::ld_wait();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-                tc::st16(col_o + 16 * c, o);
+                  for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                  tc::st16(col_o + 16 * c, o);
+                }
               }
             }
-          }
-          const float mb = m == -INFINITY ? 0.f : m;
-          const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2), minus = pack2(-mb, -mb);
-          uint64_t sum2[2] = {0, 0};
+            const float mb = m == -INFINITY ? 0.f : m;
+            minus = pack2(-mb, -mb);
+          };
           auto hand_over = [&](const uint64_t& bar) {
             tc::st_wait();
             tc::fence_before();
             __syncwarp();
             if (lane == 0) arrive(bar);
           };
-          // p of a half of the keys. The exponential unit takes 8 cycles an instruction, so everything else has to run in
-          // its shadow: the scaling of the next group, and the sum and the packing of the one before, are written between
-          // a group's exponentials.
-          auto weigh = [&](int half) {
-            constexpr int kPairs = 4, kGroups = kTile / 4 / kPairs;
-            uint32_t packed[32];
-            uint64_t a2[kPairs];
-            float e[2][2 * kPairs];
-            auto scaled = [&](int g, int i) {
-              const int k = 64 * half + 2 * (g * kPairs + i);
-              return fma2(pack2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), scale2, minus);
-            };
+          if (partly) {  // 32 keys at a time, without those that no row of the warp sees
+            float top = -INFINITY;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              const unsigned word = seen(c);
+              if (!__any_sync(0xffffffffu, word != 0)) continue;
+              uint32_t y[32];
+              ld32(col_s + 32 * c, y);
+              tc::ld_wait();
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i) a2[i] = scaled(0, i);
+              for (int j = 0; j < 32; ++j) top = (word >> j) & 1u ? fmaxf(top, __uint_as_float(y[j])) : top;
+            }
+            follow(top);
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              const unsigned word = seen(c);
+              uint32_t packed[16] = {};
+              if (__any_sync(0xffffffffu, word != 0)) {
+                uint32_t y[32];
+                ld32(col_s + 32 * c, y);
+                tc::ld_wait();
 #pragma unroll
-            for (int g = 0; g <= kGroups; ++g) {
-#pragma unroll
-              for (int i = 0; i < kPairs; ++i) {
-                if (g < kGroups) {
+                for (int j = 0; j < 16; ++j) {
                   float a, z;
-                  unpack2(a2[i], a, z);
-                  e[g % 2][2 * i] = ex2(a);
-                  e[g % 2][2 * i + 1] = ex2(z);
-                  if (g + 1 < kGroups) a2[i] = scaled(g + 1, i);
-                }
-                if (g > 0) {
-                  const float a = e[(g + 1) % 2][2 * i], z = e[(g + 1) % 2][2 * i + 1];
-                  sum2[i % 2] = add2(sum2[i % 2], pack2(a, z));
-                  packed[(g - 1) * kPairs + i] = to_bf16x2(a, z);
+                  unpack2(fma2(pack2(__uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1])), scale2, minus), a, z);
+                  a = (word >> (2 * j)) & 1u ? ex2(a) : 0.f;
+                  z = (word >> (2 * j + 1)) & 1u ? ex2(z) : 0.f;
+                  sum2[j % 2] = add2(sum2[j % 2], pack2(a, z));
+                  packed[j] = to_bf16x2(a, z);
                 }
               }
+              tc::st16(col_s + 16 * c, packed);
+              if (c == 1 && !scan) hand_over(tl.p_half[s]);
             }
-            st32(col_s + 32 * half, packed);
-          };
-          weigh(0);
-          if (!scan) hand_over(tl.p_half[s]);
-          weigh(1);
+          } else {
+            uint32_t x[kTile];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) ld32(col_s + 32 * c, x + 32 * c);
+            tc::ld_wait();
+            {
+              float part[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                part[j] = fmaxf(__uint_as_float(x[j]), __uint_as_float(x[4 + j]));
+#pragma unroll
+                for (int i = 8; i < kTile; i += 8)
+                  part[j] = fmaxf(fmaxf(part[j], __uint_as_float(x[i + j])), __uint_as_float(x[i + 4 + j]));
+              }
+              follow(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
+            }
+            // p of a half of the keys. The exponential unit takes 8 cycles an instruction, so everything else has to run in
+            // its shadow: the scaling of the next group, and the sum and the packing of the one before, are written between
+            // a group's exponentials.
+            auto weigh = [&](int half) {
+              constexpr int kPairs = 4, kGroups = kTile / 4 / kPairs;
+              uint32_t packed[32];
+              uint64_t a2[kPairs];
+              float e[2][2 * kPairs];
+              auto scaled = [&](int g, int i) {
+                const int k = 64 * half + 2 * (g * kPairs + i);
+                return fma2(pack2(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), scale2, minus);
+              };
+#pragma unroll
+              for (int i = 0; i < kPairs; ++i) a2[i] = scaled(0, i);
+#pragma unroll
+              for (int g = 0; g <= kGroups; ++g) {
+#pragma unroll
+                for (int i = 0; i < kPairs; ++i) {
+                  if (g < kGroups) {
+                    float a, z;
+                    unpack2(a2[i], a, z);
+                    e[g % 2][2 * i] = ex2(a);
+                    e[g % 2][2 * i + 1] = ex2(z);
+                    if (g + 1 < kGroups) a2[i] = scaled(g + 1, i);
+                  }
+                  if (g > 0) {
+                    const float a = e[(g + 1) % 2][2 * i], z = e[(g + 1) % 2][2 * i + 1];
+                    sum2[i % 2] = add2(sum2[i % 2], pack2(a, z));
+                    packed[(g - 1) * kPairs + i] = to_bf16x2(a, z);
+                  }
+                }
+              }
+              st32(col_s + 32 * half, packed);
+            };
+            weigh(0);
+            if (!scan) hand_over(tl.p_half[s]);
+            weigh(1);
+          }
           {
             float a, z;
             unpack2(add2(sum2[0], sum2[1]), a, z);
             l += a + z;
           }
           if (scan) {
-            wait(tl.scanned, scans & 1, abort, p.status);
+            const int slot = scans % kMasks;
+            wait(tl.scanned[slot], (scans / kMasks) & 1, abort, p.status);
             ++scans;
-            if (*reinterpret_cast<volatile int*>(&tl.found)) {  // values that are not finite, one by one
+            if (tl.found[slot][0] | tl.found[slot][1]) {  // values that are not finite, one by one
               if (t < stride) {  // the tile's product adds to the accumulator then
                 uint32_t zero[32] = {};
 #pragma unroll
@@ -1053,12 +1111,11 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               const unsigned char* v = gbase + (size_t)((2 * (tile_no + t) + 1) % L::kSlots) * L::kItem;
 #pragma unroll 1
               for (int j = 0; j < kTile; ++j) {
-                const unsigned word = j < 32 ? seen[0] : j < 64 ? seen[1] : j < 96 ? seen[2] : seen[3];
-                const bool sees = (word >> (j % 32)) & 1u;
+                const bool sees = (seen(j / 32) >> (j % 32)) & 1u;
 #pragma unroll 1
                 for (int c = 0; c < HD / 8; ++c) {
                   const uint4 w = *reinterpret_cast<const uint4*>(v + piece<HD>(j, c));
-                  if (!not_finite(w)) continue;  // the same for every lane
+                  if (!(not_finite(w) & 0x80008000u)) continue;  // the same for every lane
                   const uint32_t q[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                   for (int e = 0; e < 8; ++e) {
@@ -1175,7 +1232,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               const int e = 2 * (4 * (j / 2 % 4) + 2 * (j / 8) + j % 2);
               w[j] = l == 0.f ? 0u : to_bf16x2(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
             }
-            tc::st16(col_o + 32 * c0 + 16 * (c - c0), w);
+            tc::st16(col_o + 16 * (c0 + c), w);
           } else if (live) {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -1191,13 +1248,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           int64_t rows4[4];  // the rows this lane stores: lane / 4 and every 8th
 #pragma unroll
           for (int k = 0; k < 4; ++k) rows4[k] = __shfl_sync(0xffffffffu, row, 8 * k + lane / 4);
-#pragma unroll
-          for (int i = 0; i < HD / 32; ++i) {
-            const int c = c0 + i, dim = 32 * c + 8 * (lane % 4);
-            if (c >= c1) break;
+#pragma unroll 1
+          for (int c = c0; c < c1; ++c) {
+            const int dim = 32 * c + 8 * (lane % 4);
             uint32_t w[2][8];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) ld_across(col_o + 32 * c0 + 16 * i + ((uint32_t)(16 * k) << 16), w[k]);
+            for (int k = 0; k < 2; ++k) ld_across(col_o + 16 * (c0 + c) + ((uint32_t)(16 * k) << 16), w[k]);
             tc::ld_wait();
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -1313,6 +1369,7 @@ int make_maps(ChunkParams& p, Maps& maps) {
   if (int rc = encode(&maps.k, 5, c.k, dims, strides, boxes)) return rc;
   if (int rc = encode(&maps.v, 5, c.v, dims, strides, boxes)) return rc;
   p.box = box;
+  p.box_shift = __builtin_ctz((unsigned)box);
   p.head_atoms = beside ? HD / 64 : 0;
   p.page_heads = beside ? 1 : c.Hkv;
   return zb::kOk;
