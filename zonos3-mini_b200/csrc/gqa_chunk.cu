@@ -934,14 +934,15 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const int first_row = two ? s * stream_rows : 0, rows = min(stream_rows, u.rows - first_row);
       const bool idle = 32 * (warp % 4) >= rows;  // no lane of the warp has a row
       const int stride = two ? 1 : 2;
-      float m = -INFINITY, l = 0.f, gate = 1.f;
+      float m = -INFINITY, l = 0.f;
+      __nv_bfloat16 gate_raw = __float2bfloat16_rn(0.f);  // on its way while the tiles are worked on
       {
         int lo = 0, hi = INT32_MAX;  // a lane without a row sees everything; it is not stored
         if (32 * (warp % 4) + lane < rows)
           visible(p, u.keys, u.pos0 + p.by_group.quotient(first_row + 32 * (warp % 4) + lane), lo, hi);
         if (p.gate && u.mode != kPart0 && 32 * (warp % 4) + lane < rows) {
           const int r = first_row + 32 * (warp % 4) + lane;
-          gate = sigmoid(p.gate[(int64_t)(u.token0 + p.by_group.quotient(r)) * p.gate_stride + u.kvh * G + p.by_group.rest(r)]);
+          gate_raw = p.gate[(int64_t)(u.token0 + p.by_group.quotient(r)) * p.gate_stride + u.kvh * G + p.by_group.rest(r)];
         }
 #pragma unroll 1
         for (int t = 0; t < u.tiles; ++t) {
@@ -1185,7 +1186,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       }
       const bool done = u.mode == kFinal || adds;  // the row's output is formed here
       if ((two || s == 0 || u.tiles > 1) && !gave_up(abort)) {
-        const float f = l == 0.f ? 0.f : gate / l;  // 0 for a row that saw no key; a NaN sum stays NaN
+        const float f = l == 0.f ? 0.f : (p.gate ? sigmoid(gate_raw) : 1.f) / l;  // 0 for a row that saw no key; a NaN sum stays NaN
         const int64_t part = (int64_t)cta * 2 + (u.mode == kPart1);
         float* acc = p.acc + part * HD * p.rows_max;
         auto chunk = [&](int c) {  // 32 dims of the row's accumulator
