@@ -6,8 +6,10 @@
 //   q, k:  pair j of the first `rotary` elements turns by position * theta^(-2j / rotary); the pair is (2j, 2j + 1)
 //          (interleaved) or (j, j + rotary / 2)
 // q goes to q_out, k and v to the token's row of its request's pages. Everything is fp32 with one rounding to bf16 at
-// the end; the angle is formed in fp64 as a fraction of a turn, so that it is as good at position 10^6 as at 10 (in
-// fp32 the product position * frequency would lose a bit of the angle with every doubling of the position).
+// the end. The angle is formed as a fraction of a turn in 64-bit fixed point (position times the frequency's fraction,
+// whole turns dropping out of the top), so that it is as good at position 10^6 as at 10: in fp32 the product would lose
+// a bit of the angle with every doubling of the position. Its sine and cosine are the fast ones, within 2^-20 on
+// [-pi, pi]; the result keeps 8 bits.
 //
 // Each element is read once and written once, so the kernel is bound by HBM; a call of a few tokens is bound by its
 // latency: the token's request and page come from dependent loads (cu, keys, page table), which run while the
@@ -20,7 +22,7 @@
 
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kMaxPairs = 64;
 
 struct AppendParams {
@@ -34,7 +36,8 @@ struct AppendParams {
   float eps;
   int normalize, interleaved, rotary, Hq;
   int shares;              // warps of a token
-  double turns[kMaxPairs];  // theta^(-2j / rotary) / (2 pi)
+  float inv_hd;
+  uint64_t turns[kMaxPairs];  // the fraction of theta^(-2j / rotary) / (2 pi), times 2^64
 };
 
 // 8 consecutive elements from an address aligned to ALIGN bytes.
@@ -117,9 +120,8 @@ __global__ void __launch_bounds__(kWarps * 32) gqa_append_kernel(const __grid_co
     const int e = gl * 8 + i;
     const int pair = p.interleaved ? e / 2 : (upper ? e - half : e);
     if ((p.interleaved && i % 2) || !turned) continue;
-    double turn = (double)at * p.turns[pair];
-    turn -= rint(turn);
-    sincospif(2.f * (float)turn, &sn[i], &cs[i]);
+    const int turn = (int)(((uint64_t)(int64_t)at * p.turns[pair]) >> 32);  // of 2^32
+    __sincosf((float)turn * 1.4629180792671596e-9f, &sn[i], &cs[i]);          // 2 pi / 2^32
   }
 
   for (int h0 = first; h0 < heads + lane / GL; h0 += kBatch * step) {  // every lane of the warp takes the same turns
@@ -128,24 +130,25 @@ __global__ void __launch_bounds__(kWarps * 32) gqa_append_kernel(const __grid_co
     for (int i = 0; i < kBatch; ++i) {
       const int h = h0 + i * step;
       if (h - lane / GL >= heads) break;  // warp-uniform
-      float x[8];
-      widen(raw[i], x);
       const bool is_v = h >= p.Hq + p.kv.Hkv, is_q = h < p.Hq;
+      if (h - lane / GL >= p.Hq + p.kv.Hkv) {  // values only, for the whole warp: a copy
+        if (carries && h < heads && slot >= 0)
+          *reinterpret_cast<uint4*>(p.kv.v + slot + (int64_t)(h - p.Hq - p.kv.Hkv) * p.kv.head_stride + gl * 8) = raw[i];
+        continue;
+      }
+      float x[8], factor = 1.f;
+      widen(raw[i], x);
       if (p.normalize) {
         float ss = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
 #pragma unroll
         for (int o = GL / 2; o > 0; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float r = rsqrtf(ss / (float)hd + p.eps);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= r;
+        factor = rsqrtf(fmaf(ss, p.inv_hd, p.eps));
       }
-      if (is_q && p.temp) {
-        const float tq = fabsf(__bfloat162float(p.temp[h]));
+      if (is_q && p.temp) factor *= fabsf(__bfloat162float(p.temp[h]));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= tq;
-      }
+      for (int j = 0; j < 8; ++j) x[j] *= factor;
       if (p.interleaved) {
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
@@ -221,12 +224,16 @@ ZB_API int zb_gqa_append(const uint16_t* proj, int64_t proj_stride, const uint16
   p.interleaved = interleaved;
   p.rotary = rotary_dim;
   p.Hq = Hq;
+  p.inv_hd = 1.f / (float)hd;
   // the pairs' frequencies in turns a position, kept per thread for the next call with the same theta and width
-  thread_local double theta = 0, turns[kMaxPairs];
+  thread_local double theta = 0;
+  thread_local uint64_t turns[kMaxPairs];
   thread_local int width = 0;
   if (theta != rope_theta || width != rotary_dim) {
-    for (int j = 0; j < rotary_dim / 2; ++j)
-      turns[j] = std::pow(rope_theta, -2.0 * j / rotary_dim) / 6.283185307179586476925;
+    for (int j = 0; j < rotary_dim / 2; ++j) {
+      const double turn = std::pow(rope_theta, -2.0 * j / rotary_dim) / 6.283185307179586476925;
+      turns[j] = (uint64_t)std::ldexp(turn - std::floor(turn), 64);
+    }
     theta = rope_theta;
     width = rotary_dim;
   }
