@@ -13,8 +13,14 @@ forward(x [N, D] bf16) reads ``get_global_ctx().batch.attn_metadata`` and ``get_
     prefill: the same prologue in torch, zb_kv_store, causal softmax attention per request in torch
     y = (o * sigmoid(gate)) @ wo^T                          (cuBLAS; decode: the gate already applied)
 
-The prefill attention is plain torch: the north_star path is the decode step, and the reference runs its prefill
-attention through flash_attn_varlen_func (fa.py), a library kernel this package does not replace.
+A batch whose ``cu_seqlens_q`` is a device tensor instead of a host list runs the paged operators, whatever its requests
+bring (prompts, chunks of prompts, single tokens), over a ``SlotKVPool`` or a ``PagedKVPool``:
+
+    q = zb_gqa_append(p)                                    (q / k RMSNorm, q x |temp|, rotary embedding, k and v into
+                                                             the pages of their requests)
+    o = zb_gqa_chunk(q, caches, page_table, gate)           (causal attention over the pages, the gate in its store)
+
+The host reads no length there, so such a forward neither waits for the device nor loops over requests.
 """
 
 from __future__ import annotations
@@ -40,6 +46,26 @@ class SlotKVPool:
         self.k_buffer = torch.zeros(shape, device=device, dtype=dtype)
         self.v_buffer = torch.zeros(shape, device=device, dtype=dtype)
         self.slots = slots
+
+    def k(self, layer_id: int) -> torch.Tensor:
+        return self.k_buffer[self._index[layer_id]]
+
+    def v(self, layer_id: int) -> torch.Tensor:
+        return self.v_buffer[self._index[layer_id]]
+
+
+class PagedKVPool:
+    """K and V caches of every global-attention layer in pages of ``page_size`` tokens: ``[pages, page_size, kv_heads,
+    head_dim]`` bf16 each. A request's key position j lies in row j % page_size of page ``page_table[b, j // page_size]``.
+    Read and written by the paged operators (batches whose ``cu_seqlens_q`` is a device tensor)."""
+
+    def __init__(self, layer_ids, pages: int, page_size: int, kv_heads: int, head_dim: int, device, dtype=torch.bfloat16):
+        self.layer_ids = list(layer_ids)
+        self._index = {layer: i for i, layer in enumerate(self.layer_ids)}
+        shape = (len(self.layer_ids), pages, page_size, kv_heads, head_dim)
+        self.k_buffer = torch.zeros(shape, device=device, dtype=dtype)
+        self.v_buffer = torch.zeros(shape, device=device, dtype=dtype)
+        self.pages, self.page_size = pages, page_size
 
     def k(self, layer_id: int) -> torch.Tensor:
         return self.k_buffer[self._index[layer_id]]
@@ -99,7 +125,14 @@ class Attention(BaseOP):
         kc, vc = pool.k(self._layer_id), pool.v(self._layer_id)
         p = F.linear(x, self._proj)  # q | k | v | gate
         gate = p[:, (H + 2 * Hkv) * hd:]
-        if batch.is_decode:  # the output gate rides in the attention kernel's store
+        if isinstance(meta.cu_seqlens_q, torch.Tensor):  # a ragged batch described on the device
+            paged = (kc, vc, meta.page_table, meta.cache_seqlens, meta.cu_seqlens_q)
+            q = ops.gqa_append(p, *paged, heads=H, kv_heads=Hkv, temp=self._temp, eps=QK_NORM_EPS, rope_theta=self._theta,
+                               positions=meta.positions)
+            o = ops.gqa_chunk(q, *paged, softmax_scale=hd ** -0.5, gate=gate)
+        elif kc.dim() != 3:
+            raise RuntimeError("a paged KV pool needs attn_metadata.cu_seqlens_q as a device tensor")
+        elif batch.is_decode:  # the output gate rides in the attention kernel's store
             q = ops.gqa_prologue_decode(p, self._temp, meta.positions, kc, vc, meta.out_loc, heads=H, kv_heads=Hkv,
                                         rope_theta=self._theta, eps=QK_NORM_EPS)
             o = ops.gqa_decode(q, kc, vc, meta.page_table, meta.cache_seqlens, softmax_scale=hd ** -0.5, gate=gate)

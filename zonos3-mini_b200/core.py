@@ -30,13 +30,18 @@ class Req:
 class AttnMetadata:
     """Where the global-attention layers read and write the KV cache (page size 1, the FA backend's layout,
     servers/sgl/src/zonos3_sgl/attention/fa.py): every new row t has a position and a cache slot; request b reads
-    keys page_table[b, :cache_seqlens[b]] (its new rows included)."""
+    keys page_table[b, :cache_seqlens[b]] (its new rows included).
 
-    positions: "torch.Tensor"  # [N] int32
-    out_loc: "torch.Tensor"  # [N] int32
+    With ``cu_seqlens_q`` as a [B + 1] int32 device tensor the layers run the paged operators: ``page_table`` then holds
+    pages of the pool's page size, a new row's slot and rotary position follow from the lengths, and ``positions`` (else
+    None) overrides the latter; ``out_loc`` is not read."""
+
+    positions: "torch.Tensor | None"  # [N] int32
+    out_loc: "torch.Tensor | None"  # [N] int32
     page_table: "torch.Tensor"  # [B, max_len] int32
     cache_seqlens: "torch.Tensor"  # [B] int32
-    cu_seqlens_q: list[int] | None = None  # prefill: request b's new rows are [cu[b], cu[b+1])
+    # request b's new rows are [cu[b], cu[b+1]): a host list for a prefill, or a device tensor for any batch
+    cu_seqlens_q: "list[int] | torch.Tensor | None" = None
 
 
 @dataclass

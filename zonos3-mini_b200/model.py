@@ -27,7 +27,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib, ops
-from .attention import Attention, SlotKVPool
+from .attention import Attention, PagedKVPool, SlotKVPool
 from .attnres import FusedBlockAttnResContext, forward_layers_full
 from .base import BaseOP, OPList, Weight
 from .core import AttnMetadata, Batch, Req, forward_batch, get_global_ctx
@@ -126,11 +126,15 @@ class Zonos3ForCausalLM(BaseOP):
         """Columns of the padded head output (the logits row stride)."""
         return (self.n_codebooks * self.audio_vocab + 7) // 8 * 8
 
-    def allocate_caches(self, capacity: int, kv_slots: int, device) -> SlotKVPool:
-        """Per-slot DeltaNet state pools of ``capacity`` streams and the KV pool of ``kv_slots`` token slots."""
+    def allocate_caches(self, capacity: int, kv_slots: int, device, page_size: int | None = None):
+        """Per-slot DeltaNet state pools of ``capacity`` streams and the KV pool: a ``SlotKVPool`` of ``kv_slots`` token
+        slots, or with ``page_size`` a ``PagedKVPool`` of as many tokens in pages."""
         for gdn in self.gdn_layers():
             gdn.allocate_cache(capacity, device, torch.bfloat16)
         c = self._config
+        if page_size is not None:
+            return PagedKVPool(self.attention_layer_ids(), -(-kv_slots // page_size), page_size, c.num_kv_heads, c.head_dim,
+                               device)
         return SlotKVPool(self.attention_layer_ids(), kv_slots, c.num_kv_heads, c.head_dim, device)
 
     # ------------------------------------------------------------------ forward pieces (zonos3.py:1159-1360)
