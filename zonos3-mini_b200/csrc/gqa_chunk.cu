@@ -572,26 +572,25 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     constexpr int kCopies = kTile / kPass;   // instructions of a tile
     const int chunk = lane % kChunks, sub = lane / kChunks;
     const bool carries = chunk * 8 < hd;
-    // Rows 32 k + l of a tile are at element offset off[k] of lane l (negative: absent, zeros). `warps` warps share the
-    // tile, this one the `which`-th; the addresses of 4 copies are formed before they are issued, as each copy takes
-    // its row's offset from another lane.
-    auto copy_tile = [&](uint32_t dst, const __nv_bfloat16* src, const int64_t (&off)[4], int which, int warps) {
-      constexpr int kAhead = 4;
+    // Rows 32 k + l of a tile are at element offset off[k] of lane l (negative: absent, zeros). The three warps take 32
+    // rows each and share the last 32. The addresses of kAhead copies are formed before they are issued, as each copy
+    // takes its row's offset from another lane.
+    constexpr int kAhead = 4, kGroups = kCopies / 4 / kAhead;  // groups of copies of 32 rows
+    auto copy_group = [&](uint32_t dst, const __nv_bfloat16* src, int64_t off, int row0, int g) {
+      int64_t o[kAhead];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        constexpr int kPart = kCopies / 4;
+      for (int i = 0; i < kAhead; ++i) o[i] = __shfl_sync(0xffffffffu, off, (g * kAhead + i) * kPass + sub);
+      if (!carries) return;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        cp_async16(dst + piece<HD>(row0 + (g * kAhead + i) * kPass + sub, chunk), src + (o[i] < 0 ? 0 : o[i]) + chunk * 8, o[i] >= 0);
+    };
+    auto copy_tile = [&](uint32_t dst, const __nv_bfloat16* src, const int64_t (&off)[4], int turn) {
+      const int64_t own = lw == 0 ? off[0] : lw == 1 ? off[1] : off[2];
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) copy_group(dst, src, own, 32 * lw, g);
 #pragma unroll 1
-        for (int g = 0; g < kPart; g += kAhead) {
-          if ((k * (kPart / kAhead) + g / kAhead) % warps != which) continue;
-          int64_t o[kAhead];
-#pragma unroll
-          for (int i = 0; i < kAhead; ++i) o[i] = __shfl_sync(0xffffffffu, off[k], (g + i) * kPass + sub);
-          if (!carries) continue;
-#pragma unroll
-          for (int i = 0; i < kAhead; ++i)
-            cp_async16(dst + piece<HD>(32 * k + (g + i) * kPass + sub, chunk), src + (o[i] < 0 ? 0 : o[i]) + chunk * 8, o[i] >= 0);
-        }
-      }
+      for (int g = (lw + turn) % kLoadWarps; g < kGroups; g += kLoadWarps) copy_group(dst, src, off[3], 96, g);
     };
     // this lane's request of the window of 32 requests around the current one
     int window0 = -1;
@@ -755,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             for (int kv = 0; kv < 2; ++kv, ++item) {
               const int slot = item % L::kSlots;
               if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort, p.status);
-              copy_tile(base + slot * L::kItem, kv ? p.kv.v : p.kv.k, off, lw, kLoadWarps);
+              copy_tile(base + slot * L::kItem, kv ? p.kv.v : p.kv.k, off, item);
               cp_async_arrive(zb::smem_addr(&tl.full[slot]));
               if (warp == kLoadWarp && lane == 0) {
                 if (kv == 0) *reinterpret_cast<uint4*>(tl.mask[tile_no % kMasks]) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
