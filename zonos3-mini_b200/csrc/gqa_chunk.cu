@@ -12,8 +12,10 @@
 // stream and tile: S = Q K^T (tcgen05, fp32 in tensor memory); a thread takes a row, finds its maximum, forms p = 2^(s
 // scale log2 e - m), adds up its sum in fp32 and writes p back over S as bf16; O += P V with P read from tensor memory.
 // The two streams share each tile's K and V in shared memory and take turns: one's exponentials run while the tensor
-// cores work for the other. The subtracted maximum m only follows the true one when that has grown by more than 8 (in
-// log2): the stale one keeps p <= 2^8 and cancels in the final division, so the accumulator is hardly ever rescaled.
+// cores work for the other. The subtracted m cancels in the final division, so it need not be the maximum: it starts at 0
+// and only moves to the largest score of a tile that is more than 64 above it (or, for a row's first keys, below), which
+// keeps p within 2^64, sums and accumulators far inside fp32's range, and the largest weights' precision. So the search for
+// the maximum runs beside the exponentials instead of before them, and the accumulator is hardly ever rescaled.
 // p is rounded to bf16 because the tensor cores multiply bf16; its sum is kept from before the rounding.
 //
 // The lengths live on the device, so the split of the work does too: every CTA adds up the tiles of all units (a scan
@@ -46,7 +48,7 @@ constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
 constexpr int kMaxSlots = 10, kDescs = 4;
 constexpr int kMasks = 8;  // of key masks and of looked-through tiles: the loaders run at most 5 tiles ahead of the rows
-constexpr float kRescale = 8.f;  // log2 growth of a row's maximum that the accumulator is rescaled for
+constexpr float kRescale = 64.f;  // how far (log2) a row's largest score may be from the m that is subtracted
 constexpr int kMaxRequests = 16384;
 
 // n / d and n % d for 0 <= n < 2^31 by a multiplication: m = ceil(2^(31 + l) / d) with 2^l >= d.
@@ -933,7 +935,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const int first_row = two ? s * stream_rows : 0, rows = min(stream_rows, u.rows - first_row);
       const bool idle = 32 * (warp % 4) >= rows;  // no lane of the warp has a row
       const int stride = two ? 1 : 2;
-      float m = -INFINITY, l = 0.f;
+      float m = 0.f, l = 0.f;  // scores are first held against 0
       __nv_bfloat16 gate_raw = __float2bfloat16_rn(0.f);  // on its way while the tiles are worked on
       {
         int lo = 0, hi = INT32_MAX;  // a lane without a row sees everything; it is not stored
@@ -974,29 +976,27 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           };
           const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
           uint64_t minus, sum2[2] = {0, 0};
-          // Takes the tile's largest score: the maximum follows it, and the sum and the accumulator with it, if it has grown
-          // too far for any row of the warp.
-          auto follow = [&](float top) {
+          // Whether the weights formed with m hold for a tile whose largest score is `top` (NaN: they do); if not, m is set
+          // to it, and the sum and the accumulator follow.
+          auto holds = [&](float top) {
             top *= p.scale_log2;
-            const bool grow = top > m + kRescale;
-            if (__any_sync(0xffffffffu, grow)) {
-              const float corr = grow ? ex2(m - top) : 1.f;  // 0 for the row's first key
-              if (grow) m = top;
+            const bool off = top > m + kRescale || (l == 0.f && top < m - kRescale && top > -INFINITY);
+            if (!__any_sync(0xffffffffu, off)) return true;
+            if (t >= stride) {
+              const float corr = off && l != 0.f ? ex2(m - top) : 1.f;  // without a key so far both are 0
               l *= corr;
-              if (t >= stride) {
 #pragma unroll 1
-                for (int c = 0; c < HD / 16; ++c) {
-                  uint32_t o[16];
-                  tc::ld16(col_o + 16 * c, o);
-                  tc::ld_wait();
+              for (int c = 0; c < HD / 16; ++c) {
+                uint32_t o[16];
+                tc::ld16(col_o + 16 * c, o);
+                tc::ld_wait();
 #pragma unroll
-                  for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-                  tc::st16(col_o + 16 * c, o);
-                }
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                tc::st16(col_o + 16 * c, o);
               }
             }
-            const float mb = m == -INFINITY ? 0.f : m;
-            minus = pack2(-mb, -mb);
+            if (off) m = top;
+            return false;
           };
           auto hand_over = [&](const uint64_t& bar) {
             tc::st_wait();
@@ -1004,62 +1004,51 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             __syncwarp();
             if (lane == 0) arrive(bar);
           };
+          // The weights are formed with the m there is, and the tile's largest score is found beside them; nothing is
+          // written over the scores before it is known that they hold. A second turn is rare.
           if (partly) {  // 32 keys at a time, without those that no row of the warp sees
-            float top = -INFINITY;
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              const unsigned word = seen(c);
-              if (!__any_sync(0xffffffffu, word != 0)) continue;
-              uint32_t y[32];
-              ld32(col_s + 32 * c, y);
-              tc::ld_wait();
+            uint32_t packed[64];
+            float top;
+            do {
+              minus = pack2(-m, -m);
+              sum2[0] = sum2[1] = 0;
+              top = -INFINITY;
 #pragma unroll
-              for (int j = 0; j < 32; ++j) top = (word >> j) & 1u ? fmaxf(top, __uint_as_float(y[j])) : top;
-            }
-            follow(top);
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              const unsigned word = seen(c);
-              uint32_t packed[16] = {};
-              if (__any_sync(0xffffffffu, word != 0)) {
+              for (int c = 0; c < 4; ++c) {
+                const unsigned word = seen(c);
+                if (!__any_sync(0xffffffffu, word != 0)) {
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) packed[16 * c + j] = 0;
+                  continue;
+                }
                 uint32_t y[32];
                 ld32(col_s + 32 * c, y);
                 tc::ld_wait();
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
+                  const float s0 = (word >> (2 * j)) & 1u ? __uint_as_float(y[2 * j]) : -INFINITY;
+                  const float s1 = (word >> (2 * j + 1)) & 1u ? __uint_as_float(y[2 * j + 1]) : -INFINITY;
+                  top = fmaxf(fmaxf(top, s0), s1);
                   float a, z;
-                  unpack2(fma2(pack2(__uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1])), scale2, minus), a, z);
-                  a = (word >> (2 * j)) & 1u ? ex2(a) : 0.f;
-                  z = (word >> (2 * j + 1)) & 1u ? ex2(z) : 0.f;
+                  unpack2(fma2(pack2(s0, s1), scale2, minus), a, z);
+                  a = ex2(a);
+                  z = ex2(z);
                   sum2[j % 2] = add2(sum2[j % 2], pack2(a, z));
-                  packed[j] = to_bf16x2(a, z);
+                  packed[16 * c + j] = to_bf16x2(a, z);
                 }
               }
-              tc::st16(col_s + 16 * c, packed);
-              if (c == 1 && !scan) hand_over(tl.p_half[s]);
-            }
+            } while (!holds(top));
+            st32(col_s, packed);
+            st32(col_s + 32, packed + 32);
+            if (!scan) hand_over(tl.p_half[s]);
           } else {
             uint32_t x[kTile];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) ld32(col_s + 32 * c, x + 32 * c);
-            tc::ld_wait();
-            {
-              float part[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                part[j] = fmaxf(__uint_as_float(x[j]), __uint_as_float(x[4 + j]));
-#pragma unroll
-                for (int i = 8; i < kTile; i += 8)
-                  part[j] = fmaxf(fmaxf(part[j], __uint_as_float(x[i + j])), __uint_as_float(x[i + 4 + j]));
-              }
-              follow(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
-            }
             // p of a half of the keys. The exponential unit takes 8 cycles an instruction, so everything else has to run in
-            // its shadow: the scaling of the next group, and the sum and the packing of the one before, are written between
-            // a group's exponentials.
-            auto weigh = [&](int half) {
+            // its shadow: the scaling of the next group, the sum and the packing of the one before, and in the first half
+            // the search for the largest score are written between a group's exponentials.
+            float part[4];
+            auto weigh = [&](int half, uint32_t (&packed)[32]) {
               constexpr int kPairs = 4, kGroups = kTile / 4 / kPairs;
-              uint32_t packed[32];
               uint64_t a2[kPairs];
               float e[2][2 * kPairs];
               auto scaled = [&](int g, int i) {
@@ -1078,6 +1067,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                     e[g % 2][2 * i] = ex2(a);
                     e[g % 2][2 * i + 1] = ex2(z);
                     if (g + 1 < kGroups) a2[i] = scaled(g + 1, i);
+                    if (half == 0) {  // 4 scores to each of the group's pairs
+                      const int k = 16 * g + 4 * i;
+                      const float hi = fmaxf(__uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
+                      part[i] = g == 0 ? __uint_as_float(x[k]) : fmaxf(part[i], __uint_as_float(x[k]));
+                      part[i] = fmaxf(fmaxf(part[i], __uint_as_float(x[k + 1])), hi);
+                    }
                   }
                   if (g > 0) {
                     const float a = e[(g + 1) % 2][2 * i], z = e[(g + 1) % 2][2 * i + 1];
@@ -1086,11 +1081,20 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                   }
                 }
               }
-              st32(col_s + 32 * half, packed);
             };
-            weigh(0);
+            uint32_t packed[32];
+            do {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) ld32(col_s + 32 * c, x + 32 * c);
+              minus = pack2(-m, -m);
+              sum2[0] = sum2[1] = 0;
+              tc::ld_wait();
+              weigh(0, packed);
+            } while (!holds(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))));
+            st32(col_s, packed);
             if (!scan) hand_over(tl.p_half[s]);
-            weigh(1);
+            weigh(1, packed);
+            st32(col_s + 32, packed);
           }
           {
             float a, z;
@@ -1140,6 +1144,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         tc::fence_after();
       }
       tile_no += u.tiles;
+      if (l == 0.f) m = -INFINITY;  // no key seen: the row counts for nothing where parts are joined
       int own = 32 * (warp % 4) + lane;
       asm volatile("" : "+r"(own));  // the row is worked out here anew: kept through the tiles it would cost registers
       const bool live = own < rows;
