@@ -792,39 +792,42 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     constexpr uint32_t kIdS = tc::idesc_bf16(kStreamRows, kTile);
     constexpr uint32_t kIdO = tc::idesc_bf16(kStreamRows, HD, false, /*b_mn=*/true);
-    int item = 0, q_item = 0, scans = 0, tiles_done[2] = {0, 0};
-    auto full = [&](int i) { wait(tl.full[i % L::kSlots], (i / L::kSlots) & 1, abort, p.status); };
-    auto commit = [&](const uint64_t& bar) {
-      if (elect()) tc::commit(zb::smem_addr(&bar));
-      __syncwarp();
-    };
-    auto issue_s = [&](int s, int i, int q) {  // S_s = Q K^T of ring item i and queries q
-      full(i);
-      if (p.box == 0) tc::fence_proxy_async();  // 16-byte copies -> the tensor cores
-      if (elect()) {
-        const uint32_t kb = base + (uint32_t)(i % L::kSlots) * L::kItem, qb = base + L::kOffQ + (q % 2) * L::kItem;
-        const uint64_t kd = tc::desc_mnmajor(kb, 16, L::kGroup), qd = tc::desc_kmajor(qb);
-#pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks)
-          tc::mma(tmem + L::kColS + s * kTile, qd + ((ks / 4) * L::kQAtom + (ks % 4) * 32) / 16,
-                  kd + ((ks / 4) * 1024 + (ks % 4) * 32) / 16, kIdS, ks > 0);
-        tc::commit(zb::smem_addr(&tl.s_full[s]));
-        arrive(tl.s_full[s]);  // passes on the tile's key mask, which this thread got with the tile
+    // This warp's own time between two products is time the tensor cores stand still once their short queue is empty: ring
+    // positions are kept instead of divided out, and one lane issues a stream's products and commits in one go.
+    struct Ring {
+      int slot;
+      uint32_t phase;
+      __device__ __forceinline__ Ring after(int items) const {
+        const int to = slot + items;
+        return to >= L::kSlots ? Ring{to - L::kSlots, phase ^ 1u} : Ring{to, phase};
       }
-      __syncwarp();
     };
-    auto issue_o = [&](int s, int i, int half, bool accumulate) {  // O_s (+)= P_s V of ring item i, half of its keys
-      if (elect()) {
-        const uint32_t vb = base + (uint32_t)(i % L::kSlots) * L::kItem;
-        const uint64_t vd = tc::desc_mnmajor(vb, 1024, L::kGroup);
+    Ring at{0, 0};  // of the unit's next tile's keys; its values lie one further
+    int q_item = 0, scans = 0;
+    uint32_t parity = 0;  // bit s: of stream s's weights
+    auto full = [&](const Ring& i) { wait(tl.full[i.slot], i.phase, abort, p.status); };
+    auto commit = [&](const uint64_t& bar) { tc::commit(zb::smem_addr(&bar)); };
+    const uint64_t k_desc = tc::desc_mnmajor(base, 16, L::kGroup), v_desc = tc::desc_mnmajor(base, 1024, L::kGroup);
+    const uint64_t q_desc = tc::desc_kmajor(base + L::kOffQ);
+    // By one lane: S_s = Q K^T of a ring slot and query buffer q.
+    auto issue_s = [&](int s, int slot, int q) {
+      const uint64_t kd = k_desc + (uint32_t)slot * (L::kItem / 16), qd = q_desc + (uint32_t)(q % 2) * (L::kItem / 16);
 #pragma unroll
-        for (int k0 = 0; k0 < kTile / 32; ++k0) {
-          const int ks = k0 + half * (kTile / 32);
-          mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, vd + ks * 2 * L::kGroup / 16, kIdO,
-                 accumulate || ks > 0);
-        }
+      for (int ks = 0; ks < HD / 16; ++ks)
+        tc::mma(tmem + L::kColS + s * kTile, qd + ((ks / 4) * L::kQAtom + (ks % 4) * 32) / 16,
+                kd + ((ks / 4) * 1024 + (ks % 4) * 32) / 16, kIdS, ks > 0);
+      commit(tl.s_full[s]);
+      arrive(tl.s_full[s]);  // passes on the tile's key mask, which this thread got with the tile
+    };
+    // By one lane: O_s (+)= P_s V of a ring slot, half of its keys.
+    auto issue_o = [&](int s, int slot, int half, bool accumulate) {
+      const uint64_t vd = v_desc + (uint32_t)slot * (L::kItem / 16);
+#pragma unroll
+      for (int k0 = 0; k0 < kTile / 32; ++k0) {
+        const int ks = k0 + half * (kTile / 32);
+        mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, vd + ks * 2 * L::kGroup / 16, kIdO,
+               accumulate || ks > 0);
       }
-      __syncwarp();
     };
     for (int n = 0;; ++n) {
       const int slot = n % kDescs;
@@ -837,29 +840,36 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const int stride = two ? 1 : 2;          // tiles from one of a stream to its next
       auto wait_q = [&](int q) { wait(tl.q_full[q % 2], (q / 2) & 1, abort, p.status); };
       wait_q(q_item);
-      issue_s(0, item, q_item);
-      if (two) {
-        wait_q(q_item + 1);
-        issue_s(1, item, q_item + 1);
+      if (two) wait_q(q_item + 1);
+      full(at);
+      const bool second = !two && u.tiles > 1;  // the other half begins with the second tile
+      const Ring next = at.after(2);
+      if (second) full(next);
+      if (p.box == 0) tc::fence_proxy_async();  // 16-byte copies -> the tensor cores
+      if (elect()) {
+        issue_s(0, at.slot, q_item);
+        if (two) issue_s(1, at.slot, q_item + 1);
+        commit(tl.empty[at.slot]);
+        if (second) {
+          issue_s(1, next.slot, q_item);
+          commit(tl.empty[next.slot]);
+        }
+        if (u.tiles <= stride) {
+          commit(tl.q_empty[q_item % 2]);
+          if (two) commit(tl.q_empty[(q_item + 1) % 2]);
+        }
       }
-      commit(tl.empty[item % L::kSlots]);
-      if (!two && u.tiles > 1) {
-        issue_s(1, item + 2, q_item);
-        commit(tl.empty[(item + 2) % L::kSlots]);
-      }
-      if (u.tiles <= stride) {
-        commit(tl.q_empty[q_item % 2]);
-        if (two) commit(tl.q_empty[(q_item + 1) % 2]);
-      }
+      __syncwarp();
+      const int held = held_keys(p, u.keys);
 #pragma unroll 1
       for (int t = 0; t < u.tiles; ++t) {
         // O_s += P_s(t) V(t) as soon as P_s(t) is there, then the stream's next scores
-        const int v_item = item + 2 * t + 1, k_next = item + 2 * (t + stride);
+        const Ring v = at.after(1), k = two ? at.after(2) : at.after(2).after(2);
+        const bool more = t + stride < u.tiles, ends = t + stride == u.tiles - 1;
         const int s0 = two ? 0 : t & 1, s1 = two ? 1 : s0, first = (u.tile0 + t) * kTile;
-        unsigned char* v_tile = gbase + (v_item % L::kSlots) * L::kItem;
+        unsigned char* v_tile = gbase + v.slot * L::kItem;
         bool found = false;
-        full(v_item);
-        const int held = held_keys(p, u.keys);
+        full(v);
         // rows of the last page past the request's keys came along with a tensor copy: no key, so no value either
         if (p.box && first + kTile > held && held % p.box != 0) {
           const int r0 = held - first, r1 = (r0 + p.box - 1) / p.box * p.box;
@@ -873,10 +883,10 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           const int slot = scans % kMasks;
           wait(tl.scanned[slot], (scans / kMasks) & 1, abort, p.status);
           ++scans;
-          found = (tl.found[slot][0] | tl.found[slot][1]) != 0;
+          found = uniform(tl.found[slot][0] | tl.found[slot][1]) != 0;
           if (found) {  // every stream adds what it sees before it hands over P; then the values are zeroed
 #pragma unroll 1
-            for (int s = s0; s <= s1; ++s) wait(tl.p_full[s], tiles_done[s] & 1, abort, p.status);
+            for (int s = s0; s <= s1; ++s) wait(tl.p_full[s], (parity >> s) & 1u, abort, p.status);
             uint16_t* e = reinterpret_cast<uint16_t*>(v_tile);
 #pragma unroll 1
             for (uint32_t i = lane; i < L::kItem / 2; i += 32)
@@ -888,27 +898,39 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         if (p.box == 0) tc::fence_proxy_async();
 #pragma unroll 1
         for (int s = s0; s <= s1; ++s) {
-          wait(tl.p_half[s], tiles_done[s] & 1, abort, p.status);
+          wait(tl.p_half[s], (parity >> s) & 1u, abort, p.status);
           tc::fence_after();
-          issue_o(s, v_item, 0, t >= stride || found);
-          wait(tl.p_full[s], tiles_done[s] & 1, abort, p.status);
-          ++tiles_done[s];
+          if (elect()) issue_o(s, v.slot, 0, t >= stride || found);
+          __syncwarp();
+          wait(tl.p_full[s], (parity >> s) & 1u, abort, p.status);
           tc::fence_after();
-          issue_o(s, v_item, 1, true);
-          if (t + stride >= u.tiles) commit(tl.o_full[s]);
-          if (s == s1) commit(tl.empty[v_item % L::kSlots]);
-          if (t + stride < u.tiles) {
-            const int q = q_item + (two ? s : 0);
-            issue_s(s, k_next, q);
-            if (s == s1) commit(tl.empty[k_next % L::kSlots]);
-            if (t + stride == u.tiles - 1) commit(tl.q_empty[q % 2]);
+          if (elect()) {
+            issue_o(s, v.slot, 1, true);
+            if (s == s1) commit(tl.empty[v.slot]);
+            if (!more) commit(tl.o_full[s]);
           }
+          __syncwarp();
+          if (more) {
+            if (s == s0) {
+              full(k);
+              if (p.box == 0) tc::fence_proxy_async();
+            }
+            if (elect()) {
+              const int q = q_item + (two ? s : 0);
+              issue_s(s, k.slot, q);
+              if (s == s1) commit(tl.empty[k.slot]);
+              if (ends) commit(tl.q_empty[q % 2]);
+            }
+            __syncwarp();
+          }
+          parity ^= 1u << s;
         }
+        at = at.after(2);
       }
-      item += 2 * u.tiles;
       q_item += two ? 2 : 1;
     }
-    commit(tl.drained);  // nothing is in flight when the tensor memory is given back, also after a wait that gave up
+    if (elect()) commit(tl.drained);  // nothing is in flight when the tensor memory is given back, also after a wait that
+    __syncwarp();                     // gave up
     zb::mbar_wait_bounded(zb::smem_addr(&tl.drained), 0, p.status, zb::kStatusAttnChunkTimeout);
     __syncwarp();
   } else {
