@@ -327,7 +327,7 @@ int zb_gqa_prologue_decode(const uint16_t* proj, int64_t proj_stride, const uint
  *   page_table   [B, table_stride] int32 with max_pages columns: position j lives in row j % page_size of page
  *                page_table[b, j / page_size]; a page outside [0, num_pages) or past the columns holds no keys
  *   k_cache, v_cache bf16: page p, row r, KV head g at p * page_stride + r * slot_stride + g * head_stride elements, hd
- *                contiguous elements each; strides multiples of 8, bases 16-byte aligned. page_size * max_pages at most 2^29.
+ *                contiguous elements each; strides multiples of 8, bases 16-byte aligned. page_size * max_pages at most 2^26.
  *   hd a multiple of 8, 8 .. 128 (else status 3).
  *
  * zb_gqa_append: from projection rows proj [N, Hq*hd | Hkv*hd | Hkv*hd | ...] bf16 (q | k | v, any row stride): q and k rows

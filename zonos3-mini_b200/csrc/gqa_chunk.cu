@@ -42,7 +42,9 @@ namespace tc = zb::tc;
 
 constexpr int kTile = 128;       // keys of a tile
 constexpr int kStreamRows = 128;  // rows of a stream
-constexpr int kUnitCost = 4;     // what a unit costs besides its tiles, in tiles: the best of 1, 2, 3, 4, 6 on every batch
+// What a unit and each of its tiles cost, in fifths of a tile of one stream of rows: 1 for such a unit, 2 for one of two
+// streams. Of eight sets around the measured times the one that is within 3 % of the best on every batch.
+constexpr int kUnitCost1 = 14, kTileCost1 = 5, kUnitCost2 = 20, kTileCost2 = 7;
 constexpr int kFewRows = 32;     // up to here the row warps share a unit's rows in joining its parts
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
@@ -337,6 +339,17 @@ __device__ __forceinline__ void unit_tiles(const ChunkParams& p, const Request& 
   d.tiles = hi1 > lo0 ? (hi1 + kTile - 1) / kTile - d.tile0 : 0;
 }
 
+// A unit's cost, and the first of its tiles that begin at or behind a given cost into it.
+__device__ __forceinline__ int unit_cost(const ChunkParams& p, const Desc& d) {
+  const bool two = d.rows > p.tokens * p.G;
+  return two ? kUnitCost2 + d.tiles * kTileCost2 : kUnitCost1 + d.tiles * kTileCost1;
+}
+__device__ __forceinline__ int tile_behind(const ChunkParams& p, const Desc& d, int cost) {
+  const bool two = d.rows > p.tokens * p.G;
+  const int into = cost - (two ? kUnitCost2 : kUnitCost1);
+  return into <= 0 ? 0 : two ? (into + kTileCost2 - 1) / kTileCost2 : (into + kTileCost1 - 1) / kTileCost1;
+}
+
 // Exclusive prefix of v over the block's threads; `total` the sum. `buffer` alternates from call to call.
 __device__ __forceinline__ int block_scan(int v, Tail& tl, int buffer, int& total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -510,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     }
     Desc d;
     unit_tiles(p, at_hand(lo), j - pairs_before[lo], d);
-    return Pair{lo, j - pairs_before[lo], d.tiles + kUnitCost};
+    return Pair{lo, j - pairs_before[lo], unit_cost(p, d)};
   };
   const Pair first_pair = pair_of(tid);
   int first_total = 0;
@@ -524,7 +537,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     work += total;
   }
   work *= Hkv;
-  const int64_t share = work < INT32_MAX - ctas ? ((int)work + ctas - 1) / ctas : (work + ctas - 1) / ctas;
+  const int64_t share =
+      max((int64_t)kTileCost2, work < INT32_MAX - ctas ? ((int)work + ctas - 1) / ctas : (work + ctas - 1) / ctas);
   const int64_t begin = share * cta, end = min(work, begin + share);
   if (begin < end) {
     int64_t seen = 0;
@@ -614,13 +628,13 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     Desc d;
     unit_tiles(p, req, pair, d);
     int64_t at = begin;
-    const int unit0 = d.tiles + kUnitCost;
+    const int unit0 = unit_cost(p, d);
     int kvh = (int)(tl.start_off / unit0), off = (int)(tl.start_off % unit0);
     int item = 0, tile_no = 0, q_item = 0, scans = 0, n = 0;
     for (;;) {
-      // ---- the unit's tiles here: its work is kUnitCost, then a step a tile
-      const int unit = d.tiles + kUnitCost, to = (int)min((int64_t)unit, off + (end - at));
-      const int from_tile = max(off - kUnitCost, 0), to_tile = max(to - kUnitCost, 0);
+      // ---- the unit's tiles here: those that begin in this CTA's share, at least as long as any tile
+      const int unit = unit_cost(p, d), to = (int)min((int64_t)unit, off + (end - at));
+      const int from_tile = tile_behind(p, d, off), to_tile = tile_behind(p, d, to);
       const bool here = d.tiles > 0 ? to_tile > from_tile : off == 0;
       Desc u = d;
       u.kvh = kvh;
@@ -640,8 +654,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         const bool starts = from_tile == 0, ends = to_tile == d.tiles;
         u.mode = at >= end ? kStop : starts && ends ? kFinal : starts ? kPart1 : kPart0;
         // CTAs that hold a part of it from this one on
-        u.parts = ends ? 1 : at - off + unit < INT32_MAX ? (int)(at - off + unit - 1) / (int)share - cta + 1
-                                                         : (int)((at - off + unit - 1) / share) - cta + 1;
+        const int64_t last = at - off + unit - (u.rows > p.tokens * G ? kTileCost2 : kTileCost1);  // its last tile
+        u.parts = ends ? 1 : last < INT32_MAX ? (int)last / (int)share - cta + 1 : (int)(last / share) - cta + 1;
         if (warp == kLoadWarp && lane == 0) {
           const int slot = n % kDescs;
           if (n >= kDescs) wait(tl.desc_empty[slot], (n / kDescs - 1) & 1, abort, p.status);
@@ -662,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             if (q_item >= 2) wait(tl.q_empty[slot], (q_item / 2 - 1) & 1, abort, p.status);
             if (lane == 0) {
               zb::mbar_arrive_expect_tx(zb::smem_addr(&tl.q_full[slot]), (uint32_t)(p.tokens * G * HD * 2));
-  #pragma unroll 1
+#pragma unroll 1
               for (int a = 0; a < HD / 64; ++a)
                 load_queries(base + L::kOffQ + slot * L::kItem + a * L::kQAtom, &maps.q, a * 64, kvh * G,
                              u.token0 + s * p.tokens, zb::smem_addr(&tl.q_full[slot]));
@@ -695,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         if (p.box) {
           if (warp == kLoadWarp) {
 #pragma unroll 1
-  #pragma unroll 1
+#pragma unroll 1
           for (int t = 0; t < u.tiles; ++t, ++tile_no) {
               const int first = (u.tile0 + t) * kTile, pos = first + lane * p.box;
               const bool there = next >= 0 && next < p.kv.num_pages;
@@ -1345,7 +1359,7 @@ Launch plan(int B, int64_t N, int Hq, int Hkv, int hd, int64_t max_keys) {
   const int G = Hq / Hkv, pair_tokens = 2 * (kStreamRows / G);
   const int64_t tiles = std::max<int64_t>((max_keys + kTile - 1) / kTile, 1);
   l.pairs = N / pair_tokens + std::min<int64_t>(B, N);
-  l.ctas = (int)std::min<int64_t>(zb::sm_count(), l.pairs * Hkv * (tiles + kUnitCost));
+  l.ctas = (int)std::min<int64_t>(zb::sm_count(), l.pairs * Hkv * (tiles + kUnitCost2 / kTileCost2));
   l.splits = tiles > 1 && l.ctas > 1;
   l.rows_max = (int)std::min<int64_t>(N, pair_tokens) * G;
   if (l.splits) {

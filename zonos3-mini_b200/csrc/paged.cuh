@@ -29,8 +29,8 @@ inline int check_paged(const PagedBatch& p, const char* who) {
   ZB_REQUIRE(p.B >= 0 && p.N >= 0 && p.Hkv > 0 && p.num_pages >= 0 && p.max_pages >= 0, "%s: negative sizes", who);
   if (p.hd < 8 || p.hd > 128 || p.hd % 8 != 0)
     return fail(kUnsupported, "%s: head dim %d (a multiple of 8 up to 128)", who, p.hd);
-  ZB_REQUIRE(p.page_size >= 1 && (int64_t)p.page_size * p.max_pages <= (int64_t)1 << 29,
-             "%s: page size %d x %d table columns (at most 2^29 keys)", who, p.page_size, p.max_pages);
+  ZB_REQUIRE(p.page_size >= 1 && (int64_t)p.page_size * p.max_pages <= (int64_t)1 << 26,
+             "%s: page size %d x %d table columns (at most 2^26 keys)", who, p.page_size, p.max_pages);
   ZB_REQUIRE(p.page_stride % 8 == 0 && p.slot_stride % 8 == 0 && p.head_stride % 8 == 0 && p.page_stride >= 0 &&
                  p.slot_stride >= 0 && p.head_stride >= 0,
              "%s: cache strides (page %lld, row %lld, head %lld) must be multiples of 8", who, (long long)p.page_stride,
