@@ -400,35 +400,50 @@ __device__ __forceinline__ bool wait_parts(const ChunkParams& p, const Desc& u, 
 // Part i of a unit that began in CTA cta: the CTA's own, then those of the CTAs after it.
 __device__ __forceinline__ int64_t part_slot(int cta, int i) { return (int64_t)(cta + i) * 2 + (i == 0); }
 
-// Joins the parts of a unit of few rows, in the order of their keys: a thread of the row warps takes 8 dims of a row, its
-// loads of several parts in flight together.
+// Joins the parts of a unit of few rows, in the order of their keys: a thread of the row warps takes 8 dims of a row, the
+// loads of 8 parts in flight together.
 template <int HD>
 __device__ __forceinline__ void join_few(const ChunkParams& p, const Desc& u, int cta, int tid) {
+  constexpr int kTogether = 8;
   const int sharers = 32 * kSoftWarps / u.rows, r = tid % u.rows;  // threads of a row
   if (tid / u.rows >= sharers) return;
-  auto maximum = [&](int i) { return __ldcg(p.ml + part_slot(cta, i) * 2 * p.rows_max + r); };
-  auto sum = [&](int i) { return __ldcg(p.ml + (part_slot(cta, i) * 2 + 1) * p.rows_max + r); };
   const int h = u.kvh * p.G + p.by_group.rest(r);
   const int64_t token = u.token0 + p.by_group.quotient(r);
-  const float gate = p.gate ? sigmoid(p.gate[token * p.gate_stride + h]) : 1.f;
-  float top = -INFINITY, l = 0.f;
-#pragma unroll 8
-  for (int i = 0; i < u.parts; ++i) top = fmaxf(top, maximum(i));
-  const float mb = top == -INFINITY ? 0.f : top;
+  const __nv_bfloat16 gate = p.gate ? p.gate[token * p.gate_stride + h] : __float2bfloat16_rn(0.f);
 #pragma unroll 1
   for (int piece = tid / u.rows; piece < HD / 8; piece += sharers) {
-    float y[8] = {};
-    l = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < u.parts; ++i) {
-      const float4* a = reinterpret_cast<const float4*>(p.acc + (part_slot(cta, i) * (HD / 4) + piece * 2) * p.rows_max * 4 + r * 4);
-      const float4 v0 = __ldcg(a), v1 = __ldcg(a + p.rows_max);
-      const float w = ex2(maximum(i) - mb);  // 0 for a part none of whose keys the row sees; its accumulator is 0 too
-      l += sum(i) * w;
-      y[0] += v0.x * w, y[1] += v0.y * w, y[2] += v0.z * w, y[3] += v0.w * w;
-      y[4] += v1.x * w, y[5] += v1.y * w, y[6] += v1.z * w, y[7] += v1.w * w;
+    float y[8] = {}, top = -INFINITY, l = 0.f;
+#pragma unroll 1
+    for (int i0 = 0; i0 < u.parts; i0 += kTogether) {
+      float m[kTogether], sum[kTogether], hi = top;
+      float4 v[kTogether][2];
+#pragma unroll
+      for (int k = 0; k < kTogether; ++k) {
+        const bool there = i0 + k < u.parts;
+        const int64_t part = part_slot(cta, there ? i0 + k : 0);
+        const float* ml = p.ml + part * 2 * p.rows_max + r;
+        const float4* a = reinterpret_cast<const float4*>(p.acc + (part * (HD / 4) + piece * 2) * p.rows_max * 4 + r * 4);
+        m[k] = there ? __ldcg(ml) : -INFINITY;
+        sum[k] = there ? __ldcg(ml + p.rows_max) : 0.f;
+        v[k][0] = there ? __ldcg(a) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[k][1] = there ? __ldcg(a + p.rows_max) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int k = 0; k < kTogether; ++k) hi = fmaxf(hi, m[k]);
+      const float mb = hi == -INFINITY ? 0.f : hi, before = ex2(top - mb);
+      top = hi;
+      l *= before;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[e] *= before;
+#pragma unroll
+      for (int k = 0; k < kTogether; ++k) {
+        const float w = ex2(m[k] - mb);  // 0 for a part none of whose keys the row sees; its accumulator is 0 too
+        l += sum[k] * w;
+        y[0] += v[k][0].x * w, y[1] += v[k][0].y * w, y[2] += v[k][0].z * w, y[3] += v[k][0].w * w;
+        y[4] += v[k][1].x * w, y[5] += v[k][1].y * w, y[6] += v[k][1].z * w, y[7] += v[k][1].w * w;
+      }
     }
-    const float f = l == 0.f ? 0.f : gate / l;
+    const float f = l == 0.f ? 0.f : (p.gate ? sigmoid(gate) : 1.f) / l;
     if (piece * 8 < p.kv.hd)
       *reinterpret_cast<uint4*>(p.out + token * p.out_stride + (int64_t)h * p.kv.hd + piece * 8) =
           make_uint4(to_bf16x2(y[0] * f, y[1] * f), to_bf16x2(y[2] * f, y[3] * f), to_bf16x2(y[4] * f, y[5] * f),
