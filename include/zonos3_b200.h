@@ -336,8 +336,7 @@ int zb_gqa_prologue_decode(const uint16_t* proj, int64_t proj_stride, const uint
  * or (j, j + rotary_dim / 2) (a multiple of 16); position = positions[t], or the key position when positions is NULL.
  * fp32 with one rounding (angles in fp64). q to q_out [N, Hq, hd] (row stride q_stride, a multiple of 8; 16-byte
  * aligned; zero for a row of no request), k and v to the token's cache row (a token without a page is not stored). The
- * q/k norm, temperature, rotary and store_kv steps of Attention.forward for any batch
- * (servers/sgl/src/zonos3_sgl/models/zonos3.py:340-375). */
+ * attention layer's q/k norm, temperature, rotary embedding and KV store for any batch. */
 int zb_gqa_append(const uint16_t* proj, int64_t proj_stride, const uint16_t* temp, const int32_t* positions, float eps,
                   int normalize, double rope_theta, int rotary_dim, int interleaved, uint16_t* q_out, int64_t q_stride,
                   uint16_t* k_cache, uint16_t* v_cache, int64_t page_stride, int64_t slot_stride, int64_t head_stride,
@@ -345,9 +344,8 @@ int zb_gqa_append(const uint16_t* proj, int64_t proj_stride, const uint16_t* tem
                   const int32_t* cache_seqlens, const int32_t* cu_seqlens_q, int B, int N, int Hq, int Hkv, int hd,
                   cudaStream_t stream);
 
-/* zb_gqa_chunk: attention of the N new tokens over the pages of their requests (the FA backend's
- * flash_attn_with_kvcache for prefill, chunked prefill, decode and mixed batches,
- * servers/sgl/src/zonos3_sgl/attention/fa.py:64-81, :171-212). The token at key position p sees keys j <= p (causal; else
+/* zb_gqa_chunk: attention of the N new tokens over the pages of their requests (prompts, chunks of prompts, single
+ * tokens, or nothing, mixed as they come). The token at key position p sees keys j <= p (causal; else
  * every key of its request), j > p - window when window > 0 (causal only), in pages of the cache. out[t, h] = softmax(q[t,
  * h] . K^T * softmax_scale) V, query head h reading KV head h / (Hq / Hkv), times sigmoid(gate[t, h]) when gate is given
  * ([N, Hq] bf16, row stride gate_stride), rounded once; lse (NULL: not written) [N, Hq] fp32 = the natural logarithm of

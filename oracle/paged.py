@@ -2,9 +2,9 @@
 embedding) and the attention of a chunk of new tokens, over ragged batches described by page_table, cache_seqlens and
 cu_seqlens_q.
 
-Restates the global-attention layer of model/src/zonos3/reference/lm.py:511-537 (norms, interleaved rotary, GQA with
-query head h reading KV head h // (Hq / Hkv), scale head_dim ** -0.5, causal mask) with the FA backend's batch
-description (servers/sgl/src/zonos3_sgl/attention/fa.py:64-81). Test infrastructure only (see ``oracle/__init__.py``).
+The same attention core as ``oracle.attention`` and the pinned whole-LM oracle (norms, interleaved rotary, query head h
+reading KV head h // (Hq / Hkv), scale head_dim ** -0.5, causal mask), written out per token from the definition. Test
+infrastructure only (see ``oracle/__init__.py``).
 """
 
 from __future__ import annotations

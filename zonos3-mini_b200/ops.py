@@ -1096,10 +1096,7 @@ def _token_rows(name: str, t: torch.Tensor, index: int, N: int, heads: int, hd: 
 def gqa_append(proj, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, heads, kv_heads, temp=None,
                eps=1e-6, rope_theta=10000.0, rotary_dim=None, interleaved=True, positions=None, q_out=None):
     """The new tokens' keys and values into a paged KV cache, with the attention layer's q / k norm and rotary embedding
-    on the way, for a ragged batch (prompts, chunks of prompts, single tokens, or nothing, mixed as they come): the
-    q / k norm, ``temp``, rotary and store_kv steps of Attention.forward
-    (servers/sgl/src/zonos3_sgl/models/zonos3.py:340-375) with the FA backend's batch description
-    (servers/sgl/src/zonos3_sgl/attention/fa.py).
+    on the way, for a ragged batch: prompts, chunks of prompts, single tokens, or nothing, mixed as they come.
 
     proj [N, >= (heads + 2 kv_heads) * hd] bf16 holds q | k | v (rows contiguous, any row stride). Request b's new tokens
     are rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] ([B + 1] int32, on the device); cache_seqlens [B] int32 counts its
@@ -1143,8 +1140,7 @@ def gqa_append(proj, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, 
 def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, softmax_scale=None, causal=True, window=0,
               gate=None, out=None, lse=None, workspace=None):
     """Attention of every request's new tokens over its pages of a KV cache (which hold the new tokens' keys already:
-    :func:`gqa_append`): the FA backend's flash_attn_with_kvcache for prefill, chunked prefill, decode and batches that
-    mix them (servers/sgl/src/zonos3_sgl/attention/fa.py:64-81, :171-212).
+    :func:`gqa_append`), for prefill, chunked prefill, decode and batches that mix them.
 
     q [N, Hq, hd] bf16 (row stride allowed); the caches, page_table, cache_seqlens and cu_seqlens_q as for
     :func:`gqa_append`. Query head h reads KV head h // (Hq / Hkv). A token at key position p sees keys 0 .. p (with
