@@ -46,6 +46,10 @@ constexpr int kStreamRows = 128;  // rows of a stream
 // streams. Of eight sets around the measured times the one that is within 3 % of the best on every batch.
 constexpr int kUnitCost1 = 14, kTileCost1 = 5, kUnitCost2 = 20, kTileCost2 = 7;
 constexpr int kFewRows = 32;     // up to here the row warps share a unit's rows in joining its parts
+// Up to here a unit's products are 64 rows high instead of 128: its rows are then lanes 0-15 either way. The time of a
+// product hardly matters with so few rows, its power does: 256 single tokens over 1628 keys on average take 161 us instead of 172 where the
+// GPU is held by its power limit, 152 either way where it is not.
+constexpr int kSmallRows = 16;
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
 constexpr int kMaxSlots = 10, kDescs = 4;
@@ -819,8 +823,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   } else if (warp == kMmaWarp) {
     // =============================================================================================== tensor cores
     asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
-    constexpr uint32_t kIdS = tc::idesc_bf16(kStreamRows, kTile);
-    constexpr uint32_t kIdO = tc::idesc_bf16(kStreamRows, HD, false, /*b_mn=*/true);
+    constexpr uint32_t kIdS = tc::idesc_bf16(0, kTile), kIdO = tc::idesc_bf16(0, HD, false, /*b_mn=*/true);
+    uint32_t height = 0;  // the rest of the descriptors: the unit's rows
     // This warp's own time between two products is time the tensor cores stand still once their short queue is empty: ring
     // positions are kept instead of divided out, and one lane issues a stream's products and commits in one go.
     struct Ring {
@@ -844,7 +848,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks)
         tc::mma(tmem + L::kColS + s * kTile, qd + ((ks / 4) * L::kQAtom + (ks % 4) * 32) / 16,
-                kd + ((ks / 4) * 1024 + (ks % 4) * 32) / 16, kIdS, ks > 0);
+                kd + ((ks / 4) * 1024 + (ks % 4) * 32) / 16, kIdS | height, ks > 0);
       commit(tl.s_full[s]);
       arrive(tl.s_full[s]);  // passes on the tile's key mask, which this thread got with the tile
     };
@@ -854,7 +858,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll
       for (int k0 = 0; k0 < kTile / 32; ++k0) {
         const int ks = k0 + half * (kTile / 32);
-        mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, vd + ks * 2 * L::kGroup / 16, kIdO,
+        mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, vd + ks * 2 * L::kGroup / 16, kIdO | height,
                accumulate || ks > 0);
       }
     };
@@ -866,6 +870,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       if (u.mode == kStop || gave_up(abort)) break;
       if (u.tiles == 0) continue;
       const bool two = u.rows > p.tokens * G;  // two streams of rows share each tile, or one's two halves take turns
+      height = tc::idesc_bf16(u.rows <= kSmallRows ? 64 : kStreamRows, 0) & ~tc::idesc_bf16(0, 0);
       const int stride = two ? 1 : 2;          // tiles from one of a stream to its next
       auto wait_q = [&](int q) { wait(tl.q_full[q % 2], (q / 2) & 1, abort, p.status); };
       wait_q(q_item);
@@ -1006,15 +1011,21 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           }
           wait(tl.s_full[s], mine & 1, abort, p.status);
           ++mine;
-          if (idle) {  // whatever the tensor memory holds there, its rows are stored nowhere
+          tc::fence_after();
+          if (idle) {  // its rows are stored nowhere; zeros, because products of them take less power than of scores
             scans += scan;
+            const uint32_t zero[32] = {};
+            st32(col_s, zero);
+            st32(col_s + 32, zero);
+            tc::st_wait();
+            tc::fence_before();
+            __syncwarp();
             if (lane == 0) {
               arrive(tl.p_half[s]);
               arrive(tl.p_full[s]);
             }
             continue;
           }
-          tc::fence_after();
           const unsigned* there = tl.mask[(tile_no + t) % kMasks];
           const uint4 all4 = *reinterpret_cast<const uint4*>(there);
           const bool partly = __any_sync(0xffffffffu, first < lo || first + kTile > hi ||
