@@ -283,19 +283,16 @@ __device__ __forceinline__ unsigned not_finite(const uint4& v) {
 // Whether a tile of keys from `first` on has keys that some of the unit's rows see and others do not.
 __device__ __forceinline__ bool mixed_tile(const Desc& u, int first) { return first + kTile > u.all_hi || first < u.all_lo; }
 
-// A wait that gives up after about a second (2^31 cycles), and at once after any earlier one of the CTA did. Short, because
-// it stands in many places of loops that already fill the instruction cache.
-__device__ __forceinline__ void wait(const uint64_t& bar, uint32_t parity, int* abort, unsigned* status) {
+// A wait that gives up after about a second (a try that may sleep comes back after 4 us), and at once after any earlier one
+// of the CTA did. Short, because it stands in many places of loops that fill the instruction cache: the status is set at
+// the kernel's end.
+__device__ __forceinline__ void wait(const uint64_t& bar, uint32_t parity, int* abort) {
   const uint32_t at = zb::smem_addr(&bar);
   if (zb::mbar_try_wait(at, parity)) return;
-  const int start = clock();
-  while (!zb::mbar_try_wait_sleep(at, parity, 20000u)) {
-    if (*reinterpret_cast<volatile int*>(abort) != 0) return;
-    if ((int)clock() - start < 0) {
-      if (status) atomicOr(status, zb::kStatusAttnChunkTimeout);
-      *reinterpret_cast<volatile int*>(abort) = 1;
-    }
-  }
+#pragma unroll 1
+  for (int i = 0; i < 250000; ++i)
+    if (zb::mbar_try_wait_sleep(at, parity, 20000u) || *reinterpret_cast<volatile int*>(abort) != 0) return;
+  *reinterpret_cast<volatile int*>(abort) = 1;
 }
 // The same answer for every lane of the warp.
 __device__ __forceinline__ bool gave_up(int* abort) {
@@ -677,7 +674,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         u.parts = ends ? 1 : last < INT32_MAX ? (int)last / (int)share - cta + 1 : (int)(last / share) - cta + 1;
         if (warp == kLoadWarp && lane == 0) {
           const int slot = n % kDescs;
-          if (n >= kDescs) wait(tl.desc_empty[slot], (n / kDescs - 1) & 1, abort, p.status);
+          if (n >= kDescs) wait(tl.desc_empty[slot], (n / kDescs - 1) & 1, abort);
           tl.desc[slot] = u;
           arrive(tl.desc_full[slot]);
         }
@@ -692,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll 1
           for (int s = 0; s < (u.rows > p.tokens * G ? 2 : 1); ++s, ++q_item) {
             const int slot = q_item % 2;
-            if (q_item >= 2) wait(tl.q_empty[slot], (q_item / 2 - 1) & 1, abort, p.status);
+            if (q_item >= 2) wait(tl.q_empty[slot], (q_item / 2 - 1) & 1, abort);
             if (lane == 0) {
               zb::mbar_arrive_expect_tx(zb::smem_addr(&tl.q_full[slot]), (uint32_t)(p.tokens * G * HD * 2));
 #pragma unroll 1
@@ -707,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         auto look_through = [&](int t, int v_item) {
           const int first = (u.tile0 + t) * kTile, slot = scans % kMasks;
           if (warp == kLoadWarp || !mixed_tile(u, first)) return;
-          wait(tl.full[v_item % L::kSlots], (v_item / L::kSlots) & 1, abort, p.status);
+          wait(tl.full[v_item % L::kSlots], (v_item / L::kSlots) & 1, abort);
           constexpr uint32_t kHalf = L::kItem / 32;  // 16-byte pieces
           const uint4* v = reinterpret_cast<const uint4*>(gbase + (v_item % L::kSlots) * L::kItem);
           unsigned bad = 0;
@@ -746,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll 1
               for (int kv = 0; kv < 2; ++kv, ++item) {
                 const int slot = item % L::kSlots;
-                if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort, p.status);
+                if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort);
                 if (lane == 0) {
                   if (kv == 0) *reinterpret_cast<uint4*>(tl.mask[tile_no % kMasks]) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
                   zb::mbar_arrive_expect_tx(zb::smem_addr(&tl.full[slot]), L::kItem);
@@ -788,7 +785,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll 1
             for (int kv = 0; kv < 2; ++kv, ++item) {
               const int slot = item % L::kSlots;
-              if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort, p.status);
+              if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort);
               copy_tile(base + slot * L::kItem, kv ? p.kv.v : p.kv.k, off, item);
               cp_async_arrive(zb::smem_addr(&tl.full[slot]));
               if (warp == kLoadWarp && lane == 0) {
@@ -838,7 +835,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     Ring at{0, 0};  // of the unit's next tile's keys; its values lie one further
     int q_item = 0, scans = 0;
     uint32_t parity = 0;  // bit s: of stream s's weights
-    auto full = [&](const Ring& i) { wait(tl.full[i.slot], i.phase, abort, p.status); };
+    auto full = [&](const Ring& i) { wait(tl.full[i.slot], i.phase, abort); };
     auto commit = [&](const uint64_t& bar) { tc::commit(zb::smem_addr(&bar)); };
     const uint64_t k_desc = tc::desc_mnmajor(base, 16, L::kGroup), v_desc = tc::desc_mnmajor(base, 1024, L::kGroup);
     const uint64_t q_desc = tc::desc_kmajor(base + L::kOffQ);
@@ -864,7 +861,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     };
     for (int n = 0;; ++n) {
       const int slot = n % kDescs;
-      wait(tl.desc_full[slot], (n / kDescs) & 1, abort, p.status);
+      wait(tl.desc_full[slot], (n / kDescs) & 1, abort);
       const Desc u = uniform(tl.desc[slot]);
       if (lane == 0) arrive(tl.desc_empty[slot]);
       if (u.mode == kStop || gave_up(abort)) break;
@@ -872,94 +869,79 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const bool two = u.rows > p.tokens * G;  // two streams of rows share each tile, or one's two halves take turns
       height = tc::idesc_bf16(u.rows <= kSmallRows ? 64 : kStreamRows, 0) & ~tc::idesc_bf16(0, 0);
       const int stride = two ? 1 : 2;          // tiles from one of a stream to its next
-      auto wait_q = [&](int q) { wait(tl.q_full[q % 2], (q / 2) & 1, abort, p.status); };
-      wait_q(q_item);
-      if (two) wait_q(q_item + 1);
-      full(at);
-      const bool second = !two && u.tiles > 1;  // the other half begins with the second tile
-      const Ring next = at.after(2);
-      if (second) full(next);
-      if (p.box == 0) tc::fence_proxy_async();  // 16-byte copies -> the tensor cores
-      if (elect()) {
-        issue_s(0, at.slot, q_item);
-        if (two) issue_s(1, at.slot, q_item + 1);
-        commit(tl.empty[at.slot]);
-        if (second) {
-          issue_s(1, next.slot, q_item);
-          commit(tl.empty[next.slot]);
-        }
-        if (u.tiles <= stride) {
-          commit(tl.q_empty[q_item % 2]);
-          if (two) commit(tl.q_empty[(q_item + 1) % 2]);
-        }
-      }
-      __syncwarp();
       const int held = held_keys(p, u.keys);
+      Ring ahead = at;  // of the next tile whose scores are due
 #pragma unroll 1
-      for (int t = 0; t < u.tiles; ++t) {
-        // O_s += P_s(t) V(t) as soon as P_s(t) is there, then the stream's next scores
-        const Ring v = at.after(1), k = two ? at.after(2) : at.after(2).after(2);
+      for (int t = -stride; t < u.tiles; ++t) {
+        // O_s += P_s(t) V(t) as soon as P_s(t) is there, then the stream's next scores; before the first tile, those alone
         const bool more = t + stride < u.tiles, ends = t + stride == u.tiles - 1;
         const int s0 = two ? 0 : t & 1, s1 = two ? 1 : s0, first = (u.tile0 + t) * kTile;
+        const Ring v = at.after(1), k = ahead;
         unsigned char* v_tile = gbase + v.slot * L::kItem;
         bool found = false;
-        full(v);
-        // rows of the last page past the request's keys came along with a tensor copy: no key, so no value either
-        if (p.box && first + kTile > held && held % p.box != 0) {
-          const int r0 = held - first, r1 = (r0 + p.box - 1) / p.box * p.box;
+        if (t >= 0) {
+          full(v);
+          // rows of the last page past the request's keys came along with a tensor copy: no key, so no value either
+          if (p.box && first + kTile > held && held % p.box != 0) {
+            const int r0 = held - first, r1 = (r0 + p.box - 1) / p.box * p.box;
 #pragma unroll 1
-          for (int i = r0 * (HD / 8) + lane; i < r1 * (HD / 8); i += 32)
-            *reinterpret_cast<uint4*>(v_tile + piece<HD>(i / (HD / 8), i % (HD / 8))) = make_uint4(0, 0, 0, 0);
-          tc::fence_proxy_async();
-          __syncwarp();
-        }
-        if (mixed_tile(u, first)) {
-          const int slot = scans % kMasks;
-          wait(tl.scanned[slot], (scans / kMasks) & 1, abort, p.status);
-          ++scans;
-          found = uniform(tl.found[slot][0] | tl.found[slot][1]) != 0;
-          if (found) {  // every stream adds what it sees before it hands over P; then the values are zeroed
-#pragma unroll 1
-            for (int s = s0; s <= s1; ++s) wait(tl.p_full[s], (parity >> s) & 1u, abort, p.status);
-            uint16_t* e = reinterpret_cast<uint16_t*>(v_tile);
-#pragma unroll 1
-            for (uint32_t i = lane; i < L::kItem / 2; i += 32)
-              if ((e[i] & 0x7f80u) == 0x7f80u) e[i] = 0;
+            for (int i = r0 * (HD / 8) + lane; i < r1 * (HD / 8); i += 32)
+              *reinterpret_cast<uint4*>(v_tile + piece<HD>(i / (HD / 8), i % (HD / 8))) = make_uint4(0, 0, 0, 0);
             tc::fence_proxy_async();
             __syncwarp();
           }
+          if (mixed_tile(u, first)) {
+            const int slot = scans % kMasks;
+            wait(tl.scanned[slot], (scans / kMasks) & 1, abort);
+            ++scans;
+            found = uniform(tl.found[slot][0] | tl.found[slot][1]) != 0;
+            if (found) {  // every stream adds what it sees before it hands over P; then the values are zeroed
+#pragma unroll 1
+              for (int s = s0; s <= s1; ++s) wait(tl.p_full[s], (parity >> s) & 1u, abort);
+              uint16_t* e = reinterpret_cast<uint16_t*>(v_tile);
+#pragma unroll 1
+              for (uint32_t i = lane; i < L::kItem / 2; i += 32)
+                if ((e[i] & 0x7f80u) == 0x7f80u) e[i] = 0;
+              tc::fence_proxy_async();
+              __syncwarp();
+            }
+          }
+          if (p.box == 0) tc::fence_proxy_async();  // 16-byte copies -> the tensor cores
+          at = at.after(2);
         }
-        if (p.box == 0) tc::fence_proxy_async();
 #pragma unroll 1
         for (int s = s0; s <= s1; ++s) {
-          wait(tl.p_half[s], (parity >> s) & 1u, abort, p.status);
-          tc::fence_after();
-          if (elect()) issue_o(s, v.slot, 0, t >= stride || found);
-          __syncwarp();
-          wait(tl.p_full[s], (parity >> s) & 1u, abort, p.status);
-          tc::fence_after();
-          if (elect()) {
-            issue_o(s, v.slot, 1, true);
-            if (s == s1) commit(tl.empty[v.slot]);
-            if (!more) commit(tl.o_full[s]);
+          if (t >= 0) {
+            wait(tl.p_half[s], (parity >> s) & 1u, abort);
+            tc::fence_after();
+            if (elect()) issue_o(s, v.slot, 0, t >= stride || found);
+            __syncwarp();
+            wait(tl.p_full[s], (parity >> s) & 1u, abort);
+            tc::fence_after();
+            if (elect()) {
+              issue_o(s, v.slot, 1, true);
+              if (s == s1) commit(tl.empty[v.slot]);
+              if (!more) commit(tl.o_full[s]);
+            }
+            __syncwarp();
+            parity ^= 1u << s;
           }
-          __syncwarp();
           if (more) {
+            const int q = q_item + (two ? s : 0);
+            if (t < 0) wait(tl.q_full[q % 2], (q / 2) & 1, abort);
             if (s == s0) {
               full(k);
               if (p.box == 0) tc::fence_proxy_async();
             }
             if (elect()) {
-              const int q = q_item + (two ? s : 0);
               issue_s(s, k.slot, q);
               if (s == s1) commit(tl.empty[k.slot]);
               if (ends) commit(tl.q_empty[q % 2]);
             }
             __syncwarp();
           }
-          parity ^= 1u << s;
         }
-        at = at.after(2);
+        if (more) ahead = ahead.after(2);
       }
       q_item += two ? 2 : 1;
     }
@@ -977,12 +959,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     int tile_no = 0, mine = 0, units = 0, scans = 0, meetings = 0;  // counters of what this CTA, or this stream, has done
     auto meet = [&]() {  // the 8 row warps
       arrive(tl.halves);
-      wait(tl.halves, meetings & 1, abort, p.status);
+      wait(tl.halves, meetings & 1, abort);
       ++meetings;
     };
     for (int n = 0;; ++n) {
       const int slot = n % kDescs;
-      wait(tl.desc_full[slot], (n / kDescs) & 1, abort, p.status);
+      wait(tl.desc_full[slot], (n / kDescs) & 1, abort);
       const Desc u = uniform(tl.desc[slot]);
       if (lane == 0) arrive(tl.desc_empty[slot]);
       if (u.mode == kStop || gave_up(abort)) break;
@@ -1009,7 +991,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             scans += scan;
             continue;
           }
-          wait(tl.s_full[s], mine & 1, abort, p.status);
+          wait(tl.s_full[s], mine & 1, abort);
           ++mine;
           tc::fence_after();
           if (idle) {  // its rows are stored nowhere; zeros, because products of them take less power than of scores
@@ -1068,40 +1050,51 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           };
           // The weights are formed with the m there is, and the tile's largest score is found beside them; nothing is
           // written over the scores before it is known that they hold. A second turn is rare.
-          if (partly) {  // 32 keys at a time, without those that no row of the warp sees
-            uint32_t packed[64];
-            float top;
-            do {
-              minus = pack2(-m, -m);
-              sum2[0] = sum2[1] = 0;
-              top = -INFINITY;
+          if (partly) {  // 32 keys at a time, without those that no row of the warp sees; first their largest score
+            float top = -INFINITY;
+            auto scores = [&](int c, uint32_t (&y)[32]) {  // those that the row does not see as -infinity; whether any row sees one
+              const unsigned word = seen(c);
+              if (!__any_sync(0xffffffffu, word != 0)) return false;
+              ld32(col_s + 32 * c, y);
+              const bool all = __all_sync(0xffffffffu, word == 0xffffffffu);
+              tc::ld_wait();
+              if (!all) {
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                const unsigned word = seen(c);
-                if (!__any_sync(0xffffffffu, word != 0)) {
+                for (int j = 0; j < 32; ++j) y[j] = (word >> j) & 1u ? y[j] : 0xff800000u;
+              }
+              return true;
+            };
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t y[32];
+              if (!scores(c, y)) continue;
+              float t2 = -INFINITY;
 #pragma unroll
-                  for (int j = 0; j < 16; ++j) packed[16 * c + j] = 0;
-                  continue;
-                }
-                uint32_t y[32];
-                ld32(col_s + 32 * c, y);
-                tc::ld_wait();
+              for (int j = 0; j < 32; j += 4) {
+                top = fmaxf(fmaxf(top, __uint_as_float(y[j])), __uint_as_float(y[j + 1]));
+                t2 = fmaxf(fmaxf(t2, __uint_as_float(y[j + 2])), __uint_as_float(y[j + 3]));
+              }
+              top = fmaxf(top, t2);
+            }
+            holds(top);
+            minus = pack2(-m, -m);
+            sum2[0] = sum2[1] = 0;
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {  // the weights take half of the scores' columns: those of scores already read
+              uint32_t y[32], packed[16] = {};
+              if (scores(c, y)) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                  const float s0 = (word >> (2 * j)) & 1u ? __uint_as_float(y[2 * j]) : -INFINITY;
-                  const float s1 = (word >> (2 * j + 1)) & 1u ? __uint_as_float(y[2 * j + 1]) : -INFINITY;
-                  top = fmaxf(fmaxf(top, s0), s1);
                   float a, z;
-                  unpack2(fma2(pack2(s0, s1), scale2, minus), a, z);
+                  unpack2(fma2(pack2(__uint_as_float(y[2 * j]), __uint_as_float(y[2 * j + 1])), scale2, minus), a, z);
                   a = ex2(a);
                   z = ex2(z);
                   sum2[j % 2] = add2(sum2[j % 2], pack2(a, z));
-                  packed[16 * c + j] = to_bf16x2(a, z);
+                  packed[j] = to_bf16x2(a, z);
                 }
               }
-            } while (!holds(top));
-            st32(col_s, packed);
-            st32(col_s + 32, packed + 32);
+              tc::st16(col_s + 16 * c, packed);
+            }
             if (!scan) hand_over(tl.p_half[s]);
           } else {
             uint32_t x[kTile];
@@ -1165,7 +1158,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           }
           if (scan) {
             const int slot = scans % kMasks;
-            wait(tl.scanned[slot], (scans / kMasks) & 1, abort, p.status);
+            wait(tl.scanned[slot], (scans / kMasks) & 1, abort);
             ++scans;
             if (tl.found[slot][0] | tl.found[slot][1]) {  // values that are not finite, one by one
               if (t < stride) {  // the tile's product adds to the accumulator then
@@ -1199,12 +1192,14 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           if (scan) hand_over(tl.p_half[s]);
           hand_over(tl.p_full[s]);
         }
+      }
+      auto wait_o = [&]() {  // the stream's last product
         if (u.tiles > (two ? 0 : s)) {
-          wait(tl.o_full[s], units & 1, abort, p.status);
+          wait(tl.o_full[s], units & 1, abort);
           ++units;
         }
         tc::fence_after();
-      }
+      };
       tile_no += u.tiles;
       if (l == 0.f) m = -INFINITY;  // no key seen: the row counts for nothing where parts are joined
       int own = 32 * (warp % 4) + lane;
@@ -1215,7 +1210,9 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       // The accumulator of the row: its stream's, or both halves' of it, each half of the dims by one of the streams.
       float own_c = 1.f, other_c = 0.f;
       int c0 = 0, c1 = HD / 32;
-      if (!two && u.tiles > 1) {
+      const bool halves = !two && u.tiles > 1;
+      if (halves) {
+        wait_o();
         tl.ml[s][own][0] = m;
         tl.ml[s][own][1] = l;
         tc::fence_before();
@@ -1251,8 +1248,15 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         m = top;
       }
       const bool done = u.mode == kFinal || adds;  // the row's output is formed here
+      const float f = l == 0.f ? 0.f : (p.gate ? sigmoid(gate_raw) : 1.f) / l;  // 0 for a row that saw no key; a NaN sum stays NaN
+      int64_t rows4[4];  // where the rows go that this lane stores: lane / 4 and every 8th
+      {
+        const int64_t row = live ? token * p.out_stride + (int64_t)h * hd : -1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) rows4[k] = __shfl_sync(0xffffffffu, row, 8 * k + lane / 4);
+      }
+      if (!halves) wait_o();  // all that does not need it comes before
       if ((two || s == 0 || u.tiles > 1) && !gave_up(abort)) {
-        const float f = l == 0.f ? 0.f : (p.gate ? sigmoid(gate_raw) : 1.f) / l;  // 0 for a row that saw no key; a NaN sum stays NaN
         const int64_t part = (int64_t)cta * 2 + (u.mode == kPart1);
         float* acc = p.acc + part * HD * p.rows_max;
         auto chunk = [&](int c) {  // 32 dims of the row's accumulator
@@ -1311,10 +1315,6 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         for (int c = c0; c < c1; ++c) chunk(c);
         if (done) {
           tc::st_wait();
-          const int64_t row = live ? token * p.out_stride + (int64_t)h * hd : -1;
-          int64_t rows4[4];  // the rows this lane stores: lane / 4 and every 8th
-#pragma unroll
-          for (int k = 0; k < 4; ++k) rows4[k] = __shfl_sync(0xffffffffu, row, 8 * k + lane / 4);
 #pragma unroll 1
           for (int c = c0; c < c1; ++c) {
             const int dim = 32 * c + 8 * (lane % 4);
@@ -1370,6 +1370,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
+  if (tid == 0 && *abort != 0 && p.status) atomicOr(p.status, zb::kStatusAttnChunkTimeout);
   if (warp == kMmaWarp) tc::dealloc(tmem, 512);
 }
 
