@@ -373,7 +373,13 @@ __device__ __forceinline__ int block_scan(int v, Tail& tl, int buffer, int& tota
   return before + in - v;
 }
 
-__device__ __forceinline__ float sigmoid(__nv_bfloat16 x) { return 1.f / (1.f + expf(-__bfloat162float(x))); }
+// 1 / x to an ulp; the sums and 1 + e^-x that it is called on are far from fp32's limits, or infinite (0) or NaN (NaN).
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float sigmoid(__nv_bfloat16 x) { return reciprocal(1.f + ex2(-1.4426950408889634f * __bfloat162float(x))); }
 
 __device__ __forceinline__ void raise_flag(unsigned* flag) {
   asm volatile("st.release.gpu.global.u32 [%0], 1;" ::"l"(flag) : "memory");
@@ -444,7 +450,7 @@ __device__ __forceinline__ void join_few(const ChunkParams& p, const Desc& u, in
         y[4] += v[k][1].x * w, y[5] += v[k][1].y * w, y[6] += v[k][1].z * w, y[7] += v[k][1].w * w;
       }
     }
-    const float f = l == 0.f ? 0.f : (p.gate ? sigmoid(gate) : 1.f) / l;
+    const float f = l == 0.f ? 0.f : (p.gate ? sigmoid(gate) : 1.f) * reciprocal(l);
     if (piece * 8 < p.kv.hd)
       *reinterpret_cast<uint4*>(p.out + token * p.out_stride + (int64_t)h * p.kv.hd + piece * 8) =
           make_uint4(to_bf16x2(y[0] * f, y[1] * f), to_bf16x2(y[2] * f, y[3] * f), to_bf16x2(y[4] * f, y[5] * f),
@@ -705,16 +711,17 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           const int first = (u.tile0 + t) * kTile, slot = scans % kMasks;
           if (warp == kLoadWarp || !mixed_tile(u, first)) return;
           wait(tl.full[v_item % L::kSlots], (v_item / L::kSlots) & 1, abort);
-          constexpr uint32_t kHalf = L::kItem / 32;  // 16-byte pieces
+          // groups of 8 rows in turn; rows past the request's keys are no values (warp 8 zeroes them)
           const uint4* v = reinterpret_cast<const uint4*>(gbase + (v_item % L::kSlots) * L::kItem);
           unsigned bad = 0;
-          const bool tail = first + kTile > held;  // rows past the request's keys are no values; warp 8 zeroes them
-#pragma unroll 4
-          for (uint32_t i = (lw - 1) * kHalf + lane; i < lw * kHalf; i += 32) {
-            const int row = (int)(i / (L::kGroup / 16) * 8 + i % 64 / 8);
-            const unsigned b = not_finite(v[i]);
-            bad |= tail && first + row >= held ? 0u : b;
-          }
+          const int rows = min(kTile, held - first);
+#pragma unroll 1
+          for (int g = lw - 1; g * 8 < rows; g += kLoadWarps - 1)
+#pragma unroll
+            for (int i = 0; i < L::kGroup / 512; ++i) {
+              const unsigned b = not_finite(v[g * (L::kGroup / 16) + 32 * i + lane]);
+              bad |= g * 8 + i % 2 * 4 + lane / 8 < rows ? b : 0u;
+            }
           const bool found = __any_sync(0xffffffffu, (bad & 0x80008000u) != 0);
           if (lane == 0) {
             tl.found[slot][lw - 1] = found;
@@ -1248,7 +1255,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         m = top;
       }
       const bool done = u.mode == kFinal || adds;  // the row's output is formed here
-      const float f = l == 0.f ? 0.f : (p.gate ? sigmoid(gate_raw) : 1.f) / l;  // 0 for a row that saw no key; a NaN sum stays NaN
+      const float f = l == 0.f ? 0.f : (p.gate ? sigmoid(gate_raw) : 1.f) * reciprocal(l);  // 0 for a row that saw no key; a NaN sum stays NaN
       int64_t rows4[4];  // where the rows go that this lane stores: lane / 4 and every 8th
       {
         const int64_t row = live ? token * p.out_stride + (int64_t)h * hd : -1;
