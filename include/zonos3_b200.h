@@ -334,7 +334,7 @@ int zb_gqa_prologue_decode(const uint16_t* proj, int64_t proj_stride, const uint
  * divided by sqrt(mean(x^2) + eps) when normalize, q multiplied by |temp[h]| (NULL: not), the first rotary_dim elements
  * turned by position * rope_theta^(-2j / rotary_dim) in pairs (2j, 2j + 1) when interleaved (rotary_dim a multiple of 8)
  * or (j, j + rotary_dim / 2) (a multiple of 16); position = positions[t], or the key position when positions is NULL.
- * fp32 with one rounding (angles in fp64). q to q_out [N, Hq, hd] (row stride q_stride, a multiple of 8; 16-byte
+ * fp32 with one rounding (angles in 64-bit fixed point). q to q_out [N, Hq, hd] (row stride q_stride, a multiple of 8; 16-byte
  * aligned; zero for a row of no request), k and v to the token's cache row (a token without a page is not stored). The
  * attention layer's q/k norm, temperature, rotary embedding and KV store for any batch. */
 int zb_gqa_append(const uint16_t* proj, int64_t proj_stride, const uint16_t* temp, const int32_t* positions, float eps,

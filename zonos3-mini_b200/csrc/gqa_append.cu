@@ -16,6 +16,11 @@
 // projection row's loads are in flight. A warp takes a token (or a share of its heads when there are few tokens): a
 // group of lanes, 8 elements each, holds a head, so a warp moves 512 bytes an instruction and turns its lanes' pairs by
 // sines and cosines that it computes once for all heads.
+//
+// Measured (B200): 16210 tokens of 16 query and 4 KV heads of 128 (199 MB) 45 us, 4.4 TB/s, 0.68 of a copy's 6.46: the
+// schedulers issue in 65 % of the cycles, a norm, a turn and a rounding for every element, where a copy would issue in few.
+// Four warps a block and four passes of heads in flight is the best of 2-8 by 1-8; several tokens to a warp (64-66 us) and
+// a token over several warps (66-75) are slower there. 256 single tokens 5.5 us, one 3.4.
 #include <cmath>
 
 #include "paged.cuh"

@@ -30,6 +30,26 @@
 // A key hidden from some rows of a tile must not reach them even when its value is not finite, and 0 x inf is NaN in a
 // matrix product. So where a tile's keys are visible to some of its rows only, warps 10 and 11 look through the V tile while
 // the scores are being worked on; values that are not finite are added to the rows that see them one by one, then zeroed.
+//
+// What bounds it, and what it measured (B200, 16 query and 4 KV heads of 128, captured calls back to back):
+// * A long prompt (8192 tokens, causal; 275 GFLOP): 235 us, 1170 TFLOP/s, 0.71 of the 1638 that a library product of
+//   8192^3 reaches. Per stream and tile the chain scores (512 cycles), weights (1024 of the exponential unit, 2048 with the
+//   other stream's beside them), hand-over, values' product (its second half 256) comes to 3100-3500 cycles for two tiles'
+//   2048 cycles of tensor-core work; without the row warps' work the loop takes 195 us. Held by the power limit it is 270 us,
+//   as the clock falls from 1.95 to 1.62 GHz. 4 x 512 tokens behind 8192 cached ones (142 GFLOP): 131 us, 1080 TFLOP/s.
+// * Single tokens are bound by HBM: 256 requests of 1628 keys (856 MB), 149 us, 5.7 TB/s, 0.89 of a copy's
+//   6.46; 2 of 65000 keys over all CTAs, 56 us, 4.7 TB/s.
+// * Many short units (256 prompts of up to 128 tokens) are bound by the latency of a unit's steps, 8000-10000 cycles,
+//   and by their balance, not by bytes (26 us of them): 68 us. Each unit runs through about 30 KB of code once, more than
+//   the instruction cache keeps beside the other warps' (a third of its requests missed at 148 KB of kernel, a fifth at
+//   131 KB). So code that runs once a unit is kept small before it is kept fast: loops over 32 keys or dims instead of whole
+//   rows (unrolled whole, the epilogue made it 75 -> 79 us), one place for each stream's products (70.7 -> 69.2), waits that
+//   count (73.7 -> 70.7).
+// * One request of one token: 14.7 us, about 7 of them the way from the launch to the first scores.
+//
+// Pages: with rows of 64 or 128 elements and a page size with a factor of 8 or more, a lane copies a page's rows in one
+// tensor copy; 16-byte copies by three warps otherwise. On 128 requests of 2000 keys and pages of 8 the first takes 125 us
+// against 158 with heads of 128, 120 against 120 with heads of 64.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -47,8 +67,8 @@ constexpr int kStreamRows = 128;  // rows of a stream
 constexpr int kUnitCost1 = 14, kTileCost1 = 5, kUnitCost2 = 20, kTileCost2 = 7;
 constexpr int kFewRows = 32;     // up to here the row warps share a unit's rows in joining its parts
 // Up to here a unit's products are 64 rows high instead of 128: its rows are then lanes 0-15 either way. The time of a
-// product hardly matters with so few rows, its power does: 256 single tokens over 1628 keys on average take 161 us instead of 172 where the
-// GPU is held by its power limit, 152 either way where it is not.
+// product hardly matters with so few rows, its power does: 256 single tokens over 1628 keys take 161 us instead
+// of 172 where the GPU is held by its power limit, 152 either way where it is not.
 constexpr int kSmallRows = 16;
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
@@ -732,8 +752,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         if (p.box) {
           if (warp == kLoadWarp) {
 #pragma unroll 1
-#pragma unroll 1
-          for (int t = 0; t < u.tiles; ++t, ++tile_no) {
+            for (int t = 0; t < u.tiles; ++t, ++tile_no) {
               const int first = (u.tile0 + t) * kTile, pos = first + lane * p.box;
               const bool there = next >= 0 && next < p.kv.num_pages;
               const int page = there ? next * p.page_heads + (p.page_heads > 1 ? kvh : 0)
@@ -1055,8 +1074,6 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             __syncwarp();
             if (lane == 0) arrive(bar);
           };
-          // The weights are formed with the m there is, and the tile's largest score is found beside them; nothing is
-          // written over the scores before it is known that they hold. A second turn is rare.
           if (partly) {  // 32 keys at a time, without those that no row of the warp sees; first their largest score
             float top = -INFINITY;
             auto scores = [&](int c, uint32_t (&y)[32]) {  // those that the row does not see as -infinity; whether any row sees one
@@ -1104,6 +1121,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             }
             if (!scan) hand_over(tl.p_half[s]);
           } else {
+            // The weights are formed with the m there is, and the tile's largest score is found beside them; nothing is
+            // written over the scores before it is known that they hold. A second turn is rare.
             uint32_t x[kTile];
             // p of a half of the keys. The exponential unit takes 8 cycles an instruction, so everything else has to run in
             // its shadow: the scaling of the next group, the sum and the packing of the one before, and in the first half
