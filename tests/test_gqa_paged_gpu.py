@@ -458,3 +458,40 @@ def test_refusals(zb):
         with pytest.raises(ValueError):
             zb.ops.gqa_append(**{**base, **change})
     assert zb.ops.gqa_append(**{**base, "proj": proj[:0], "cu_seqlens_q": torch.zeros_like(cu)}).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("Hq, Hkv, hd, page, window", [(16, 4, 128, 16, 0), (16, 1, 128, 1, 0), (14, 2, 64, 24, 300),
+                                                       (8, 8, 40, 8, 0), (4, 4, 128, 128, 0)])
+def test_units_of_few_rows_keep_their_weights(zb, Hq, Hkv, hd, page, window):
+    """Single tokens (up to 16 rows a KV head): the weights' roundings to bf16 are multiplied too, which leaves 2^-16 of a
+    weight. Beside that a weight and the sum that divides it are each off by the exponential's 2^-15 and a score's error;
+    the output is rounded once (2^-8 of it)."""
+    gen = torch.Generator().manual_seed(11)
+    q, k, v, table, seqlens, cu = _chunk_inputs(gen, [1, 1, 1, 0, 1, 1], [0, 1, 700, 40, 128, 5000], Hq, Hkv, hd, page)
+    out = _check_chunk(zb, q, k, v, table, seqlens, cu, window=window)
+    ref, spread, _, size = paged.chunk(q, k, v, table, seqlens, cu, window=window)
+    _close(out, ref, 2.0 ** -8 * ref.abs() + 2 * spread * (2.0 ** -16 + 2.0 ** -15 + hd * 2.0 ** -23 * size[..., None]))
+
+
+@pytest.mark.parametrize("new", [1, 3, 40, 200])
+def test_a_row_that_sees_one_key_is_its_value(zb, new):
+    """A prompt's first token sees its own key alone: its weight is divided by itself, and the output is v."""
+    gen = torch.Generator().manual_seed(new)
+    q, k, v, table, seqlens, cu = _chunk_inputs(gen, [new, new], [0, 0], 8, 2, 128, 16, spread=3.0)
+    out = _check_chunk(zb, q, k, v, table, seqlens, cu).cpu()
+    for b in range(2):
+        first = v[int(table[b, 0]), 0].repeat_interleave(4, 0)
+        assert torch.equal(out[b * new], first)
+
+
+def test_few_rows_over_infinite_values(zb):
+    """A value that is infinite and seen makes its dim infinite, of its sign, also where a weight's rounding left nothing."""
+    gen = torch.Generator().manual_seed(5)
+    q, k, v, table, seqlens, cu = _chunk_inputs(gen, [1, 1], [299, 511], 16, 4, 128, 16)
+    for b, key, sign in ((0, 17, 1.0), (1, 500, -1.0)):
+        v[int(table[b, key // 16]), key % 16, :, 3] = sign * math.inf
+    d = [t.to(DEV) for t in (q, k, v, table, seqlens, cu)]
+    out = zb.ops.gqa_chunk(*d).float().cpu()
+    assert (out[0, :, 3] == math.inf).all() and (out[1, :, 3] == -math.inf).all()
+    rest = torch.cat([out[..., :3], out[..., 4:]], -1)
+    assert torch.isfinite(rest).all()

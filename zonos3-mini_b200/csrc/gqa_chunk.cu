@@ -16,7 +16,9 @@
 // and only moves to the largest score of a tile that is more than 64 above it (or, for a row's first keys, below), which
 // keeps p within 2^64, sums and accumulators far inside fp32's range, and the largest weights' precision. So the search for
 // the maximum runs beside the exponentials instead of before them, and the accumulator is hardly ever rescaled.
-// p is rounded to bf16 because the tensor cores multiply bf16; its sum is kept from before the rounding.
+// p is rounded to bf16 because the tensor cores multiply bf16; its sum is kept from before the rounding. Where that would
+// be the largest error for nothing it is avoided: units of few rows multiply what the rounding left off too, and rows whose
+// first keys lie in a partly visible tile start with m at their largest score, whose p is 1.
 //
 // The lengths live on the device, so the split of the work does too: every CTA adds up the tiles of all units (a scan
 // over the requests) and takes an equal run of them. A unit that spans CTAs leaves partial results (accumulator,
@@ -37,15 +39,15 @@
 //   other stream's beside them), hand-over, values' product (its second half 256) comes to 3100-3500 cycles for two tiles'
 //   2048 cycles of tensor-core work; without the row warps' work the loop takes 195 us. Held by the power limit it is 270 us,
 //   as the clock falls from 1.95 to 1.62 GHz. 4 x 512 tokens behind 8192 cached ones (142 GFLOP): 131 us, 1080 TFLOP/s.
-// * Single tokens are bound by HBM: 256 requests of 1628 keys (856 MB), 149 us, 5.7 TB/s, 0.89 of a copy's
-//   6.46; 2 of 65000 keys over all CTAs, 56 us, 4.7 TB/s.
+// * Single tokens are bound by HBM: 256 requests of 1628 keys (856 MB), 152 us, 5.6 TB/s, 0.87 of a copy's
+//   6.46; 2 of 65000 keys over all CTAs, 57 us, 4.7 TB/s.
 // * Many short units (256 prompts of up to 128 tokens) are bound by the latency of a unit's steps, 8000-10000 cycles,
-//   and by their balance, not by bytes (26 us of them): 68 us. Each unit runs through about 30 KB of code once, more than
+//   and by their balance, not by bytes (26 us of them): 71 us. Each unit runs through about 30 KB of code once, more than
 //   the instruction cache keeps beside the other warps' (a third of its requests missed at 148 KB of kernel, a fifth at
 //   131 KB). So code that runs once a unit is kept small before it is kept fast: loops over 32 keys or dims instead of whole
 //   rows (unrolled whole, the epilogue made it 75 -> 79 us), one place for each stream's products (70.7 -> 69.2), waits that
 //   count (73.7 -> 70.7).
-// * One request of one token: 14.7 us, about 7 of them the way from the launch to the first scores.
+// * One request of one token: 15 us, about 7 of them the way from the launch to the first scores.
 //
 // Pages: with rows of 64 or 128 elements and a page size with a factor of 8 or more, a lane copies a page's rows in one
 // tensor copy; 16-byte copies by three warps otherwise. On 128 requests of 2000 keys and pages of 8 the first takes 125 us
@@ -66,10 +68,12 @@ constexpr int kStreamRows = 128;  // rows of a stream
 // streams. Of eight sets around the measured times the one that is within 3 % of the best on every batch.
 constexpr int kUnitCost1 = 14, kTileCost1 = 5, kUnitCost2 = 20, kTileCost2 = 7;
 constexpr int kFewRows = 32;     // up to here the row warps share a unit's rows in joining its parts
-// Up to here a unit's products are 64 rows high instead of 128: its rows are then lanes 0-15 either way. The time of a
-// product hardly matters with so few rows, its power does: 256 single tokens over 1628 keys take 161 us instead
-// of 172 where the GPU is held by its power limit, 152 either way where it is not.
-constexpr int kSmallRows = 16;
+// Up to here a unit's rows are lanes 0-15 of products that are 64 rows high instead of 128, and a thread takes 64 of two
+// rows' scores. The time of a product hardly matters with so few rows, so a second one takes what rounding a weight to bf16
+// leaves off, which leaves 2^-16 of a weight instead of 2^-8: the output of single tokens is then as good as fp32's, 0.0017 of
+// its norm from the exact one (its own rounding) instead of 0.0023. It costs 256 single tokens over 1628 keys 149 -> 152 us,
+// 161 -> 168 where the GPU is held by its power limit; products of 128 rows took 172 there with one product.
+constexpr int kFineRows = 16;
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
 constexpr int kMaxSlots = 10, kDescs = 4;
@@ -234,6 +238,40 @@ __device__ __forceinline__ void ld_across(uint32_t taddr, uint32_t (&r)[8]) {
   asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr));
+}
+// 16 rows' 128 columns: thread T gets, for block b of 8, columns 2 (T % 4), + 1 of row T / 4 in r[4 b], r[4 b + 1] and of
+// row T / 4 + 8 in the next two.
+__device__ __forceinline__ void ld_fine(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+                 "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+                 "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+                 "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+                 "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+                 "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+                 "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+                 "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr));
+}
+// 16 rows' 64 columns: thread T's r[2 b] goes to column 4 b + T % 4 of row T / 4, r[2 b + 1] to the row 8 further.
+__device__ __forceinline__ void st_fine(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// What threads 4 r of the warp hold of rows r and r + 8, for the lane's row.
+__device__ __forceinline__ float of_row(float a, float b, int lane) {
+  const float x = __shfl_sync(0xffffffffu, a, 4 * (lane % 8)), y = __shfl_sync(0xffffffffu, b, 4 * (lane % 8));
+  return lane & 8 ? y : x;
 }
 __device__ __forceinline__ uint32_t ld1(uint32_t taddr) {
   uint32_t r;
@@ -875,8 +913,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       commit(tl.s_full[s]);
       arrive(tl.s_full[s]);  // passes on the tile's key mask, which this thread got with the tile
     };
-    // By one lane: O_s (+)= P_s V of a ring slot, half of its keys.
-    auto issue_o = [&](int s, int slot, int half, bool accumulate) {
+    // By one lane: O_s (+)= P_s V of a ring slot, half of its keys; the product of the weights' rests too where they have some.
+    auto issue_o = [&](int s, int slot, int half, bool accumulate, bool fine) {
       const uint64_t vd = v_desc + (uint32_t)slot * (L::kItem / 16);
 #pragma unroll
       for (int k0 = 0; k0 < kTile / 32; ++k0) {
@@ -884,6 +922,13 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, vd + ks * 2 * L::kGroup / 16, kIdO | height,
                accumulate || ks > 0);
       }
+      if (fine)
+#pragma unroll
+        for (int k0 = 0; k0 < kTile / 32; ++k0) {
+          const int ks = k0 + half * (kTile / 32);
+          mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + kTile / 2 + 8 * ks, vd + ks * 2 * L::kGroup / 16,
+                 kIdO | height, true);
+        }
     };
     for (int n = 0;; ++n) {
       const int slot = n % kDescs;
@@ -893,7 +938,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       if (u.mode == kStop || gave_up(abort)) break;
       if (u.tiles == 0) continue;
       const bool two = u.rows > p.tokens * G;  // two streams of rows share each tile, or one's two halves take turns
-      height = tc::idesc_bf16(u.rows <= kSmallRows ? 64 : kStreamRows, 0) & ~tc::idesc_bf16(0, 0);
+      const bool fine = u.rows <= kFineRows;
+      height = tc::idesc_bf16(fine ? 64 : kStreamRows, 0) & ~tc::idesc_bf16(0, 0);
       const int stride = two ? 1 : 2;          // tiles from one of a stream to its next
       const int held = held_keys(p, u.keys);
       Ring ahead = at;  // of the next tile whose scores are due
@@ -940,12 +986,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           if (t >= 0) {
             wait(tl.p_half[s], (parity >> s) & 1u, abort);
             tc::fence_after();
-            if (elect()) issue_o(s, v.slot, 0, t >= stride || found);
+            if (elect()) issue_o(s, v.slot, 0, t >= stride || found, fine);
             __syncwarp();
             wait(tl.p_full[s], (parity >> s) & 1u, abort);
             tc::fence_after();
             if (elect()) {
-              issue_o(s, v.slot, 1, true);
+              issue_o(s, v.slot, 1, true, fine);
               if (s == s1) commit(tl.empty[v.slot]);
               if (!more) commit(tl.o_full[s]);
             }
@@ -997,9 +1043,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const int stream_rows = p.tokens * G;
       const bool two = u.rows > stream_rows;
       const int first_row = two ? s * stream_rows : 0, rows = min(stream_rows, u.rows - first_row);
+      const bool fine = u.rows <= kFineRows;
       const bool idle = 32 * (warp % 4) >= rows;  // no lane of the warp has a row
       const int stride = two ? 1 : 2;
       float m = 0.f, l = 0.f;  // scores are first held against 0
+      float m2[2] = {}, l2[2] = {};  // fine: of rows lane / 4 and 8 further; l of this thread's keys only
+      bool any2[2] = {};             // whether they saw a key
       __nv_bfloat16 gate_raw = __float2bfloat16_rn(0.f);  // on its way while the tiles are worked on
       {
         int lo = 0, hi = INT32_MAX;  // a lane without a row sees everything; it is not stored
@@ -1023,8 +1072,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           if (idle) {  // its rows are stored nowhere; zeros, because products of them take less power than of scores
             scans += scan;
             const uint32_t zero[32] = {};
-            st32(col_s, zero);
-            st32(col_s + 32, zero);
+#pragma unroll 1
+            for (int c = 0; c < (fine ? 4 : 2); ++c) st32(col_s + 32 * c, zero);
             tc::st_wait();
             tc::fence_before();
             __syncwarp();
@@ -1046,15 +1095,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           };
           const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
           uint64_t minus, sum2[2] = {0, 0};
-          // Whether the weights formed with m hold for a tile whose largest score is `top` (NaN: they do); if not, m is set
-          // to it, and the sum and the accumulator follow.
-          auto holds = [&](float top) {
-            top *= p.scale_log2;
-            const bool off = top > m + kRescale || (l == 0.f && top < m - kRescale && top > -INFINITY);
-            if (!__any_sync(0xffffffffu, off)) return true;
+          auto rescale = [&](float corr) {  // the lane's row of the accumulator
             if (t >= stride) {
-              const float corr = off && l != 0.f ? ex2(m - top) : 1.f;  // without a key so far both are 0
-              l *= corr;
 #pragma unroll 1
               for (int c = 0; c < HD / 16; ++c) {
                 uint32_t o[16];
@@ -1065,6 +1107,16 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                 tc::st16(col_o + 16 * c, o);
               }
             }
+          };
+          // Whether the weights formed with m hold for a tile whose largest score is `top` (NaN: they do); if not, m is set
+          // to it, and the sum and the accumulator follow.
+          auto holds = [&](float top, float below) {
+            top *= p.scale_log2;
+            const bool off = top > m + kRescale || (l == 0.f && top < m + below && top > -INFINITY);
+            if (!__any_sync(0xffffffffu, off)) return true;
+            const float corr = off && l != 0.f ? ex2(m - top) : 1.f;  // without a key so far both are 0
+            l *= corr;
+            rescale(corr);
             if (off) m = top;
             return false;
           };
@@ -1074,7 +1126,89 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             __syncwarp();
             if (lane == 0) arrive(bar);
           };
-          if (partly) {  // 32 keys at a time, without those that no row of the warp sees; first their largest score
+          if (fine) {
+            // Two rows' keys 8 b + 2 (lane % 4), + 1: x[4 b], x[4 b + 1] of row lane / 4, the next two of the row 8 further.
+            uint32_t x[64], hi16[32], rest[32];
+            ld_fine(col_s, x);
+            const uint64_t less = pack2(-1.f + 0x1p-24f, -1.f + 0x1p-24f);
+            tc::ld_wait();
+            if (partly) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  const unsigned word = seen(c);
+                  const unsigned wa = __shfl_sync(0xffffffffu, word, lane / 4) >> 2 * (lane % 4);
+                  const unsigned wb = __shfl_sync(0xffffffffu, word, lane / 4 + 8) >> 2 * (lane % 4);
+#pragma unroll
+                  for (int b = 0; b < 4; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                      if (!((e < 2 ? wa : wb) >> (8 * b + e % 2) & 1u)) x[16 * c + 4 * b + e] = 0xff800000u;
+                }
+            }
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int q = 0; q < 32; ++q)
+              top[q % 2] = fmaxf(fmaxf(top[q % 2], __uint_as_float(x[2 * q])), __uint_as_float(x[2 * q + 1]));
+            bool off[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+              top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * p.scale_log2;
+              off[r] = top[r] > m2[r] + kRescale || (!any2[r] && top[r] < m2[r] - kRescale && top[r] > -INFINITY);
+            }
+            if (__any_sync(0xffffffffu, off[0] || off[1])) {
+              float corr[2];
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                corr[r] = off[r] && any2[r] ? ex2(m2[r] - top[r]) : 1.f;
+                l2[r] *= corr[r];
+                if (off[r]) m2[r] = top[r];
+              }
+              rescale(of_row(corr[0], corr[1], lane));
+            }
+            any2[0] |= top[0] > -INFINITY;
+            any2[1] |= top[1] > -INFINITY;
+            const uint64_t minus_a = pack2(-m2[0], -m2[0]), minus_b = pack2(-m2[1], -m2[1]);
+            sum2[0] = sum2[1] = 0;
+            constexpr int kPairs = 4, kGroups = 32 / kPairs;
+            float e[2][2 * kPairs];
+#pragma unroll
+            for (int g = 0; g <= kGroups; ++g)
+#pragma unroll
+              for (int i = 0; i < kPairs; ++i) {
+                if (g < kGroups) {
+                  const int q = g * kPairs + i;
+                  float a, z;
+                  unpack2(fma2(pack2(__uint_as_float(x[2 * q]), __uint_as_float(x[2 * q + 1])), scale2, q % 2 ? minus_b : minus_a),
+                          a, z);
+                  e[g % 2][2 * i] = ex2(a);
+                  e[g % 2][2 * i + 1] = ex2(z);
+                }
+                if (g > 0) {
+                  // A weight's upper 16 bits, and the rest. 2^-24 of the weight stays in the rest, so that it is not 0 where the
+                  // weight is not: 0 times an infinite value would be NaN.
+                  const int q = (g - 1) * kPairs + i;
+                  const uint64_t w = pack2(e[(g + 1) % 2][2 * i], e[(g + 1) % 2][2 * i + 1]);
+                  const uint32_t a = __float_as_uint(e[(g + 1) % 2][2 * i]) & 0xffff0000u;
+                  const uint32_t z = __float_as_uint(e[(g + 1) % 2][2 * i + 1]) & 0xffff0000u;
+                  sum2[i % 2] = add2(sum2[i % 2], w);
+                  hi16[q] = a >> 16 | z;
+                  float r0, r1;
+                  unpack2(fma2(pack2(__uint_as_float(a), __uint_as_float(z)), less, w), r0, r1);
+                  rest[q] = to_bf16x2(r0, r1);
+                }
+              }
+            st_fine(col_s, hi16);
+            st_fine(col_s + kTile / 2, rest);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              float a, z;
+              unpack2(sum2[r], a, z);
+              l2[r] += a + z;
+            }
+            sum2[0] = sum2[1] = 0;
+            if (!scan) hand_over(tl.p_half[s]);
+          } else if (partly) {  // 32 keys at a time, without those that no row of the warp sees; first their largest score
             float top = -INFINITY;
             auto scores = [&](int c, uint32_t (&y)[32]) {  // those that the row does not see as -infinity; whether any row sees one
               const unsigned word = seen(c);
@@ -1100,7 +1234,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               }
               top = fmaxf(top, t2);
             }
-            holds(top);
+            // The first keys of a unit's row set m to their largest score, whose weight is 1 then, and exact.
+            holds(top, t < stride ? kRescale : -kRescale);
             minus = pack2(-m, -m);
             sum2[0] = sum2[1] = 0;
 #pragma unroll 1
@@ -1171,7 +1306,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               sum2[0] = sum2[1] = 0;
               tc::ld_wait();
               weigh(0, packed);
-            } while (!holds(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))));
+            } while (!holds(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])), -kRescale));
             st32(col_s, packed);
             if (!scan) hand_over(tl.p_half[s]);
             weigh(1, packed);
@@ -1226,6 +1361,15 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         }
         tc::fence_after();
       };
+      if (fine) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          l2[r] += __shfl_xor_sync(0xffffffffu, l2[r], 1);
+          l2[r] += __shfl_xor_sync(0xffffffffu, l2[r], 2);
+        }
+        m = of_row(m2[0], m2[1], lane);
+        l = of_row(l2[0], l2[1], lane);
+      }
       tile_no += u.tiles;
       if (l == 0.f) m = -INFINITY;  // no key seen: the row counts for nothing where parts are joined
       int own = 32 * (warp % 4) + lane;
