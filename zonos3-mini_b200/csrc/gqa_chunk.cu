@@ -12,13 +12,16 @@
 // stream and tile: S = Q K^T (tcgen05, fp32 in tensor memory); a thread takes a row, finds its maximum, forms p = 2^(s
 // scale log2 e - m), adds up its sum in fp32 and writes p back over S as bf16; O += P V with P read from tensor memory.
 // The two streams share each tile's K and V in shared memory and take turns: one's exponentials run while the tensor
-// cores work for the other. The subtracted m cancels in the final division, so it need not be the maximum: it starts at 0
-// and only moves to the largest score of a tile that is more than 64 above it (or, for a row's first keys, below), which
-// keeps p within 2^64, sums and accumulators far inside fp32's range, and the largest weights' precision. So the search for
-// the maximum runs beside the exponentials instead of before them, and the accumulator is hardly ever rescaled.
+// cores work for the other. The subtracted m cancels in the final division, so it need not be the maximum: it lies at it
+// or up to 16 (log2) above it, and moves to 16 above a tile's largest score when that is larger than m. So no p is above 1, as
+// with the maximum itself: the accumulator stays below sum |v_j|, and no finite values overflow that do not with exact
+// softmax; and the largest p is at least 2^-16, so that what falls below fp32's 2^-126 is below 2^-110 of the largest. m starts
+// at 16, which holds for first keys whose largest score is 0 to 16 (with q and k normalised to a mean square of 1, no score
+// of 128 dims is above 16.3). So the search for the maximum runs beside the exponentials instead of before them, and the
+// accumulator is hardly ever rescaled.
 // p is rounded to bf16 because the tensor cores multiply bf16; its sum is kept from before the rounding. Where that would
 // be the largest error for nothing it is avoided: units of few rows multiply what the rounding left off too, and rows whose
-// first keys lie in a partly visible tile start with m at their largest score, whose p is 1.
+// first keys lie in a partly visible tile start with m 16 above their largest score, whose p is 2^-16 and exact.
 //
 // The lengths live on the device, so the split of the work does too: every CTA adds up the tiles of all units (a scan
 // over the requests) and takes an equal run of them. A unit that spans CTAs leaves partial results (accumulator,
@@ -78,7 +81,7 @@ constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
 constexpr int kMaxSlots = 10, kDescs = 4;
 constexpr int kMasks = 8;  // of key masks and of looked-through tiles: the loaders run at most 5 tiles ahead of the rows
-constexpr float kRescale = 64.f;  // how far (log2) a row's largest score may be from the m that is subtracted
+constexpr float kAbove = 16.f;  // how far (log2) the m that is subtracted may lie above a row's largest score
 constexpr int kMaxRequests = 16384;
 
 // n / d and n % d for 0 <= n < 2^31 by a multiplication: m = ceil(2^(31 + l) / d) with 2^l >= d.
@@ -1046,7 +1049,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const bool fine = u.rows <= kFineRows;
       const bool idle = 32 * (warp % 4) >= rows;  // no lane of the warp has a row
       const int stride = two ? 1 : 2;
-      float m = 0.f, l = 0.f;  // scores are first held against 0
+      float m = kAbove, l = 0.f;
       float m2[2] = {}, l2[2] = {};  // fine: of rows lane / 4 and 8 further; l of this thread's keys only
       bool any2[2] = {};             // whether they saw a key
       __nv_bfloat16 gate_raw = __float2bfloat16_rn(0.f);  // on its way while the tiles are worked on
@@ -1109,11 +1112,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             }
           };
           // Whether the weights formed with m hold for a tile whose largest score is `top` (NaN: they do); if not, m is set
-          // to it, and the sum and the accumulator follow.
-          auto holds = [&](float top, float below) {
+          // by it, and the sum and the accumulator follow. `set`: first keys set m whatever it is.
+          auto holds = [&](float top, bool set) {
             top *= p.scale_log2;
-            const bool off = top > m + kRescale || (l == 0.f && top < m + below && top > -INFINITY);
+            const bool off = top > m || (l == 0.f && (set || top < m - kAbove) && top > -INFINITY);
             if (!__any_sync(0xffffffffu, off)) return true;
+            top += kAbove;
             const float corr = off && l != 0.f ? ex2(m - top) : 1.f;  // without a key so far both are 0
             l *= corr;
             rescale(corr);
@@ -1154,15 +1158,15 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             for (int r = 0; r < 2; ++r) {
               top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
               top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * p.scale_log2;
-              off[r] = top[r] > m2[r] + kRescale || (!any2[r] && top[r] < m2[r] - kRescale && top[r] > -INFINITY);
+              off[r] = top[r] > m2[r] || (!any2[r] && top[r] > -INFINITY);
             }
             if (__any_sync(0xffffffffu, off[0] || off[1])) {
               float corr[2];
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                corr[r] = off[r] && any2[r] ? ex2(m2[r] - top[r]) : 1.f;
+                corr[r] = off[r] && any2[r] ? ex2(m2[r] - (top[r] + kAbove)) : 1.f;
                 l2[r] *= corr[r];
-                if (off[r]) m2[r] = top[r];
+                if (off[r]) m2[r] = top[r] + kAbove;
               }
               rescale(of_row(corr[0], corr[1], lane));
             }
@@ -1234,8 +1238,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               }
               top = fmaxf(top, t2);
             }
-            // The first keys of a unit's row set m to their largest score, whose weight is 1 then, and exact.
-            holds(top, t < stride ? kRescale : -kRescale);
+            // The first keys of a unit's row set m by their largest score, whose weight is a power of 2 then, and exact.
+            holds(top, t < stride);
             minus = pack2(-m, -m);
             sum2[0] = sum2[1] = 0;
 #pragma unroll 1
@@ -1257,7 +1261,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             if (!scan) hand_over(tl.p_half[s]);
           } else {
             // The weights are formed with the m there is, and the tile's largest score is found beside them; nothing is
-            // written over the scores before it is known that they hold. A second turn is rare.
+            // written over the scores before it is known that they hold. A second turn is rare, and the last.
             uint32_t x[kTile];
             // p of a half of the keys. The exponential unit takes 8 cycles an instruction, so everything else has to run in
             // its shadow: the scaling of the next group, the sum and the packing of the one before, and in the first half
@@ -1299,6 +1303,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               }
             };
             uint32_t packed[32];
+            bool again = false;
             do {
 #pragma unroll
               for (int c = 0; c < 4; ++c) ld32(col_s + 32 * c, x + 32 * c);
@@ -1306,7 +1311,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               sum2[0] = sum2[1] = 0;
               tc::ld_wait();
               weigh(0, packed);
-            } while (!holds(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])), -kRescale));
+              again = !again && !holds(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])), false);
+            } while (again);
             st32(col_s, packed);
             if (!scan) hand_over(tl.p_half[s]);
             weigh(1, packed);
