@@ -36,3 +36,36 @@ def test_chunk_values_of_any_size(zb, news, caches, offset, binade):
     _close(out, ref, spread * (2.0 ** -7 * (1 + 2.0 ** -4) + 2 * score[..., None]))
     _close(lse, ref_lse, score)
     assert zb.ops.device_status() == 0
+
+
+FLAG_BYTES = 4096  # of a workspace's start
+
+
+def _workspace_calls(gen):
+    """Calls whose units span CTAs, on grids of 5 CTAs up to all of the GPU's."""
+    calls = []
+    for news, caches, heads, kv, hd, page in (([1], [383], 1, 1, 64, 16), ([1, 40, 3], [9000, 300, 2000], 16, 4, 128, 16),
+                                              ([1], [700], 2, 1, 128, 16), ([3, 1], [4000, 90], 8, 2, 64, 64)):
+        calls.append([t.to(DEV) for t in _chunk_inputs(gen, news, caches, heads, kv, hd, page)])
+    return calls
+
+
+def _need(zb, x):
+    q, k, _, table, _, _ = x
+    return zb.ops.gqa_chunk_workspace_bytes(q.shape[0], q.shape[1], table, k)
+
+
+def test_chunk_calls_of_different_grids_share_a_workspace(zb):
+    """What a call leaves in its parts does not lie where another call has its flags: those are zero after every call, and
+    the results are those on a workspace of their own."""
+    calls = _workspace_calls(torch.Generator().manual_seed(17))
+    needs = [_need(zb, x) for x in calls]
+    assert all(n > 0 for n in needs)
+    shared = torch.zeros(max(needs), dtype=torch.uint8, device=DEV)
+    for i in (0, 1, 2, 0, 3, 1, 2, 1, 0, 3):
+        own = torch.zeros(needs[i], dtype=torch.uint8, device=DEV)
+        expected = zb.ops.gqa_chunk(*calls[i], workspace=own)
+        got = zb.ops.gqa_chunk(*calls[i], workspace=shared)
+        assert torch.equal(got, expected)
+        assert not shared[:FLAG_BYTES].any() and not own[:FLAG_BYTES].any()
+    assert zb.ops.device_status() == 0

@@ -83,6 +83,9 @@ constexpr int kMaxSlots = 10, kDescs = 4;
 constexpr int kMasks = 8;  // of key masks and of looked-through tiles: the loaders run at most 5 tiles ahead of the rows
 constexpr float kAbove = 16.f;  // how far (log2) the m that is subtracted may lie above a row's largest score
 constexpr int kMaxRequests = 16384;
+// The flags' part of a workspace, of every call's alike: calls of different grids take turns on one workspace, and what one
+// leaves in its parts must not lie where another has its flags.
+constexpr int64_t kFlagBytes = 4096;
 
 // n / d and n % d for 0 <= n < 2^31 by a multiplication: m = ceil(2^(31 + l) / d) with 2^l >= d.
 struct Divisor {
@@ -1562,12 +1565,12 @@ Launch plan(int B, int64_t N, int Hq, int Hkv, int hd, int64_t max_keys) {
   const int G = Hq / Hkv, pair_tokens = 2 * (kStreamRows / G);
   const int64_t tiles = std::max<int64_t>((max_keys + kTile - 1) / kTile, 1);
   l.pairs = N / pair_tokens + std::min<int64_t>(B, N);
-  l.ctas = (int)std::min<int64_t>(zb::sm_count(), l.pairs * Hkv * (tiles + kUnitCost2 / kTileCost2));
+  l.ctas = (int)std::min<int64_t>(std::min<int64_t>(zb::sm_count(), kFlagBytes / 4), l.pairs * Hkv * (tiles + kUnitCost2 / kTileCost2));
   l.splits = tiles > 1 && l.ctas > 1;
   l.rows_max = (int)std::min<int64_t>(N, pair_tokens) * G;
   if (l.splits) {
     const int64_t width = hd <= 64 ? 64 : 128;
-    l.flag_bytes = ((int64_t)l.ctas * 4 + 255) / 256 * 256;
+    l.flag_bytes = kFlagBytes;
     l.acc_bytes = (int64_t)l.ctas * 2 * l.rows_max * width * 4;
     l.ml_bytes = (int64_t)l.ctas * 4 * l.rows_max * 4;
   }
