@@ -69,3 +69,21 @@ def test_chunk_calls_of_different_grids_share_a_workspace(zb):
         assert torch.equal(got, expected)
         assert not shared[:FLAG_BYTES].any() and not own[:FLAG_BYTES].any()
     assert zb.ops.device_status() == 0
+
+
+def test_chunk_takes_no_notice_of_flags_that_another_call_left(zb):
+    """A call whose waits gave up can leave its flags raised. On such a workspace, the caller's and the stream's own, later
+    calls wait for their own CTAs all the same."""
+    for x in _workspace_calls(torch.Generator().manual_seed(18)):
+        workspace = torch.zeros(_need(zb, x), dtype=torch.uint8, device=DEV)
+        expected = zb.ops.gqa_chunk(*x, workspace=workspace)
+        for _ in range(3):
+            workspace[FLAG_BYTES:].random_(0, 256)  # and parts that are not this call's
+            workspace[:FLAG_BYTES].view(torch.int32).fill_(1)  # raised by this process's first call
+            assert torch.equal(zb.ops.gqa_chunk(*x, workspace=workspace), expected)
+        zb.ops.gqa_chunk(*x)
+        for own in zb.ops._CHUNK_WS.values():
+            own[FLAG_BYTES:].random_(0, 256)
+            own[:FLAG_BYTES].view(torch.int32).fill_(1)
+        assert torch.equal(zb.ops.gqa_chunk(*x), expected)
+    assert zb.ops.device_status() == 0

@@ -116,9 +116,10 @@ struct ChunkParams {
   __nv_bfloat16* out;  // [N, Hq, hd]
   int64_t out_stride;
   float* lse;  // [N, Hq] or null
-  // workspace: per CTA a flag (0 between calls) and two slots of partial results, rows_max rows each: of the unit that
-  // began before this CTA, and of the one that goes on after it
+  // workspace: per CTA a flag (raised to the call's `raised`, put back to 0 by the CTA that waited for it) and two slots of
+  // partial results, rows_max rows each: of the unit that began before this CTA, and of the one that goes on after it
   unsigned* flags;
+  unsigned raised;  // of every call another, so that a flag left by a call whose waits gave up is no other call's
   float* acc;  // [CTA][2][HD / 4][rows_max][4]
   float* ml;   // [CTA][2][2][rows_max]: maximum, sum
   int rows_max;
@@ -446,16 +447,16 @@ __device__ __forceinline__ float reciprocal(float x) {
 }
 __device__ __forceinline__ float sigmoid(__nv_bfloat16 x) { return reciprocal(1.f + ex2(-1.4426950408889634f * __bfloat162float(x))); }
 
-__device__ __forceinline__ void raise_flag(unsigned* flag) {
-  asm volatile("st.release.gpu.global.u32 [%0], 1;" ::"l"(flag) : "memory");
+__device__ __forceinline__ void raise_flag(unsigned* flag, unsigned raised) {
+  asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(flag), "r"(raised) : "memory");
 }
 // Whether the flag was raised within a second.
-__device__ __forceinline__ bool wait_flag(const unsigned* flag) {
+__device__ __forceinline__ bool wait_flag(const unsigned* flag, unsigned raised) {
   const uint64_t start = zb::globaltimer_ns();
   for (;;) {
     unsigned v;
     asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
-    if (v != 0) return true;
+    if (v == raised) return true;
     if (zb::globaltimer_ns() - start > 1000000000ull) return false;
   }
 }
@@ -464,7 +465,7 @@ __device__ __forceinline__ bool wait_flag(const unsigned* flag) {
 __device__ __forceinline__ bool wait_parts(const ChunkParams& p, const Desc& u, int cta, int lane) {
   bool there = true;
 #pragma unroll 1
-  for (int i = 1 + lane; i < u.parts; i += 32) there = wait_flag(p.flags + cta + i) && there;
+  for (int i = 1 + lane; i < u.parts; i += 32) there = wait_flag(p.flags + cta + i, p.raised) && there;
   there = __all_sync(0xffffffffu, there);
   if (!there && p.status && lane == 0) atomicOr(p.status, zb::kStatusAttnChunkTimeout);
   return there;
@@ -1526,7 +1527,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         if (!done) __threadfence();
         meet();
         if (u.mode == kPart0) {
-          if (tid == 0) raise_flag(p.flags + cta);
+          if (tid == 0) raise_flag(p.flags + cta, p.raised);
         } else {
           if (few && wait_parts(p, u, cta, lane)) join_few<HD>(p, u, cta, tid);
           meet();  // every thread is done with the parts
@@ -1700,6 +1701,9 @@ ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_c
   p.lse = lse;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   p.flags = reinterpret_cast<unsigned*>(ws);
+  static std::atomic<unsigned> calls{0};
+  do p.raised = calls.fetch_add(1, std::memory_order_relaxed) + 1;
+  while (p.raised == 0);
   p.acc = reinterpret_cast<float*>(ws + l.flag_bytes);
   p.ml = reinterpret_cast<float*>(ws + l.flag_bytes + l.acc_bytes);
   p.rows_max = l.rows_max;

@@ -1150,8 +1150,9 @@ def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, s
     contiguous [N, Hq] fp32 tensor that receives the natural logarithm of the softmax denominators. A token that sees
     no key, or belongs to no request, gets zeros and an lse of -inf. The lengths are read on the device: a captured
     graph follows them. workspace: optional uint8 tensor of at least :func:`gqa_chunk_workspace_bytes` bytes, its first
-    4096 zero before the first call (every call leaves them zero) and not shared by calls that may overlap; absent, the
-    stream's own is used. hd: a multiple of 8 up to 128. Returns out [N, Hq, hd] bf16."""
+    4096 zero before the first call and not shared by calls that may overlap (a call leaves them zero unless its waits gave
+    up, :func:`device_status` bit 64; eager calls take no notice of what that left, a captured one asks for zeros again before
+    its next replay); absent, the stream's own is used. hd: a multiple of 8 up to 128. Returns out [N, Hq, hd] bf16."""
     paged, index, Hkv, hd = _paged(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, None)
     N, Hq = q.shape[0], q.shape[1]
     q_stride = _token_rows("q", q, index, N, Hq, hd)
@@ -1188,7 +1189,7 @@ def _chunk_workspace_bytes(B, N, Hq, Hkv, hd, max_keys) -> int:
     return _lib.load().zb_gqa_chunk_workspace_bytes(B, N, Hq, Hkv, hd, max_keys)
 
 
-_CHUNK_WS: dict = {}  # (device, stream) -> the workspace of eager calls on that stream (its flags zero between calls)
+_CHUNK_WS: dict = {}  # (device, stream) -> the workspace of eager calls on that stream (flags another call left do not count)
 _CHUNK_FLAG_BYTES = 4096  # the flags lie at the workspace's start
 
 
