@@ -657,8 +657,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     __syncthreads();
 #pragma unroll 1
     for (uint32_t i = tid; i < L::kOffTail / 16; i += kThreads) reinterpret_cast<uint4*>(gbase)[i] = make_uint4(0, 0, 0, 0);
-    tc::fence_proxy_async();
   }
+  tc::fence_proxy_async();  // the plan's tables and the zeros come before the tensor copies over them
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
