@@ -320,8 +320,8 @@ int zb_gqa_prologue_decode(const uint16_t* proj, int64_t proj_stride, const uint
 
 /* The new tokens of a ragged batch over a paged KV cache. Both entry points below describe the batch the same way (all
  * device pointers; nothing is read on the host, so captured graphs follow the lengths):
- *   cu_seqlens_q [B + 1] int32, non-decreasing: request b's new tokens are rows cu[b] .. cu[b + 1] of the N rows; rows
- *                outside [cu[0], cu[B]) belong to no request
+ *   cu_seqlens_q [B + 1] int32, non-decreasing, within [0, N]: request b's new tokens are rows cu[b] .. cu[b + 1] of the
+ *                N rows; rows outside [cu[0], cu[B]) belong to no request
  *   cache_seqlens [B] int32: request b's keys, its new tokens included as the last ones: row t is key position
  *                cache_seqlens[b] - (cu[b + 1] - t)
  *   page_table   [B, table_stride] int32 with max_pages columns: position j lives in row j % page_size of page
@@ -354,7 +354,8 @@ int zb_gqa_append(const uint16_t* proj, int64_t proj_stride, const uint16_t* tem
  * least zb_gqa_chunk_workspace_bytes(B, N, Hq, Hkv, hd, page_size * max_pages) bytes, not shared by overlapping calls; its
  * first 4096 bytes (flags) must be zero before the first call and are left zero by each. A call whose waits gave up (status bit
  * 64) may leave some non-zero. Later calls take no notice, as each raises them to a value of its own; a captured call has one
- * value for all its replays, so zero them before it is replayed again. Status bit 128: cu_seqlens_q decreases, nothing was written. */
+ * value for all its replays, so zero them before it is replayed again. Status bit 128: cu_seqlens_q
+ * decreases or leaves [0, N], nothing was written. */
 int64_t zb_gqa_chunk_workspace_bytes(int B, int N, int Hq, int Hkv, int hd, int64_t max_keys);
 int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache,
                  int64_t page_stride, int64_t slot_stride, int64_t head_stride, int64_t num_pages, int page_size,

@@ -87,3 +87,31 @@ def test_chunk_takes_no_notice_of_flags_that_another_call_left(zb):
             own[:FLAG_BYTES].view(torch.int32).fill_(1)
         assert torch.equal(zb.ops.gqa_chunk(*x), expected)
     assert zb.ops.device_status() == 0
+
+
+@pytest.mark.parametrize("cu", [[0, 5, 3, 8], [0, 10, 5, 20], [3, 2, 2, 2], [0, 400, 0, 400], [-1, 2, 3, 8], [0, 2, 5, 9],
+                                [0, 2, 1 << 30, 8]])
+def test_chunk_refuses_bounds_out_of_order(zb, cu):
+    """cu_seqlens_q that decreases, or leaves the rows there are, is the device status's bit 128, and nothing is written."""
+    gen = torch.Generator().manual_seed(19)
+    N = 8 if cu[-1] == 9 else max(cu[-1], 4)  # [.., 9]: one row more than there is
+    q, k, v, table, seqlens, _ = (t.to(DEV) for t in _chunk_inputs(gen, [N, 1, 1], [40, 300, 70], 8, 2, 64, 16))
+    out, lse = torch.full_like(q[:N], 3.0), torch.full((N, 8), 7.0, device=DEV)
+    zb.ops.device_status()
+    zb.ops.gqa_chunk(q[:N], k, v, table, seqlens, torch.tensor(cu, dtype=torch.int32, device=DEV), out=out, lse=lse)
+    assert zb.ops.device_status() == 128
+    assert out.eq(3.0).all() and lse.eq(7.0).all()
+
+
+def test_chunk_takes_bounds_at_the_ends(zb):
+    """Requests without tokens at either end, and all rows of no request, are in order."""
+    gen = torch.Generator().manual_seed(20)
+    q, k, v, table, seqlens, _ = (t.to(DEV) for t in _chunk_inputs(gen, [6, 1, 1], [40, 300, 70], 8, 2, 64, 16))
+    for cu in ([0, 0, 8, 8], [8, 8, 8, 8], [0, 0, 0, 0], [0, 8, 8, 8]):
+        lse = torch.full((8, 8), 7.0, device=DEV)
+        bounds = torch.tensor(cu, dtype=torch.int32)
+        out = zb.ops.gqa_chunk(q, k, v, table, seqlens, bounds.to(DEV), lse=lse)
+        ref, spread, ref_lse, _ = paged.chunk(*(t.cpu() for t in (q, k, v, table, seqlens)), bounds)
+        _close(out, ref, 2.0 ** -7 * (1 + 2.0 ** -4) * spread)
+        assert torch.equal(lse.cpu() == -torch.inf, ref_lse == -torch.inf)
+        assert zb.ops.device_status() == 0

@@ -48,7 +48,7 @@ enum DeviceStatusBits : unsigned {
   kStatusAttnDecodeTimeout = 1u << 4,
   kStatusEmbedIndex = 1u << 5,  // an embedding id outside its table (read as a zero row)
   kStatusAttnChunkTimeout = 1u << 6,
-  kStatusAttnChunkBatch = 1u << 7,  // a chunk attention call whose cu_seqlens_q decreases (no output written)
+  kStatusAttnChunkBatch = 1u << 7,  // a chunk attention call whose cu_seqlens_q decreases or leaves [0, N] (nothing written)
 };
 
 }  // namespace zb

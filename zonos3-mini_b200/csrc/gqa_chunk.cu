@@ -123,7 +123,6 @@ struct ChunkParams {
   float* acc;  // [CTA][2][HD / 4][rows_max][4]
   float* ml;   // [CTA][2][2][rows_max]: maximum, sum
   int rows_max;
-  int pairs_max;  // units of a KV head, at most
   unsigned* status;
   int box, box_shift;  // rows of a page that one tensor copy brings; 0: K and V rows come by 16-byte copies
   int head_atoms, page_heads;  // a KV head's atom offset, and a page's index step, in the tensor maps
@@ -583,19 +582,20 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   if (tid < B) requests[tid] = mine;
   int64_t all_pairs = 0;
   int buffer = 0;
+  bool out_of_order = false;  // bounds that decrease or leave the rows: two requests would write the same ones
 #pragma unroll 1
   for (int b0 = 0; b0 < B; b0 += kThreads, buffer ^= 1) {
     const int b = b0 + tid;
     const int n = b < B ? stream_pairs(p, b0 == 0 ? mine.tokens : request(p, b).tokens) : 0;
+    if (b < B) out_of_order |= p.kv.cu[b + 1] < p.kv.cu[b] || p.kv.cu[b] < 0 || p.kv.cu[b + 1] > p.kv.N;
     int total;
     const int before = block_scan(n, tl, buffer, total);
     if (b < B) pairs_before[b] = (int)(all_pairs + before);
     all_pairs += total;
   }
-  __syncthreads();
-  // more than the tokens can make: cu decreases somewhere, nothing is done
-  const int pairs = all_pairs <= p.pairs_max ? (int)all_pairs : 0;
-  if (all_pairs > p.pairs_max && blockIdx.x == 0 && tid == 0 && p.status) atomicOr(p.status, zb::kStatusAttnChunkBatch);
+  const bool refused = __syncthreads_or(out_of_order);  // nothing is done then
+  const int pairs = refused ? 0 : (int)all_pairs;
+  if (refused && blockIdx.x == 0 && tid == 0 && p.status) atomicOr(p.status, zb::kStatusAttnChunkBatch);
   struct Pair {
     int b, pair, work;  // work: for one KV head
   };
@@ -1539,7 +1539,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     }
   }
   // ---- rows of no request
-  const int idle = tl.idle[0] + p.kv.N - tl.idle[1];
+  const int idle = refused ? 0 : tl.idle[0] + p.kv.N - tl.idle[1];
 #pragma unroll 1
   for (int i = cta * (kThreads / 32) + warp; i < idle; i += ctas * (kThreads / 32)) {
     const int64_t t = i < tl.idle[0] ? i : tl.idle[1] + i - tl.idle[0];
@@ -1561,15 +1561,15 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 struct Launch {
   int ctas, rows_max;
   bool splits;
-  int64_t pairs, flag_bytes, acc_bytes, ml_bytes;
+  int64_t flag_bytes, acc_bytes, ml_bytes;
 };
 Launch plan(int B, int64_t N, int Hq, int Hkv, int hd, int64_t max_keys) {
   Launch l{};
   if (Hkv < 1 || B < 1 || N < 1 || Hq < Hkv || Hq / Hkv > kStreamRows) return l;
   const int G = Hq / Hkv, pair_tokens = 2 * (kStreamRows / G);
   const int64_t tiles = std::max<int64_t>((max_keys + kTile - 1) / kTile, 1);
-  l.pairs = N / pair_tokens + std::min<int64_t>(B, N);
-  l.ctas = (int)std::min<int64_t>(std::min<int64_t>(zb::sm_count(), kFlagBytes / 4), l.pairs * Hkv * (tiles + kUnitCost2 / kTileCost2));
+  const int64_t pairs = N / pair_tokens + std::min<int64_t>(B, N);  // units of a KV head, at most
+  l.ctas = (int)std::min<int64_t>(std::min<int64_t>(zb::sm_count(), kFlagBytes / 4), pairs * Hkv * (tiles + kUnitCost2 / kTileCost2));
   l.splits = tiles > 1 && l.ctas > 1;
   l.rows_max = (int)std::min<int64_t>(N, pair_tokens) * G;
   if (l.splits) {
@@ -1707,7 +1707,6 @@ ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_c
   p.acc = reinterpret_cast<float*>(ws + l.flag_bytes);
   p.ml = reinterpret_cast<float*>(ws + l.flag_bytes + l.acc_bytes);
   p.rows_max = l.rows_max;
-  p.pairs_max = (int)l.pairs;
   p.status = zb::device_status_ptr();
   return hd <= 64 ? launch_chunk<64>(p, l, stream) : launch_chunk<128>(p, l, stream);
 }

@@ -1149,7 +1149,8 @@ def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, s
     stride allowed); head h's output is multiplied by sigmoid(gate[t, h]) before its one rounding. lse: optional
     contiguous [N, Hq] fp32 tensor that receives the natural logarithm of the softmax denominators. A token that sees
     no key, or belongs to no request, gets zeros and an lse of -inf. The lengths are read on the device: a captured
-    graph follows them. workspace: optional uint8 tensor of at least :func:`gqa_chunk_workspace_bytes` bytes, its first
+    graph follows them, and cu_seqlens_q that decreases or leaves [0, N] shows as :func:`device_status` bit 128 (nothing is
+    written then). workspace: optional uint8 tensor of at least :func:`gqa_chunk_workspace_bytes` bytes, its first
     4096 zero before the first call and not shared by calls that may overlap (a call leaves them zero unless its waits gave
     up, :func:`device_status` bit 64; eager calls take no notice of what that left, a captured one asks for zeros again before
     its next replay); absent, the stream's own is used. hd: a multiple of 8 up to 128. Returns out [N, Hq, hd] bf16."""
