@@ -350,14 +350,18 @@ __device__ __forceinline__ bool mixed_tile(const Desc& u, int first) { return fi
 
 // A wait that gives up after about a second (a try that may sleep comes back after 4 us), and at once after any earlier one
 // of the CTA did. Short, because it stands in many places of loops that fill the instruction cache: the status is set at
-// the kernel's end.
-__device__ __forceinline__ void wait(const uint64_t& bar, uint32_t parity, int* abort) {
+// the kernel's end. False: it gave up. Only those who copy into what they waited for have to stop then; what the others go on
+// to read and write is the CTA's own, up to the end of the unit.
+__device__ __forceinline__ bool wait(const uint64_t& bar, uint32_t parity, int* abort) {
   const uint32_t at = zb::smem_addr(&bar);
-  if (zb::mbar_try_wait(at, parity)) return;
+  if (zb::mbar_try_wait(at, parity)) return true;
 #pragma unroll 1
-  for (int i = 0; i < 250000; ++i)
-    if (zb::mbar_try_wait_sleep(at, parity, 20000u) || *reinterpret_cast<volatile int*>(abort) != 0) return;
+  for (int i = 0; i < 250000; ++i) {
+    if (zb::mbar_try_wait_sleep(at, parity, 20000u)) return true;
+    if (*reinterpret_cast<volatile int*>(abort) != 0) return false;
+  }
   *reinterpret_cast<volatile int*>(abort) = 1;
+  return false;
 }
 // The same answer for every lane of the warp.
 __device__ __forceinline__ bool gave_up(int* abort) {
@@ -719,7 +723,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     const int unit0 = unit_cost(p, d);
     int kvh = (int)(tl.start_off / unit0), off = (int)(tl.start_off % unit0);
     int item = 0, tile_no = 0, q_item = 0, scans = 0, n = 0;
-    for (;;) {
+    bool going = true;  // until a wait for room gave up
+    auto room = [&](const uint64_t& bar, uint32_t parity) {
+      going = __all_sync(0xffffffffu, wait(bar, parity, abort));
+      return going;
+    };
+    while (going) {
       // ---- the unit's tiles here: those that begin in this CTA's share, at least as long as any tile
       const int unit = unit_cost(p, d), to = (int)min((int64_t)unit, off + (end - at));
       const int from_tile = tile_behind(p, d, off), to_tile = tile_behind(p, d, to);
@@ -744,13 +753,15 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         // CTAs that hold a part of it from this one on
         const int64_t last = at - off + unit - (u.rows > p.tokens * G ? kTileCost2 : kTileCost1);  // its last tile
         u.parts = ends ? 1 : last < INT32_MAX ? (int)last / (int)share - cta + 1 : (int)(last / share) - cta + 1;
-        if (warp == kLoadWarp && lane == 0) {
+        if (warp == kLoadWarp) {
           const int slot = n % kDescs;
-          if (n >= kDescs) wait(tl.desc_empty[slot], (n / kDescs - 1) & 1, abort);
-          tl.desc[slot] = u;
-          arrive(tl.desc_full[slot]);
+          if (n >= kDescs && !room(tl.desc_empty[slot], (n / kDescs - 1) & 1)) break;
+          if (lane == 0) {
+            tl.desc[slot] = u;
+            arrive(tl.desc_full[slot]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
         ++n;
         if (u.mode == kStop) break;
       } else {
@@ -761,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll 1
           for (int s = 0; s < (u.rows > p.tokens * G ? 2 : 1); ++s, ++q_item) {
             const int slot = q_item % 2;
-            if (q_item >= 2) wait(tl.q_empty[slot], (q_item / 2 - 1) & 1, abort);
+            if (q_item >= 2 && !room(tl.q_empty[slot], (q_item / 2 - 1) & 1)) break;
             if (lane == 0) {
               zb::mbar_arrive_expect_tx(zb::smem_addr(&tl.q_full[slot]), (uint32_t)(p.tokens * G * HD * 2));
 #pragma unroll 1
@@ -798,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         if (p.box) {
           if (warp == kLoadWarp) {
 #pragma unroll 1
-            for (int t = 0; t < u.tiles; ++t, ++tile_no) {
+            for (int t = 0; t < u.tiles && going; ++t, ++tile_no) {
               const int first = (u.tile0 + t) * kTile, pos = first + lane * p.box;
               const bool there = next >= 0 && next < p.kv.num_pages;
               const int page = there ? next * p.page_heads + (p.page_heads > 1 ? kvh : 0)
@@ -815,7 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll 1
               for (int kv = 0; kv < 2; ++kv, ++item) {
                 const int slot = item % L::kSlots;
-                if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort);
+                if (item >= L::kSlots && !room(tl.empty[slot], (item / L::kSlots - 1) & 1)) break;
                 if (lane == 0) {
                   if (kv == 0) *reinterpret_cast<uint4*>(tl.mask[tile_no % kMasks]) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
                   zb::mbar_arrive_expect_tx(zb::smem_addr(&tl.full[slot]), L::kItem);
@@ -841,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           };
           look(u.tile0);
 #pragma unroll 1
-          for (int t = 0; t < u.tiles; ++t, ++tile_no) {
+          for (int t = 0; t < u.tiles && going; ++t, ++tile_no) {
             int64_t off[4];
             unsigned bits[4];
 #pragma unroll
@@ -857,7 +868,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll 1
             for (int kv = 0; kv < 2; ++kv, ++item) {
               const int slot = item % L::kSlots;
-              if (item >= L::kSlots) wait(tl.empty[slot], (item / L::kSlots - 1) & 1, abort);
+              if (item >= L::kSlots && !room(tl.empty[slot], (item / L::kSlots - 1) & 1)) break;
               copy_tile(base + slot * L::kItem, kv ? p.kv.v : p.kv.k, off, item);
               cp_async_arrive(zb::smem_addr(&tl.full[slot]));
               if (warp == kLoadWarp && lane == 0) {
@@ -865,7 +876,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                 arrive(tl.full[slot]);
               }
             }
-            look_through(t, item - 1);
+            if (going) look_through(t, item - 1);
           }
         }
       }
@@ -889,6 +900,15 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    // Nothing is in flight when the CTA's shared memory goes to another, also where a wait gave up: a lane waits for the last
+    // copies into a slot.
+    auto landed = [&](const uint64_t* full, int slots, int items) {
+      if (lane < min(slots, items))
+        zb::mbar_wait_bounded(zb::smem_addr(full + lane), (items - 1 - lane) / slots & 1, p.status, zb::kStatusAttnChunkTimeout);
+      __syncwarp();
+    };
+    if (warp == kLoadWarp && p.box) landed(tl.full, L::kSlots, item);
+    if (warp == kLoadWarp + 1) landed(tl.q_full, 2, q_item);
   } else if (warp == kMmaWarp) {
     // =============================================================================================== tensor cores
     asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
