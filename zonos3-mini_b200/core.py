@@ -34,13 +34,14 @@ class AttnMetadata:
 
     With ``cu_seqlens_q`` as a [B + 1] int32 device tensor the layers run the paged operators: ``page_table`` then holds
     pages of the pool's page size, a new row's slot and rotary position follow from the lengths, and ``positions`` (else
-    None) overrides the latter; ``out_loc`` is not read."""
+    None) overrides the latter; ``out_loc`` is not read. A decode batch over a pool of page size 1 that has ``positions``
+    and ``out_loc`` runs the decode kernels all the same."""
 
     positions: "torch.Tensor | None"  # [N] int32
     out_loc: "torch.Tensor | None"  # [N] int32
     page_table: "torch.Tensor"  # [B, max_len] int32
     cache_seqlens: "torch.Tensor"  # [B] int32
-    # request b's new rows are [cu[b], cu[b+1]): a host list for a prefill, or a device tensor for any batch
+    # request b's new rows are [cu[b], cu[b+1]): a host list or tensor for a prefill, an int32 device tensor for any batch
     cu_seqlens_q: "list[int] | torch.Tensor | None" = None
 
 
