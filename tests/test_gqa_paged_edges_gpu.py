@@ -115,3 +115,28 @@ def test_chunk_takes_bounds_at_the_ends(zb):
         _close(out, ref, 2.0 ** -7 * (1 + 2.0 ** -4) * spread)
         assert torch.equal(lse.cpu() == -torch.inf, ref_lse == -torch.inf)
         assert zb.ops.device_status() == 0
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5, 2 ** 40])
+def test_chunk_windows_past_32_bits(zb, window):
+    """A window longer than any cache is none."""
+    gen = torch.Generator().manual_seed(21)
+    x = [t.to(DEV) for t in _chunk_inputs(gen, [40, 1], [260, 511], 8, 2, 64, 16)]
+    assert torch.equal(zb.ops.gqa_chunk(*x, window=window), zb.ops.gqa_chunk(*x))
+
+
+@pytest.mark.parametrize("window", [-1, -(2 ** 32) + 5, -(2 ** 31)])
+def test_chunk_refuses_negative_windows(zb, window):
+    gen = torch.Generator().manual_seed(22)
+    x = [t.to(DEV) for t in _chunk_inputs(gen, [40, 1], [260, 511], 8, 2, 64, 16)]
+    with pytest.raises(ValueError):
+        zb.ops.gqa_chunk(*x, window=window)
+
+
+@pytest.mark.parametrize("rotary", [2 ** 32, 2 ** 32 + 64, -8, 72])
+def test_append_refuses_rotary_dims_outside_the_head(zb, rotary):
+    gen = torch.Generator().manual_seed(23)
+    q, k, v, table, seqlens, cu = (t.to(DEV) for t in _chunk_inputs(gen, [4, 1], [20, 9], 4, 2, 64, 16))
+    proj = torch.zeros(5, 8 * 64, device=DEV, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        zb.ops.gqa_append(proj, k, v, table, seqlens, cu, heads=4, kv_heads=2, rotary_dim=rotary)

@@ -1035,7 +1035,7 @@ def decode_advance(codes, ids, positions, cache_seqlens, out_loc, page_table, co
 
 # These calls serve single tokens too, where the host's time is the call's: the checks build their messages only to raise
 # them, and read each attribute once.
-_BF16, _I32 = torch.bfloat16, torch.int32
+_BF16, _I32, _I32_MAX = torch.bfloat16, torch.int32, 2 ** 31 - 1
 
 
 def _raw_stream(device_index: int) -> int:
@@ -1117,6 +1117,10 @@ def gqa_append(proj, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, 
             shape[1] > 1 and proj.stride(1) != 1):
         raise ValueError(f"proj must be a bfloat16 [N, >= {(heads + 2 * Hkv) * hd}] tensor with contiguous rows")
     N = shape[0]
+    if rotary_dim is None:
+        rotary_dim = hd
+    elif not 0 <= rotary_dim <= hd:
+        raise ValueError(f"rotary_dim must be between 0 and {hd}, got {rotary_dim}")
     if temp is not None and (temp.dtype is not _BF16 or temp.get_device() != index or temp.numel() != heads
                              or not temp.is_contiguous()):
         raise ValueError(f"temp must hold {heads} bfloat16 values on {proj.device}")
@@ -1132,7 +1136,7 @@ def gqa_append(proj, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, 
         q_stride = _token_rows("q_out", q_out, index, N, heads, hd)
     _lib.call("zb_gqa_append", proj.data_ptr(), proj.stride(0) if N > 1 else shape[1],
               None if temp is None else temp.data_ptr(), None if positions is None else positions.data_ptr(),
-              0.0 if eps is None else eps, eps is not None, rope_theta, hd if rotary_dim is None else rotary_dim,
+              0.0 if eps is None else eps, eps is not None, rope_theta, rotary_dim,
               interleaved, q_out.data_ptr(), q_stride, *paged, N, heads, Hkv, hd, _raw_stream(index))
     return q_out
 
@@ -1171,6 +1175,9 @@ def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, s
     if lse is not None and (lse.dtype is not torch.float32 or lse.get_device() != index or lse.shape != (N, Hq)
                             or not lse.is_contiguous()):
         raise ValueError(f"lse must be a contiguous float32 [{N}, {Hq}] tensor on {q.device}")
+    if window < 0:
+        raise ValueError(f"window must not be negative, got {window}")
+    window = min(window, _I32_MAX)  # the C argument's range; no cache holds as many keys
     need = _chunk_workspace_bytes(paged[12], N, Hq, Hkv, hd, paged[9] * paged[6])
     stream = _raw_stream(index)
     if workspace is None:
