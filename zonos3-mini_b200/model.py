@@ -128,7 +128,8 @@ class Zonos3ForCausalLM(BaseOP):
 
     def allocate_caches(self, capacity: int, kv_slots: int, device, page_size: int | None = None):
         """Per-slot DeltaNet state pools of ``capacity`` streams and the KV pool: a ``SlotKVPool`` of ``kv_slots`` token
-        slots, or with ``page_size`` a ``PagedKVPool`` of as many tokens in pages."""
+        slots, or with ``page_size`` a ``PagedKVPool`` of as many tokens in pages (for batches described on the device;
+        ``DecodeGraph`` takes the former)."""
         for gdn in self.gdn_layers():
             gdn.allocate_cache(capacity, device, torch.bfloat16)
         c = self._config
@@ -192,10 +193,14 @@ class DecodeGraph:
     ``input_ids`` <- the sampled codes, every position and cache length + 1, ``out_loc`` <- the next slot of each
     stream's page table, the codes appended to the repetition window, the sampler's draw counter + 1. So replays
     alone run an autoregressive decode; ``step()`` instead loads host ids / metadata first (the server's path).
+
+    The pool has page size 1 (``SlotKVPool``): the step's bookkeeping moves every stream from slot to slot.
     """
 
     def __init__(self, model: Zonos3ForCausalLM, pool: SlotKVPool, batch_size: int, page_table: torch.Tensor,
                  slots: torch.Tensor | None = None, sampling: SamplingConfig | None = None, stop_id: int | None = None):
+        if any(pool.k(layer).dim() != 3 for layer in model.attention_layer_ids()):
+            raise ValueError("DecodeGraph needs a pool of page size 1 (allocate_caches without page_size)")
         c = model.config
         dev = page_table.device
         self.model, self.pool, self.bs = model, pool, batch_size
