@@ -40,8 +40,8 @@ inline int check_paged(const PagedBatch& p, const char* who) {
   if (p.B == 0 || p.N == 0) return kOk;
   ZB_REQUIRE(p.cu && p.keys && (p.table || p.max_pages == 0) && ((p.k && p.v) || p.num_pages == 0), "%s: null pointer",
              who);
-  ZB_REQUIRE_ALIGNED(p.k, 16, "the K cache");
-  ZB_REQUIRE_ALIGNED(p.v, 16, "the V cache");
+  ZB_REQUIRE((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) % 16 == 0,
+             "%s: the K and V caches must be 16-byte aligned", who);
   return kOk;
 }
 
