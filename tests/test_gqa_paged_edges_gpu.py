@@ -140,3 +140,74 @@ def test_append_refuses_rotary_dims_outside_the_head(zb, rotary):
     proj = torch.zeros(5, 8 * 64, device=DEV, dtype=torch.bfloat16)
     with pytest.raises(ValueError):
         zb.ops.gqa_append(proj, k, v, table, seqlens, cu, heads=4, kv_heads=2, rotary_dim=rotary)
+
+
+def _definition(q, k, v, table, seqlens, cu, b, window, gate=None):
+    """(out, spread) of request b in 64 bits on the device, from dense scores; values that are not finite reach no row that
+    does not see them."""
+    first, last, keys, page = int(cu[b]), int(cu[b + 1]), int(seqlens[b]), k.shape[1]
+    at = torch.arange(keys)
+    where = table[b, at // page].long().to(DEV), (at % page).to(DEV)
+    key, value = k.to(DEV)[where].double(), v.to(DEV)[where].double()  # [keys, Hkv, hd]
+    rows = torch.arange(keys - (last - first), keys, device=DEV)[:, None]
+    hidden = (at.to(DEV)[None] > rows) | (at.to(DEV)[None] <= rows - window if window else False)
+    x = q[first:last].to(DEV).double()
+    out, spread = torch.empty_like(x), torch.empty_like(x)
+    group = q.shape[1] // k.shape[2]
+    for h in range(q.shape[1]):
+        s = (x[:, h] @ key[:, h // group].t() * q.shape[2] ** -0.5).masked_fill(hidden, float("-inf"))
+        w = torch.softmax(s, -1)
+        out[:, h], spread[:, h] = w @ value[:, h // group], w @ value[:, h // group].abs()
+    return out, spread
+
+
+LONG = [
+    # news, caches, Hq, Hkv, hd, page, window: units with runs of tiles that every row sees between tiles that hide keys
+    ([1747] * 8, [5] * 8, 16, 2, 64, 24, 0),
+    ([1400] * 12, [0] * 12, 16, 4, 128, 16, 0),
+    ([2000, 900, 3000], [300, 1200, 0], 6, 2, 128, 64, 0),
+    ([512, 511, 100], [8192, 6001, 3000], 16, 4, 128, 32, 0),
+    ([1, 80, 1, 1, 40, 300] * 8, [5000, 3000, 1856, 4100, 2500, 900] * 8, 8, 8, 128, 16, 1856),
+    ([597] * 40, [154] * 40, 8, 2, 128, 64, 964),
+    ([1] * 64, [3000] * 64, 14, 2, 64, 128, 1000),
+]
+
+
+@pytest.mark.parametrize("case", LONG)
+def test_chunk_long_runs_of_tiles(zb, case):
+    """Page copies against the definition; then with values that are not finite in every request, in the future of its first
+    new tokens and, with a window, behind it: they reach the rows that see them and no others, as with 16-byte copies of the
+    same tiles (pages of one row)."""
+    news, caches, Hq, Hkv, hd, page, window = case
+    gen = torch.Generator().manual_seed(LONG.index(case))
+    q, k, v, table, seqlens, cu = _chunk_inputs(gen, news, caches, Hq, Hkv, hd, page)
+    # the same rows as pages of one row
+    rows = (table.long()[:, :, None] * page + torch.arange(page)).flatten(1).clamp(min=-1).to(torch.int32)
+
+    def both(v):
+        slots = [t.reshape(-1, Hkv, hd).to(DEV) for t in (k, v)]
+        paged = zb.ops.gqa_chunk(*(t.to(DEV) for t in (q, k, v, table, seqlens, cu)), window=window)
+        assert zb.ops.device_status() == 0
+        single = zb.ops.gqa_chunk(q.to(DEV), *slots, rows.to(DEV), seqlens.to(DEV), cu.to(DEV), window=window)
+        assert zb.ops.device_status() == 0
+        return paged, single
+
+    clean, _ = both(v)
+    for b in {0, len(news) // 2, len(news) - 1}:
+        ref, spread = _definition(q, k, v, table, seqlens, cu, b, window)
+        got = clean[int(cu[b]):int(cu[b + 1])]
+        _close(got, ref.cpu(), 2.0 ** -7 * (1 + 2.0 ** -4) * spread.cpu())
+    dirty, unseen = v.clone(), torch.ones(len(q), dtype=torch.bool)
+    for b, (n, c) in enumerate(zip(news, caches)):
+        for j, bad in ((c + n - 1, torch.nan), (c + n // 2, torch.inf), (c - window if window else -1, -torch.inf)):
+            if j < 0:
+                continue
+            dirty[int(table[b, j // page]), j % page, :, 5] = bad
+            seen = torch.arange(n) + c >= j
+            if window:
+                seen &= torch.arange(n) + c < j + window
+            unseen[int(cu[b]):int(cu[b + 1])][seen] = False
+    paged, single = both(dirty)
+    assert paged[unseen.to(DEV)].isfinite().all()
+    assert torch.equal(paged.isnan(), single.isnan()) and torch.equal(paged.isinf(), single.isinf())
+    assert not paged[(~unseen).to(DEV)][..., 5].isfinite().any()

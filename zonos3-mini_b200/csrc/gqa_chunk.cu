@@ -149,7 +149,7 @@ struct Tail {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t q_full[2], q_empty[2];
   uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
-  uint64_t scanned[kMasks], drained, halves;
+  uint64_t armed[kMasks], scanned[kMasks], drained, halves;
   uint64_t desc_full[kDescs], desc_empty[kDescs];
   alignas(16) unsigned mask[kMasks][4];  // keys of a tile that exist
   Desc desc[kDescs];
@@ -558,7 +558,10 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       zb::mbar_init(zb::smem_addr(&tl.p_full[s]), kSoftWarps / 2);
       zb::mbar_init(zb::smem_addr(&tl.o_full[s]), 1);
     }
-    for (int s = 0; s < kMasks; ++s) zb::mbar_init(zb::smem_addr(&tl.scanned[s]), kLoadWarps - 1);
+    for (int s = 0; s < kMasks; ++s) {
+      zb::mbar_init(zb::smem_addr(&tl.armed[s]), 1);
+      zb::mbar_init(zb::smem_addr(&tl.scanned[s]), kLoadWarps - 1);
+    }
     zb::mbar_init(zb::smem_addr(&tl.drained), 1);
     zb::mbar_init(zb::smem_addr(&tl.halves), 32 * kSoftWarps);
     for (int s = 0; s < kDescs; ++s) {
@@ -784,9 +787,13 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           }
         }
         // The last two warps look through the values of tiles that hold keys hidden from some rows, half of a tile each.
+        // A phase's parity says that the phase is over only to those who know that it is the current one or the last. With
+        // tensor copies these warps pass over whole tiles, so they would get to one whose slot is phases behind, and take an
+        // older phase for the tile's: they wait until the tile's copies have been started.
         auto look_through = [&](int t, int v_item) {
           const int first = (u.tile0 + t) * kTile, slot = scans % kMasks;
           if (warp == kLoadWarp || !mixed_tile(u, first)) return;
+          if (p.box) wait(tl.armed[slot], (scans / kMasks) & 1, abort);
           wait(tl.full[v_item % L::kSlots], (v_item / L::kSlots) & 1, abort);
           // groups of 8 rows in turn; rows past the request's keys are no values (warp 8 zeroes them)
           const uint4* v = reinterpret_cast<const uint4*>(gbase + (v_item % L::kSlots) * L::kItem);
@@ -811,6 +818,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 #pragma unroll 1
             for (int t = 0; t < u.tiles && going; ++t, ++tile_no) {
               const int first = (u.tile0 + t) * kTile, pos = first + lane * p.box;
+              const bool mixed = mixed_tile(u, first);
               const bool there = next >= 0 && next < p.kv.num_pages;
               const int page = there ? next * p.page_heads + (p.page_heads > 1 ? kvh : 0)
                                      : (int)(p.kv.num_pages * p.page_heads);  // past the end: zeros
@@ -830,12 +838,14 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                 if (lane == 0) {
                   if (kv == 0) *reinterpret_cast<uint4*>(tl.mask[tile_no % kMasks]) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
                   zb::mbar_arrive_expect_tx(zb::smem_addr(&tl.full[slot]), L::kItem);
+                  if (kv == 1 && mixed) arrive(tl.armed[scans % kMasks]);
                 }
                 __syncwarp();
                 if (lane < boxes)
                   load_rows(base + slot * L::kItem + lane * (p.box / 8) * L::kGroup, kv ? &maps.v : &maps.k,
                             kvh * p.head_atoms, group, page, zb::smem_addr(&tl.full[slot]));
               }
+              scans += mixed;
             }
           } else {
 #pragma unroll 1
