@@ -175,9 +175,8 @@ LONG = [
 
 @pytest.mark.parametrize("case", LONG)
 def test_chunk_long_runs_of_tiles(zb, case):
-    """Page copies against the definition; then with values that are not finite in every request, in the future of its first
-    new tokens and, with a window, behind it: they reach the rows that see them and no others, as with 16-byte copies of the
-    same tiles (pages of one row)."""
+    """Page copies against 16-byte copies of the same tiles (pages of one row), bit by bit, and against the definition;
+    then with values that are not finite in every request, in the future of its first new tokens and, with a window, behind it."""
     news, caches, Hq, Hkv, hd, page, window = case
     gen = torch.Generator().manual_seed(LONG.index(case))
     q, k, v, table, seqlens, cu = _chunk_inputs(gen, news, caches, Hq, Hkv, hd, page)
@@ -192,7 +191,8 @@ def test_chunk_long_runs_of_tiles(zb, case):
         assert zb.ops.device_status() == 0
         return paged, single
 
-    clean, _ = both(v)
+    clean, single = both(v)
+    assert torch.equal(clean, single)
     for b in {0, len(news) // 2, len(news) - 1}:
         ref, spread = _definition(q, k, v, table, seqlens, cu, b, window)
         got = clean[int(cu[b]):int(cu[b + 1])]
@@ -208,6 +208,29 @@ def test_chunk_long_runs_of_tiles(zb, case):
                 seen &= torch.arange(n) + c < j + window
             unseen[int(cu[b]):int(cu[b + 1])][seen] = False
     paged, single = both(dirty)
-    assert paged[unseen.to(DEV)].isfinite().all()
-    assert torch.equal(paged.isnan(), single.isnan()) and torch.equal(paged.isinf(), single.isinf())
+    assert torch.equal(paged[unseen.to(DEV)], clean[unseen.to(DEV)])
+    assert torch.equal(paged.isnan(), single.isnan()) and torch.equal(paged.nan_to_num(), single.nan_to_num())
     assert not paged[(~unseen).to(DEV)][..., 5].isfinite().any()
+
+
+@pytest.mark.parametrize("news, caches, Hq", [([200, 40], [0, 300], 8), ([130], [600], 6), ([5, 1, 1, 3], [700, 300, 20, 0], 8),
+                                              ([1, 1, 1], [500, 40, 260], 6)])
+def test_chunk_rows_keep_their_bits_whatever_stands_beside_them(zb, news, caches, Hq):
+    """Other requests' queries, and keys in a token's own future, leave every bit of its output as it was, also where they
+    make other rows' scores thousands of times as large."""
+    gen = torch.Generator().manual_seed(24 + len(news))
+    x = _chunk_inputs(gen, news, caches, Hq, 2, 128, 16)
+    clean = zb.ops.gqa_chunk(*(t.to(DEV) for t in x))
+    q, k, v, table, seqlens, cu = x
+    for b, n in enumerate(news):
+        first, last = int(cu[b]), int(cu[b + 1])
+        loud = q.clone()  # every request but b
+        loud[:first], loud[last:] = 1000.0 * q[:first], 1000.0 * q[last:]
+        got = zb.ops.gqa_chunk(*(t.to(DEV) for t in (loud, k, v, table, seqlens, cu)))
+        assert torch.equal(got[first:last], clean[first:last])
+        for i in sorted({n - 1, n // 2, n // 3}):
+            j = caches[b] + i  # token i's own key: tokens before it do not see it
+            loud = k.clone()
+            loud[int(table[b, j // 16]), j % 16] *= 1000.0
+            got = zb.ops.gqa_chunk(*(t.to(DEV) for t in (q, loud, v, table, seqlens, cu)))
+            assert torch.equal(got[first:first + i], clean[first:first + i])

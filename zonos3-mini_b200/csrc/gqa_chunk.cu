@@ -16,10 +16,9 @@
 // or up to 24 (log2) above it, and moves to 24 above a tile's largest score when that is larger than m. So no p is above 1, as
 // with the maximum itself: the accumulator stays below sum |v_j|, and no finite values overflow that do not with the maximum;
 // and the largest p is at least 2^-24, so that weights below 2^-102 of it count as 0, and values down to 2^-100 keep their
-// precision. m starts at 24, which holds for first keys whose largest score is 0 to 24 (with q and k normalised to a mean
-// square of 1, no score of 128 dims is above 16.3). So the search for the maximum runs beside the exponentials instead of
-// before them, and the accumulator is hardly ever rescaled: 4 x 512 tokens behind 8192 take 132 us with scores that spread
-// by 1 nat, 136 by 4, 138 by 8, 158 by 16 (16 above instead of 24: 132, 134, 152, 175).
+// precision. m starts at 24, which holds for first keys whose largest score is 0 to 12 (for larger ones it would be reached
+// too soon). So the search for the maximum runs beside the exponentials instead of before them, and the accumulator is hardly
+// ever rescaled: 4 x 512 tokens behind 8192 take 131 us with scores that spread by 1 nat, 134 by 4, 141 by 8, 190 by 16.
 // p is rounded to bf16 because the tensor cores multiply bf16; its sum is kept from before the rounding. Where that would
 // be the largest error for nothing it is avoided: units of few rows multiply what the rounding left off too, and rows whose
 // first keys lie in a partly visible tile start with m 24 above their largest score, whose p is 2^-24 and exact.
@@ -1147,17 +1146,18 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             }
           };
           // Whether the weights formed with m hold for a tile whose largest score is `top` (NaN: they do); if not, m is set
-          // by it, and the sum and the accumulator follow. Every row of the warp takes its m up then, so that the others do
-          // not ask for turns of their own soon after. `set`: first keys set m whatever it is.
+          // by it, and the sum and the accumulator follow. A row's m goes by its own scores alone: with those of the warp's
+          // other rows in it, what rounding makes of a token's output would hang on tokens behind it, and on what lies in
+          // lanes without a row. `set`: first keys set m whatever it is.
           auto holds = [&](float top, bool set) {
             top *= p.scale_log2;
-            const bool off = top > m || (l == 0.f && (set || top < m - kAbove) && top > -INFINITY);
+            const bool off = l != 0.f ? top > m : (set || top > m - kAbove / 2 || top < m - kAbove) && top > -INFINITY;
             if (!__any_sync(0xffffffffu, off)) return true;
-            const float to = off && l == 0.f ? top + kAbove : fmaxf(m, top + kAbove);
-            const float corr = l != 0.f ? ex2(m - to) : 1.f;  // without a key so far both are 0
+            top += kAbove;
+            const float corr = off && l != 0.f ? ex2(m - top) : 1.f;  // without a key so far both are 0
             l *= corr;
             rescale(corr);
-            m = to;
+            if (off) m = top;
             return false;
           };
           auto hand_over = [&](const uint64_t& bar) {
@@ -1200,10 +1200,9 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
               float corr[2];
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                const float to = any2[r] ? fmaxf(m2[r], top[r] + kAbove) : off[r] ? top[r] + kAbove : 0.f;
-                corr[r] = any2[r] ? ex2(m2[r] - to) : 1.f;
+                corr[r] = off[r] && any2[r] ? ex2(m2[r] - (top[r] + kAbove)) : 1.f;
                 l2[r] *= corr[r];
-                m2[r] = to;
+                if (off[r]) m2[r] = top[r] + kAbove;
               }
               rescale(of_row(corr[0], corr[1], lane));
             }
