@@ -350,12 +350,13 @@ int zb_gqa_append(const uint16_t* proj, int64_t proj_stride, const uint16_t* tem
  * h] . K^T * softmax_scale) V, query head h reading KV head h / (Hq / Hkv), times sigmoid(gate[t, h]) when gate is given
  * ([N, Hq] bf16, row stride gate_stride), rounded once; lse (NULL: not written) [N, Hq] fp32 = the natural logarithm of
  * the softmax denominator. A row that sees no key or belongs to no request: zeros, lse -inf. q / out [N, Hq, hd] bf16 with
- * row strides (multiples of 8), 16-byte aligned; softmax_scale > 0; Hq a multiple of Hkv. workspace: 16-byte aligned, at
- * least zb_gqa_chunk_workspace_bytes(B, N, Hq, Hkv, hd, page_size * max_pages) bytes, not shared by overlapping calls; its
- * first 4096 bytes (flags) must be zero before the first call and are left zero by each. A call whose waits gave up (status bit
- * 64) may leave some non-zero. Later calls take no notice, as each raises them to a value of its own; a captured call has one
- * value for all its replays, so zero them before it is replayed again. Status bit 128: cu_seqlens_q
- * decreases or leaves [0, N], nothing was written. */
+ * row strides (multiples of 8), 16-byte aligned; softmax_scale > 0; Hq a multiple of Hkv, at most 128
+ * times it, and B at most 16384 (else status 3). workspace: 16-byte aligned, at least
+ * zb_gqa_chunk_workspace_bytes(B, N, Hq, Hkv, hd, page_size * max_pages) bytes, not shared by overlapping calls; its first
+ * 4096 bytes (flags) must be zero before the first call and are left zero by each. A call whose waits gave up (status bit 64)
+ * may leave some non-zero. Later calls take no notice, as each raises them to a value of its own; a captured call has one
+ * value for all its replays, so zero them before it is replayed again. Status bit 128: cu_seqlens_q decreases or leaves
+ * [0, N], nothing was written. */
 int64_t zb_gqa_chunk_workspace_bytes(int B, int N, int Hq, int Hkv, int hd, int64_t max_keys);
 int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache,
                  int64_t page_stride, int64_t slot_stride, int64_t head_stride, int64_t num_pages, int page_size,

@@ -36,25 +36,29 @@
 // matrix product. So where a tile's keys are visible to some of its rows only, warps 10 and 11 look through the V tile while
 // the scores are being worked on; values that are not finite are added to the rows that see them one by one, then zeroed.
 //
-// What bounds it, and what it measured (B200, 16 query and 4 KV heads of 128, captured calls back to back):
-// * A long prompt (8192 tokens, causal; 275 GFLOP): 235 us, 1170 TFLOP/s, 0.71 of the 1638 that a library product of
-//   8192^3 reaches. Per stream and tile the chain scores (512 cycles), weights (1024 of the exponential unit, 2048 with the
-//   other stream's beside them), hand-over, values' product (its second half 256) comes to 3100-3500 cycles for two tiles'
-//   2048 cycles of tensor-core work; without the row warps' work the loop takes 195 us. Held by the power limit it is 270 us,
-//   as the clock falls from 1.95 to 1.62 GHz. 4 x 512 tokens behind 8192 cached ones (142 GFLOP): 131 us, 1080 TFLOP/s.
-// * Single tokens are bound by HBM: 256 requests of 1628 keys (856 MB), 152 us, 5.6 TB/s, 0.87 of a copy's
-//   6.46; 2 of 65000 keys over all CTAs, 57 us, 4.7 TB/s.
+// What bounds it, and what it measured (B200, 16 query and 4 KV heads of 128; calls one after the other without end, and in
+// brackets bursts of 20 captured calls, before the power limit lowers the clock):
+// * A long prompt (8192 tokens, causal; 275 GFLOP): 278 us, 988 TFLOP/s (231 us, 1190), 0.60 (0.73) of the 1638 that a library
+//   product of 8192^3 reaches in a burst. Per stream and tile the chain scores (512 cycles), weights (1024 of the exponential
+//   unit, 2048 with the other stream's beside them), hand-over, values' product (its second half 256) comes to 3100-3500
+//   cycles for two tiles' 2048 cycles of tensor-core work; without the row warps' work the loop takes 195 us. At the power
+//   limit the clock falls from 1.95 to 1.62 GHz. 4 x 512 tokens behind 8192 cached ones (142 GFLOP): 156 us, 908 TFLOP/s (131).
+// * Single tokens are bound by HBM and power: 256 requests of 1628 keys (856 MB), 171 us, 5.0 TB/s, 0.78 of a copy's 6.46
+//   (153 us, 0.87); 2 of 65000 keys over all CTAs, 57 us, 4.7 TB/s. Products 64 rows high for the 4 rows of a token are what
+//   takes the power; with pages of one row the decode kernel, whose products are 16 wide, takes 155 us and this one 237.
 // * Many short units (256 prompts of up to 128 tokens) are bound by the latency of a unit's steps, 8000-10000 cycles,
-//   and by their balance, not by bytes (26 us of them): 71 us. Each unit runs through about 30 KB of code once, more than
-//   the instruction cache keeps beside the other warps' (a third of its requests missed at 148 KB of kernel, a fifth at
-//   131 KB). So code that runs once a unit is kept small before it is kept fast: loops over 32 keys or dims instead of whole
-//   rows (unrolled whole, the epilogue made it 75 -> 79 us), one place for each stream's products (70.7 -> 69.2), waits that
-//   count (73.7 -> 70.7).
+//   and by their balance, not by bytes (26 us of them): 72 us. Each unit runs through about 30 KB of code once, more than
+//   the instruction cache keeps beside the other warps' (a fifth of its requests miss at the present 147 KB of kernel). So code
+//   that runs once a unit is kept small before it is kept fast: loops over 32 keys or dims instead of whole rows (unrolled
+//   whole, the epilogue made it 75 -> 79 us), one place for each stream's products (70.7 -> 69.2), waits that count (73.7 ->
+//   70.7).
 // * One request of one token: 15 us, about 7 of them the way from the launch to the first scores.
 //
 // Pages: with rows of 64 or 128 elements and a page size with a factor of 8 or more, a lane copies a page's rows in one
 // tensor copy; 16-byte copies by three warps otherwise. On 128 requests of 2000 keys and pages of 8 the first takes 125 us
-// against 158 with heads of 128, 120 against 120 with heads of 64.
+// against 158 with heads of 128, 120 against 120 with heads of 64. The 16-byte copies cost most on pages of one row: the 4 x 512
+// tokens take 199 us, the prompts 84; and where a head dim is padded: 96 dims 192 us for the 4 x 512 tokens, 32 dims 180 us for
+// 256 single tokens, more than 64 dims do (115, 127).
 #include <algorithm>
 
 #include "paged.cuh"
@@ -74,8 +78,9 @@ constexpr int kFewRows = 32;     // up to here the row warps share a unit's rows
 // Up to here a unit's rows are lanes 0-15 of products that are 64 rows high instead of 128, and a thread takes 64 of two
 // rows' scores. The time of a product hardly matters with so few rows, so a second one takes what rounding a weight to bf16
 // leaves off, which leaves 2^-16 of a weight instead of 2^-8: the output of single tokens is then as good as fp32's, 0.0017 of
-// its norm from the exact one (its own rounding) instead of 0.0023. It costs 256 single tokens over 1628 keys 149 -> 152 us,
-// 161 -> 168 where the GPU is held by its power limit; products of 128 rows took 172 there with one product.
+// its norm from the exact one (its own rounding) instead of 0.0023. The second product costs 256 single tokens over 1628 keys
+// 149 -> 152 us, 161 -> 168 where the GPU is held by its power limit (before it, products of 64 rows instead of 128 had taken
+// that time from 181 to 167 on another GPU).
 constexpr int kFineRows = 16;
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
@@ -287,8 +292,6 @@ __device__ __forceinline__ uint32_t ld1(uint32_t taddr) {
 __device__ __forceinline__ void st1(uint32_t taddr, uint32_t r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r) : "memory");
 }
-// One lane of a converged warp, always the same. Code under it stays uniform for the compiler, so that the operands of
-// the tensor-core instructions are kept in uniform registers.
 // A value that is the same on every lane, told to the compiler: it and what follows from it stay in uniform registers,
 // which the tensor-core instructions take their operands from.
 __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
@@ -307,6 +310,8 @@ __device__ __forceinline__ Desc uniform(const Desc& d) {
   u.all_hi = uniform(d.all_hi);
   return u;
 }
+// One lane of a converged warp, always the same. Code under it stays uniform for the compiler, so that the operands of
+// the tensor-core instructions are kept in uniform registers.
 __device__ __forceinline__ bool elect() {
   uint32_t yes;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(yes));
@@ -379,10 +384,11 @@ __device__ __forceinline__ Request request(const ChunkParams& p, int b) {
   return r;
 }
 
-// Keys [lo, hi) that the token at position pos of a request with `keys` keys sees.
+// Keys of a request that the page table's columns can hold.
 __device__ __forceinline__ int held_keys(const ChunkParams& p, int keys) {
   return min(keys, p.kv.max_pages * p.kv.page_size);
 }
+// Keys [lo, hi) that the token at position pos of a request with `keys` keys sees.
 __device__ __forceinline__ void visible(const ChunkParams& p, int keys, int pos, int& lo, int& hi) {
   const int held = held_keys(p, keys);
   hi = max(p.causal ? min(held, pos + 1) : held, 0);

@@ -1157,7 +1157,9 @@ def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, s
     written then). workspace: optional uint8 tensor of at least :func:`gqa_chunk_workspace_bytes` bytes, its first
     4096 zero before the first call and not shared by calls that may overlap (a call leaves them zero unless its waits gave
     up, :func:`device_status` bit 64; eager calls take no notice of what that left, a captured one asks for zeros again before
-    its next replay); absent, the stream's own is used. hd: a multiple of 8 up to 128. Returns out [N, Hq, hd] bf16."""
+    its next replay); absent, the stream's own is used. hd: a multiple of 8 up to 128; at most 16384 requests and 128 query
+    heads a KV head. Single tokens over a cache of one token a page are faster by :func:`gqa_decode`. Returns out [N, Hq, hd]
+    bf16."""
     paged, index, Hkv, hd = _paged(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, None)
     N, Hq = q.shape[0], q.shape[1]
     q_stride = _token_rows("q", q, index, N, Hq, hd)
