@@ -365,6 +365,53 @@ int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_cache, c
                  int window, const uint16_t* gate, int64_t gate_stride, uint16_t* out, int64_t out_stride, float* lse,
                  void* workspace, int64_t workspace_bytes, cudaStream_t stream);
 
+/* zb_gqa_chunk_sinks: the same with first keys that stay visible: with window > 0 a token also sees the keys j < sinks
+ * (j <= p) of its request, as streams far behind their beginning need them. sinks >= 0; 0, or no window: as zb_gqa_chunk. */
+int zb_gqa_chunk_sinks(const uint16_t* q, int64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache,
+                       int64_t page_stride, int64_t slot_stride, int64_t head_stride, int64_t num_pages, int page_size,
+                       const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* cache_seqlens,
+                       const int32_t* cu_seqlens_q, int B, int N, int Hq, int Hkv, int hd, float softmax_scale, int causal,
+                       int window, int sinks, const uint16_t* gate, int64_t gate_stride, uint16_t* out, int64_t out_stride,
+                       float* lse, void* workspace, int64_t workspace_bytes, cudaStream_t stream);
+
+/* The same three over a paged KV cache in 4 bits. The batch is described as above; the cache is one buffer of bytes, KV head
+ * g of page p at p * page_stride + g * head_stride BYTES (multiples of 16, 16-byte aligned): page_size / 16 blocks of 20 hd
+ * bytes one after the other (page_size a multiple of 16; hd 32, 64, 96 or 128, else status 3). A block holds 16 tokens of a
+ * head: [0, 8 hd) the codes of their keys, 16 rows of hd / 2 bytes; [8 hd, 16 hd) those of their values; [16 hd, 18 hd) the
+ * pairs of their keys, 16 rows of hd / 32; [18 hd, 20 hd) those of their values. 32 consecutive elements of a row are a group
+ * with a pair (s, m) of bf16 (a 32-bit word, s in its lower half), and stand for m + s c, c their codes 0 .. 15. A row's codes
+ * are 32-bit words: word t * (hd / 32) + g holds elements 32 g + 8 t + e, e = 0 .. 7, element e in bits 4 (e / 2 + 4 (e % 2))
+ * and up. A pair with a magnitude of 2^100 or more or a NaN (never written) stands for zeros. Replaces no part of the
+ * reference, whose cache is bf16.
+ *
+ * zb_gqa_append_q4: as zb_gqa_append; k, rounded to bf16, and v go into the cache with m the smallest element of a group, s =
+ * bf16((largest - m) / 15), 0 below 2^-100, c = floor((x - m) / s + 1/2). NaN is stored as 0, magnitudes above 2^99 as that.
+ * Hq may be 0 (proj holds k | v; q_out is not used). */
+int zb_gqa_append_q4(const uint16_t* proj, int64_t proj_stride, const uint16_t* temp, const int32_t* positions, float eps,
+                     int normalize, double rope_theta, int rotary_dim, int interleaved, uint16_t* q_out, int64_t q_stride,
+                     uint8_t* kv_cache, int64_t page_stride, int64_t head_stride, int64_t num_pages, int page_size,
+                     const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* cache_seqlens,
+                     const int32_t* cu_seqlens_q, int B, int N, int Hq, int Hkv, int hd, cudaStream_t stream);
+
+/* zb_kv_read_q4: the last cu[b + 1] - cu[b] keys and values of every request as bf16 rows k_out, v_out [N, Hkv, hd] (row
+ * strides, multiples of 8; 16-byte aligned), m + s c rounded once. Zeros for a row of no request and where no page holds the
+ * key. */
+int zb_kv_read_q4(const uint8_t* kv_cache, int64_t page_stride, int64_t head_stride, int64_t num_pages, int page_size,
+                  const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* cache_seqlens,
+                  const int32_t* cu_seqlens, int B, int N, int Hkv, int hd, uint16_t* k_out, int64_t k_stride,
+                  uint16_t* v_out, int64_t v_stride, cudaStream_t stream);
+
+/* zb_gqa_chunk_q4: as zb_gqa_chunk_sinks, over the values the cache stands for. max_new (0: not known): no request brings more
+ * new tokens than so many; a request that does sets status bit 256 and its rows may be left unwritten. The workspace is that of
+ * zb_gqa_chunk_q4_workspace_bytes with the same max_new; its first 8192 bytes are the flags. */
+int64_t zb_gqa_chunk_q4_workspace_bytes(int B, int N, int Hq, int Hkv, int hd, int64_t max_keys, int max_new);
+int zb_gqa_chunk_q4(const uint16_t* q, int64_t q_stride, const uint8_t* kv_cache, int64_t page_stride, int64_t head_stride,
+                    int64_t num_pages, int page_size, const int32_t* page_table, int64_t table_stride, int max_pages,
+                    const int32_t* cache_seqlens, const int32_t* cu_seqlens_q, int B, int N, int Hq, int Hkv, int hd,
+                    float softmax_scale, int causal, int window, int sinks, int max_new, const uint16_t* gate,
+                    int64_t gate_stride, uint16_t* out, int64_t out_stride, float* lse, void* workspace,
+                    int64_t workspace_bytes, cudaStream_t stream);
+
 /* ---------------------------------------------------------------------------------------------- TTS sampler */
 
 /* Next audio codes from per-codebook logits [B, C, V] (row (b, c) of V at b * batch_stride + c * row_stride elements,

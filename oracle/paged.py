@@ -66,8 +66,8 @@ def append(proj, k_cache, v_cache, table, seqlens, cu, *, heads, kv_heads, temp=
     return q, q_mag, k_mag
 
 
-def chunk(q, k_cache, v_cache, table, seqlens, cu, *, scale=None, causal=True, window=0, gate=None):
-    """(out, spread, lse, size): out [N, Hq, hd] float64; spread = sum_j p_j |v_j| (gated), the scale of out's rounding
+def chunk(q, k_cache, v_cache, table, seqlens, cu, *, scale=None, causal=True, window=0, sinks=0, gate=None):
+    """(out, spread, lse, size): out [N, Hq, hd] float64 (with a window the first ``sinks`` keys stay visible); spread = sum_j p_j |v_j| (gated), the scale of out's rounding
     errors; lse [N, Hq]; size = max_j scale * sum_d |q_d k_jd|, the scale of a score's rounding error."""
     N, Hq, hd = q.shape
     pages, page_size, Hkv, _ = k_cache.shape
@@ -88,7 +88,7 @@ def chunk(q, k_cache, v_cache, table, seqlens, cu, *, scale=None, causal=True, w
             if causal:
                 seen &= at <= p
             if window:
-                seen &= at > p - window
+                seen &= (at > p - window) | (at < sinks)
             if not seen.any():
                 continue
             for h in range(Hq):

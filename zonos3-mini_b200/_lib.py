@@ -111,6 +111,22 @@ SIGNATURES: dict[str, list] = {
                      _f32, _i32, _i32, _p, _i64, _p, _i64, _p, _p, _i64, _p],
     # B, N, Hq, Hkv, hd, max_keys -> bytes (int64)
     "zb_gqa_chunk_workspace_bytes": [_i32, _i32, _i32, _i32, _i32, _i64],
+    # as zb_gqa_chunk, with sinks behind window
+    "zb_gqa_chunk_sinks": [_p, _i64, _p, _p, _i64, _i64, _i64, _i64, _i32, _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _i32,
+                           _i32, _f32, _i32, _i32, _i32, _p, _i64, _p, _i64, _p, _p, _i64, _p],
+    # as zb_gqa_append, with kv_cache, page_stride, head_stride (bytes) for the caches and their strides
+    "zb_gqa_append_q4": [_p, _i64, _p, _p, _f32, _i32, ctypes.c_double, _i32, _i32, _p, _i64, _p, _i64, _i64, _i64,
+                         _i32, _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _p],
+    # kv_cache, page_stride, head_stride, num_pages, page_size, page_table, table_stride, max_pages, cache_seqlens,
+    # cu_seqlens, B, N, Hkv, hd, k_out, k_stride, v_out, v_stride, stream
+    "zb_kv_read_q4": [_p, _i64, _i64, _i64, _i32, _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _i32, _p, _i64, _p, _i64, _p],
+    # q, q_stride, kv_cache, page_stride, head_stride, num_pages, page_size, page_table, table_stride, max_pages,
+    # cache_seqlens, cu_seqlens_q, B, N, Hq, Hkv, hd, scale, causal, window, sinks, max_new, gate, gate_stride, out,
+    # out_stride, lse, workspace, workspace_bytes, stream
+    "zb_gqa_chunk_q4": [_p, _i64, _p, _i64, _i64, _i64, _i32, _p, _i64, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32,
+                        _f32, _i32, _i32, _i32, _i32, _p, _i64, _p, _i64, _p, _p, _i64, _p],
+    # B, N, Hq, Hkv, hd, max_keys, max_new -> bytes (int64)
+    "zb_gqa_chunk_q4_workspace_bytes": [_i32, _i32, _i32, _i32, _i32, _i64, _i32],
     # n, out (complex float64 [n]), stream
     "zb_istft_twiddles": [_i32, _p, _p],
     # y0, y0_stride, y1, y1_stride, y_is_f64, streams, cols, n0, n1, hop, window0, window1, twiddle0, twiddle1,
@@ -125,7 +141,7 @@ SIGNATURES: dict[str, list] = {
 }
 _RESTYPES = {"zb_last_error": ctypes.c_char_p, "zb_clear_error": None, "zb_launch_count": ctypes.c_uint64,
              "zb_gdn_chunk_prefill_workspace_bytes": ctypes.c_int64, "zb_proj_gemm_workspace_bytes": ctypes.c_int64,
-             "zb_gqa_chunk_workspace_bytes": ctypes.c_int64}
+             "zb_gqa_chunk_workspace_bytes": ctypes.c_int64, "zb_gqa_chunk_q4_workspace_bytes": ctypes.c_int64}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

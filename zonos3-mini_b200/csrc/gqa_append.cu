@@ -21,9 +21,12 @@
 // schedulers issue in 65 % of the cycles, a norm, a turn and a rounding for every element, where a copy would issue in few.
 // Four warps a block and four passes of heads in flight is the best of 2-8 by 1-8; several tokens to a warp (64-66 us) and
 // a token over several warps (66-75) are slower there. 256 single tokens 5.5 us, one 3.4.
+//
+// With Q4 the cache is one of 4 bits (kv_q4.cuh): k rounded to bf16 as above, and v, go to their groups' codes and pairs. A
+// lane's 8 elements are one word of codes, the 4 lanes of a group find its bounds with two exchanges.
 #include <cmath>
 
-#include "paged.cuh"
+#include "kv_q4.cuh"
 
 namespace {
 
@@ -75,7 +78,7 @@ __device__ __forceinline__ void widen(const uint4& r, float (&x)[8]) {
 }
 
 // GL lanes hold a head (hd / 8 of them carry elements).
-template <int GL, int ALIGN>
+template <int GL, int ALIGN, bool Q4>
 __global__ void __launch_bounds__(kWarps * 32) gqa_append_kernel(const __grid_constant__ AppendParams p) {
   zb::pdl_enter();
   constexpr int kHeads = 32 / GL;  // heads of a pass
@@ -109,9 +112,12 @@ __global__ void __launch_bounds__(kWarps * 32) gqa_append_kernel(const __grid_co
     if (pos >= 0 && pos / p.kv.page_size < p.kv.max_pages) {
       const int page = p.kv.table[(int64_t)b * p.kv.table_stride + pos / p.kv.page_size];
       if (page >= 0 && page < p.kv.num_pages)
-        slot = (int64_t)page * p.kv.page_stride + (int64_t)(pos % p.kv.page_size) * p.kv.slot_stride;
+        slot = (int64_t)page * p.kv.page_stride +
+               (Q4 ? (int64_t)(pos % p.kv.page_size / zb::q4::kBlock) * zb::q4::block_bytes(hd)
+                   : (int64_t)(pos % p.kv.page_size) * p.kv.slot_stride);
     }
   }
+  const int row4 = at % zb::q4::kBlock;  // of the block; at is not negative where the token has a slot
   if (p.positions) at = p.positions[t];
   // the lane's rotation: interleaved, pairs gl * 4 ..; halves, the 8 pairs its elements belong to
   float cs[8], sn[8];
@@ -136,7 +142,7 @@ __global__ void __launch_bounds__(kWarps * 32) gqa_append_kernel(const __grid_co
       const int h = h0 + i * step;
       if (h - lane / GL >= heads) break;  // warp-uniform
       const bool is_v = h >= p.Hq + p.kv.Hkv, is_q = h < p.Hq;
-      if (h - lane / GL >= p.Hq + p.kv.Hkv) {  // values only, for the whole warp: a copy
+      if (!Q4 && h - lane / GL >= p.Hq + p.kv.Hkv) {  // values only, for the whole warp: a copy
         if (carries && h < heads && slot >= 0)
           *reinterpret_cast<uint4*>(p.kv.v + slot + (int64_t)(h - p.Hq - p.kv.Hkv) * p.kv.head_stride + gl * 8) = raw[i];
         continue;
@@ -170,11 +176,22 @@ __global__ void __launch_bounds__(kWarps * 32) gqa_append_kernel(const __grid_co
           if (turned) x[j] = upper ? other * sn[j] + x[j] * cs[j] : x[j] * cs[j] - other * sn[j];
         }
       }
-      if (!carries || h >= heads) continue;
       const uint4 packed = is_v ? raw[i] : zb::pack_bf16x8(x);
+      uint32_t word = 0, pair = 0;
+      if (Q4 && h - lane / GL + kHeads > p.Hq) word = zb::q4::write_word(packed, pair);  // the warp has keys or values
+      if (!carries || h >= heads) continue;
       if (is_q) {
         const uint4 zero = make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4*>(p.q_out + (int64_t)t * p.q_stride + (int64_t)h * hd + gl * 8) = b >= 0 ? packed : zero;
+      } else if (Q4) {
+        if (slot >= 0) {
+          const int groups = hd / zb::q4::kGroup, group = gl / 4, part = gl % 4;
+          unsigned char* block = reinterpret_cast<unsigned char*>(p.kv.k) + slot +
+                                 (int64_t)(h - p.Hq - (is_v ? p.kv.Hkv : 0)) * p.kv.head_stride;
+          *reinterpret_cast<uint32_t*>(block + (is_v ? 8 : 0) * hd + row4 * (hd / 2) + 4 * (part * groups + group)) = word;
+          if (part == 0)
+            *reinterpret_cast<uint32_t*>(block + (is_v ? 18 : 16) * hd + 4 * (row4 * groups + group)) = pair;
+        }
       } else if (slot >= 0) {
         __nv_bfloat16* cache = is_v ? p.kv.v : p.kv.k;
         const int g = h - p.Hq - (is_v ? p.kv.Hkv : 0);
@@ -184,40 +201,33 @@ __global__ void __launch_bounds__(kWarps * 32) gqa_append_kernel(const __grid_co
   }
 }
 
-template <int GL>
+template <int GL, bool Q4>
 cudaError_t launch_append(const AppendParams& p, int align, cudaStream_t stream) {
   const int64_t units = (int64_t)p.kv.N * p.shares;
   const dim3 grid((unsigned)((units + kWarps - 1) / kWarps)), block(kWarps * 32);
-  if (align >= 16) return zb::launch(gqa_append_kernel<GL, 16>, grid, block, 0, stream, 1, p);
-  if (align >= 4) return zb::launch(gqa_append_kernel<GL, 4>, grid, block, 0, stream, 1, p);
-  return zb::launch(gqa_append_kernel<GL, 2>, grid, block, 0, stream, 1, p);
+  if (align >= 16) return zb::launch(gqa_append_kernel<GL, 16, Q4>, grid, block, 0, stream, 1, p);
+  if (align >= 4) return zb::launch(gqa_append_kernel<GL, 4, Q4>, grid, block, 0, stream, 1, p);
+  return zb::launch(gqa_append_kernel<GL, 2, Q4>, grid, block, 0, stream, 1, p);
 }
 
-}  // namespace
-
-ZB_API int zb_gqa_append(const uint16_t* proj, int64_t proj_stride, const uint16_t* temp, const int32_t* positions,
-                         float eps, int normalize, double rope_theta, int rotary_dim, int interleaved, uint16_t* q_out,
-                         int64_t q_stride, uint16_t* k_cache, uint16_t* v_cache, int64_t page_stride,
-                         int64_t slot_stride, int64_t head_stride, int64_t num_pages, int page_size,
-                         const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* cache_seqlens,
-                         const int32_t* cu_seqlens_q, int B, int N, int Hq, int Hkv, int hd, cudaStream_t stream) {
-  AppendParams p;
-  p.kv = zb::PagedBatch{reinterpret_cast<__nv_bfloat16*>(k_cache), reinterpret_cast<__nv_bfloat16*>(v_cache),
-                        page_stride, slot_stride, head_stride, num_pages, page_size, page_table, table_stride,
-                        max_pages, cache_seqlens, cu_seqlens_q, B, N, Hkv, hd};
-  if (int rc = zb::check_paged(p.kv, "gqa_append")) return rc;
-  ZB_REQUIRE(Hq > 0, "gqa_append: %d query heads", Hq);
+// The checks that follow those of the cache, and the launch; `who` names the entry point.
+template <bool Q4>
+int append(AppendParams& p, const char* who, const uint16_t* proj, int64_t proj_stride, const uint16_t* temp,
+           const int32_t* positions, float eps, int normalize, double rope_theta, int rotary_dim, int interleaved,
+           uint16_t* q_out, int64_t q_stride, int Hq, cudaStream_t stream) {
+  const int N = p.kv.N, Hkv = p.kv.Hkv, hd = p.kv.hd;
+  ZB_REQUIRE(Q4 ? Hq >= 0 : Hq > 0, "%s: %d query heads", who, Hq);
   ZB_REQUIRE(rotary_dim >= 0 && rotary_dim <= hd && rotary_dim % (interleaved ? 8 : 16) == 0,
-             "gqa_append: rotary_dim %d (at most %d, a multiple of %d)", rotary_dim, hd, interleaved ? 8 : 16);
-  ZB_REQUIRE(rope_theta > 0 && eps >= 0.f, "gqa_append: rope_theta %g > 0, eps %g >= 0", rope_theta, (double)eps);
-  ZB_REQUIRE(proj_stride >= (int64_t)(Hq + 2 * Hkv) * hd || N <= 1, "gqa_append: proj_stride %lld < %lld",
+             "%s: rotary_dim %d (at most %d, a multiple of %d)", who, rotary_dim, hd, interleaved ? 8 : 16);
+  ZB_REQUIRE(rope_theta > 0 && eps >= 0.f, "%s: rope_theta %g > 0, eps %g >= 0", who, rope_theta, (double)eps);
+  ZB_REQUIRE(proj_stride >= (int64_t)(Hq + 2 * Hkv) * hd || N <= 1, "%s: proj_stride %lld < %lld", who,
              (long long)proj_stride, (long long)(Hq + 2 * Hkv) * hd);
-  ZB_REQUIRE(q_stride >= (int64_t)Hq * hd && q_stride % 8 == 0, "gqa_append: q_stride %lld", (long long)q_stride);
+  ZB_REQUIRE(q_stride >= (int64_t)Hq * hd && q_stride % 8 == 0, "%s: q_stride %lld", who, (long long)q_stride);
   if (N == 0) return zb::kOk;
-  ZB_REQUIRE(B > 0, "gqa_append: %d tokens of no request", N);
-  ZB_REQUIRE(proj && q_out, "gqa_append: null pointer");
-  ZB_REQUIRE_ALIGNED(q_out, 16, "gqa_append q_out");
-  ZB_REQUIRE_ALIGNED(proj, 2, "gqa_append proj");
+  ZB_REQUIRE(p.kv.B > 0, "%s: %d tokens of no request", who, N);
+  ZB_REQUIRE(proj && (q_out || Hq == 0), "%s: null pointer", who);
+  ZB_REQUIRE(reinterpret_cast<uintptr_t>(q_out) % 16 == 0, "%s q_out must be 16-byte aligned", who);
+  ZB_REQUIRE(reinterpret_cast<uintptr_t>(proj) % 2 == 0, "%s proj must be 2-byte aligned", who);
   p.proj = reinterpret_cast<const __nv_bfloat16*>(proj);
   p.proj_stride = proj_stride;
   p.temp = reinterpret_cast<const __nv_bfloat16*>(temp);
@@ -251,13 +261,41 @@ ZB_API int zb_gqa_append(const uint16_t* proj, int64_t proj_stride, const uint16
   const uintptr_t spread = reinterpret_cast<uintptr_t>(proj) | (uintptr_t)(N > 1 ? proj_stride * 2 : 0);
   const int align = spread % 16 == 0 ? 16 : spread % 4 == 0 ? 4 : 2;
   cudaError_t err = cudaSuccess;
-  switch (group) {
-    case 1: err = launch_append<1>(p, align, stream); break;
-    case 2: err = launch_append<2>(p, align, stream); break;
-    case 4: err = launch_append<4>(p, align, stream); break;
-    case 8: err = launch_append<8>(p, align, stream); break;
-    default: err = launch_append<16>(p, align, stream); break;
-  }
+  if (group == 4) err = launch_append<4, Q4>(p, align, stream);
+  else if (group == 8) err = launch_append<8, Q4>(p, align, stream);
+  else if (group == 16) err = launch_append<16, Q4>(p, align, stream);
+  else if constexpr (!Q4) err = group == 1 ? launch_append<1, Q4>(p, align, stream) : launch_append<2, Q4>(p, align, stream);
   ZB_CUDA(err);
-  return zb::check_launch("gqa_append");
+  return zb::check_launch(who);
+}
+
+}  // namespace
+
+ZB_API int zb_gqa_append(const uint16_t* proj, int64_t proj_stride, const uint16_t* temp, const int32_t* positions,
+                         float eps, int normalize, double rope_theta, int rotary_dim, int interleaved, uint16_t* q_out,
+                         int64_t q_stride, uint16_t* k_cache, uint16_t* v_cache, int64_t page_stride,
+                         int64_t slot_stride, int64_t head_stride, int64_t num_pages, int page_size,
+                         const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* cache_seqlens,
+                         const int32_t* cu_seqlens_q, int B, int N, int Hq, int Hkv, int hd, cudaStream_t stream) {
+  AppendParams p;
+  p.kv = zb::PagedBatch{reinterpret_cast<__nv_bfloat16*>(k_cache), reinterpret_cast<__nv_bfloat16*>(v_cache),
+                        page_stride, slot_stride, head_stride, num_pages, page_size, page_table, table_stride,
+                        max_pages, cache_seqlens, cu_seqlens_q, B, N, Hkv, hd};
+  if (int rc = zb::check_paged(p.kv, "gqa_append")) return rc;
+  return append<false>(p, "gqa_append", proj, proj_stride, temp, positions, eps, normalize, rope_theta, rotary_dim,
+                       interleaved, q_out, q_stride, Hq, stream);
+}
+
+ZB_API int zb_gqa_append_q4(const uint16_t* proj, int64_t proj_stride, const uint16_t* temp, const int32_t* positions,
+                            float eps, int normalize, double rope_theta, int rotary_dim, int interleaved, uint16_t* q_out,
+                            int64_t q_stride, uint8_t* kv_cache, int64_t page_stride, int64_t head_stride,
+                            int64_t num_pages, int page_size, const int32_t* page_table, int64_t table_stride,
+                            int max_pages, const int32_t* cache_seqlens, const int32_t* cu_seqlens_q, int B, int N, int Hq,
+                            int Hkv, int hd, cudaStream_t stream) {
+  AppendParams p;
+  p.kv = zb::PagedBatch{reinterpret_cast<__nv_bfloat16*>(kv_cache), nullptr, page_stride, 0, head_stride, num_pages,
+                        page_size, page_table, table_stride, max_pages, cache_seqlens, cu_seqlens_q, B, N, Hkv, hd};
+  if (int rc = zb::q4::check_cache(p.kv, "gqa_append_q4")) return rc;
+  return append<true>(p, "gqa_append_q4", proj, proj_stride, temp, positions, eps, normalize, rope_theta, rotary_dim,
+                      interleaved, q_out, q_stride, Hq, stream);
 }

@@ -61,7 +61,7 @@
 // 256 single tokens, more than 64 dims do (115, 127).
 #include <algorithm>
 
-#include "paged.cuh"
+#include "kv_q4.cuh"
 #include "tc.cuh"
 #include "tc_pair.cuh"
 
@@ -85,6 +85,8 @@ constexpr int kFineRows = 16;
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
 constexpr int kMaxSlots = 10, kDescs = 4;
+// 4 bits: stages of 64 keys (their values too) as they lie in the cache, which two warps write out as bf16 tiles.
+constexpr int kRawStages = 3, kRawBlocks = 4;
 constexpr int kMasks = 8;  // of key masks and of looked-through tiles: the loaders run at most 5 tiles ahead of the rows
 constexpr float kAbove = 24.f;  // how far (log2) the m that is subtracted may lie above a row's largest score
 constexpr int kMaxRequests = 16384;
@@ -114,7 +116,8 @@ struct ChunkParams {
   int Hq, G;
   int tokens;  // of a stream: kStreamRows / G
   float scale_log2;  // softmax scale * log2(e)
-  int causal, window;
+  int causal, window, sinks;
+  int few;  // requests of up to so many rows (more than 0) are another kernel's
   const __nv_bfloat16* gate;  // [N, Hq] or null
   int64_t gate_stride;
   __nv_bfloat16* out;  // [N, Hq, hd]
@@ -143,6 +146,8 @@ struct Desc {
   int rows;       // (token, head) rows
   int kvh;
   int tile0, tiles;  // tiles of keys; 0: no row sees a key
+  int sink_tiles, gap;  // tiles from sink_tiles on are counted without the `gap` tiles that lie between sinks and window
+  int from;             // keys from the sinks' end to here are hidden from every row
   int mode;          // kFinal, kPart0, kPart1, kStop
   int parts;
   int all_lo, all_hi;  // no key of [all_lo, all_hi) is hidden from some row (a key the request does not have is a zero)
@@ -153,7 +158,7 @@ struct Tail {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t q_full[2], q_empty[2];
   uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
-  uint64_t armed[kMasks], scanned[kMasks], drained, halves;
+  uint64_t armed[kMasks], scanned[kMasks], drained, halves;  // with 4 bits, armed: a stage is there; scanned: it is free
   uint64_t desc_full[kDescs], desc_empty[kDescs];
   alignas(16) unsigned mask[kMasks][4];  // keys of a tile that exist
   Desc desc[kDescs];
@@ -167,16 +172,18 @@ struct Tail {
   int found[kMasks][2];  // either half of the tile's values holds some that are not finite
 };
 
-template <int HD>
+template <int HD, bool Q4 = false>
 struct Shape {
   // A tile of 128 rows: 8 rows x 64 dims (128 swizzled bytes each) are an atom; an 8-row group's atoms lie together, so
   // that one tensor copy of whole rows of a page, of any multiple of 8, lands in place.
   static constexpr uint32_t kGroup = HD / 64 * 1024;
   static constexpr uint32_t kItem = kTile / 8 * kGroup;
   static constexpr uint32_t kQAtom = kStreamRows * 128;  // the queries lie dims apart: 64 dims of all rows, then the next
-  static constexpr int kSlots = HD == 128 ? 5 : 10;
+  static constexpr int kSlots = Q4 ? (HD == 128 ? 4 : 6) : HD == 128 ? 5 : 10;
+  static constexpr uint32_t kRaw = Q4 ? kRawBlocks * zb::q4::block_bytes(HD) : 0;  // a stage
   static constexpr uint32_t kOffQ = kSlots * kItem;
-  static constexpr uint32_t kOffTail = kOffQ + 2 * kItem;
+  static constexpr uint32_t kOffRaw = kOffQ + 2 * kItem;
+  static constexpr uint32_t kOffTail = kOffRaw + kRawStages * kRaw;
   static constexpr size_t kSmem = kOffTail + sizeof(Tail);
   static_assert(kSlots * kItem >= kMaxRequests * 4 + kThreads * 16, "the plan's tables fit the ring");
   static_assert(kSmem <= 232448, "shared memory");
@@ -304,6 +311,8 @@ __device__ __forceinline__ Desc uniform(const Desc& d) {
   u.kvh = uniform(d.kvh);
   u.tile0 = uniform(d.tile0);
   u.tiles = uniform(d.tiles);
+  u.sink_tiles = uniform(d.sink_tiles);
+  u.gap = uniform(d.gap);
   u.mode = uniform(d.mode);
   u.parts = uniform(d.parts);
   u.all_lo = uniform(d.all_lo);
@@ -350,7 +359,16 @@ __device__ __forceinline__ unsigned not_finite(const uint4& v) {
   return not_finite(v.x) | not_finite(v.y) | not_finite(v.z) | not_finite(v.w);
 }
 // Whether a tile of keys from `first` on has keys that some of the unit's rows see and others do not.
-__device__ __forceinline__ bool mixed_tile(const Desc& u, int first) { return first + kTile > u.all_hi || first < u.all_lo; }
+template <bool SINKS>
+__device__ __forceinline__ bool mixed_tile(const Desc& u, int first, int sinks) {
+  return first + kTile > u.all_hi || (first < u.all_lo && (!SINKS || first + kTile > sinks));
+}
+// The first key of tile t of a unit.
+template <bool SINKS>
+__device__ __forceinline__ int first_key(const Desc& u, int t) {
+  const int tile = u.tile0 + t;
+  return (SINKS && tile >= u.sink_tiles ? tile + u.gap : tile) * kTile;
+}
 
 // A wait that gives up after about a second (a try that may sleep comes back after 4 us), and at once after any earlier one
 // of the CTA did. Short, because it stands in many places of loops that fill the instruction cache: the status is set at
@@ -380,6 +398,7 @@ __device__ __forceinline__ Request request(const ChunkParams& p, int b) {
   Request r;
   r.row0 = min(max(p.kv.cu[b], 0), p.kv.N);
   r.tokens = min(max(p.kv.cu[b + 1], r.row0), p.kv.N) - r.row0;
+  if (r.tokens * p.G <= p.few) r.tokens = 0;
   r.keys = max(p.kv.keys[b], 0);
   return r;
 }
@@ -388,11 +407,12 @@ __device__ __forceinline__ Request request(const ChunkParams& p, int b) {
 __device__ __forceinline__ int held_keys(const ChunkParams& p, int keys) {
   return min(keys, p.kv.max_pages * p.kv.page_size);
 }
-// Keys [lo, hi) that the token at position pos of a request with `keys` keys sees.
+// Keys [lo, hi) that the token at position pos of a request with `keys` keys sees, beside those below min(sinks, hi).
 __device__ __forceinline__ void visible(const ChunkParams& p, int keys, int pos, int& lo, int& hi) {
   const int held = held_keys(p, keys);
   hi = max(p.causal ? min(held, pos + 1) : held, 0);
   lo = p.window > 0 ? (int)max((int64_t)0, (int64_t)pos + 1 - p.window) : 0;
+  if (lo <= p.sinks) lo = 0;
 }
 
 // Streams of a request's rows come in pairs; a pair's unit of work for one KV head: its rows and key tiles.
@@ -410,8 +430,17 @@ __device__ __forceinline__ void unit_tiles(const ChunkParams& p, const Request& 
   visible(p, r.keys, d.pos0 + tokens - 1, lo1, hi1);
   d.all_lo = lo1;
   d.all_hi = hi0 == held_keys(p, r.keys) ? INT32_MAX : hi0;
+  d.from = lo0;
   d.tile0 = lo0 / kTile;
   d.tiles = hi1 > lo0 ? (hi1 + kTile - 1) / kTile - d.tile0 : 0;
+  d.sink_tiles = d.gap = 0;
+  const int seen_first = min(p.sinks, hi1);
+  if (lo0 > 0 && seen_first > 0) {  // the sinks' tiles come before the window's
+    d.sink_tiles = min((seen_first + kTile - 1) / kTile, d.tile0);
+    d.gap = d.tile0 - d.sink_tiles;
+    d.tiles += d.sink_tiles;
+    d.tile0 = 0;
+  }
 }
 
 // A unit's cost, and the first of its tiles that begin at or behind a given cost into it.
@@ -533,10 +562,12 @@ __device__ __forceinline__ void join_few(const ChunkParams& p, const Desc& u, in
   }
 }
 
-template <int HD>
+// Q4: the cache holds 4 bits (and may leave requests of few rows to another kernel). SINKS: there are first keys that stay
+// visible; a kernel of its own, as the few registers it takes would be spilled ones for the rest.
+template <int HD, bool Q4, bool SINKS>
 __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_constant__ ChunkParams p,
                                                                 const __grid_constant__ Maps maps) {
-  using L = Shape<HD>;
+  using L = Shape<HD, Q4>;
   extern __shared__ __align__(1024) unsigned char gbase[];
   const uint32_t base = zb::smem_addr(gbase);
   if (base % 1024 != 0) {  // the swizzled tiles ask for it; there is no static shared memory before them
@@ -730,7 +761,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     int64_t at = begin;
     const int unit0 = unit_cost(p, d);
     int kvh = (int)(tl.start_off / unit0), off = (int)(tl.start_off % unit0);
-    int item = 0, tile_no = 0, q_item = 0, scans = 0, n = 0;
+    int item = 0, tile_no = 0, q_item = 0, scans = 0, n = 0, raws = 0;
     bool going = true;  // until a wait for room gave up
     auto room = [&](const uint64_t& bar, uint32_t parity) {
       going = __all_sync(0xffffffffu, wait(bar, parity, abort));
@@ -747,12 +778,13 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       const int32_t* table = p.kv.table + (int64_t)min(b, B - 1) * p.kv.table_stride;
       // Page lookups, a tile ahead of their use and before anything that can wait. A lane's box of a tile:
       const int boxes = p.box ? kTile >> p.box_shift : 0;
-      auto look_box = [&](int t) {
-        const int pos = t * kTile + lane * p.box;
-        return lane < boxes && pos < held ? table[p.by_page.quotient(pos)] : -1;
+      auto look_box = [&](int t) {  // of tile t of the unit's from from_tile on
+        const int pos = first_key<SINKS>(d, from_tile + t) + lane * p.box;
+        const bool hidden = SINKS && pos >= p.sinks && pos + p.box <= d.from;  // from every row: not brought
+        return lane < boxes && pos < held && !hidden ? table[p.by_page.quotient(pos)] : -1;
       };
       int next = -1;
-      if (p.box && here && warp == kLoadWarp) next = look_box(d.tile0 + from_tile);
+      if (p.box && here && warp == kLoadWarp) next = look_box(0);
       if (here || at >= end) {
         u.tile0 = d.tile0 + from_tile;
         u.tiles = to_tile - from_tile;
@@ -796,8 +828,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         // tensor copies these warps pass over whole tiles, so they would get to one whose slot is phases behind, and take an
         // older phase for the tile's: they wait until the tile's copies have been started.
         auto look_through = [&](int t, int v_item) {
-          const int first = (u.tile0 + t) * kTile, slot = scans % kMasks;
-          if (warp == kLoadWarp || !mixed_tile(u, first)) return;
+          const int first = first_key<SINKS>(u, t), slot = scans % kMasks;
+          if (warp == kLoadWarp || !mixed_tile<SINKS>(u, first, p.sinks)) return;
           if (p.box) wait(tl.armed[slot], (scans / kMasks) & 1, abort);
           wait(tl.full[v_item % L::kSlots], (v_item / L::kSlots) & 1, abort);
           // groups of 8 rows in turn; rows past the request's keys are no values (warp 8 zeroes them)
@@ -818,12 +850,102 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           }
           ++scans;
         };
-        if (p.box) {
+        if (Q4) {
+          const int block = zb::q4::block_bytes(hd);
+          if (warp == kLoadWarp) {  // blocks of 16 keys as they lie in the cache, a bulk copy each
+#pragma unroll 1
+            for (int t = 0; t < u.tiles && going; ++t, ++tile_no) {
+              const int first = first_key<SINKS>(u, t), pos = first + lane * zb::q4::kBlock;
+              const bool there = next >= 0 && next < p.kv.num_pages;
+              const int64_t from = there ? (int64_t)next * p.kv.page_stride + (int64_t)kvh * p.kv.head_stride +
+                                               (int64_t)(p.by_page.rest(pos) / zb::q4::kBlock) * block
+                                         : 0;
+              const unsigned live = __ballot_sync(0xffffffffu, there);
+              unsigned bits[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const int r = 32 * k + lane;
+                bits[k] = __ballot_sync(0xffffffffu, first + r < held && (live >> (r / zb::q4::kBlock) & 1u));
+              }
+              if (t + 1 < u.tiles) next = look_box(t + 1);
+#pragma unroll 1
+              for (int half = 0; half < 2; ++half, ++raws) {
+                const int slot = raws % kRawStages;
+                if (raws >= kRawStages && !room(tl.scanned[slot], (raws / kRawStages - 1) & 1)) break;
+                if (lane == 0) {
+                  if (half == 0) *reinterpret_cast<uint4*>(tl.mask[tile_no % kMasks]) = make_uint4(bits[0], bits[1], bits[2], bits[3]);
+                  zb::mbar_arrive_expect_tx(zb::smem_addr(&tl.armed[slot]),
+                                            (uint32_t)(__popc(live >> (kRawBlocks * half) & ((1u << kRawBlocks) - 1)) * block));
+                }
+                __syncwarp();
+                if (there && lane / kRawBlocks == half)
+                  zb::bulk_g2s(base + L::kOffRaw + slot * L::kRaw + lane % kRawBlocks * block,
+                               reinterpret_cast<const unsigned char*>(p.kv.k) + from, (uint32_t)block,
+                               zb::smem_addr(&tl.armed[slot]));
+              }
+            }
+          } else {  // the keys (warp 10) and values (warp 11) of a tile as bf16, absent ones as zeros
+            const int kv = lw - 1, part = lane % 4, groups = hd / zb::q4::kGroup;
+            // The 8 rows that a warp takes at a time, ordered so that two rows of a quarter of its lanes read and write other
+            // banks: 64 bytes of codes and, in the swizzled tile, 4 pieces of 16 bytes each.
+            const int row8 = (0x63724150u >> (4 * (lane / 4))) & 7;
+#pragma unroll 1
+            for (int t = 0; t < u.tiles && going; ++t, ++tile_no, item += 2) {
+              const int slot = (item + kv) % L::kSlots;
+              uint4 exist{};
+#pragma unroll 1
+              for (int half = 0; half < 2; ++half, ++raws) {
+                const int stage = raws % kRawStages;
+                if (!wait(tl.armed[stage], (raws / kRawStages) & 1, abort)) going = false;
+                if (half == 0) {
+                  if (item >= L::kSlots && !room(tl.empty[slot], (item / L::kSlots - 1) & 1)) break;
+                  exist = *reinterpret_cast<const uint4*>(tl.mask[tile_no % kMasks]);
+                }
+                const unsigned char* raw = gbase + L::kOffRaw + stage * L::kRaw;
+                const unsigned lower = half ? exist.z : exist.x, upper = half ? exist.w : exist.y;
+#pragma unroll 4
+                for (int i = 0; i < 8; ++i) {
+                  const int r = 8 * i + row8, in = r % zb::q4::kBlock;  // of the stage, of the block
+                  const unsigned char* from = raw + r / zb::q4::kBlock * block;
+                  const bool exists = ((i < 4 ? lower : upper) >> (r % 32)) & 1u;
+                  uint32_t words[HD / 32], pairs[HD / 32];
+                  const uint32_t* w = reinterpret_cast<const uint32_t*>(from + 8 * kv * hd + in * (hd / 2)) + part * groups;
+                  const uint32_t* q = reinterpret_cast<const uint32_t*>(from + (16 + 2 * kv) * hd) + in * groups;
+                  if (HD == 128 && hd == HD) {
+                    *reinterpret_cast<uint4*>(words) = *reinterpret_cast<const uint4*>(w);
+                    *reinterpret_cast<uint4*>(pairs) = *reinterpret_cast<const uint4*>(q);
+                  } else if (HD == 64 && hd == HD) {
+                    *reinterpret_cast<uint2*>(words) = *reinterpret_cast<const uint2*>(w);
+                    *reinterpret_cast<uint2*>(pairs) = *reinterpret_cast<const uint2*>(q);
+                  } else {
+#pragma unroll
+                    for (int g = 0; g < HD / 32; ++g) {
+                      words[g] = g < groups ? w[g] : 0;
+                      pairs[g] = g < groups ? q[g] : 0;
+                    }
+                  }
+#pragma unroll
+                  for (int g = 0; g < HD / 32; ++g) {
+                    const uint32_t pair = exists && !zb::q4::pair_is_none(pairs[g]) ? pairs[g] : 0u;
+                    if (g < groups)
+                      *reinterpret_cast<uint4*>(gbase + slot * L::kItem + piece<HD>(64 * half + r, 4 * g + part)) =
+                          zb::q4::read_word(words[g], pair);
+                  }
+                }
+                __syncwarp();
+                if (lane == 0) arrive(tl.scanned[stage]);
+              }
+              tc::fence_proxy_async();  // what was written -> the tensor cores
+              __syncwarp();
+              if (lane == 0) arrive(tl.full[slot]);
+            }
+          }
+        } else if (p.box) {
           if (warp == kLoadWarp) {
 #pragma unroll 1
             for (int t = 0; t < u.tiles && going; ++t, ++tile_no) {
-              const int first = (u.tile0 + t) * kTile, pos = first + lane * p.box;
-              const bool mixed = mixed_tile(u, first);
+              const int first = first_key<SINKS>(u, t), pos = first + lane * p.box;
+              const bool mixed = mixed_tile<SINKS>(u, first, p.sinks);
               const bool there = next >= 0 && next < p.kv.num_pages;
               const int page = there ? next * p.page_heads + (p.page_heads > 1 ? kvh : 0)
                                      : (int)(p.kv.num_pages * p.page_heads);  // past the end: zeros
@@ -835,7 +957,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                 const int r = 32 * k + lane;
                 bits[k] = __ballot_sync(0xffffffffu, first + r < held && (live >> (r >> p.box_shift) & 1u));
               }
-              if (t + 1 < u.tiles) next = look_box(u.tile0 + t + 1);
+              if (t + 1 < u.tiles) next = look_box(t + 1);
 #pragma unroll 1
               for (int kv = 0; kv < 2; ++kv, ++item) {
                 const int slot = item % L::kSlots;
@@ -861,25 +983,26 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           auto look = [&](int t) {  // pages of the lane's rows of tile t
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const int pos = t * kTile + 32 * k + lane;
-              pages[k] = pos < held ? table[p.by_page.quotient(pos)] : -1;
+              const int pos = first_key<SINKS>(u, t) + 32 * k + lane;
+              const bool hidden = SINKS && pos >= p.sinks && pos < u.from;  // from every row: not brought
+              pages[k] = pos < held && !hidden ? table[p.by_page.quotient(pos)] : -1;
             }
           };
-          look(u.tile0);
+          look(0);
 #pragma unroll 1
           for (int t = 0; t < u.tiles && going; ++t, ++tile_no) {
             int64_t off[4];
             unsigned bits[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const int pos = (u.tile0 + t) * kTile + 32 * k + lane;
+              const int pos = first_key<SINKS>(u, t) + 32 * k + lane;
               const bool there = pages[k] >= 0 && pages[k] < p.kv.num_pages;
               off[k] = there ? (int64_t)pages[k] * p.kv.page_stride + (int64_t)p.by_page.rest(pos) * p.kv.slot_stride +
                                    (int64_t)kvh * p.kv.head_stride
                              : -1;
               bits[k] = __ballot_sync(0xffffffffu, there);
             }
-            if (t + 1 < u.tiles) look(u.tile0 + t + 1);
+            if (t + 1 < u.tiles) look(t + 1);
 #pragma unroll 1
             for (int kv = 0; kv < 2; ++kv, ++item) {
               const int slot = item % L::kSlots;
@@ -922,7 +1045,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         zb::mbar_wait_bounded(zb::smem_addr(full + lane), (items - 1 - lane) / slots & 1, p.status, zb::kStatusAttnChunkTimeout);
       __syncwarp();
     };
-    if (warp == kLoadWarp && p.box) landed(tl.full, L::kSlots, item);
+    if (warp == kLoadWarp && p.box && !Q4) landed(tl.full, L::kSlots, item);
+    if (warp == kLoadWarp && Q4) landed(tl.armed, kRawStages, raws);
     if (warp == kLoadWarp + 1) landed(tl.q_full, 2, q_item);
   } else if (warp == kMmaWarp) {
     // =============================================================================================== tensor cores
@@ -990,14 +1114,14 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       for (int t = -stride; t < u.tiles; ++t) {
         // O_s += P_s(t) V(t) as soon as P_s(t) is there, then the stream's next scores; before the first tile, those alone
         const bool more = t + stride < u.tiles, ends = t + stride == u.tiles - 1;
-        const int s0 = two ? 0 : t & 1, s1 = two ? 1 : s0, first = (u.tile0 + t) * kTile;
+        const int s0 = two ? 0 : t & 1, s1 = two ? 1 : s0, first = first_key<SINKS>(u, t);
         const Ring v = at.after(1), k = ahead;
         unsigned char* v_tile = gbase + v.slot * L::kItem;
         bool found = false;
         if (t >= 0) {
           full(v);
           // rows of the last page past the request's keys came along with a tensor copy: no key, so no value either
-          if (p.box && first + kTile > held && held % p.box != 0) {
+          if (!Q4 && p.box && first + kTile > held && held % p.box != 0) {
             const int r0 = held - first, r1 = (r0 + p.box - 1) / p.box * p.box;
 #pragma unroll 1
             for (int i = r0 * (HD / 8) + lane; i < r1 * (HD / 8); i += 32)
@@ -1005,7 +1129,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
             tc::fence_proxy_async();
             __syncwarp();
           }
-          if (mixed_tile(u, first)) {
+          if (!Q4 && mixed_tile<SINKS>(u, first, p.sinks)) {
             const int slot = scans % kMasks;
             wait(tl.scanned[slot], (scans / kMasks) & 1, abort);
             ++scans;
@@ -1103,8 +1227,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
         }
 #pragma unroll 1
         for (int t = 0; t < u.tiles; ++t) {
-          const int first = (u.tile0 + t) * kTile;
-          const bool scan = mixed_tile(u, first);
+          const int first = first_key<SINKS>(u, t);
+          const bool scan = !Q4 && mixed_tile<SINKS>(u, first, p.sinks);
           if (!two && (t & 1) != s) {  // the other half's tile
             scans += scan;
             continue;
@@ -1128,13 +1252,16 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
           }
           const unsigned* there = tl.mask[(tile_no + t) % kMasks];
           const uint4 all4 = *reinterpret_cast<const uint4*>(there);
-          const bool partly = __any_sync(0xffffffffu, first < lo || first + kTile > hi ||
+          const bool partly = __any_sync(0xffffffffu, (first < lo && (!SINKS || first + kTile > p.sinks)) || first + kTile > hi ||
                                                           (all4.x & all4.y & all4.z & all4.w) != 0xffffffffu);
           auto seen = [&](int c) {  // which of keys 32 c .. of the tile the row sees
             const int a = min(max(lo - first - 32 * c, 0), 32), z = min(max(hi - first - 32 * c, 0), 32);
             const unsigned below = z >= 32 ? 0xffffffffu : (1u << z) - 1u;
             const unsigned under = a >= 32 ? 0xffffffffu : (1u << a) - 1u;
-            return there[c] & below & ~under;
+            if (!SINKS) return there[c] & below & ~under;
+            const int k = min(max(p.sinks - first - 32 * c, 0), 32);
+            const unsigned kept = k >= 32 ? 0xffffffffu : (1u << k) - 1u;
+            return there[c] & below & (~under | kept);
           };
           const uint64_t scale2 = pack2(p.scale_log2, p.scale_log2);
           uint64_t minus, sum2[2] = {0, 0};
@@ -1619,7 +1746,7 @@ Launch plan(int B, int64_t N, int Hq, int Hkv, int hd, int64_t max_keys) {
 // Tensor maps: the queries, and over the caches for copies of whole page rows: [64 dims, 8 rows, atoms, row groups, pages], with the KV
 // heads folded into the atoms (a row's heads side by side) or the pages (a page's heads one after the other). p.box
 // stays 0 where the layout, the page size or the head dim does not allow them.
-template <int HD>
+template <int HD, bool Q4>
 int make_maps(ChunkParams& p, Maps& maps) {
   const zb::PagedBatch& c = p.kv;
   auto fn = zb::tcp::encode_fn();
@@ -1638,6 +1765,11 @@ int make_maps(ChunkParams& p, Maps& maps) {
     const cuuint32_t boxes[3] = {64, (cuuint32_t)p.G, (cuuint32_t)p.tokens};
     ZB_REQUIRE(p.q_stride < (int64_t)1 << 38, "gqa_chunk: q_stride %lld", (long long)p.q_stride);
     if (int rc = encode(&maps.q, 3, p.q, dims, strides, boxes)) return rc;
+  }
+  if (Q4) {  // blocks come by bulk copies
+    p.box = zb::q4::kBlock;
+    p.box_shift = 4;
+    return zb::kOk;
   }
   p.box = 0;
   int box = 1;
@@ -1661,74 +1793,63 @@ int make_maps(ChunkParams& p, Maps& maps) {
   return zb::kOk;
 }
 
-template <int HD>
+template <int HD, bool Q4, bool SINKS>
 int launch_chunk(ChunkParams& p, const Launch& l, cudaStream_t stream) {
   Maps maps = {};
-  if (int rc = make_maps<HD>(p, maps)) return rc;
-  auto kernel = gqa_chunk_kernel<HD>;
+  if (int rc = make_maps<HD, Q4>(p, maps)) return rc;
+  auto kernel = gqa_chunk_kernel<HD, Q4, SINKS>;
   static bool configured[64] = {false};  // the shared-memory attribute, set once per device
   int dev = 0;
   ZB_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !configured[dev]) {
-    ZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD>::kSmem));
+    ZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD, Q4>::kSmem));
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  ZB_CUDA(zb::launch(kernel, dim3((unsigned)l.ctas), dim3(kThreads), Shape<HD>::kSmem, stream, 1, p, maps));
+  ZB_CUDA(zb::launch(kernel, dim3((unsigned)l.ctas), dim3(kThreads), Shape<HD, Q4>::kSmem, stream, 1, p, maps));
   return zb::check_launch("gqa_chunk");
 }
 
-}  // namespace
-
-ZB_API int64_t zb_gqa_chunk_workspace_bytes(int B, int N, int Hq, int Hkv, int hd, int64_t max_keys) {
-  const Launch l = plan(B, N, Hq, Hkv, hd, max_keys);
-  return l.flag_bytes + l.acc_bytes + l.ml_bytes;
-}
-
-ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache,
-                        int64_t page_stride, int64_t slot_stride, int64_t head_stride, int64_t num_pages, int page_size,
-                        const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* cache_seqlens,
-                        const int32_t* cu_seqlens_q, int B, int N, int Hq, int Hkv, int hd, float softmax_scale,
-                        int causal, int window, const uint16_t* gate, int64_t gate_stride, uint16_t* out,
-                        int64_t out_stride, float* lse, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
-  ChunkParams p;
-  p.kv = zb::PagedBatch{reinterpret_cast<__nv_bfloat16*>(const_cast<uint16_t*>(k_cache)),
-                        reinterpret_cast<__nv_bfloat16*>(const_cast<uint16_t*>(v_cache)), page_stride, slot_stride,
-                        head_stride, num_pages, page_size, page_table, table_stride, max_pages, cache_seqlens,
-                        cu_seqlens_q, B, N, Hkv, hd};
-  if (int rc = zb::check_paged(p.kv, "gqa_chunk")) return rc;
-  ZB_REQUIRE(Hq > 0 && Hq % Hkv == 0, "gqa_chunk: %d query heads do not group over %d KV heads", Hq, Hkv);
-  ZB_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, "gqa_chunk: softmax_scale %g must be positive",
+// What both caches' entry points do once the cache has been checked; `who` names the entry point.
+template <bool Q4>
+int chunk(ChunkParams& p, const char* who, const uint16_t* q, int64_t q_stride, int Hq, float softmax_scale, int causal,
+          int window, int sinks, int few, const uint16_t* gate, int64_t gate_stride, uint16_t* out, int64_t out_stride,
+          float* lse, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
+  const int B = p.kv.B, N = p.kv.N, Hkv = p.kv.Hkv, hd = p.kv.hd;
+  ZB_REQUIRE(Hq > 0 && Hq % Hkv == 0, "%s: %d query heads do not group over %d KV heads", who, Hq, Hkv);
+  ZB_REQUIRE(softmax_scale > 0.f && softmax_scale < INFINITY, "%s: softmax_scale %g must be positive", who,
              (double)softmax_scale);
-  ZB_REQUIRE(window >= 0 && (causal || window == 0), "gqa_chunk: window %d (>= 0, and only with causal)", window);
+  ZB_REQUIRE(window >= 0 && (causal || window == 0), "%s: window %d (>= 0, and only with causal)", who, window);
+  ZB_REQUIRE(sinks >= 0, "%s: sinks %d must not be negative", who, sinks);
   ZB_REQUIRE(q_stride >= (int64_t)Hq * hd && q_stride % 8 == 0 && out_stride >= (int64_t)Hq * hd && out_stride % 8 == 0 &&
                  (!gate || gate_stride >= Hq),
-             "gqa_chunk: strides (q %lld, out %lld, gate %lld)", (long long)q_stride, (long long)out_stride,
+             "%s: strides (q %lld, out %lld, gate %lld)", who, (long long)q_stride, (long long)out_stride,
              (long long)gate_stride);
-  ZB_REQUIRE((int64_t)N * Hq < (int64_t)1 << 31, "gqa_chunk: %d tokens x %d heads", N, Hq);
+  ZB_REQUIRE((int64_t)N * Hq < (int64_t)1 << 31, "%s: %d tokens x %d heads", who, N, Hq);
   if (Hq / Hkv > kStreamRows)
-    return zb::fail(zb::kUnsupported, "gqa_chunk: %d query heads a KV head (at most %d)", Hq / Hkv, kStreamRows);
-  if (B > kMaxRequests) return zb::fail(zb::kUnsupported, "gqa_chunk: %d requests (at most %d)", B, kMaxRequests);
+    return zb::fail(zb::kUnsupported, "%s: %d query heads a KV head (at most %d)", who, Hq / Hkv, kStreamRows);
+  if (B > kMaxRequests) return zb::fail(zb::kUnsupported, "%s: %d requests (at most %d)", who, B, kMaxRequests);
   if (N == 0) return zb::kOk;
-  ZB_REQUIRE(B > 0, "gqa_chunk: %d tokens of no request", N);
-  ZB_REQUIRE(q && out, "gqa_chunk: null pointer");
-  ZB_REQUIRE_ALIGNED(q, 16, "gqa_chunk q");
-  ZB_REQUIRE_ALIGNED(out, 16, "gqa_chunk out");
-  const Launch l = plan(B, N, Hq, Hkv, hd, (int64_t)page_size * max_pages);
+  ZB_REQUIRE(B > 0, "%s: %d tokens of no request", who, N);
+  ZB_REQUIRE(q && out, "%s: null pointer", who);
+  ZB_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 == 0,
+             "%s: q, out and workspace must be 16-byte aligned", who);
+  const Launch l = plan(B, N, Hq, Hkv, hd, (int64_t)p.kv.page_size * p.kv.max_pages);
   const int64_t need = l.flag_bytes + l.acc_bytes + l.ml_bytes;
-  ZB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "gqa_chunk: a workspace of %lld bytes, got %lld",
+  ZB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "%s: a workspace of %lld bytes, got %lld", who,
              (long long)need, (long long)workspace_bytes);
-  ZB_REQUIRE_ALIGNED(workspace, 16, "gqa_chunk workspace");
   p.q = reinterpret_cast<const __nv_bfloat16*>(q);
   p.q_stride = q_stride;
   p.Hq = Hq;
   p.G = Hq / Hkv;
   p.tokens = kStreamRows / p.G;
-  p.by_page.set(page_size);
+  p.by_page.set(p.kv.page_size);
   p.by_group.set(p.G);
   p.by_pair.set(2 * p.tokens);
   p.scale_log2 = softmax_scale * 1.4426950408889634f;
   p.causal = causal;
   p.window = window;
+  p.sinks = window > 0 ? sinks : 0;
+  p.few = few;
   p.gate = reinterpret_cast<const __nv_bfloat16*>(gate);
   p.gate_stride = gate_stride;
   p.out = reinterpret_cast<__nv_bfloat16*>(out);
@@ -1743,5 +1864,64 @@ ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_c
   p.ml = reinterpret_cast<float*>(ws + l.flag_bytes + l.acc_bytes);
   p.rows_max = l.rows_max;
   p.status = zb::device_status_ptr();
-  return hd <= 64 ? launch_chunk<64>(p, l, stream) : launch_chunk<128>(p, l, stream);
+  if constexpr (!Q4)
+    if (p.sinks == 0) return hd <= 64 ? launch_chunk<64, false, false>(p, l, stream) : launch_chunk<128, false, false>(p, l, stream);
+  return hd <= 64 ? launch_chunk<64, Q4, true>(p, l, stream) : launch_chunk<128, Q4, true>(p, l, stream);
+}
+
+}  // namespace
+
+ZB_API int64_t zb_gqa_chunk_workspace_bytes(int B, int N, int Hq, int Hkv, int hd, int64_t max_keys) {
+  const Launch l = plan(B, N, Hq, Hkv, hd, max_keys);
+  return l.flag_bytes + l.acc_bytes + l.ml_bytes;
+}
+
+ZB_API int zb_gqa_chunk_sinks(const uint16_t* q, int64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache,
+                              int64_t page_stride, int64_t slot_stride, int64_t head_stride, int64_t num_pages,
+                              int page_size, const int32_t* page_table, int64_t table_stride, int max_pages,
+                              const int32_t* cache_seqlens, const int32_t* cu_seqlens_q, int B, int N, int Hq, int Hkv,
+                              int hd, float softmax_scale, int causal, int window, int sinks, const uint16_t* gate,
+                              int64_t gate_stride, uint16_t* out, int64_t out_stride, float* lse, void* workspace,
+                              int64_t workspace_bytes, cudaStream_t stream) {
+  ChunkParams p;
+  p.kv = zb::PagedBatch{reinterpret_cast<__nv_bfloat16*>(const_cast<uint16_t*>(k_cache)),
+                        reinterpret_cast<__nv_bfloat16*>(const_cast<uint16_t*>(v_cache)), page_stride, slot_stride,
+                        head_stride, num_pages, page_size, page_table, table_stride, max_pages, cache_seqlens,
+                        cu_seqlens_q, B, N, Hkv, hd};
+  if (int rc = zb::check_paged(p.kv, "gqa_chunk")) return rc;
+  return chunk<false>(p, "gqa_chunk", q, q_stride, Hq, softmax_scale, causal, window, sinks, 0, gate, gate_stride, out,
+                      out_stride, lse, workspace, workspace_bytes, stream);
+}
+
+ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_cache, const uint16_t* v_cache,
+                        int64_t page_stride, int64_t slot_stride, int64_t head_stride, int64_t num_pages, int page_size,
+                        const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* cache_seqlens,
+                        const int32_t* cu_seqlens_q, int B, int N, int Hq, int Hkv, int hd, float softmax_scale,
+                        int causal, int window, const uint16_t* gate, int64_t gate_stride, uint16_t* out,
+                        int64_t out_stride, float* lse, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
+  return zb_gqa_chunk_sinks(q, q_stride, k_cache, v_cache, page_stride, slot_stride, head_stride, num_pages, page_size,
+                            page_table, table_stride, max_pages, cache_seqlens, cu_seqlens_q, B, N, Hq, Hkv, hd,
+                            softmax_scale, causal, window, 0, gate, gate_stride, out, out_stride, lse, workspace,
+                            workspace_bytes, stream);
+}
+
+ZB_API int64_t zb_gqa_chunk_q4_workspace_bytes(int B, int N, int Hq, int Hkv, int hd, int64_t max_keys, int max_new) {
+  (void)max_new;
+  return zb_gqa_chunk_workspace_bytes(B, N, Hq, Hkv, hd, max_keys);
+}
+
+ZB_API int zb_gqa_chunk_q4(const uint16_t* q, int64_t q_stride, const uint8_t* kv_cache, int64_t page_stride,
+                           int64_t head_stride, int64_t num_pages, int page_size, const int32_t* page_table,
+                           int64_t table_stride, int max_pages, const int32_t* cache_seqlens, const int32_t* cu_seqlens_q,
+                           int B, int N, int Hq, int Hkv, int hd, float softmax_scale, int causal, int window, int sinks,
+                           int max_new, const uint16_t* gate, int64_t gate_stride, uint16_t* out, int64_t out_stride,
+                           float* lse, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
+  ChunkParams p;
+  p.kv = zb::PagedBatch{reinterpret_cast<__nv_bfloat16*>(const_cast<uint8_t*>(kv_cache)), nullptr, page_stride, 0,
+                        head_stride, num_pages, page_size, page_table, table_stride, max_pages, cache_seqlens,
+                        cu_seqlens_q, B, N, Hkv, hd};
+  if (int rc = zb::q4::check_cache(p.kv, "gqa_chunk_q4")) return rc;
+  ZB_REQUIRE(max_new >= 0, "gqa_chunk_q4: max_new %d must not be negative", max_new);
+  return chunk<true>(p, "gqa_chunk_q4", q, q_stride, Hq, softmax_scale, causal, window, sinks, 0, gate, gate_stride, out,
+                     out_stride, lse, workspace, workspace_bytes, stream);
 }

@@ -1,0 +1,127 @@
+// A paged KV cache in 4 bits: its layout, and the arithmetic of its groups.
+//
+// 32 consecutive elements of a token's key or value of one KV head are a group; it is kept as 4-bit codes c and a pair (s, m)
+// of bf16, and stands for x = m + s c. From x (bf16; NaN counts as 0, and what is beyond +-2^99 as that):
+//   m = min x,  s = bf16((max x - min x) / 15) (0 where that is below 2^-100),  c = floor((x - m) / s + 1/2), 0 .. 15 (0 where s = 0)
+// m is one of the elements, so storing it rounds nothing; s is rounded before it divides, so c allows for it. A pair with a
+// magnitude of 2^100 or more, or a NaN, is never written and stands for zeros: rows that no token wrote hold anything, and
+// 0 x inf would be NaN in a matrix product that counts them with weight 0.
+//
+// 16 consecutive keys of a head are a block of 20 hd bytes, a page of a head is page_size / 16 blocks one after the other:
+//   [0, 8 hd) codes of the keys, 16 rows of hd / 2 bytes; [8 hd, 16 hd) codes of the values;
+//   [16 hd, 18 hd) pairs of the keys, 16 rows of hd / 32 (s in the lower half of a 32-bit word); [18 hd, 20 hd) of the values.
+// So one bulk copy of 20 hd bytes (2560 at hd 128) brings the keys and values of 16 tokens of a head. A row's codes are
+// 32-bit words: word t * (hd / 32) + g holds elements e = 0 .. 7 of dims 32 g + 8 t + e, element e in bits 4 (e / 2 + 4 (e % 2))
+// and up. (w >> 4 i) & 0x000f000f is then the pair of elements 2 i, 2 i + 1, as matrix fragments hold them; a word lies in one
+// group; and the words of a t are consecutive, which are what one lane of a fragment of 16 keys needs of a row.
+#pragma once
+
+#include "paged.cuh"
+
+namespace zb {
+namespace q4 {
+
+constexpr int kBlock = 16;   // keys of a block
+constexpr int kGroup = 32;   // elements of a group
+constexpr float kLargest = 0x1p99f, kSmallestStep = 0x1p-100f;
+
+__host__ __device__ constexpr int block_bytes(int hd) { return 20 * hd; }
+
+// The cache as a PagedBatch: `k` is its first byte, strides are in bytes, `v` and slot_stride are not used.
+inline int check_cache(const PagedBatch& p, const char* who) {
+  ZB_REQUIRE(p.B >= 0 && p.N >= 0 && p.Hkv > 0 && p.num_pages >= 0 && p.max_pages >= 0, "%s: negative sizes", who);
+  if (p.hd < kGroup || p.hd > 128 || p.hd % kGroup != 0)
+    return fail(kUnsupported, "%s: head dim %d (32, 64, 96 or 128)", who, p.hd);
+  ZB_REQUIRE(p.page_size >= kBlock && p.page_size % kBlock == 0 && (int64_t)p.page_size * p.max_pages <= (int64_t)1 << 26,
+             "%s: page size %d (a multiple of 16) x %d table columns (at most 2^26 keys)", who, p.page_size, p.max_pages);
+  ZB_REQUIRE(p.page_stride % 16 == 0 && p.head_stride % 16 == 0 && p.page_stride >= 0 && p.head_stride >= 0,
+             "%s: cache strides (page %lld, head %lld bytes) must be multiples of 16", who, (long long)p.page_stride,
+             (long long)p.head_stride);
+  ZB_REQUIRE(p.table_stride >= p.max_pages || p.B <= 1, "%s: table stride %lld < %d columns", who,
+             (long long)p.table_stride, p.max_pages);
+  if (p.B == 0 || p.N == 0) return kOk;
+  ZB_REQUIRE(p.cu && p.keys && (p.table || p.max_pages == 0) && (p.k || p.num_pages == 0), "%s: null pointer", who);
+  ZB_REQUIRE(reinterpret_cast<uintptr_t>(p.k) % 16 == 0, "%s: the cache must be 16-byte aligned", who);
+  return kOk;
+}
+
+// A pair as the rule above has it: 0 where one of its numbers is not finite or has a magnitude of 2^100 or more (its exponent
+// field is 227 or more: added to 0x8000 - 0x7180 it carries into the sign).
+__device__ __forceinline__ bool pair_is_none(uint32_t pair) { return (((pair & 0x7fff7fffu) + 0x0e800e80u) & 0x80008000u) != 0; }
+
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
+__device__ __forceinline__ uint32_t as_word(__nv_bfloat162 h) { return *reinterpret_cast<const uint32_t*>(&h); }
+
+// 128 + c of codes 2 i, 2 i + 1 of a word, as bf16: 128 has its last bit at 1, so a code is the lower bits of the significand.
+template <int I>
+__device__ __forceinline__ uint32_t codes_128(uint32_t word) {
+  return ((word >> (4 * I)) & 0x000f000fu) | 0x43004300u;
+}
+// m + s c of two codes, rounded once: s2, m2 hold s and m twice (or those of two tokens).
+__device__ __forceinline__ uint32_t stands_for(uint32_t c128, uint32_t s2, uint32_t m2) {
+  return as_word(__hfma2(__hsub2(as_bf162(c128), as_bf162(0x43004300u)), as_bf162(s2), as_bf162(m2)));
+}
+// The 8 elements of a word of codes, as bf16.
+__device__ __forceinline__ uint4 read_word(uint32_t word, uint32_t pair) {
+  const uint32_t s2 = __byte_perm(pair, 0, 0x1010), m2 = __byte_perm(pair, 0, 0x3232);
+  return make_uint4(stands_for(codes_128<0>(word), s2, m2), stands_for(codes_128<1>(word), s2, m2),
+                    stands_for(codes_128<2>(word), s2, m2), stands_for(codes_128<3>(word), s2, m2));
+}
+
+// 8 bf16 elements of a group whose other elements are on the lanes' neighbours (4 lanes of a group, lane % 4 = t): their
+// word of codes and the group's pair. Every lane of the warp takes part.
+__device__ __forceinline__ uint32_t write_word(uint4 x, uint32_t& pair) {
+  uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  // the smallest element and the negated largest, as a pair of bf16; a NaN anywhere comes out as NaN
+  auto bounds = [&]() {
+    const __nv_bfloat162 lo = __hmin2_nan(__hmin2_nan(as_bf162(w[0]), as_bf162(w[1])), __hmin2_nan(as_bf162(w[2]), as_bf162(w[3])));
+    const __nv_bfloat162 hi = __hmax2_nan(__hmax2_nan(as_bf162(w[0]), as_bf162(w[1])), __hmax2_nan(as_bf162(w[2]), as_bf162(w[3])));
+    const uint32_t l = as_word(lo), h = as_word(hi) ^ 0x80008000u;
+    __nv_bfloat162 b = __hmin2_nan(as_bf162(__byte_perm(l, h, 0x5410)), as_bf162(__byte_perm(l, h, 0x7632)));
+#pragma unroll
+    for (int o = 1; o < 4; o *= 2) b = __hmin2_nan(b, as_bf162(__shfl_xor_sync(0xffffffffu, as_word(b), o)));
+    return as_word(b);
+  };
+  uint32_t b = bounds();
+  float low = __uint_as_float(b << 16), high = -__uint_as_float(b & 0xffff0000u);
+  if (__any_sync(0xffffffffu, !(low >= -kLargest && high <= kLargest))) {  // elements that 4 bits do not keep
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t fixed = 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float v = __uint_as_float(e ? w[i] & 0xffff0000u : w[i] << 16);
+        const float kept = v != v ? 0.f : fminf(fmaxf(v, -kLargest), kLargest);  // exact in bf16
+        fixed |= e ? __float_as_uint(kept) : __float_as_uint(kept) >> 16;
+      }
+      w[i] = fixed;
+    }
+    b = bounds();
+    low = __uint_as_float(b << 16);
+    high = -__uint_as_float(b & 0xffff0000u);
+  }
+  float s = bf16_round(__fdiv_rn(high - low, 15.f));
+  if (s < kSmallestStep) s = 0.f;
+  pair = (__float_as_uint(s) >> 16) | (__float_as_uint(low) & 0xffff0000u);
+  const float r = s > 0.f ? __frcp_rn(s) : 0.f, half = 0.5f * s;
+  constexpr float kMagic = 12582912.f;  // 1.5 x 2^23: a sum with it has the nearest integer in its lower bits
+  uint32_t word = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float d = __uint_as_float(e ? w[i] & 0xffff0000u : w[i] << 16) - low;
+      float c = fmaf(d, r, kMagic) - kMagic;
+      // d r may be an ulp off, and rounds halves to even: what is left of d after c steps tells which code it is
+      const float left = fmaf(-c, s, d);
+      if (left >= half) c += 1.f;
+      if (left < -half) c -= 1.f;
+      c = s > 0.f ? fminf(c, 15.f) : 0.f;
+      word |= (__float_as_uint(c + kMagic) & 15u) << (4 * (i + 4 * e));
+    }
+  }
+  return word;
+}
+
+}  // namespace q4
+}  // namespace zb

@@ -1142,13 +1142,13 @@ def gqa_append(proj, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, 
 
 
 def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, softmax_scale=None, causal=True, window=0,
-              gate=None, out=None, lse=None, workspace=None):
+              sinks=0, gate=None, out=None, lse=None, workspace=None):
     """Attention of every request's new tokens over its pages of a KV cache (which hold the new tokens' keys already:
     :func:`gqa_append`), for prefill, chunked prefill, decode and batches that mix them.
 
     q [N, Hq, hd] bf16 (row stride allowed); the caches, page_table, cache_seqlens and cu_seqlens_q as for
     :func:`gqa_append`. Query head h reads KV head h // (Hq / Hkv). A token at key position p sees keys 0 .. p (with
-    ``window`` > 0 the last ``window`` of them; with ``causal=False`` every key of its request); a page outside
+    ``window`` > 0 the last ``window`` of them, and the first ``sinks``; with ``causal=False`` every key of its request); a page outside
     [0, pages) masks its keys. softmax_scale (> 0) defaults to hd ** -0.5. gate: optional [N, Hq] bf16 logits (row
     stride allowed); head h's output is multiplied by sigmoid(gate[t, h]) before its one rounding. lse: optional
     contiguous [N, Hq] fp32 tensor that receives the natural logarithm of the softmax denominators. A token that sees
@@ -1180,6 +1180,8 @@ def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, s
     if window < 0:
         raise ValueError(f"window must not be negative, got {window}")
     window = min(window, _I32_MAX)  # the C argument's range; no cache holds as many keys
+    if sinks < 0:
+        raise ValueError(f"sinks must not be negative, got {sinks}")
     need = _chunk_workspace_bytes(paged[12], N, Hq, Hkv, hd, paged[9] * paged[6])
     stream = _raw_stream(index)
     if workspace is None:
@@ -1187,8 +1189,9 @@ def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, s
     elif (workspace.dtype is not torch.uint8 or workspace.get_device() != index or not workspace.is_contiguous()
           or workspace.numel() < need):
         raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on {q.device}")
-    _lib.call("zb_gqa_chunk", q.data_ptr(), q_stride, *paged, N, Hq, Hkv, hd,
-              hd ** -0.5 if softmax_scale is None else softmax_scale, causal, window, gate_ptr, gate_stride,
+    name, more = ("zb_gqa_chunk_sinks", (min(sinks, _I32_MAX),)) if sinks else ("zb_gqa_chunk", ())
+    _lib.call(name, q.data_ptr(), q_stride, *paged, N, Hq, Hkv, hd,
+              hd ** -0.5 if softmax_scale is None else softmax_scale, causal, window, *more, gate_ptr, gate_stride,
               out.data_ptr(), out_stride, None if lse is None else lse.data_ptr(),
               None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(), stream)
     return out
@@ -1199,19 +1202,20 @@ def _chunk_workspace_bytes(B, N, Hq, Hkv, hd, max_keys) -> int:
     return _lib.load().zb_gqa_chunk_workspace_bytes(B, N, Hq, Hkv, hd, max_keys)
 
 
-_CHUNK_WS: dict = {}  # (device, stream) -> the workspace of eager calls on that stream (flags another call left do not count)
+_CHUNK_WS: dict = {}  # (device, stream, bytes of flags) -> the workspace of eager calls on that stream (flags another call left do not count)
 _CHUNK_FLAG_BYTES = 4096  # the flags lie at the workspace's start
+_CHUNK_Q4_FLAG_BYTES = 8192
 
 
-def _chunk_workspace(q: torch.Tensor, stream: int, nbytes: int) -> torch.Tensor:
-    """A workspace with its flags zero. Eager calls on a stream share one, in stream order; under capture every call gets
+def _chunk_workspace(q: torch.Tensor, stream: int, nbytes: int, flag_bytes: int = _CHUNK_FLAG_BYTES) -> torch.Tensor:
+    """A workspace with its flags zero (one for each size of them: what one operator has for flags is another's partial results). Eager calls on a stream share one, in stream order; under capture every call gets
     its own (from the graph's pool, its flags zeroed by the graph), as a replay may run beside eager calls."""
-    key = q.get_device(), stream
+    key = q.get_device(), stream, flag_bytes
     capturing = torch.cuda.is_current_stream_capturing()
     ws = None if capturing else _CHUNK_WS.get(key)
     if ws is None or ws.numel() < nbytes:  # a smaller one goes back to the allocator, which reuses it in stream order
         ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
-        ws[:_CHUNK_FLAG_BYTES].zero_()
+        ws[:flag_bytes].zero_()
         if not capturing:
             _CHUNK_WS[key] = ws
     return ws
@@ -1222,3 +1226,188 @@ def gqa_chunk_workspace_bytes(tokens: int, heads: int, page_table, k_cache) -> i
     page_size = k_cache.shape[1] if k_cache.dim() == 4 else 1
     return _chunk_workspace_bytes(page_table.shape[0], tokens, heads, k_cache.shape[-2], k_cache.shape[-1],
                                   page_table.shape[1] * page_size)
+
+
+# ------------------------------------------------------------------------------------------- a paged KV cache in 4 bits
+
+
+_U8 = torch.uint8
+KV_Q4_BLOCK = 16  # tokens of a block
+
+
+def kv_q4_block_bytes(head_dim: int) -> int:
+    """Bytes of 16 tokens' keys and values of one KV head in 4 bits (5 bits an element, the groups' pairs included)."""
+    if head_dim not in (32, 64, 96, 128):
+        raise ValueError(f"a 4-bit cache holds heads of 32, 64, 96 or 128, got {head_dim}")
+    return 20 * head_dim
+
+
+def kv_q4_cache(pages: int, page_size: int, kv_heads: int, head_dim: int, device) -> torch.Tensor:
+    """An empty cache of 4 bits: uint8 [pages, kv_heads, page_size / 16, 20 head_dim] (page_size a multiple of 16), zeros."""
+    if page_size < 1 or page_size % KV_Q4_BLOCK:
+        raise ValueError(f"a 4-bit cache has pages of a multiple of {KV_Q4_BLOCK} tokens, got {page_size}")
+    return torch.zeros(pages, kv_heads, page_size // KV_Q4_BLOCK, kv_q4_block_bytes(head_dim), device=device, dtype=_U8)
+
+
+def _paged_q4(first, kv_cache, page_table, cache_seqlens, cu_seqlens_q, kv_heads):
+    """As :func:`_paged`, for a cache of 4 bits (``first``: the operator's query-side input, or the cache)."""
+    index = first.get_device()
+    if index < 0:
+        raise ValueError("the paged KV operators take CUDA tensors (the B200 kernels have no CPU path)")
+    if (kv_cache.dtype is not _U8 or page_table.dtype is not _I32 or cache_seqlens.dtype is not _I32
+            or cu_seqlens_q.dtype is not _I32 or kv_cache.get_device() != index or page_table.get_device() != index
+            or cache_seqlens.get_device() != index or cu_seqlens_q.get_device() != index):
+        raise ValueError("kv_cache must be uint8, page_table, cache_seqlens and cu_seqlens_q int32 tensors "
+                         f"on {first.device}, got " + ", ".join(f"{t.dtype} on {t.device}" for t in (
+                             kv_cache, page_table, cache_seqlens, cu_seqlens_q)))
+    shape, strides = kv_cache.shape, kv_cache.stride()
+    if len(shape) != 4 or shape[3] % 20 or shape[2] < 1:
+        raise ValueError(f"kv_cache must be [pages, Hkv, page_size / 16, 20 hd], got {tuple(shape)}")
+    pages, Hkv, blocks, block = shape
+    if (strides[3] != 1 and block > 1) or (strides[2] != block and blocks > 1):
+        raise ValueError("the blocks of a page of kv_cache must be contiguous")
+    if kv_heads is not None and Hkv != kv_heads:
+        raise ValueError(f"the cache holds {Hkv} KV heads, expected {kv_heads}")
+    table_shape, table_strides = page_table.shape, page_table.stride()
+    B = cache_seqlens.shape[0] if cache_seqlens.dim() == 1 else -1
+    if len(table_shape) != 2 or table_shape[0] != B or cu_seqlens_q.shape != (B + 1,):
+        raise ValueError(f"page_table, cache_seqlens and cu_seqlens_q must be [B, pages], [B] and [B + 1], got "
+                         f"{tuple(table_shape)}, {tuple(cache_seqlens.shape)}, {tuple(cu_seqlens_q.shape)}")
+    columns = table_shape[1]
+    if (table_strides[1] != 1 and columns > 1) or not cache_seqlens.is_contiguous() or not cu_seqlens_q.is_contiguous():
+        raise ValueError("page_table rows, cache_seqlens and cu_seqlens_q must be contiguous")
+    return (kv_cache.data_ptr(), strides[0] if pages > 1 else 0, strides[1] if Hkv > 1 else 0, pages, blocks * KV_Q4_BLOCK,
+            page_table.data_ptr(), table_strides[0] if B > 1 else columns, columns, cache_seqlens.data_ptr(),
+            cu_seqlens_q.data_ptr(), B), index, Hkv, block // 20
+
+
+def gqa_append_q4(proj, kv_cache, page_table, cache_seqlens, cu_seqlens_q, *, heads, kv_heads, temp=None, eps=1e-6,
+                  rope_theta=10000.0, rotary_dim=None, interleaved=True, positions=None, q_out=None):
+    """:func:`gqa_append` into a KV cache of 4 bits, quantised as it is written.
+
+    kv_cache: uint8 [pages, kv_heads, page_size / 16, 20 hd] (:func:`kv_q4_cache`; page and head strides allowed, multiples
+    of 16); hd 32, 64, 96 or 128. The other arguments as for :func:`gqa_append`; ``heads`` may be 0, for a proj of k | v alone
+    (with ``eps=None, rotary_dim=0`` they are stored as they come), and None is returned then.
+
+    k after its norm and rotation, rounded to bf16, and v are kept in groups of 32 elements: x = m + s c, m the group's
+    smallest element, s = bf16((largest - smallest) / 15) (0 below 2^-100), c = floor((x - m) / s + 1/2) in 4 bits. So an
+    element is kept to s / 2 (and 2^-9 of the group's range for the rounding of s). NaN is kept as 0, magnitudes beyond 2^99
+    as that."""
+    paged, index, Hkv, hd = _paged_q4(proj, kv_cache, page_table, cache_seqlens, cu_seqlens_q, kv_heads)
+    shape = proj.shape
+    if heads < 0:
+        raise ValueError(f"heads must not be negative, got {heads}")
+    if proj.dtype is not _BF16 or len(shape) != 2 or shape[1] < (heads + 2 * Hkv) * hd or (
+            shape[1] > 1 and proj.stride(1) != 1):
+        raise ValueError(f"proj must be a bfloat16 [N, >= {(heads + 2 * Hkv) * hd}] tensor with contiguous rows")
+    N = shape[0]
+    if rotary_dim is None:
+        rotary_dim = hd
+    elif not 0 <= rotary_dim <= hd:
+        raise ValueError(f"rotary_dim must be between 0 and {hd}, got {rotary_dim}")
+    if temp is not None and (temp.dtype is not _BF16 or temp.get_device() != index or temp.numel() != heads
+                             or not temp.is_contiguous()):
+        raise ValueError(f"temp must hold {heads} bfloat16 values on {proj.device}")
+    if positions is not None and (positions.dtype is not _I32 or positions.get_device() != index
+                                  or positions.shape != (N,) or not positions.is_contiguous()):
+        raise ValueError(f"positions must be a contiguous int32 [{N}] tensor on {proj.device}")
+    if heads == 0:
+        if q_out is not None:
+            raise ValueError("q_out without query heads")
+        q_ptr, q_stride = None, 0
+    else:
+        if q_out is None:
+            q_out = proj.new_empty((N, heads, hd))
+            q_stride = heads * hd
+        else:
+            q_stride = _token_rows("q_out", q_out, index, N, heads, hd)
+        q_ptr = q_out.data_ptr()
+    _lib.call("zb_gqa_append_q4", proj.data_ptr(), proj.stride(0) if N > 1 else shape[1],
+              None if temp is None else temp.data_ptr(), None if positions is None else positions.data_ptr(),
+              0.0 if eps is None else eps, eps is not None, rope_theta, rotary_dim,
+              interleaved, q_ptr, q_stride, *paged, N, heads, Hkv, hd, _raw_stream(index))
+    return q_out
+
+
+def kv_read_q4(kv_cache, page_table, cache_seqlens, cu_seqlens, rows, *, k_out=None, v_out=None):
+    """Keys and values read back from a KV cache of 4 bits: the last cu_seqlens[b + 1] - cu_seqlens[b] of every request's
+    cache_seqlens[b], as rows cu_seqlens[b] .. of k, v [rows, Hkv, hd] bf16 (``k_out``, ``v_out`` when given; row strides
+    allowed). With the batch of a :func:`gqa_append_q4` these are the new tokens'; with cu_seqlens = the running sum of
+    cache_seqlens, all of them. ``rows``: of the result (cu_seqlens is on the device; the last of its values as a rule). A row
+    of no request, and one whose page is outside the cache, is zeros. Each element is m + s c rounded once."""
+    paged, index, Hkv, hd = _paged_q4(kv_cache, kv_cache, page_table, cache_seqlens, cu_seqlens, None)
+    if rows < 0:
+        raise ValueError(f"rows must not be negative, got {rows}")
+    strides = []
+    found = []
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t is None:
+            t = torch.empty((rows, Hkv, hd), dtype=_BF16, device=kv_cache.device)
+            strides.append(Hkv * hd)
+        else:
+            strides.append(_token_rows(name, t, index, rows, Hkv, hd))
+        found.append(t)
+    _lib.call("zb_kv_read_q4", *paged, rows, Hkv, hd, found[0].data_ptr(), strides[0], found[1].data_ptr(), strides[1],
+              _raw_stream(index))
+    return found[0], found[1]
+
+
+def gqa_chunk_q4(q, kv_cache, page_table, cache_seqlens, cu_seqlens_q, *, softmax_scale=None, causal=True, window=0, sinks=0,
+                 max_new=None, gate=None, out=None, lse=None, workspace=None):
+    """:func:`gqa_chunk` over a KV cache of 4 bits (:func:`gqa_append_q4`): attention of every request's new tokens over the
+    values that the cache stands for.
+
+    kv_cache as for :func:`gqa_append_q4`; the other arguments as for :func:`gqa_chunk`. ``max_new``: no request brings more new
+    tokens than so many, when the caller knows (1 for a decode batch); a small one saves the launch for requests of many rows.
+    A request that brings more all the same sets :func:`device_status` bit 256 and its rows may be left unwritten.
+    workspace: at least :func:`gqa_chunk_q4_workspace_bytes` bytes, its first 8192 zero before the first call. Returns out
+    [N, Hq, hd] bf16."""
+    paged, index, Hkv, hd = _paged_q4(q, kv_cache, page_table, cache_seqlens, cu_seqlens_q, None)
+    N, Hq = q.shape[0], q.shape[1]
+    q_stride = _token_rows("q", q, index, N, Hq, hd)
+    if out is None:
+        out = torch.empty_like(q) if q_stride == Hq * hd else q.new_empty((N, Hq, hd))
+        out_stride = Hq * hd
+    else:
+        out_stride = _token_rows("out", out, index, N, Hq, hd)
+    gate_ptr, gate_stride = None, 0
+    if gate is not None:
+        if gate.dtype is not _BF16 or gate.get_device() != index or gate.shape != (N, Hq) or (
+                Hq > 1 and gate.stride(1) != 1):
+            raise ValueError(f"gate must be a bfloat16 [{N}, {Hq}] tensor on {q.device} with contiguous rows")
+        gate_ptr, gate_stride = gate.data_ptr(), gate.stride(0) if N > 1 else Hq
+    if lse is not None and (lse.dtype is not torch.float32 or lse.get_device() != index or lse.shape != (N, Hq)
+                            or not lse.is_contiguous()):
+        raise ValueError(f"lse must be a contiguous float32 [{N}, {Hq}] tensor on {q.device}")
+    if window < 0 or sinks < 0:
+        raise ValueError(f"window and sinks must not be negative, got {window} and {sinks}")
+    window, sinks = min(window, _I32_MAX), min(sinks, _I32_MAX)
+    if max_new is None:
+        max_new = 0
+    elif max_new < 1:
+        raise ValueError(f"max_new must be positive, got {max_new}")
+    else:
+        max_new = min(max_new, max(N, 1))
+    need = _chunk_q4_workspace_bytes(paged[10], N, Hq, Hkv, hd, paged[7] * paged[4], max_new)
+    stream = _raw_stream(index)
+    if workspace is None:
+        workspace = _chunk_workspace(q, stream, need, _CHUNK_Q4_FLAG_BYTES) if need else None
+    elif (workspace.dtype is not torch.uint8 or workspace.get_device() != index or not workspace.is_contiguous()
+          or workspace.numel() < need):
+        raise ValueError(f"workspace must be a contiguous uint8 tensor of at least {need} bytes on {q.device}")
+    _lib.call("zb_gqa_chunk_q4", q.data_ptr(), q_stride, *paged, N, Hq, Hkv, hd,
+              hd ** -0.5 if softmax_scale is None else softmax_scale, causal, window, sinks, max_new, gate_ptr, gate_stride,
+              out.data_ptr(), out_stride, None if lse is None else lse.data_ptr(),
+              None if workspace is None else workspace.data_ptr(), 0 if workspace is None else workspace.numel(), stream)
+    return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _chunk_q4_workspace_bytes(B, N, Hq, Hkv, hd, max_keys, max_new) -> int:
+    return _lib.load().zb_gqa_chunk_q4_workspace_bytes(B, N, Hq, Hkv, hd, max_keys, max_new)
+
+
+def gqa_chunk_q4_workspace_bytes(tokens: int, heads: int, page_table, kv_cache, max_new: int | None = None) -> int:
+    """Bytes of workspace :func:`gqa_chunk_q4` needs for ``tokens`` rows of ``heads`` query heads over these tables."""
+    return _chunk_q4_workspace_bytes(page_table.shape[0], tokens, heads, kv_cache.shape[1], kv_cache.shape[3] // 20,
+                                     page_table.shape[1] * kv_cache.shape[2] * KV_Q4_BLOCK, max_new or 0)
