@@ -272,7 +272,63 @@ def test_chunk_matches_oracle(zb, case, mode):
     gate = torch.randn(x[0].shape[0], Hq, generator=gen).bfloat16() if mode == "gate" else None
     kw = {"window": dict(window=37), "sinks": dict(window=37, sinks=5), "full": dict(causal=False),
           "count": dict(window=100, sinks=3)}.get(mode, {})
-    _check_chunk(zb, *x, gate=gate, **kw)
+    for max_new in (None, max(news)):
+        _check_chunk(zb, *x, gate=gate, max_new=max_new, **kw)
+
+
+FEW = [
+    # news, caches, Hq, Hkv, hd, page: rows of up to 8 and of up to 16 heads of tokens
+    ([1, 1, 0, 1, 1], [0, 15, 3, 16, 17], 8, 1, 128, 16),
+    ([2, 1, 2, 0, 2], [0, 300, 127, 5, 1000], 16, 4, 64, 32),
+    ([8, 3, 1], [5, 77, 640], 4, 4, 128, 64),
+    ([4, 1, 3], [130, 0, 2000], 16, 4, 128, 48),
+    ([1, 1], [33, 700], 16, 1, 64, 16),
+    ([16, 7, 2], [0, 9, 250], 2, 2, 128, 16),
+    ([1, 1, 1], [1, 900, 31], 12, 1, 128, 256),
+]
+
+
+@pytest.mark.parametrize("case", FEW)
+@pytest.mark.parametrize("mode", ["causal", "sinks", "full", "gate", "count"])
+def test_chunk_of_few_rows_matches_oracle(zb, case, mode):
+    """Batches whose every request has few rows, known to have them: the kernel of few rows alone. Its scores and weights are
+    nearer to the oracle's than the bound for rounded keys: without the keys' rounding it is the bf16 cache's."""
+    news, caches, Hq, Hkv, hd, page = case
+    gen = torch.Generator().manual_seed(200 + FEW.index(case))
+    x = _chunk_inputs(gen, news, caches, Hq, Hkv, hd, page, spread=0.0 if mode == "count" else 1.0)
+    gate = torch.randn(x[0].shape[0], Hq, generator=gen).bfloat16() if mode == "gate" else None
+    kw = {"sinks": dict(window=37, sinks=5), "full": dict(causal=False), "count": dict(window=100, sinks=3)}.get(mode, {})
+    before = zb._lib.launch_count()
+    out = _check_chunk(zb, *x, gate=gate, max_new=max(news), **kw)
+    assert zb._lib.launch_count() - before == 1
+    _, spread, _, _ = ref = paged.chunk(x[0], *paged_q4.read(x[1]), *x[2:], gate=gate, **kw)
+    _close(out, ref[0], 2.0 ** -7 * (1 + 2.0 ** -4) * spread)
+
+
+def test_chunk_of_more_new_tokens_than_said(zb):
+    """A status bit; the other requests are as they are without it."""
+    gen = torch.Generator().manual_seed(20)
+    x = [t.to(DEV) for t in _chunk_inputs(gen, [1, 3, 1], [500, 300, 90], 16, 4, 128, 16)]
+    expected = zb.ops.gqa_chunk_q4(*x)
+    assert zb.ops.device_status() == 0
+    out = zb.ops.gqa_chunk_q4(*x, max_new=1)
+    assert zb.ops.device_status() == 256
+    assert torch.equal(out[0], expected[0]) and torch.equal(out[4], expected[4])
+
+
+@pytest.mark.parametrize("news", [[1, 2], [40, 3]])
+@pytest.mark.parametrize("scale", [2.0 ** -60, 2.0 ** -20, 2.0 ** -12, 2.0 ** 12, 2.0 ** 20, 2.0 ** 90])
+def test_chunk_values_of_all_magnitudes(zb, news, scale):
+    """Values outside fp16's range, all of them and every third group alone: as precise as any."""
+    gen = torch.Generator().manual_seed(21)
+    for alone in (False, True):
+        table, seqlens, cu, pages = _batch(gen, news, [100, 300], 16)
+        k, v = (torch.randn(pages, 16, 2, 128, generator=gen) for _ in range(2))
+        v *= torch.where(torch.rand(pages, 16, 2, 4, 1, generator=gen).lt(0.3) if alone else torch.ones(1).bool(), scale,
+                         1.0).expand(pages, 16, 2, 4, 32).flatten(-2)
+        cache = paged_q4.store_all(k.bfloat16(), v.bfloat16())
+        q = torch.randn(int(cu[-1]), 8, 128, generator=gen).bfloat16()
+        _check_chunk(zb, q, cache, table, seqlens, cu)
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 1), (2, 0), (128, 128), (500, 4), (3, 300), (130, 17), (1 << 40, 1 << 40)])

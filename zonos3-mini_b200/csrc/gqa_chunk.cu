@@ -61,7 +61,7 @@
 // 256 single tokens, more than 64 dims do (115, 127).
 #include <algorithm>
 
-#include "kv_q4.cuh"
+#include "few_q4.cuh"
 #include "tc.cuh"
 #include "tc_pair.cuh"
 
@@ -1809,10 +1809,17 @@ int launch_chunk(ChunkParams& p, const Launch& l, cudaStream_t stream) {
   return zb::check_launch("gqa_chunk");
 }
 
+// 4 bits: both kernels' flags, then the partial results of whichever runs.
+int64_t q4_workspace_bytes(const Launch& l, int B, int N, int Hkv, int hd, int few, bool only_few) {
+  const int64_t parts = only_few ? 0 : l.acc_bytes + l.ml_bytes;
+  const int64_t few_parts = few > 0 ? zb::q4::few_workspace_bytes(B, N, Hkv, hd, few) - zb::q4::kFewFlagBytes : 0;
+  return parts + few_parts > 0 ? kFlagBytes + zb::q4::kFewFlagBytes + std::max(parts, few_parts) : 0;
+}
+
 // What both caches' entry points do once the cache has been checked; `who` names the entry point.
 template <bool Q4>
 int chunk(ChunkParams& p, const char* who, const uint16_t* q, int64_t q_stride, int Hq, float softmax_scale, int causal,
-          int window, int sinks, int few, const uint16_t* gate, int64_t gate_stride, uint16_t* out, int64_t out_stride,
+          int window, int sinks, int max_new, const uint16_t* gate, int64_t gate_stride, uint16_t* out, int64_t out_stride,
           float* lse, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
   const int B = p.kv.B, N = p.kv.N, Hkv = p.kv.Hkv, hd = p.kv.hd;
   ZB_REQUIRE(Hq > 0 && Hq % Hkv == 0, "%s: %d query heads do not group over %d KV heads", who, Hq, Hkv);
@@ -1834,7 +1841,9 @@ int chunk(ChunkParams& p, const char* who, const uint16_t* q, int64_t q_stride, 
   ZB_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(workspace)) % 16 == 0,
              "%s: q, out and workspace must be 16-byte aligned", who);
   const Launch l = plan(B, N, Hq, Hkv, hd, (int64_t)p.kv.page_size * p.kv.max_pages);
-  const int64_t need = l.flag_bytes + l.acc_bytes + l.ml_bytes;
+  const int few = Q4 ? zb::q4::few_rows(hd, Hq / Hkv, max_new) : 0;
+  const bool only_few = few > 0 && (int64_t)max_new * (Hq / Hkv) <= few;
+  const int64_t need = Q4 ? q4_workspace_bytes(l, B, N, Hkv, hd, few, only_few) : l.flag_bytes + l.acc_bytes + l.ml_bytes;
   ZB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "%s: a workspace of %lld bytes, got %lld", who,
              (long long)need, (long long)workspace_bytes);
   p.q = reinterpret_cast<const __nv_bfloat16*>(q);
@@ -1860,10 +1869,17 @@ int chunk(ChunkParams& p, const char* who, const uint16_t* q, int64_t q_stride, 
   static std::atomic<unsigned> calls{0};
   do p.raised = calls.fetch_add(1, std::memory_order_relaxed) + 1;
   while (p.raised == 0);
-  p.acc = reinterpret_cast<float*>(ws + l.flag_bytes);
-  p.ml = reinterpret_cast<float*>(ws + l.flag_bytes + l.acc_bytes);
+  unsigned char* parts = ws + (Q4 ? kFlagBytes + zb::q4::kFewFlagBytes : l.flag_bytes);
+  p.acc = reinterpret_cast<float*>(parts);
+  p.ml = reinterpret_cast<float*>(parts + l.acc_bytes);
   p.rows_max = l.rows_max;
   p.status = zb::device_status_ptr();
+  if (Q4 && few > 0) {
+    const zb::q4::FewCall call{p.kv, p.q, q_stride, Hq, p.scale_log2, causal, window, p.sinks, few, only_few, p.gate,
+                               gate_stride, p.out, out_stride, lse, ws + kFlagBytes};
+    const int rc = zb::q4::launch_few(call, stream);
+    if (rc != zb::kOk || only_few) return rc;
+  }
   if constexpr (!Q4)
     if (p.sinks == 0) return hd <= 64 ? launch_chunk<64, false, false>(p, l, stream) : launch_chunk<128, false, false>(p, l, stream);
   return hd <= 64 ? launch_chunk<64, Q4, true>(p, l, stream) : launch_chunk<128, Q4, true>(p, l, stream);
@@ -1906,8 +1922,11 @@ ZB_API int zb_gqa_chunk(const uint16_t* q, int64_t q_stride, const uint16_t* k_c
 }
 
 ZB_API int64_t zb_gqa_chunk_q4_workspace_bytes(int B, int N, int Hq, int Hkv, int hd, int64_t max_keys, int max_new) {
-  (void)max_new;
-  return zb_gqa_chunk_workspace_bytes(B, N, Hq, Hkv, hd, max_keys);
+  const Launch l = plan(B, N, Hq, Hkv, hd, max_keys);
+  if (l.ctas == 0) return 0;
+  max_new = max_new > 0 ? std::min(max_new, N) : N;
+  const int few = zb::q4::few_rows(hd, Hq / Hkv, max_new);
+  return q4_workspace_bytes(l, B, N, Hkv, hd, few, few > 0 && (int64_t)max_new * (Hq / Hkv) <= few);
 }
 
 ZB_API int zb_gqa_chunk_q4(const uint16_t* q, int64_t q_stride, const uint8_t* kv_cache, int64_t page_stride,
@@ -1922,6 +1941,7 @@ ZB_API int zb_gqa_chunk_q4(const uint16_t* q, int64_t q_stride, const uint8_t* k
                         cu_seqlens_q, B, N, Hkv, hd};
   if (int rc = zb::q4::check_cache(p.kv, "gqa_chunk_q4")) return rc;
   ZB_REQUIRE(max_new >= 0, "gqa_chunk_q4: max_new %d must not be negative", max_new);
-  return chunk<true>(p, "gqa_chunk_q4", q, q_stride, Hq, softmax_scale, causal, window, sinks, 0, gate, gate_stride, out,
-                     out_stride, lse, workspace, workspace_bytes, stream);
+  return chunk<true>(p, "gqa_chunk_q4", q, q_stride, Hq, softmax_scale, causal, window, sinks,
+                     max_new > 0 ? std::min(max_new, N) : N, gate, gate_stride, out, out_stride, lse, workspace,
+                     workspace_bytes, stream);
 }
