@@ -24,12 +24,12 @@ struct FewCall {
   unsigned char* workspace;  // its first kFewFlagBytes zero, and left zero
 };
 
-constexpr int64_t kFewFlagBytes = 4096;
+constexpr int64_t kFewFlagBytes = 32768;
 
 // Rows of a request that the kernel takes in a call (0: none): 8 or 16 (token, head) pairs. No request has more new tokens than
 // `max_new`.
 int few_rows(int hd, int G, int max_new);
-int64_t few_workspace_bytes(int B, int N, int Hkv, int hd, int rows);
+int64_t few_workspace_bytes(int B, int N, int Hkv, int hd, int rows, int64_t max_keys);
 int launch_few(const FewCall& call, cudaStream_t stream);
 
 }  // namespace q4

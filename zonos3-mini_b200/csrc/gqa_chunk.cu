@@ -1810,9 +1810,9 @@ int launch_chunk(ChunkParams& p, const Launch& l, cudaStream_t stream) {
 }
 
 // 4 bits: both kernels' flags, then the partial results of whichever runs.
-int64_t q4_workspace_bytes(const Launch& l, int B, int N, int Hkv, int hd, int few, bool only_few) {
+int64_t q4_workspace_bytes(const Launch& l, int B, int N, int Hkv, int hd, int64_t max_keys, int few, bool only_few) {
   const int64_t parts = only_few ? 0 : l.acc_bytes + l.ml_bytes;
-  const int64_t few_parts = few > 0 ? zb::q4::few_workspace_bytes(B, N, Hkv, hd, few) - zb::q4::kFewFlagBytes : 0;
+  const int64_t few_parts = few > 0 ? zb::q4::few_workspace_bytes(B, N, Hkv, hd, few, max_keys) - zb::q4::kFewFlagBytes : 0;
   return parts + few_parts > 0 ? kFlagBytes + zb::q4::kFewFlagBytes + std::max(parts, few_parts) : 0;
 }
 
@@ -1843,7 +1843,7 @@ int chunk(ChunkParams& p, const char* who, const uint16_t* q, int64_t q_stride, 
   const Launch l = plan(B, N, Hq, Hkv, hd, (int64_t)p.kv.page_size * p.kv.max_pages);
   const int few = Q4 ? zb::q4::few_rows(hd, Hq / Hkv, max_new) : 0;
   const bool only_few = few > 0 && (int64_t)max_new * (Hq / Hkv) <= few;
-  const int64_t need = Q4 ? q4_workspace_bytes(l, B, N, Hkv, hd, few, only_few) : l.flag_bytes + l.acc_bytes + l.ml_bytes;
+  const int64_t need = Q4 ? q4_workspace_bytes(l, B, N, Hkv, hd, (int64_t)p.kv.page_size * p.kv.max_pages, few, only_few) : l.flag_bytes + l.acc_bytes + l.ml_bytes;
   ZB_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "%s: a workspace of %lld bytes, got %lld", who,
              (long long)need, (long long)workspace_bytes);
   p.q = reinterpret_cast<const __nv_bfloat16*>(q);
@@ -1926,7 +1926,7 @@ ZB_API int64_t zb_gqa_chunk_q4_workspace_bytes(int B, int N, int Hq, int Hkv, in
   if (l.ctas == 0) return 0;
   max_new = max_new > 0 ? std::min(max_new, N) : N;
   const int few = zb::q4::few_rows(hd, Hq / Hkv, max_new);
-  return q4_workspace_bytes(l, B, N, Hkv, hd, few, few > 0 && (int64_t)max_new * (Hq / Hkv) <= few);
+  return q4_workspace_bytes(l, B, N, Hkv, hd, max_keys, few, few > 0 && (int64_t)max_new * (Hq / Hkv) <= few);
 }
 
 ZB_API int zb_gqa_chunk_q4(const uint16_t* q, int64_t q_stride, const uint8_t* kv_cache, int64_t page_stride,

@@ -5,9 +5,9 @@
 // reads every code once, so the work is the codes' way from HBM and their unpacking; the products are few. So they are
 // formed from registers (m16n8k16: 16 keys or dims by 8 rows), where a code goes from the loaded word into a matrix fragment
 // with two instructions for two codes, and nothing is written out in between as a tensor-memory product would need it:
-//   scores^T [16 keys, 8 rows] = sum over groups g of  s_g (c . q)_g + m_g (sum q)_g:  the codes themselves are the operand, as
-//     128 + c in bf16 (exact), the products' sums are fp32, and the pair of a key's group goes onto them in fp32: the scores have
-//     the precision of fp32;
+//   scores^T [16 keys, 8 rows] = sum over groups g of  s_g ((128 + c) . q)_g + (m_g - 128 s_g) (sum q)_g:  the codes themselves are
+//     the operand, as 128 + c in bf16 (exact), s goes onto the products' sums in fp32; the second term is a product of its own, the
+//     pairs as they lie in the cache times the queries' sums, split into three bf16 each: the scores have the precision of fp32;
 //   out^T [16 dims, 8 rows] += V^T p^T with V = m + s c and the weights in fp16, 2^-12 of each: bf16's 2^-9 would be the largest
 //     error here. fp16 has less range, so a block whose pairs are not all within it (magnitudes of 2^-10 to 2^14, or 0) takes bf16.
 // A weight is 2^(score - m + 15) with m a row's reference, its largest score or up to 8 (log2) above it when it is set; it is set
@@ -16,11 +16,16 @@
 // The keys of a 16-key block stand in the scores' rows in the order 0 1 3 2 4 5 7 6 and 8 on: the two rows of a quarter of the lanes then
 // read other banks, and the four rows that a lane's values come from too, as far as 64-byte rows allow.
 //
-// A warp takes one block of 16 keys at a time (at hd 128 one bulk copy of 2560 bytes), its products and its own m, sum and
-// accumulator; 7 such warps are a CTA, two CTAs an SM. An eighth warp looks up pages and starts the copies, 24 blocks ahead and across
-// units. The CTAs take equal runs of all units' blocks (as in gqa_chunk.cu); at the end of a unit's part the warps'
-// accumulators are joined through shared memory in order, and where a unit spans CTAs the last one to arrive joins the parts
-// in the order of their keys: no CTA waits for another, and results do not depend on timing.
+// Every warp works for itself. All units' keys are one long run of items (two blocks of 16 keys, at hd 128 2560 bytes
+// each), of which a warp takes an equal share (the split is as in gqa_chunk.cu, to warps instead of CTAs): it looks up the places of
+// its blocks, has the copies of the next item under way while it computes one, and keeps m, the sum and the accumulator of a unit in
+// its registers, where a lane has 8 consecutive elements of up to four rows' outputs. A unit that spans warps leaves a part of each
+// in the workspace; the warp that finishes the last of up to 16 neighbouring parts joins them in the order of their keys, and so on
+// for the joined ones. No warp waits for another, and results do not depend on timing.
+//
+// Measured ways that were slower (256 tokens of 16 / 4 heads of 128 over 1628 keys): seven warps a CTA that share a unit's items, an eighth
+// that starts the copies, the accumulators joined in shared memory: 105-112 us. Each warp waited for copies and at every
+// unit's end for the slowest; half of the cycles issued nothing.
 #include <algorithm>
 
 #include "few_q4.cuh"
@@ -29,84 +34,99 @@ namespace {
 
 namespace q4 = zb::q4;
 
-// Warps that compute. With the one that copies, 8 a CTA: of nine, an SM's quarter would get five of two CTAs, and a thread 96
-// registers instead of 128.
-constexpr int kWarps = 7;
-constexpr int kThreads = 32 * (kWarps + 1);
-constexpr int kCtas = 2;                        // of an SM
-constexpr int kStages = 24, kDescs = 4;
-constexpr int kUnitCost = 8;                    // of a unit, in blocks
-constexpr int kMinShare = 16;                   // blocks of a CTA, its units' cost among them
+constexpr int kItem = 2;      // blocks of an item
+constexpr int kUnitCost = 1;  // of a unit, in items
+constexpr int kMinShare = 3;  // items of a warp, its units' cost among them
+constexpr int kJoin = 16;     // parts that are joined at once
 constexpr float kAbove = 8.f, kShift = 15.f;
-constexpr float kNone = -3.0e38f;               // m of a row that has seen no key
+constexpr float kNone = -3.0e38f;  // m of a row that has seen no key
 
 struct FewParams {
   q4::FewCall c;
-  int G;
+  int G, workers;
   unsigned page_mul, page_shift;  // division by the page size
-  // [CTA]: the call's tag and, below it, the parts that have arrived of the unit that began there and goes on; 0 again when
-  // all have. What a call whose waits gave up has left has another tag.
+  // [warp][2]: the call's tag and, below it, the parts that have arrived of those that are joined with one of the warp's (the first
+  // of them; [0]: of the unit that began there, [1]: of one that had begun before); 0 again when all have. What a call whose waits
+  // gave up has left has another tag.
   unsigned* counters;
   unsigned tag;
-  float* acc;                     // [CTA][2][rows][hd]
-  float* ml;                      // [CTA][2][2][rows]: m, sum
+  float* acc;  // [warp][2][rows][hd]: parts
+  float* ml;   // [warp][2][2][rows]: m, sum
   unsigned* status;
 };
 
+// What a warp does with one unit.
 struct Desc {
   int token0, pos0, keys;  // first token row, its key position, keys of the request
   int rows, kvh;
-  int item0, items;  // blocks here; -1: the end
-  int index, parts;  // of the unit's parts, this one and their number
-  int first_cta;     // where the unit's first part is
-  int from;          // keys from the sinks' end to here are hidden from every row
-  int all_lo, all_hi;  // keys of [all_lo, all_hi), and those below min(sinks, all_hi), are seen by every row
+  int items;
+  int index, parts, first;  // of the unit's parts this one, their number, and the warp that has the first
+  int from;                 // keys from the sinks' end to here are hidden from every row
+  int all_lo, all_hi;       // keys of [all_lo, all_hi), and those below min(sinks, all_hi), are seen by every row
+};
+// Where a block lies; its first key, and how many of its keys there are.
+struct Place {
+  const unsigned char* at;
+  int key0, exist;
+};
+// A warp's own shared memory, behind its stages and queries.
+struct Own {
+  alignas(16) int2 info[2][kItem];  // of the stages' blocks: first key, and how many there are
+  alignas(16) Place places[32];
+  Desc desc[2];
+  // the unit after those opened: how far its request and the share have got
+  int64_t at;
+  int b, kvh, off;
+  int row0, tokens, keys;
+  // of the unit opened last: blocks whose places are not looked up yet, and what that takes
+  int next, end, n, sink_blocks, gap, of_b, of_kvh, held;
 };
 
 template <int GROUPS, int NT>
 struct Shape {
   static constexpr int kHd = GROUPS * q4::kGroup, kBlockBytes = q4::block_bytes(kHd), kRows = 8 * NT;
-  static constexpr int kJoinRow = kHd + 4;  // floats of a row in the join's buffer: rows 2 t of its writers begin 8 banks apart
-  static constexpr int kOffQ = kStages * kBlockBytes;
-  static constexpr int kOffJoin = kOffQ + kDescs * kRows * kHd * 2;
-  static constexpr int kOffSums = kOffJoin + kWarps * 8 * kJoinRow * 4;  // the groups' sums of the queries, of a unit
-  static constexpr int kOffTail = kOffSums + kWarps * GROUPS * kRows * 4;
+  static constexpr int kStage = kItem * kBlockBytes;
+  static constexpr int kOffQ = 2 * kStage;
+  static constexpr int kOffPairs = kOffQ + kRows * kHd * 2;  // pairs of values, as the lanes need them
+  static constexpr int kOffOwn = kOffPairs + kItem * GROUPS * 64;
+  static constexpr int kPerWarp = (kOffOwn + (int)sizeof(Own) + 127) / 128 * 128;
+  // 16 warps an SM have 128 registers a thread; with 16 rows the accumulators alone are 64, so 12 have 168
+  static constexpr int kWarps = NT == 1 ? 8 : 6, kCtas = 2, kThreads = 32 * kWarps;
   // The queries' fragments stay in registers, or are read again for every block where the accumulators take those.
   static constexpr bool kKeep = NT == 1;
 };
 struct Tail {
-  uint64_t full[kStages], empty[kStages];
-  uint64_t desc_full[kDescs], desc_empty[kDescs], met;
-  int2 info[kStages];  // a block's first key, and how many of its keys there are
-  Desc desc[kDescs];
-  float m[kWarps][16], l[kWarps][16];
-  int sums[2][kWarps + 1];
-  int64_t start_off;
-  int start_b;
+  int sums[2][8];
+  int before[256], cost[256];
   int idle[2];
-  int last;
-  int abort;
 };
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
-  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// D += A B
 template <bool HALF>
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (HALF)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// D = A B of bf16
+__device__ __forceinline__ void mma_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 template <bool HALF>
@@ -119,30 +139,32 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 __device__ __forceinline__ float low_of(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float high_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
 
-// Whether m + s c of a pair and its neighbours keep fp16's 11 bits, or near them: the larger of |m| and 16 s lies in [2^-10, 2^14),
-// or the pair is 0.
+// Whether fp16 keeps m + s c of a pair to near its 11 bits: |m| is below 2^14 and s below 2^10, and either |m| is 2^-10 or more or
+// s 2^-14, or the pair is 0.
 __device__ __forceinline__ bool half_holds(uint32_t pair) {
-  const uint32_t a = pair & 0x7fff7fffu, top = max(a >> 16, (a & 0xffffu) + 0x200u);  // 16 s: the exponent 4 more
-  return a == 0 || top - 0x3a80u < 0x4680u - 0x3a80u;
+  const uint32_t a = pair & 0x7fff7fffu;
+  const uint32_t over = a + (((0x8000u - 0x4680u) << 16) | (0x8000u - 0x4480u));
+  const uint32_t under = a + (((0x8000u - 0x3a80u) << 16) | (0x8000u - 0x3880u));
+  return (over & 0x80008000u) == 0 && ((under & 0x80008000u) != 0 || a == 0);
 }
 
-// A wait that gives up after about a second, and at once after any earlier one of the CTA did.
-__device__ __forceinline__ bool wait(const uint64_t& bar, uint32_t parity, int* abort) {
-  const uint32_t at = zb::smem_addr(&bar);
-  if (zb::mbar_try_wait(at, parity)) return true;
-#pragma unroll 1
-  for (int i = 0; i < 250000; ++i) {
-    if (zb::mbar_try_wait_sleep(at, parity, 20000u)) return true;
-    if (*reinterpret_cast<volatile int*>(abort) != 0) return false;
-  }
-  *reinterpret_cast<volatile int*>(abort) = 1;
-  return false;
+// (x & mask) | bits, in one instruction.
+__device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(mask), "r"(bits));
+  return d;
 }
-__device__ __forceinline__ void arrive(const uint64_t& bar) { zb::mbar_arrive(zb::smem_addr(&bar)); }
-// What was written to shared memory comes before the next copy over it.
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// 16 bytes into shared memory, asynchronously and for this thread's next commit.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_copies() {  // all but the last N groups of this thread
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
-// A request's new rows (none where they are another kernel's) and its blocks of keys. Blocks from sink_blocks on are counted
+// A request's new rows (none where they are another kernel's) and its blocks of keys, which are taken two at a time. Blocks from sink_blocks on are counted
 // without the `gap` blocks between the first keys and the windows.
 struct Request {
   int row0, tokens, keys;
@@ -189,11 +211,13 @@ __device__ __forceinline__ Blocks blocks_of(const FewParams& p, const Request& r
   }
   return x;
 }
+
 __device__ __forceinline__ int cost_of(const FewParams& p, const Request& r) {
-  return r.tokens > 0 ? kUnitCost + blocks_of(p, r).n : 0;
+  return r.tokens > 0 ? kUnitCost + (blocks_of(p, r).n + kItem - 1) / kItem : 0;
 }
 
 // Exclusive prefix of v over the block's threads; `total` the sum. `buffer` alternates from call to call.
+template <int WARPS>
 __device__ __forceinline__ int block_scan(int v, Tail& tl, int buffer, int& total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int in = v;
@@ -207,7 +231,7 @@ __device__ __forceinline__ int block_scan(int v, Tail& tl, int buffer, int& tota
   int before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w <= kWarps; ++w) {
+  for (int w = 0; w < WARPS; ++w) {
     const int s = tl.sums[buffer][w];
     if (w < warp) before += s;
     total += s;
@@ -217,34 +241,24 @@ __device__ __forceinline__ int block_scan(int v, Tail& tl, int buffer, int& tota
 
 __device__ __forceinline__ float sigmoid(__nv_bfloat16 x) { return 1.f / (1.f + ex2(-1.4426950408889634f * __bfloat162float(x))); }
 
-// Part `index` of a unit whose first part is CTA `first`'s: the slots are its own second one, then the first ones of the CTAs after it.
+// Part `index` of a unit whose first part is warp `first`'s: the slots are its own second one, then the first ones of those after it.
 __device__ __forceinline__ int64_t part_slot(int first, int index) { return (int64_t)(first + index) * 2 + (index == 0); }
 
 template <int GROUPS, int NT>
-__global__ void __launch_bounds__(kThreads, kCtas) gqa_few_q4_kernel(const __grid_constant__ FewParams p) {
+__global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>::kCtas)
+    gqa_few_q4_kernel(const __grid_constant__ FewParams p) {
   using L = Shape<GROUPS, NT>;
+  constexpr int hd = L::kHd, kWarps = L::kWarps, kThreads = L::kThreads;
   extern __shared__ __align__(128) unsigned char gbase[];
-  Tail& tl = *reinterpret_cast<Tail*>(gbase + L::kOffTail);
+  Tail& tl = *reinterpret_cast<Tail*>(gbase + kWarps * L::kPerWarp);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
+  unsigned char* own = gbase + warp * L::kPerWarp;
+  Own& my = *reinterpret_cast<Own*>(own + L::kOffOwn);
   const int B = p.c.kv.B, Hkv = p.c.kv.Hkv;
-  const int ctas = gridDim.x, cta = blockIdx.x;
-  constexpr int hd = L::kHd;
-  if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      zb::mbar_init(zb::smem_addr(&tl.full[s]), 1);
-      zb::mbar_init(zb::smem_addr(&tl.empty[s]), 1);
-    }
-    for (int s = 0; s < kDescs; ++s) {
-      zb::mbar_init(zb::smem_addr(&tl.desc_full[s]), 1);
-      zb::mbar_init(zb::smem_addr(&tl.desc_empty[s]), kWarps);
-    }
-    zb::mbar_init(zb::smem_addr(&tl.met), 32 * kWarps);
-    zb::fence_mbar_init();
-    tl.abort = 0;
-  }
+  const int worker = warp * gridDim.x + blockIdx.x;  // few of them are spread over the SMs
   zb::pdl_enter();
 
-  // ---- the plan: the work of all units, and where this CTA's begins
+  // ---- the plan: the work of all units, and where this warp's begins
   bool more = false, out_of_order = false;
   const Request mine = tid < B ? request(p, tid, more) : Request{0, 0, 0};
   const int mine_cost = cost_of(p, mine);
@@ -260,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) gqa_few_q4_kernel(const __gri
     if (b < B) out_of_order |= p.c.kv.cu[b + 1] < p.c.kv.cu[b] || p.c.kv.cu[b] < 0 || p.c.kv.cu[b + 1] > p.c.kv.N;
     const int cost = b0 == 0 ? mine_cost : b < B ? cost_of(p, request(p, b, more)) : 0;
     int total;
-    const int before = block_scan(cost, tl, buffer, total);
+    const int before = block_scan<kWarps>(cost, tl, buffer, total);
     if (b0 == 0) {
       mine_before = before;
       mine_total = total;
@@ -269,12 +283,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) gqa_few_q4_kernel(const __gri
   }
   const bool refused = __syncthreads_or(out_of_order);
   const bool left_out = __syncthreads_or(more) && p.c.only;
-  if (cta == 0 && tid == 0 && p.status && (refused || left_out))
+  if (worker == 0 && lane == 0 && p.status && (refused || left_out))
     atomicOr(p.status, refused ? zb::kStatusAttnChunkBatch : zb::kStatusAttnFewRows);
   work = refused ? 0 : work * Hkv;
-  const int64_t share = max((int64_t)kMinShare, (work + ctas - 1) / ctas);
-  const int64_t begin = share * cta, end = min(work, begin + share);
-  if (begin < end) {
+  const int64_t share = max((int64_t)kMinShare, (work + p.workers - 1) / p.workers);
+  const int64_t begin = share * worker, end = min(work, begin + share);
+  {
     int64_t seen = 0;
 #pragma unroll 1
     for (int b0 = 0; b0 < B; b0 += kThreads) {
@@ -282,182 +296,220 @@ __global__ void __launch_bounds__(kThreads, kCtas) gqa_few_q4_kernel(const __gri
       if (b0 > 0) {
         cost = b0 + tid < B ? cost_of(p, request(p, b0 + tid, more)) : 0;
         buffer ^= 1;
-        before = block_scan(cost, tl, buffer, total);
+        before = block_scan<kWarps>(cost, tl, buffer, total);
       }
-      const int64_t at = (seen + before) * Hkv;
-      if (cost > 0 && begin >= at && begin < at + (int64_t)cost * Hkv) {
-        tl.start_b = b0 + tid;
-        tl.start_off = begin - at;
+      if (work > 0) {
+        tl.before[tid] = before;
+        tl.cost[tid] = cost;
+      }
+      __syncthreads();
+      if (begin < end && begin >= seen * Hkv && begin < (seen + total) * Hkv) {
+#pragma unroll 1
+        for (int i = lane; i < kThreads; i += 32) {
+          const int64_t at = (seen + tl.before[i]) * Hkv;
+          if (tl.cost[i] > 0 && begin >= at && begin < at + (int64_t)tl.cost[i] * Hkv) {
+            bool ignored = false;
+            const Request r = request(p, b0 + i, ignored);
+            my.at = begin;
+            my.b = b0 + i;
+            my.kvh = (int)((begin - at) / tl.cost[i]);
+            my.off = (int)((begin - at) % tl.cost[i]);
+            my.row0 = r.row0;
+            my.tokens = r.tokens;
+            my.keys = r.keys;
+          }
+        }
       }
       seen += total;
-      if (begin < seen * Hkv) break;
+      __syncthreads();
     }
   }
-  __syncthreads();
-  int* abort = &tl.abort;
-
-  if (begin >= end) {
-    // nothing for this CTA
-  } else if (warp == kWarps) {
-    // =============================================================================================== copies
-    int b = tl.start_b, item = 0, n = 0;
-    bool ignored = false, going = true;
-    Request req = request(p, b, ignored);
-    int cost = max(cost_of(p, req), 1);
-    int kvh = (int)(tl.start_off / cost), off = (int)(tl.start_off % cost);
-    int64_t at = begin;
-    int window0 = -1;
-    Request window{};
-    auto room = [&](const uint64_t& bar, uint32_t parity) {
-      going = __all_sync(0xffffffffu, wait(bar, parity, abort));
-      return going;
-    };
-    while (going && at < end) {
-      const Blocks x = blocks_of(p, req);
-      const int to_cost = (int)min((int64_t)cost, off + (end - at));
-      const int from = max(off - kUnitCost, 0), to = max(to_cost - kUnitCost, 0);
-      if (to > from || (x.n == 0 && off == 0)) {
-        const int slot = n % kDescs;
-        if (n >= kDescs && !room(tl.desc_empty[slot], (n / kDescs - 1) & 1)) break;
-        const int64_t first = at - off + kUnitCost;  // of the unit's blocks
-        if (lane == 0) {
-          Desc d;
-          d.token0 = req.row0;
-          d.pos0 = req.keys - req.tokens;
-          d.keys = req.keys;
-          d.rows = req.tokens * p.G;
-          d.kvh = kvh;
-          d.item0 = item;
-          d.items = to - from;
-          d.first_cta = x.n > 0 ? (int)(first / share) : cta;
-          d.index = cta - d.first_cta;
-          d.parts = x.n > 0 ? (int)((first + x.n - 1) / share) - d.first_cta + 1 : 1;
-          d.from = x.lo_first;
-          d.all_lo = x.lo_last;
-          d.all_hi = x.hi_first;
-          tl.desc[slot] = d;
-          zb::mbar_arrive_expect_tx(zb::smem_addr(&tl.desc_full[slot]), (uint32_t)(req.tokens * p.G * hd * 2));
-        }
-        __syncwarp();
-        if (lane < req.tokens)  // the queries: a token's heads of the group lie side by side
-          zb::bulk_g2s(zb::smem_addr(gbase + L::kOffQ + slot * (L::kRows * hd * 2) + lane * p.G * hd * 2),
-                       p.c.q + (int64_t)(req.row0 + lane) * p.c.q_stride + (int64_t)kvh * p.G * hd, (uint32_t)(p.G * hd * 2),
-                       zb::smem_addr(&tl.desc_full[slot]));
-        ++n;
-        const int held = held_keys(p, req.keys);
-        const int32_t* table = p.c.kv.table + (int64_t)b * p.c.kv.table_stride;
-#pragma unroll 1
-        for (int j0 = from; j0 < to && going; j0 += 32) {  // a lane's block
-          const int j = j0 + lane, block = j < x.sink_blocks ? j : j + x.gap, key0 = block * q4::kBlock;
-          const int column = (int)(((uint64_t)(unsigned)key0 * p.page_mul) >> p.page_shift);
-          const int page = j < to && key0 < held ? table[column] : -1;
-          const bool there = page >= 0 && page < p.c.kv.num_pages;
-          const unsigned char* src = reinterpret_cast<const unsigned char*>(p.c.kv.k) + (there ? (int64_t)page * p.c.kv.page_stride : 0) +
-                                     (int64_t)kvh * p.c.kv.head_stride +
-                                     (int64_t)(key0 - column * p.c.kv.page_size) / q4::kBlock * L::kBlockBytes;
-          const int exist = there ? min(q4::kBlock, held - key0) : 0;
-#pragma unroll 1
-          for (int g = 0; g < 32 && j0 + g < to; g += 8) {  // 8 at a time: waiting for room for all would drain the ring
-            const bool own = lane / 8 == g / 8 && j < to;
-            const int i = item + j - from, stage = i % kStages;
-            bool ready = true;
-            if (own && i >= kStages) ready = wait(tl.empty[stage], (i / kStages - 1) & 1, abort);
-            going = __all_sync(0xffffffffu, ready);
-            if (!going) break;
-            if (own) {
-              tl.info[stage] = make_int2(key0, exist);
-              if (there) {
-                zb::mbar_arrive_expect_tx(zb::smem_addr(&tl.full[stage]), L::kBlockBytes);
-                zb::bulk_g2s(zb::smem_addr(gbase + stage * L::kBlockBytes), src, L::kBlockBytes, zb::smem_addr(&tl.full[stage]));
-              } else {
-                arrive(tl.full[stage]);
-              }
-            }
-            __syncwarp();
-          }
-        }
-        item += to - from;
-      }
-      // ---- the next unit: KV head, then request
-      at += to_cost - off;
-      off = 0;
-      if (at >= end) break;
-      if (++kvh == Hkv) {
-        kvh = 0;
-        do {
-          ++b;
-          if (b / 32 != window0) {
-            window0 = b / 32;
-            const int i = window0 * 32 + lane;
-            window = i < B ? request(p, i, ignored) : Request{0, 0, 0};
-          }
-          req.row0 = __shfl_sync(0xffffffffu, window.row0, b % 32);
-          req.tokens = __shfl_sync(0xffffffffu, window.tokens, b % 32);
-          req.keys = __shfl_sync(0xffffffffu, window.keys, b % 32);
-        } while (b < B - 1 && req.tokens == 0);
-        cost = cost_of(p, req);
-        if (cost == 0) break;  // not while the lengths stay as they were when the work was added up
-      }
-    }
-    const int slot = n % kDescs;
-    if (going && (n < kDescs || room(tl.desc_empty[slot], (n / kDescs - 1) & 1))) {
-      if (lane == 0) {
-        tl.desc[slot].items = -1;
-        arrive(tl.desc_full[slot]);
-      }
-      ++n;
-    }
-    __syncwarp();
-    // nothing is in flight when the CTA's shared memory goes to another, also where a wait gave up
-    if (lane < min(kStages, item))
-      zb::mbar_wait_bounded(zb::smem_addr(&tl.full[lane]), (item - 1 - lane) / kStages & 1, p.status, zb::kStatusAttnChunkTimeout);
-    if (lane < min(kDescs, n))
-      zb::mbar_wait_bounded(zb::smem_addr(&tl.desc_full[lane]), (n - 1 - lane) / kDescs & 1, p.status, zb::kStatusAttnChunkTimeout);
-  } else {
-    // =============================================================================================== blocks
+  if (begin < end) {
     const int gid = lane / 4, t4 = lane % 4;
     const int key_row = gid ^ ((gid >> 1) & 1);             // the key of scores' row gid; 8 more for row gid + 8
     const int va = 2 * t4 + (t4 & 1), vb = va ^ 1;  // the keys of rows 2 t4 and 2 t4 + 1
-    int meetings = 0;
-    auto meet = [&]() {  // the warps that compute; a wait with a limit, as all are
-      arrive(tl.met);
-      wait(tl.met, meetings & 1, abort);
-      ++meetings;
+    int opened = 0, done = 0;      // units
+    int fetched = 0, computed = 0;  // items
+    int place = 0, places = 0;      // the next of the places looked up, and their number
+    bool loaded = false, more_units = true;  // the queries of unit `done` have been taken from shared memory
+
+    // Opens the next unit of which items lie in the share: its description, and its queries' copy.
+    auto open_unit = [&]() {
+      __syncwarp();
+      int64_t at = my.at;
+      int b = my.b, kvh = my.kvh, off = my.off;
+      Request req{my.row0, my.tokens, my.keys};
+      bool found = false;
+      __syncwarp();
+#pragma unroll 1
+      while (!found && at < end) {
+        const Blocks x = blocks_of(p, req);
+        const int unit_items = (x.n + kItem - 1) / kItem, cost = kUnitCost + unit_items;
+        const int to_cost = (int)min((int64_t)cost, off + (end - at));
+        const int from = max(off - kUnitCost, 0), to = max(to_cost - kUnitCost, 0);
+        if (to > from || (x.n == 0 && off == 0)) {
+          found = true;
+          const int64_t first = at - off + kUnitCost;  // of the unit's items
+          if (lane == 0) {
+            Desc d;
+            d.token0 = req.row0;
+            d.pos0 = req.keys - req.tokens;
+            d.keys = req.keys;
+            d.rows = req.tokens * p.G;
+            d.kvh = kvh;
+            d.items = to - from;
+            d.first = x.n > 0 ? (int)(first / share) : worker;
+            d.index = worker - d.first;
+            d.parts = x.n > 0 ? (int)((first + unit_items - 1) / share) - d.first + 1 : 1;
+            d.from = x.lo_first;
+            d.all_lo = x.lo_last;
+            d.all_hi = x.hi_first;
+            my.desc[opened % 2] = d;
+            my.next = from * kItem;
+            my.end = to * kItem;
+            my.n = x.n;
+            my.sink_blocks = x.sink_blocks;
+            my.gap = x.gap;
+            my.of_b = b;
+            my.of_kvh = kvh;
+            my.held = held_keys(p, req.keys);
+          }
+          // the queries, with the copies of the unit's first item: a token's heads of the group lie side by side
+          const int pieces = p.G * (hd / 8);
+#pragma unroll 1
+          for (int i = lane; i < (to > from ? req.tokens * pieces : 0); i += 32)
+            copy16(zb::smem_addr(own + L::kOffQ) + i * 16,
+                   p.c.q + (int64_t)(req.row0 + i / pieces) * p.c.q_stride + (int64_t)kvh * p.G * hd + i % pieces * 8);
+        }
+        // the next unit: KV head, then request
+        at += to_cost - off;
+        off = 0;
+        if (at < end && ++kvh == Hkv) {
+          kvh = 0;
+          req.tokens = 0;
+#pragma unroll 1
+          for (++b; b < B; b += 32) {  // 32 requests at a time
+            bool ignored = false;
+            const Request r = b + lane < B ? request(p, b + lane, ignored) : Request{0, 0, 0};
+            const unsigned have = __ballot_sync(0xffffffffu, r.tokens > 0);
+            if (have == 0) continue;
+            const int k = __ffs(have) - 1;
+            b += k;
+            req.row0 = __shfl_sync(0xffffffffu, r.row0, k);
+            req.tokens = __shfl_sync(0xffffffffu, r.tokens, k);
+            req.keys = __shfl_sync(0xffffffffu, r.keys, k);
+            break;
+          }
+          if (req.tokens == 0) at = end;  // not while the lengths stay as they were when the work was added up
+        }
+      }
+      if (lane == 0) {
+        my.at = at;
+        my.b = b;
+        my.kvh = kvh;
+        my.off = off;
+        my.row0 = req.row0;
+        my.tokens = req.tokens;
+        my.keys = req.keys;
+      }
+      __syncwarp();
+      place = places = 0;
+      opened += found;
+      more_units = found;
     };
-    for (int n = 0;; ++n) {
-      const int slot = n % kDescs;
-      if (!wait(tl.desc_full[slot], (n / kDescs) & 1, abort)) break;
-      const Desc d = tl.desc[slot];
-      if (d.items < 0) break;
-      // ---- queries: B fragments, and their groups' sums
-      const unsigned char* q_rows = gbase + L::kOffQ + slot * (L::kRows * hd * 2);
-      float* sums = reinterpret_cast<float*>(gbase + L::kOffSums) + warp * GROUPS * L::kRows;
+    // Starts the copies of the next item. Those of a unit after the one that is computed wait until its queries are in registers,
+    // which makes room for theirs.
+    auto fetch = [&]() {
+#pragma unroll 1
+      while (place == places) {
+        const int next = my.next, stop = my.end;
+        if (opened > done && next < stop) {  // a lane's block
+          const int j = next + lane, block = j < my.sink_blocks ? j : j + my.gap, key0 = block * q4::kBlock;
+          const int column = (int)(((uint64_t)(unsigned)key0 * p.page_mul) >> p.page_shift);
+          const int page = j < min(stop, my.n) && key0 < my.held ? p.c.kv.table[(int64_t)my.of_b * p.c.kv.table_stride + column] : -1;
+          const bool there = page >= 0 && page < p.c.kv.num_pages;
+          Place found;
+          found.at = reinterpret_cast<const unsigned char*>(p.c.kv.k) + (there ? (int64_t)page * p.c.kv.page_stride : 0) +
+                     (int64_t)my.of_kvh * p.c.kv.head_stride + (int64_t)(key0 - column * p.c.kv.page_size) / q4::kBlock * L::kBlockBytes;
+          found.key0 = key0;
+          found.exist = there ? min(q4::kBlock, my.held - key0) : 0;
+          __syncwarp();
+          my.places[lane] = found;
+          place = 0;
+          places = min(32, stop - next);
+          if (lane == 0) my.next = next + places;
+          __syncwarp();
+        } else {
+          if (!more_units || opened - done > 1 || (opened - done == 1 && !(L::kKeep && loaded))) return;
+          open_unit();
+        }
+      }
+      const int stage = fetched % 2;
+#pragma unroll
+      for (int x = 0; x < kItem; ++x) {
+        const Place found = my.places[place + x];
+        const uint32_t to = zb::smem_addr(own + stage * L::kStage + x * L::kBlockBytes) + lane * 16;
+        if (lane == 0) my.info[stage][x] = make_int2(found.key0, found.exist);
+        if (found.exist > 0)
+#pragma unroll
+          for (int i = 0; i < L::kBlockBytes; i += 512)
+            if (i + 512 <= L::kBlockBytes || lane * 16 < L::kBlockBytes - i) copy16(to + i, found.at + i + lane * 16);
+      }
+      commit_copies();
+      place += kItem;
+      ++fetched;
+    };
+    // Masks that the compiler does not see through stay in registers, and a code takes one instruction with the constant it is
+    // joined to; with both as immediates it takes two.
+    uint32_t low4 = 0x000f000fu, high4 = 0x00f000f0u;
+    asm("" : "+r"(low4), "+r"(high4));
+
+    fetch();
+    fetch();
+#pragma unroll 1
+    while (true) {
+      if (opened == done) open_unit();
+      if (opened == done) break;
+      const Desc d = my.desc[done % 2];
+      // The copies of the item to be computed, and with them those of its unit's queries.
+      auto arrived = [&]() {
+        if (fetched - computed > 1) wait_copies<1>();
+        else wait_copies<0>();
+        __syncwarp();
+      };
+      if (fetched == computed) fetch();
+      arrived();
+      // ---- queries: B fragments; and of what a group's pair multiplies, -128 and 1 times the sum of its elements of the query, as
+      // three bf16 each: (c . q) comes with 128 instead of 0 for every code's zero
+      const unsigned char* q_rows = own + L::kOffQ;
       auto fragment = [&](int nt, int g) {
         return 8 * nt + gid < d.rows ? *reinterpret_cast<const uint4*>(q_rows + (8 * nt + gid) * hd * 2 + (32 * g + 8 * t4) * 2)
                                      : make_uint4(0, 0, 0, 0);
       };
       uint4 q[L::kKeep ? GROUPS : 1];
-      float2 qs[L::kKeep ? GROUPS : 1];
+      uint32_t qs[NT][3];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float of_group = 0.f;  // t4
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
           const uint4 w = fragment(nt, g);
           float sum = low_of(w.x) + high_of(w.x) + (low_of(w.y) + high_of(w.y)) + (low_of(w.z) + high_of(w.z)) + (low_of(w.w) + high_of(w.w));
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          if (L::kKeep) {
-            q[g] = w;
-            qs[g].x = __shfl_sync(0xffffffffu, sum, 8 * t4);
-            qs[g].y = __shfl_sync(0xffffffffu, sum, 8 * t4 + 4);
-          } else if (t4 == 0) {
-            sums[g * L::kRows + 8 * nt + gid] = sum;
-          }
+          if (g == t4) of_group = sum;
+          if (L::kKeep) q[g] = w;
         }
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          const float kept = zb::bf16_round(of_group);
+          qs[nt][i] = pack<false>(-128.f * kept, kept);
+          of_group -= kept;
+        }
+      }
       __syncwarp();
-      if (L::kKeep && lane == 0) arrive(tl.desc_empty[slot]);
-      // hidden keys: of the lane's rows 2 t4, 2 t4 + 1 (and 8 on)
-      float m[NT][2], l[NT][2], o[NT][2 * GROUPS][4];
+      loaded = true;
+      float m[NT][2], l[NT][2], o[NT][2 * GROUPS][4];  // of rows 2 t4 and 2 t4 + 1 (and 8 on)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         m[nt][0] = m[nt][1] = kNone;
@@ -465,346 +517,395 @@ __global__ void __launch_bounds__(kThreads, kCtas) gqa_few_q4_kernel(const __gri
 #pragma unroll
         for (int i = 0; i < 2 * GROUPS; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
       }
-      const int item_end = d.item0 + d.items, turn = d.item0 % kWarps;
-      auto skips = [&](int w) { return w >= turn ? w - turn : w - turn + kWarps; };  // blocks before warp w's first one
+      uint32_t* pairs_out = reinterpret_cast<uint32_t*>(own + L::kOffPairs);
 #pragma unroll 1
-      for (int item = d.item0 + skips(warp); item < item_end; item += kWarps) {
-        const int stage = item % kStages;
-        wait(tl.full[stage], (item / kStages) & 1, abort);
-        const int2 info = tl.info[stage];
-        unsigned char* block = gbase + stage * L::kBlockBytes;
-        uint32_t* k_pairs = reinterpret_cast<uint32_t*>(block + 16 * hd);
-        uint32_t* v_pairs = reinterpret_cast<uint32_t*>(block + 18 * hd);
-        const int key0 = info.x;
-        if (info.y < q4::kBlock || (key0 < d.from && key0 + q4::kBlock > p.c.sinks)) {
-          // rows that are no keys hold anything, and what no row sees shall not choose the values' type either
-          for (int i = lane; i < 16 * GROUPS; i += 32) {
-            const int j = i / GROUPS, key = key0 + j;
-            if (j >= info.y || (key >= p.c.sinks && key < d.from)) k_pairs[i] = v_pairs[i] = 0;
+      for (int item = 0; item < d.items; ++item) {
+        while (fetched - computed < 2) {
+          const int before = fetched;
+          fetch();
+          if (fetched == before) break;
+        }
+        const int stage = computed % 2;
+        arrived();
+        const int4 info = *reinterpret_cast<const int4*>(my.info[stage]);
+        unsigned char* blocks = own + stage * L::kStage;
+        auto k_pairs = [&](int x) { return reinterpret_cast<uint32_t*>(blocks + x * L::kBlockBytes + 16 * hd); };
+        auto v_pairs = [&](int x) { return reinterpret_cast<uint32_t*>(blocks + x * L::kBlockBytes + 18 * hd); };
+        // keys that some rows do not see
+        bool partly = false;
+#pragma unroll
+        for (int x = 0; x < kItem; ++x) {
+          const int key0 = x ? info.z : info.x, exist = x ? info.w : info.y;
+          partly |= exist < q4::kBlock || key0 + q4::kBlock > d.all_hi || (key0 < d.all_lo && key0 + q4::kBlock > p.c.sinks);
+        }
+        if (partly) {  // rows that are no keys hold anything, and what no row sees shall not choose the values' type either
+          for (int i = lane; i < kItem * 16 * GROUPS; i += 32) {
+            const int x = i / (16 * GROUPS), j = i / GROUPS % 16, key = (x ? info.z : info.x) + j;
+            if (j >= (x ? info.w : info.y) || (key >= p.c.sinks && key < d.from))
+              k_pairs(x)[i % (16 * GROUPS)] = v_pairs(x)[i % (16 * GROUPS)] = 0;
           }
-          fence_proxy_async();
           __syncwarp();
         }
+        // Pairs: none of the keys' may count as one that is not finite; the values' go to where the lanes that need them read
+        // them, two keys' s and m beside each other.
         bool half = true;
         {
+          const int g = lane / 8 % GROUPS, t = lane % 4, h = lane / 4 % 2;  // a group, and the keys of scores' rows 2 t + 8 h, + 1
+          const int row = 2 * t + (t & 1) + 8 * h;
           bool k_none = false;
+          uint32_t a[kItem], b[kItem];
 #pragma unroll
-          for (int i = 0; i < GROUPS / 2; ++i) {
-            k_none |= q4::pair_is_none(k_pairs[lane + 32 * i]);
-            half &= half_holds(v_pairs[lane + 32 * i]);
+          for (int x = 0; x < kItem; ++x) {
+            const uint2 k2 = GROUPS == 4 ? reinterpret_cast<const uint2*>(k_pairs(x))[lane] : make_uint2(k_pairs(x)[lane], 0);
+            k_none |= q4::pair_is_none(k2.x) || q4::pair_is_none(k2.y);
+            a[x] = v_pairs(x)[row * GROUPS + g];
+            b[x] = v_pairs(x)[(row ^ 1) * GROUPS + g];
+            half &= half_holds(a[x]) && half_holds(b[x]);
+          }
+          half = __all_sync(0xffffffffu, half);
+#pragma unroll
+          for (int x = 0; x < kItem; ++x) {
+            uint2 w;
+            if (half) {
+              w = make_uint2(pack<true>(low_of(a[x]), low_of(b[x])), pack<true>(high_of(a[x]), high_of(b[x])));
+            } else {
+              if (q4::pair_is_none(a[x])) a[x] = 0;
+              if (q4::pair_is_none(b[x])) b[x] = 0;
+              w = make_uint2(__byte_perm(a[x], b[x], 0x5410), __byte_perm(a[x], b[x], 0x7632));
+            }
+            if (lane < 8 * GROUPS) *reinterpret_cast<uint2*>(pairs_out + ((x * GROUPS + g) * 4 + t) * 4 + 2 * h) = w;
           }
           if (__any_sync(0xffffffffu, k_none)) {
 #pragma unroll
-            for (int i = 0; i < GROUPS / 2; ++i)
-              if (q4::pair_is_none(k_pairs[lane + 32 * i])) k_pairs[lane + 32 * i] = 0;
-            fence_proxy_async();
-            __syncwarp();
-          }
-          half = __all_sync(0xffffffffu, half);
+            for (int x = 0; x < kItem; ++x)
+              for (int i = lane; i < 16 * GROUPS; i += 32)
+                if (q4::pair_is_none(k_pairs(x)[i])) k_pairs(x)[i] = 0;
+            }
+          __syncwarp();
         }
-        // ---- scores
-        float s[NT][4];
+        auto body = [&](auto type) {
+          constexpr bool HALF = decltype(type)::value;
+          // ---- scores
+          float s[kItem][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-        {
-          uint32_t w[2][GROUPS], pr[2][GROUPS];
+          for (int x = 0; x < kItem; ++x) {
+            uint32_t w[2][GROUPS], pr[2][GROUPS], mine[2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const unsigned char* from = block + (key_row + 8 * h) * (hd / 2) + t4 * GROUPS * 4;
-            const uint32_t* pairs = k_pairs + (key_row + 8 * h) * GROUPS;
-            if constexpr (GROUPS == 4) {
-              *reinterpret_cast<uint4*>(w[h]) = *reinterpret_cast<const uint4*>(from);
-              *reinterpret_cast<uint4*>(pr[h]) = *reinterpret_cast<const uint4*>(pairs);
-            } else {
-              *reinterpret_cast<uint2*>(w[h]) = *reinterpret_cast<const uint2*>(from);
-              *reinterpret_cast<uint2*>(pr[h]) = *reinterpret_cast<const uint2*>(pairs);
+            for (int h = 0; h < 2; ++h) {
+              const unsigned char* from = blocks + x * L::kBlockBytes + (key_row + 8 * h) * (hd / 2) + t4 * GROUPS * 4;
+              const uint32_t* pairs = k_pairs(x) + (key_row + 8 * h) * GROUPS;
+              if constexpr (GROUPS == 4) {
+                *reinterpret_cast<uint4*>(w[h]) = *reinterpret_cast<const uint4*>(from);
+                *reinterpret_cast<uint4*>(pr[h]) = *reinterpret_cast<const uint4*>(pairs);
+              } else {
+                *reinterpret_cast<uint2*>(w[h]) = *reinterpret_cast<const uint2*>(from);
+                *reinterpret_cast<uint2*>(pr[h]) = *reinterpret_cast<const uint2*>(pairs);
+              }
+              mine[h] = pairs[t4 % GROUPS];
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {  // the pairs with the queries' sums
+              mma_new(s[x][nt], mine[0], mine[1], mine[0], mine[1], qs[nt][0], qs[nt][1]);
+              mma<false>(s[x][nt], mine[0], mine[1], 0u, 0u, qs[nt][2], 0u);
+            }
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+              uint32_t a[2][4];  // 128 + c
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) a[h][i] = masked_or(w[h][g] >> (4 * i), low4, 0x43004300u);
+              const float s0 = low_of(pr[0][g]), s1 = low_of(pr[1][g]);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                float dot[4];
+                const uint4 f = L::kKeep ? q[g] : fragment(nt, g);
+                mma_new(dot, a[0][0], a[1][0], a[0][1], a[1][1], f.x, f.y);
+                mma<false>(dot, a[0][2], a[1][2], a[0][3], a[1][3], f.z, f.w);
+                s[x][nt][0] = fmaf(s0, dot[0], s[x][nt][0]);
+                s[x][nt][1] = fmaf(s0, dot[1], s[x][nt][1]);
+                s[x][nt][2] = fmaf(s1, dot[2], s[x][nt][2]);
+                s[x][nt][3] = fmaf(s1, dot[3], s[x][nt][3]);
+              }
             }
           }
+          if (partly) {
+            const int held = held_keys(p, d.keys);
 #pragma unroll
-          for (int g = 0; g < GROUPS; ++g) {
-            const uint32_t a[2][4] = {{q4::codes_128<0>(w[0][g]), q4::codes_128<1>(w[0][g]), q4::codes_128<2>(w[0][g]), q4::codes_128<3>(w[0][g])},
-                                      {q4::codes_128<0>(w[1][g]), q4::codes_128<1>(w[1][g]), q4::codes_128<2>(w[1][g]), q4::codes_128<3>(w[1][g])}};
-            const float s0 = low_of(pr[0][g]), s1 = low_of(pr[1][g]);
-            const float m0 = fmaf(-128.f, s0, high_of(pr[0][g])), m1 = fmaf(-128.f, s1, high_of(pr[1][g]));
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int row = 8 * nt + 2 * t4 + e, pos = d.pos0 + min(row, d.rows - 1) / p.G;
+                const int lo = first_seen(p, pos), hi = behind_seen(p, held, pos);
+#pragma unroll
+                for (int x = 0; x < kItem; ++x)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const int j = key_row + 8 * h, key = (x ? info.z : info.x) + j;
+                    if (j >= (x ? info.w : info.y) || key >= hi || (key < lo && key >= p.c.sinks)) s[x][nt][2 * h + e] = -INFINITY;
+                  }
+              }
+          }
+          // ---- weights
+          float e[kItem][NT][4];
+          bool above = false;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int x = 0; x < kItem; ++x) {
+                e[x][nt][i] = fmaf(s[x][nt][i], p.c.scale_log2, kShift - m[nt][i % 2]);
+                above |= e[x][nt][i] > kShift;
+              }
+          if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                float top = fmaxf(fmaxf(s[0][nt][r], s[0][nt][2 + r]), fmaxf(s[1][nt][r], s[1][nt][2 + r])) * p.c.scale_log2;
+#pragma unroll
+                for (int w = 4; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                if (top > m[nt][r]) {  // of a row: all its lanes
+                  const float corr = ex2(m[nt][r] - (top + kAbove));
+                  m[nt][r] = top + kAbove;
+                  l[nt][r] *= corr;
+#pragma unroll
+                  for (int i = 0; i < 2 * GROUPS; ++i) {
+                    o[nt][i][r] *= corr;
+                    o[nt][i][2 + r] *= corr;
+                  }
+                }
+#pragma unroll
+                for (int x = 0; x < kItem; ++x)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) e[x][nt][2 * h + r] = fmaf(s[x][nt][2 * h + r], p.c.scale_log2, kShift - m[nt][r]);
+              }
+          }
+          uint32_t pb[kItem][NT][2];
+#pragma unroll
+          for (int x = 0; x < kItem; ++x)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              float dot[4] = {0.f, 0.f, 0.f, 0.f};
-              const uint4 f = L::kKeep ? q[g] : fragment(nt, g);
-              const float2 sum = L::kKeep ? qs[g] : *reinterpret_cast<const float2*>(sums + g * L::kRows + 8 * nt + 2 * t4);
-              mma<false>(dot, a[0][0], a[1][0], a[0][1], a[1][1], f.x, f.y);
-              mma<false>(dot, a[0][2], a[1][2], a[0][3], a[1][3], f.z, f.w);
-              s[nt][0] = fmaf(s0, dot[0], fmaf(m0, sum.x, s[nt][0]));
-              s[nt][1] = fmaf(s0, dot[1], fmaf(m0, sum.y, s[nt][1]));
-              s[nt][2] = fmaf(s1, dot[2], fmaf(m1, sum.x, s[nt][2]));
-              s[nt][3] = fmaf(s1, dot[3], fmaf(m1, sum.y, s[nt][3]));
+#pragma unroll
+              for (int i = 0; i < 4; ++i) e[x][nt][i] = ex2(e[x][nt][i]);
+              l[nt][0] += e[x][nt][0] + e[x][nt][2];
+              l[nt][1] += e[x][nt][1] + e[x][nt][3];
+              pb[x][nt][0] = transpose8(pack<HALF>(e[x][nt][0], e[x][nt][1]));
+              pb[x][nt][1] = transpose8(pack<HALF>(e[x][nt][2], e[x][nt][3]));
             }
-          }
-        }
-        if (info.y < q4::kBlock || key0 + q4::kBlock > d.all_hi || (key0 < d.all_lo && key0 + q4::kBlock > p.c.sinks)) {
-          const int held = held_keys(p, d.keys);
+          // ---- values
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int x = 0; x < kItem; ++x) {
+            constexpr int W = GROUPS / 2;  // words of a key here
+            uint32_t w[4][W];
+            uint4 sm[W];  // s and m of the keys of rows 2 t4, + 1, and of those 8 on
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int row = 8 * nt + 2 * t4 + e, pos = d.pos0 + min(row, d.rows - 1) / p.G;
-              const int lo = first_seen(p, pos), hi = behind_seen(p, held, pos);
+            for (int k = 0; k < 4; ++k) {
+              const int row = (k % 2 ? vb : va) + 8 * (k / 2);
+              const unsigned char* from = blocks + x * L::kBlockBytes + 8 * hd + row * (hd / 2) + gid * W * 4;
+              if constexpr (W == 2) *reinterpret_cast<uint2*>(w[k]) = *reinterpret_cast<const uint2*>(from);
+              else w[k][0] = *reinterpret_cast<const uint32_t*>(from);
+            }
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int j = key_row + 8 * h, key = key0 + j;
-                if (j >= info.y || key >= hi || (key < lo && key >= p.c.sinks)) s[nt][2 * h + e] = -INFINITY;
+            for (int i = 0; i < W; ++i)
+              sm[i] = *reinterpret_cast<const uint4*>(pairs_out + ((x * GROUPS + (gid * W) % GROUPS + i) * 4 + t4) * 4);
+            // codes of two keys beside each other: nibbles 0-3 and 4-7 of each word
+            uint32_t part[2][W][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int i = 0; i < W; ++i) {
+                part[h][i][0] = __byte_perm(w[2 * h][i], w[2 * h + 1][i], 0x5410);
+                part[h][i][1] = __byte_perm(w[2 * h][i], w[2 * h + 1][i], 0x7632);
               }
-            }
-        }
-        // ---- weights
-        float e[NT][4];
-        bool above = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            e[nt][i] = fmaf(s[nt][i], p.c.scale_log2, kShift - m[nt][i % 2]);
-            above |= e[nt][i] > kShift;
-          }
-        if (__any_sync(0xffffffffu, above)) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              float top = fmaxf(s[nt][r], s[nt][2 + r]) * p.c.scale_log2;
-#pragma unroll
-              for (int w = 4; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-              if (top > m[nt][r]) {  // of a row: all its lanes
-                const float corr = ex2(m[nt][r] - (top + kAbove));
-                m[nt][r] = top + kAbove;
-                l[nt][r] *= corr;
-#pragma unroll
-                for (int i = 0; i < 2 * GROUPS; ++i) {
-                  o[nt][i][r] *= corr;
-                  o[nt][i][2 + r] *= corr;
-                }
-              }
-#pragma unroll
-              for (int h = 0; h < 2; ++h) e[nt][2 * h + r] = fmaf(s[nt][2 * h + r], p.c.scale_log2, kShift - m[nt][r]);
-            }
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) e[nt][i] = ex2(e[nt][i]);
-          l[nt][0] += e[nt][0] + e[nt][2];
-          l[nt][1] += e[nt][1] + e[nt][3];
-        }
-        // ---- values
-        auto values = [&](auto type) {
-          constexpr bool HALF = decltype(type)::value;
-          uint32_t pb[NT][2];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            pb[nt][0] = transpose8(pack<HALF>(e[nt][0], e[nt][1]));
-            pb[nt][1] = transpose8(pack<HALF>(e[nt][2], e[nt][3]));
-          }
-          constexpr int W = GROUPS / 2;  // words of a key here
-          uint32_t w[4][W], pr[4][W];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int row = (k % 2 ? vb : va) + 8 * (k / 2);
-            const unsigned char* from = block + 8 * hd + row * (hd / 2) + gid * W * 4;
-            const uint32_t* pairs = v_pairs + row * GROUPS + (gid * W) % GROUPS;
-            if constexpr (W == 2) {
-              *reinterpret_cast<uint2*>(w[k]) = *reinterpret_cast<const uint2*>(from);
-              *reinterpret_cast<uint2*>(pr[k]) = *reinterpret_cast<const uint2*>(pairs);
-            } else {
-              w[k][0] = *reinterpret_cast<const uint32_t*>(from);
-              pr[k][0] = *pairs;
-            }
-            if constexpr (!HALF)
-#pragma unroll
-              for (int i = 0; i < W; ++i) pr[k][i] = q4::pair_is_none(pr[k][i]) ? 0u : pr[k][i];
-          }
-          // codes of two keys beside each other: nibbles 0-3 and 4-7 of each word; and the keys' s and m
-          uint32_t part[2][W][2], s2[2][W], m2[2][W];
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-              part[h][i][0] = __byte_perm(w[2 * h][i], w[2 * h + 1][i], 0x5410);
-              part[h][i][1] = __byte_perm(w[2 * h][i], w[2 * h + 1][i], 0x7632);
+            auto value = [&](uint32_t codes, int nibble, uint32_t sc, uint32_t mn) {
               if constexpr (HALF) {
-                s2[h][i] = pack<true>(low_of(pr[2 * h][i]), low_of(pr[2 * h + 1][i]));
-                m2[h][i] = pack<true>(high_of(pr[2 * h][i]), high_of(pr[2 * h + 1][i]));
+                // the even nibbles as 1024 + c, the odd ones, 4 bits higher in the significand, as 64 + c
+                const uint32_t y = nibble >= 2 ? codes >> 8 : codes, zero = nibble % 2 ? 0x54005400u : 0x64006400u;
+                const uint32_t c = masked_or(y, nibble % 2 ? high4 : low4, zero);
+                const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), *reinterpret_cast<const __half2*>(&zero)),
+                                          *reinterpret_cast<const __half2*>(&sc), *reinterpret_cast<const __half2*>(&mn));
+                return *reinterpret_cast<const uint32_t*>(&v);
               } else {
-                s2[h][i] = __byte_perm(pr[2 * h][i], pr[2 * h + 1][i], 0x5410);
-                m2[h][i] = __byte_perm(pr[2 * h][i], pr[2 * h + 1][i], 0x7632);
+                return q4::stands_for(((codes >> (4 * nibble)) & 0x000f000fu) | 0x43004300u, sc, mn);
               }
-            }
-          auto value = [&](uint32_t codes, uint32_t sc, uint32_t mn) {
-            if constexpr (HALF) {
-              const uint32_t c = codes | 0x64006400u, k1024 = 0x64006400u;  // 1024 + c
-              const __half2 x = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), *reinterpret_cast<const __half2*>(&k1024)),
-                                        *reinterpret_cast<const __half2*>(&sc), *reinterpret_cast<const __half2*>(&mn));
-              return *reinterpret_cast<const uint32_t*>(&x);
-            } else {
-              return q4::stands_for(codes | 0x43004300u, sc, mn);
-            }
-          };
+            };
 #pragma unroll
-          for (int i = 0; i < 2 * GROUPS; ++i) {
-            // rows gid and gid + 8 of the product: nibble i of the lane's two words, or nibbles i and i + 4 of its one
-            const int x0 = 0, x1 = W - 1, n0 = i, n1 = W == 2 ? i : i + 4;
-            const uint32_t a0 = value((part[0][x0][n0 / 4] >> (4 * (n0 % 4))) & 0x000f000fu, s2[0][x0], m2[0][x0]);
-            const uint32_t a1 = value((part[0][x1][n1 / 4] >> (4 * (n1 % 4))) & 0x000f000fu, s2[0][x1], m2[0][x1]);
-            const uint32_t a2 = value((part[1][x0][n0 / 4] >> (4 * (n0 % 4))) & 0x000f000fu, s2[1][x0], m2[1][x0]);
-            const uint32_t a3 = value((part[1][x1][n1 / 4] >> (4 * (n1 % 4))) & 0x000f000fu, s2[1][x1], m2[1][x1]);
+            for (int i = 0; i < 2 * GROUPS; ++i) {
+              // rows gid and gid + 8 of the product: nibble i of the lane's two words, or nibbles i and i + 4 of its one
+              const int x1 = W - 1, n1 = W == 2 ? i : i + 4;
+              const uint32_t a0 = value(part[0][0][i / 4], i % 4, sm[0].x, sm[0].y);
+              const uint32_t a1 = value(part[0][x1][n1 / 4], n1 % 4, sm[x1].x, sm[x1].y);
+              const uint32_t a2 = value(part[1][0][i / 4], i % 4, sm[0].z, sm[0].w);
+              const uint32_t a3 = value(part[1][x1][n1 / 4], n1 % 4, sm[x1].z, sm[x1].w);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma<HALF>(o[nt][i], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+              for (int nt = 0; nt < NT; ++nt) mma<HALF>(o[nt][i], a0, a1, a2, a3, pb[x][nt][0], pb[x][nt][1]);
+            }
           }
         };
-        if (half) values(std::true_type{});
-        else values(std::false_type{});
+        if (half) body(std::true_type{});
+        else body(std::false_type{});
         __syncwarp();
-        if (lane == 0) arrive(tl.empty[stage]);
+        ++computed;
       }
-      __syncwarp();
-      if (!L::kKeep && lane == 0) arrive(tl.desc_empty[slot]);
-      // ---- the warps' accumulators together
-      const bool whole = d.parts == 1;
+      // ---- the unit's part: a lane has words' 8 elements of rows 2 t4, + 1: of two words, or one
+      constexpr int W = GROUPS / 2;
+      auto element = [&](int nt, int word, int r, int e) -> float& {  // element e lies in nibble e / 2 + 4 (e % 2)
+        const int nibble = e / 2 + 4 * (e % 2);
+        return W == 2 ? o[nt][nibble][2 * word + r] : o[nt][nibble % 4][2 * (nibble / 4) + r];
+      };
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        if (8 * nt >= d.rows) break;
-        float* join = reinterpret_cast<float*>(gbase + L::kOffJoin);
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           float sum = l[nt][r];
 #pragma unroll
           for (int w = 4; w < 32; w *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-          if (gid == 0) {
-            tl.m[warp][8 * nt + 2 * t4 + r] = m[nt][r];
-            tl.l[warp][8 * nt + 2 * t4 + r] = sum;
-          }
-        }
-        const bool any = d.items > skips(warp);  // the warp had a block
-        if (any && 8 * nt + 2 * t4 < d.rows)
-#pragma unroll
-          for (int i = 0; i < 2 * GROUPS; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) join[(warp * 8 + 2 * t4 + r % 2) * L::kJoinRow + 16 * i + gid + 8 * (r / 2)] = o[nt][i][r];
-        meet();
-        // a thread takes 4 elements of a row: element e of word w lies in nibble e / 2 + 4 (e % 2) of it
-        constexpr int kQuads = hd / 4;
-        for (int x = tid; x < 8 * kQuads; x += 32 * kWarps) {
-          const int row = 8 * nt + x / kQuads, quad = x % kQuads, word = quad / 2;
-          if (row >= d.rows) break;
-          int at[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int nibble = (quad % 2 * 4 + e) / 2 + 4 * (e % 2);
-            at[e] = GROUPS == 4 ? 16 * nibble + word / 2 + 8 * (word % 2) : 16 * (nibble % 4) + word + 8 * (nibble / 4);
-          }
-          float top = kNone;
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, tl.m[w][row]);
-          float sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            if (d.items <= skips(w)) continue;
-            const float f = ex2(tl.m[w][row] - top);
-            sum = fmaf(tl.l[w][row], f, sum);
-            const float* from = join + (w * 8 + x / kQuads) * L::kJoinRow;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = fmaf(from[at[e]], f, y[e]);
-          }
-          // the quad's dims: word t * GROUPS + g holds 32 g + 8 t on
-          const int dim = 32 * (word % GROUPS) + 8 * (word / GROUPS) + quad % 2 * 4;
-          if (whole) {
+          const int row = 8 * nt + 2 * t4 + r;
+          if (row >= d.rows) continue;
+          if (d.parts == 1) {
             const int64_t token = d.token0 + row / p.G;
             const int head = d.kvh * p.G + row % p.G;
             float f = sum == 0.f ? 0.f : 1.f / sum;
             if (p.c.gate && sum != 0.f) f *= sigmoid(p.c.gate[token * p.c.gate_stride + head]);
-            uint2 w;
-            w.x = sum == 0.f ? 0u : pack<false>(y[0] * f, y[1] * f);
-            w.y = sum == 0.f ? 0u : pack<false>(y[2] * f, y[3] * f);
-            *reinterpret_cast<uint2*>(p.c.out + token * p.c.out_stride + (int64_t)head * hd + dim) = w;
-            if (p.c.lse && quad == 0)
-              p.c.lse[token * p.c.Hq + head] = sum == 0.f ? -INFINITY : (top - kShift + log2f(sum)) * 0.6931471805599453f;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+              const int word = gid * W + i;  // of dims 32 (word % GROUPS) + 8 (word / GROUPS) on
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                w[e] = sum == 0.f ? 0u : pack<false>(element(nt, i, r, 2 * e) * f, element(nt, i, r, 2 * e + 1) * f);
+              *reinterpret_cast<uint4*>(p.c.out + token * p.c.out_stride + (int64_t)head * hd + 32 * (word % GROUPS) +
+                                        8 * (word / GROUPS)) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            if (p.c.lse && gid == 0)
+              p.c.lse[token * p.c.Hq + head] = sum == 0.f ? -INFINITY : (m[nt][r] - kShift + log2f(sum)) * 0.6931471805599453f;
           } else {
-            const int64_t part = part_slot(d.first_cta, d.index);
-            __stcg(reinterpret_cast<float4*>(p.acc + (part * p.c.rows + row) * hd + dim), make_float4(y[0], y[1], y[2], y[3]));
-            if (quad == 0) {
-              __stcg(p.ml + part * 2 * p.c.rows + row, sum == 0.f ? kNone : top);
+            const int64_t part = part_slot(d.first, d.index);
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+              const int word = gid * W + i;
+              float* to = p.acc + (part * p.c.rows + row) * hd + 32 * (word % GROUPS) + 8 * (word / GROUPS);
+              __stcg(reinterpret_cast<float4*>(to), make_float4(element(nt, i, r, 0), element(nt, i, r, 1), element(nt, i, r, 2), element(nt, i, r, 3)));
+              __stcg(reinterpret_cast<float4*>(to) + 1, make_float4(element(nt, i, r, 4), element(nt, i, r, 5), element(nt, i, r, 6), element(nt, i, r, 7)));
+            }
+            if (gid == 0) {
+              __stcg(p.ml + part * 2 * p.c.rows + row, sum == 0.f ? kNone : m[nt][r]);
               __stcg(p.ml + (part * 2 + 1) * p.c.rows + row, sum);
             }
           }
         }
-        if (!whole) __threadfence();
-        meet();  // the buffer is free, the part is written
-      }
-      if (!whole) {
-        if (tid == 0) {
-          unsigned* counter = p.counters + d.first_cta;
+      // ---- parts that are all there are joined, 16 neighbours at a time: into the first one's slot, or to the output
+      int index = d.index, parts = d.parts, stride = 1, level = 0;
+#pragma unroll 1
+      while (parts > 1) {
+        __threadfence();
+        __syncwarp();
+        const int leader = index / kJoin * kJoin, count = min(kJoin, parts - leader);  // in units of `stride` parts
+        int last = 0;
+        if (lane == 0) {
+          // the warps between two first ones are inside the unit: theirs are free for the joins of joined parts
+          unsigned* counter = p.counters + ((int64_t)(d.first + leader * stride + level) * 2 + (leader != 0));
           unsigned old = *reinterpret_cast<volatile unsigned*>(counter), seen, arrived;
           do {
             seen = old;
             arrived = (seen >> 12 == p.tag ? seen & 0xfffu : 0u) + 1;
-            old = atomicCAS(counter, seen, arrived == (unsigned)d.parts ? 0u : p.tag << 12 | arrived);
+            old = atomicCAS(counter, seen, arrived == (unsigned)count ? 0u : p.tag << 12 | arrived);
           } while (old != seen);
-          tl.last = arrived == (unsigned)d.parts;
+          last = arrived == (unsigned)count;
           __threadfence();
         }
-        meet();
-        if (tl.last) {
-          constexpr int kQuads = hd / 4, kTogether = 8;
-          for (int x = tid; x < d.rows * kQuads; x += 32 * kWarps) {
-            const int row = x / kQuads, quad = x % kQuads;
-            float top = kNone, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+        last = __shfl_sync(0xffffffffu, last, 0);
+        if (!last) break;
+        const bool final = parts <= kJoin;
+        constexpr int kQuads = hd / 4, kTogether = 4, kAtOnce = 2;  // of a lane: rows' pieces, parts whose loads are in flight
+        const int64_t to = part_slot(d.first, leader * stride);
 #pragma unroll 1
-            for (int i0 = 0; i0 < d.parts; i0 += kTogether) {
-              float pm[kTogether], pl[kTogether], high = top;
-              float4 v[kTogether];
+        for (int x0 = lane; x0 < d.rows * kQuads; x0 += 32 * kAtOnce) {
+          float top[kAtOnce], sum[kAtOnce], y[kAtOnce][4];
+#pragma unroll
+          for (int a = 0; a < kAtOnce; ++a) {
+            top[a] = kNone;
+            sum[a] = y[a][0] = y[a][1] = y[a][2] = y[a][3] = 0.f;
+          }
+#pragma unroll 1
+          for (int i0 = 0; i0 < count; i0 += kTogether) {
+            float pm[kAtOnce][kTogether], pl[kAtOnce][kTogether];
+            float4 v[kAtOnce][kTogether];
+#pragma unroll
+            for (int a = 0; a < kAtOnce; ++a)
 #pragma unroll
               for (int k = 0; k < kTogether; ++k) {
-                const bool there = i0 + k < d.parts;
-                const int64_t part = part_slot(d.first_cta, there ? i0 + k : 0);
-                pm[k] = there ? __ldcg(p.ml + part * 2 * p.c.rows + row) : kNone;
-                pl[k] = there ? __ldcg(p.ml + (part * 2 + 1) * p.c.rows + row) : 0.f;
-                v[k] = there ? __ldcg(reinterpret_cast<const float4*>(p.acc + (part * p.c.rows + row) * hd + quad * 4))
-                             : make_float4(0.f, 0.f, 0.f, 0.f);
+                const int x = x0 + 32 * a, row = x / kQuads, quad = x % kQuads;
+                const bool there = i0 + k < count && row < d.rows;
+                const int64_t part = part_slot(d.first, (leader + (there ? i0 + k : 0)) * stride);
+                pm[a][k] = there ? __ldcg(p.ml + part * 2 * p.c.rows + row) : kNone;
+                pl[a][k] = there ? __ldcg(p.ml + (part * 2 + 1) * p.c.rows + row) : 0.f;
+                v[a][k] = there ? __ldcg(reinterpret_cast<const float4*>(p.acc + (part * p.c.rows + row) * hd + quad * 4))
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
               }
 #pragma unroll
-              for (int k = 0; k < kTogether; ++k) high = fmaxf(high, pm[k]);
-              const float before = ex2(top - high);
-              top = high;
-              sum *= before;
+            for (int a = 0; a < kAtOnce; ++a) {
+              float high = top[a];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) y[e] *= before;
+              for (int k = 0; k < kTogether; ++k) high = fmaxf(high, pm[a][k]);
+              const float before = ex2(top[a] - high);
+              top[a] = high;
+              sum[a] *= before;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) y[a][e] *= before;
 #pragma unroll
               for (int k = 0; k < kTogether; ++k) {
-                const float f = ex2(pm[k] - top);
-                sum = fmaf(pl[k], f, sum);
-                y[0] = fmaf(v[k].x, f, y[0]), y[1] = fmaf(v[k].y, f, y[1]);
-                y[2] = fmaf(v[k].z, f, y[2]), y[3] = fmaf(v[k].w, f, y[3]);
+                const float f = ex2(pm[a][k] - high);
+                sum[a] = fmaf(pl[a][k], f, sum[a]);
+                y[a][0] = fmaf(v[a][k].x, f, y[a][0]), y[a][1] = fmaf(v[a][k].y, f, y[a][1]);
+                y[a][2] = fmaf(v[a][k].z, f, y[a][2]), y[a][3] = fmaf(v[a][k].w, f, y[a][3]);
               }
             }
-            const int64_t token = d.token0 + row / p.G;
-            const int head = d.kvh * p.G + row % p.G;
-            float f = sum == 0.f ? 0.f : 1.f / sum;
-            if (p.c.gate && sum != 0.f) f *= sigmoid(p.c.gate[token * p.c.gate_stride + head]);
-            uint2 w;
-            w.x = sum == 0.f ? 0u : pack<false>(y[0] * f, y[1] * f);
-            w.y = sum == 0.f ? 0u : pack<false>(y[2] * f, y[3] * f);
-            *reinterpret_cast<uint2*>(p.c.out + token * p.c.out_stride + (int64_t)head * hd + quad * 4) = w;
-            if (p.c.lse && quad == 0)
-              p.c.lse[token * p.c.Hq + head] = sum == 0.f ? -INFINITY : (top - kShift + log2f(sum)) * 0.6931471805599453f;
           }
+          // (the first part's m and sum are rewritten only when every lane has read them)
+          if (!final) __syncwarp();
+#pragma unroll
+          for (int a = 0; a < kAtOnce; ++a) {
+            const int x = x0 + 32 * a, row = x / kQuads, quad = x % kQuads;
+            if (row >= d.rows) continue;
+            if (final) {
+              const int64_t token = d.token0 + row / p.G;
+              const int head = d.kvh * p.G + row % p.G;
+              float f = sum[a] == 0.f ? 0.f : 1.f / sum[a];
+              if (p.c.gate && sum[a] != 0.f) f *= sigmoid(p.c.gate[token * p.c.gate_stride + head]);
+              uint2 w;
+              w.x = sum[a] == 0.f ? 0u : pack<false>(y[a][0] * f, y[a][1] * f);
+              w.y = sum[a] == 0.f ? 0u : pack<false>(y[a][2] * f, y[a][3] * f);
+              *reinterpret_cast<uint2*>(p.c.out + token * p.c.out_stride + (int64_t)head * hd + quad * 4) = w;
+              if (p.c.lse && quad == 0)
+                p.c.lse[token * p.c.Hq + head] = sum[a] == 0.f ? -INFINITY : (top[a] - kShift + log2f(sum[a])) * 0.6931471805599453f;
+            } else {
+              __stcg(reinterpret_cast<float4*>(p.acc + (to * p.c.rows + row) * hd + quad * 4), make_float4(y[a][0], y[a][1], y[a][2], y[a][3]));
+              if (quad == 0) {
+                __stcg(p.ml + to * 2 * p.c.rows + row, top[a]);
+                __stcg(p.ml + (to * 2 + 1) * p.c.rows + row, sum[a]);
+              }
+            }
+          }
+          if (!final) __syncwarp();
         }
-        meet();  // tl.last has been read
+        index = leader / kJoin;
+        parts = (parts + kJoin - 1) / kJoin;
+        stride *= kJoin;
+        ++level;
       }
+      ++done;
+      loaded = false;
     }
+    wait_copies<0>();
   }
   // ---- rows of no request, where no other kernel takes them
   if (p.c.only && !refused) {
     const int idle = tl.idle[0] + p.c.kv.N - tl.idle[1];
 #pragma unroll 1
-    for (int i = cta * (kWarps + 1) + warp; i < idle; i += ctas * (kWarps + 1)) {
+    for (int i = worker; i < idle; i += p.workers) {
       const int64_t t = i < tl.idle[0] ? i : tl.idle[1] + i - tl.idle[0];
 #pragma unroll 1
       for (int c = lane; c < p.c.Hq * hd / 8; c += 32)
@@ -814,15 +915,22 @@ __global__ void __launch_bounds__(kThreads, kCtas) gqa_few_q4_kernel(const __gri
         for (int h = lane; h < p.c.Hq; h += 32) p.c.lse[t * p.c.Hq + h] = -INFINITY;
     }
   }
-  __syncthreads();
-  if (tid == 0 && *abort != 0 && p.status) atomicOr(p.status, zb::kStatusAttnChunkTimeout);
+}
+
+// The CTAs of a launch: those that are on the GPU at once, or as many as a batch can have a share for.
+int ctas_of(int B, int N, int Hkv, int64_t max_keys, int warps) {
+  const int64_t items = (max_keys + kItem * q4::kBlock - 1) / (kItem * q4::kBlock) + 1;  // of a unit; sinks may add one
+  const int64_t shares = std::min<int64_t>(B, N) * Hkv * (items + kUnitCost) / kMinShare + 1;
+  const int64_t most = std::min<int64_t>((int64_t)zb::sm_count() * 2, q4::kFewFlagBytes / 8 / warps - 1);
+  return (int)std::max<int64_t>(1, std::min(most, shares));  // a warp of each first: few shares are spread over the SMs
 }
 
 template <int GROUPS, int NT>
 int launch(FewParams& p, int ctas, cudaStream_t stream) {
+  using L = Shape<GROUPS, NT>;
   auto kernel = gqa_few_q4_kernel<GROUPS, NT>;
-  constexpr int kSmem = Shape<GROUPS, NT>::kOffTail + (int)sizeof(Tail);
-  static_assert(kSmem * kCtas <= 227 * 1024, "shared memory");
+  constexpr int kSmem = L::kWarps * L::kPerWarp + (int)sizeof(Tail);
+  static_assert((kSmem + 1024) * L::kCtas <= 228 * 1024, "shared memory");
   static bool configured[64] = {false};  // the shared-memory attribute, set once per device
   int dev = 0;
   ZB_CUDA(cudaGetDevice(&dev));
@@ -830,11 +938,12 @@ int launch(FewParams& p, int ctas, cudaStream_t stream) {
     ZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  ZB_CUDA(zb::launch(kernel, dim3((unsigned)ctas), dim3(kThreads), (size_t)kSmem, stream, 1, p));
+  p.workers = ctas * L::kWarps;
+  ZB_CUDA(zb::launch(kernel, dim3((unsigned)ctas), dim3(L::kThreads), (size_t)kSmem, stream, 1, p));
   return zb::check_launch("gqa_chunk_q4");
 }
 
-int ctas_of() { return (int)std::min<int64_t>((int64_t)zb::sm_count() * kCtas, q4::kFewFlagBytes / 4); }
+int warps_of(int rows) { return rows <= 8 ? 8 : 6; }
 
 }  // namespace
 
@@ -849,9 +958,9 @@ int few_rows(int hd, int G, int max_new) {
   return G <= 8 ? 8 : G <= 16 ? 16 : 0;
 }
 
-int64_t few_workspace_bytes(int B, int N, int Hkv, int hd, int rows) {
+int64_t few_workspace_bytes(int B, int N, int Hkv, int hd, int rows, int64_t max_keys) {
   if (rows == 0 || B < 1 || N < 1) return 0;
-  return kFewFlagBytes + (int64_t)ctas_of() * 2 * rows * (hd + 2) * 4;
+  return kFewFlagBytes + (int64_t)ctas_of(B, N, Hkv, max_keys, warps_of(rows)) * warps_of(rows) * 2 * rows * (hd + 2) * 4;
 }
 
 int launch_few(const FewCall& call, cudaStream_t stream) {
@@ -862,13 +971,14 @@ int launch_few(const FewCall& call, cudaStream_t stream) {
   while ((1u << l) < (unsigned)call.kv.page_size) ++l;
   p.page_shift = 31 + l;
   p.page_mul = (unsigned)((((uint64_t)1 << p.page_shift) + call.kv.page_size - 1) / call.kv.page_size);
-  const int ctas = ctas_of();
+  const int warps = warps_of(call.rows);
+  const int ctas = ctas_of(call.kv.B, call.kv.N, call.kv.Hkv, (int64_t)call.kv.page_size * call.kv.max_pages, warps);
   static std::atomic<unsigned> calls{0};
   do p.tag = (calls.fetch_add(1, std::memory_order_relaxed) + 1) & 0xfffffu;
   while (p.tag == 0);
   p.counters = reinterpret_cast<unsigned*>(call.workspace);
   p.acc = reinterpret_cast<float*>(call.workspace + kFewFlagBytes);
-  p.ml = p.acc + (int64_t)ctas * 2 * call.rows * call.kv.hd;
+  p.ml = p.acc + (int64_t)ctas * warps * 2 * call.rows * call.kv.hd;
   p.status = device_status_ptr();
   if (call.kv.hd == 128) return call.rows == 8 ? launch<4, 1>(p, ctas, stream) : launch<4, 2>(p, ctas, stream);
   return call.rows == 8 ? launch<2, 1>(p, ctas, stream) : launch<2, 2>(p, ctas, stream);

@@ -1204,7 +1204,7 @@ def _chunk_workspace_bytes(B, N, Hq, Hkv, hd, max_keys) -> int:
 
 _CHUNK_WS: dict = {}  # (device, stream, bytes of flags) -> the workspace of eager calls on that stream (flags another call left do not count)
 _CHUNK_FLAG_BYTES = 4096  # the flags lie at the workspace's start
-_CHUNK_Q4_FLAG_BYTES = 8192
+_CHUNK_Q4_FLAG_BYTES = 36864
 
 
 def _chunk_workspace(q: torch.Tensor, stream: int, nbytes: int, flag_bytes: int = _CHUNK_FLAG_BYTES) -> torch.Tensor:
@@ -1360,7 +1360,7 @@ def gqa_chunk_q4(q, kv_cache, page_table, cache_seqlens, cu_seqlens_q, *, softma
     kv_cache as for :func:`gqa_append_q4`; the other arguments as for :func:`gqa_chunk`. ``max_new``: no request brings more new
     tokens than so many, when the caller knows (1 for a decode batch); a small one saves the launch for requests of many rows.
     A request that brings more all the same sets :func:`device_status` bit 256 and its rows may be left unwritten.
-    workspace: at least :func:`gqa_chunk_q4_workspace_bytes` bytes, its first 8192 zero before the first call. Returns out
+    workspace: at least :func:`gqa_chunk_q4_workspace_bytes` bytes, its first 36864 zero before the first call. Returns out
     [N, Hq, hd] bf16."""
     paged, index, Hkv, hd = _paged_q4(q, kv_cache, page_table, cache_seqlens, cu_seqlens_q, None)
     N, Hq = q.shape[0], q.shape[1]
