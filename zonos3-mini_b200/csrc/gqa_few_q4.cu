@@ -5,16 +5,18 @@
 // reads every code once, so the work is the codes' way from HBM and their unpacking; the products are few. So they are
 // formed from registers (m16n8k16: 16 keys or dims by 8 rows), where a code goes from the loaded word into a matrix fragment
 // with two instructions for two codes, and nothing is written out in between as a tensor-memory product would need it:
-//   scores^T [16 keys, 8 rows] = sum over groups g of  s_g ((128 + c) . q)_g + (m_g - 128 s_g) (sum q)_g:  the codes themselves are
-//     the operand, as 128 + c in bf16 (exact), s goes onto the products' sums in fp32; the second term is a product of its own, the
-//     pairs as they lie in the cache times the queries' sums, split into three bf16 each: the scores have the precision of fp32;
-//   out^T [16 dims, 8 rows] += V^T p^T with V = m + s c and the weights in fp16, 2^-12 of each: bf16's 2^-9 would be the largest
-//     error here. fp16 has less range, so a block whose pairs are not all within it (magnitudes of 2^-10 to 2^14, or 0) takes bf16.
+//   scores^T [16 keys, 8 rows] = sum over groups g of  s_g (c . q)_g + m_g (sum q)_g:  the codes themselves are the operand, as fp16
+//     subnormals, which takes one instruction for two of them; the queries, scaled into fp16's range, keep their 8 bits. s goes onto
+//     the products' sums in fp32; the second term is a product of its own, the pairs as they lie in the cache times the queries'
+//     sums, split into three bf16. So the scores are as good as fp32's, down to 2^-35 of a row's largest element;
+//   out^T [16 dims of a group, 8 rows] += c (s_g p^T), and p^T m_g and the sum of p by a product more. Weights are fp16, 2^-12 of
+//     each: bf16's 2^-9 would be the largest error here. fp16 has less range, so an item whose pairs are not all within it
+//     (half_holds()) and those after it take bf16.
 // A weight is 2^(score - m + 15) with m a row's reference, its largest score or up to 8 (log2) above it when it is set; it is set
 // anew by a score above it, hardly ever after the first block. So weights lie in fp16's range: up to 2^15, the largest not below 2^7
 // when m is set, and those below 2^-39 of m count as 0. m and the sum cancel in the end.
 // The keys of a 16-key block stand in the scores' rows in the order 0 1 3 2 4 5 7 6 and 8 on: the two rows of a quarter of the lanes then
-// read other banks, and the four rows that a lane's values come from too, as far as 64-byte rows allow.
+// read other banks, and the four rows that a quarter's values come from too, as far as 64-byte rows allow.
 //
 // Every warp works for itself. All units' keys are one long run of items (two blocks of 16 keys, at hd 128 2560 bytes
 // each), of which a warp takes an equal share (the split is as in gqa_chunk.cu, to warps instead of CTAs): it looks up the places of
@@ -35,7 +37,8 @@ namespace {
 namespace q4 = zb::q4;
 
 constexpr int kItem = 2;      // blocks of an item
-constexpr int kUnitCost = 1;  // of a unit, in items
+constexpr int kStages = 2;    // items of a warp: one that is computed, and copies under way
+constexpr int kUnitCost = 4;  // of a unit, in items
 constexpr int kMinShare = 3;  // items of a warp, its units' cost among them
 constexpr int kJoin = 16;     // parts that are joined at once
 constexpr float kAbove = 8.f, kShift = 15.f;
@@ -45,13 +48,11 @@ struct FewParams {
   q4::FewCall c;
   int G, workers;
   unsigned page_mul, page_shift;  // division by the page size
-  // [warp][2]: the call's tag and, below it, the parts that have arrived of those that are joined with one of the warp's (the first
-  // of them; [0]: of the unit that began there, [1]: of one that had begun before); 0 again when all have. What a call whose waits
-  // gave up has left has another tag.
+  // [warp][2]: how many parts have arrived of those that are joined with one of the warp's (the first of them; [0]: of the unit that
+  // began there, [1]: of one that had begun before); 0 again when all have
   unsigned* counters;
-  unsigned tag;
   float* acc;  // [warp][2][rows][hd]: parts
-  float* ml;   // [warp][2][2][rows]: m, sum
+  float2* ml;  // [warp][2][rows]: m, sum
   unsigned* status;
 };
 
@@ -62,16 +63,16 @@ struct Desc {
   int items;
   int index, parts, first;  // of the unit's parts this one, their number, and the warp that has the first
   int from;                 // keys from the sinks' end to here are hidden from every row
-  int all_lo, all_hi;       // keys of [all_lo, all_hi), and those below min(sinks, all_hi), are seen by every row
 };
-// Where a block lies; its first key, and how many of its keys there are.
+// Where a block lies; its first key; how many of its keys there are, and kPartly if some rows do not see some of its keys.
 struct Place {
   const unsigned char* at;
   int key0, exist;
 };
+constexpr int kPartly = 256;
 // A warp's own shared memory, behind its stages and queries.
 struct Own {
-  alignas(16) int2 info[2][kItem];  // of the stages' blocks: first key, and how many there are
+  int2 info[kStages][kItem];  // of the stages' blocks: a Place's key0 and exist
   alignas(16) Place places[32];
   Desc desc[2];
   // the unit after those opened: how far its request and the share have got
@@ -79,14 +80,14 @@ struct Own {
   int b, kvh, off;
   int row0, tokens, keys;
   // of the unit opened last: blocks whose places are not looked up yet, and what that takes
-  int next, end, n, sink_blocks, gap, of_b, of_kvh, held;
+  int next, end, n, sink_blocks, gap, of_b, of_kvh, held, all_lo, all_hi;
 };
 
 template <int GROUPS, int NT>
 struct Shape {
   static constexpr int kHd = GROUPS * q4::kGroup, kBlockBytes = q4::block_bytes(kHd), kRows = 8 * NT;
   static constexpr int kStage = kItem * kBlockBytes;
-  static constexpr int kOffQ = 2 * kStage;
+  static constexpr int kOffQ = kStages * kStage;
   static constexpr int kOffPairs = kOffQ + kRows * kHd * 2;  // pairs of values, as the lanes need them
   static constexpr int kOffOwn = kOffPairs + kItem * GROUPS * 64;
   static constexpr int kPerWarp = (kOffOwn + (int)sizeof(Own) + 127) / 128 * 128;
@@ -94,11 +95,6 @@ struct Shape {
   static constexpr int kWarps = NT == 1 ? 8 : 6, kCtas = 2, kThreads = 32 * kWarps;
   // The queries' fragments stay in registers, or are read again for every block where the accumulators take those.
   static constexpr bool kKeep = NT == 1;
-};
-struct Tail {
-  int sums[2][8];
-  int before[256], cost[256];
-  int idle[2];
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -118,9 +114,20 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// D = A B of bf16
+// The same with half the depth, of bf16.
+__device__ __forceinline__ void mma8(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0));
+}
+__device__ __forceinline__ void mma8_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(b0), "f"(0.f));
+}
+// D = A B of fp16
 __device__ __forceinline__ void mma_new(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
@@ -139,21 +146,15 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
 __device__ __forceinline__ float low_of(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float high_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
 
-// Whether fp16 keeps m + s c of a pair to near its 11 bits: |m| is below 2^14 and s below 2^10, and either |m| is 2^-10 or more or
-// s 2^-14, or the pair is 0.
-__device__ __forceinline__ bool half_holds(uint32_t pair) {
+// Whether fp16 keeps a pair's s and 2^8 m well: s is below 2 and |m| below 2^7 (a sign bit of `over` else), and s is 2^-12 or
+// more, or the pair is 0 (`holds`).
+__device__ __forceinline__ void half_holds(uint32_t pair, uint32_t& over, bool& holds) {
   const uint32_t a = pair & 0x7fff7fffu;
-  const uint32_t over = a + (((0x8000u - 0x4680u) << 16) | (0x8000u - 0x4480u));
-  const uint32_t under = a + (((0x8000u - 0x3a80u) << 16) | (0x8000u - 0x3880u));
-  return (over & 0x80008000u) == 0 && ((under & 0x80008000u) != 0 || a == 0);
+  over |= a + (((0x8000u - 0x4300u) << 16) | (0x8000u - 0x4000u));
+  holds &= pair << 16 >= 0x3980u << 16 || a == 0;
 }
 
-// (x & mask) | bits, in one instruction.
-__device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t mask, uint32_t bits) {
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(mask), "r"(bits));
-  return d;
-}
+__device__ __forceinline__ void fence_gpu() { asm volatile("fence.acq_rel.gpu;" ::: "memory"); }
 // 16 bytes into shared memory, asynchronously and for this thread's next commit.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -183,6 +184,15 @@ __device__ __forceinline__ Request request(const FewParams& p, int b, bool& more
 struct Blocks {
   int n, sink_blocks, gap;
   int lo_first, lo_last, hi_first;
+};
+// While the work is split, over the first warp's stages: a round of requests, and their places in it.
+struct Round {
+  int before[256], cost[256];
+  Request request[256];
+};
+struct Tail {
+  int sums[2][16];
+  int idle[2];
 };
 __device__ __forceinline__ int held_keys(const FewParams& p, int keys) { return min(keys, p.c.kv.max_pages * p.c.kv.page_size); }
 __device__ __forceinline__ int first_seen(const FewParams& p, int pos) {  // of a token's window
@@ -216,6 +226,9 @@ __device__ __forceinline__ int cost_of(const FewParams& p, const Request& r) {
   return r.tokens > 0 ? kUnitCost + (blocks_of(p, r).n + kItem - 1) / kItem : 0;
 }
 
+// n / d, whose quotient fits 32 bits; n hardly ever does not.
+__device__ __forceinline__ int quotient(int64_t n, int d) { return n <= INT32_MAX ? (int)n / d : (int)(n / d); }
+
 // Exclusive prefix of v over the block's threads; `total` the sum. `buffer` alternates from call to call.
 template <int WARPS>
 __device__ __forceinline__ int block_scan(int v, Tail& tl, int buffer, int& total) {
@@ -242,7 +255,7 @@ __device__ __forceinline__ int block_scan(int v, Tail& tl, int buffer, int& tota
 __device__ __forceinline__ float sigmoid(__nv_bfloat16 x) { return 1.f / (1.f + ex2(-1.4426950408889634f * __bfloat162float(x))); }
 
 // Part `index` of a unit whose first part is warp `first`'s: the slots are its own second one, then the first ones of those after it.
-__device__ __forceinline__ int64_t part_slot(int first, int index) { return (int64_t)(first + index) * 2 + (index == 0); }
+__device__ __forceinline__ unsigned part_slot(int first, int index) { return (unsigned)(first + index) * 2 + (index == 0); }
 
 template <int GROUPS, int NT>
 __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>::kCtas)
@@ -252,6 +265,7 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
   extern __shared__ __align__(128) unsigned char gbase[];
   Tail& tl = *reinterpret_cast<Tail*>(gbase + kWarps * L::kPerWarp);
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid / 32, 0), lane = tid % 32;
+  Round& round = *reinterpret_cast<Round*>(gbase);
   unsigned char* own = gbase + warp * L::kPerWarp;
   Own& my = *reinterpret_cast<Own*>(own + L::kOffOwn);
   const int B = p.c.kv.B, Hkv = p.c.kv.Hkv;
@@ -286,37 +300,41 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
   if (worker == 0 && lane == 0 && p.status && (refused || left_out))
     atomicOr(p.status, refused ? zb::kStatusAttnChunkBatch : zb::kStatusAttnFewRows);
   work = refused ? 0 : work * Hkv;
-  const int64_t share = max((int64_t)kMinShare, (work + p.workers - 1) / p.workers);
-  const int64_t begin = share * worker, end = min(work, begin + share);
+  const int share = max(kMinShare, quotient(work + p.workers - 1, p.workers));
+  const int64_t begin = (int64_t)share * worker, end = min(work, begin + share);
   {
+    const int64_t of_head = begin <= INT32_MAX ? (int)begin / Hkv : begin / Hkv;  // how far the share's begin is into the work of one head
     int64_t seen = 0;
 #pragma unroll 1
     for (int b0 = 0; b0 < B; b0 += kThreads) {
       int cost = mine_cost, before = mine_before, total = mine_total;
+      Request r = mine;
       if (b0 > 0) {
-        cost = b0 + tid < B ? cost_of(p, request(p, b0 + tid, more)) : 0;
+        r = b0 + tid < B ? request(p, b0 + tid, more) : Request{0, 0, 0};
+        cost = cost_of(p, r);
         buffer ^= 1;
         before = block_scan<kWarps>(cost, tl, buffer, total);
       }
       if (work > 0) {
-        tl.before[tid] = before;
-        tl.cost[tid] = cost;
+        round.before[tid] = before;
+        round.cost[tid] = cost;
+        round.request[tid] = r;
       }
       __syncthreads();
-      if (begin < end && begin >= seen * Hkv && begin < (seen + total) * Hkv) {
-#pragma unroll 1
+      if (begin < end && of_head >= seen && of_head < seen + total) {
+        const int into = (int)(of_head - seen);
+#pragma unroll 2
         for (int i = lane; i < kThreads; i += 32) {
-          const int64_t at = (seen + tl.before[i]) * Hkv;
-          if (tl.cost[i] > 0 && begin >= at && begin < at + (int64_t)tl.cost[i] * Hkv) {
-            bool ignored = false;
-            const Request r = request(p, b0 + i, ignored);
+          if (into >= round.before[i] && into - round.before[i] < round.cost[i]) {
+            const int64_t rest = begin - (seen + round.before[i]) * Hkv;
+            const int kvh = quotient(rest, round.cost[i]);
             my.at = begin;
             my.b = b0 + i;
-            my.kvh = (int)((begin - at) / tl.cost[i]);
-            my.off = (int)((begin - at) % tl.cost[i]);
-            my.row0 = r.row0;
-            my.tokens = r.tokens;
-            my.keys = r.keys;
+            my.kvh = kvh;
+            my.off = (int)(rest - (int64_t)kvh * round.cost[i]);
+            my.row0 = round.request[i].row0;
+            my.tokens = round.request[i].tokens;
+            my.keys = round.request[i].keys;
           }
         }
       }
@@ -358,12 +376,10 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
             d.rows = req.tokens * p.G;
             d.kvh = kvh;
             d.items = to - from;
-            d.first = x.n > 0 ? (int)(first / share) : worker;
+            d.first = x.n > 0 ? quotient(first, share) : worker;
             d.index = worker - d.first;
-            d.parts = x.n > 0 ? (int)((first + unit_items - 1) / share) - d.first + 1 : 1;
+            d.parts = x.n > 0 ? quotient(first + unit_items - 1, share) - d.first + 1 : 1;
             d.from = x.lo_first;
-            d.all_lo = x.lo_last;
-            d.all_hi = x.hi_first;
             my.desc[opened % 2] = d;
             my.next = from * kItem;
             my.end = to * kItem;
@@ -373,6 +389,8 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
             my.of_b = b;
             my.of_kvh = kvh;
             my.held = held_keys(p, req.keys);
+            my.all_lo = x.lo_last;
+            my.all_hi = x.hi_first;
           }
           // the queries, with the copies of the unit's first item: a token's heads of the group lie side by side
           const int pieces = p.G * (hd / 8);
@@ -432,7 +450,10 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
           found.at = reinterpret_cast<const unsigned char*>(p.c.kv.k) + (there ? (int64_t)page * p.c.kv.page_stride : 0) +
                      (int64_t)my.of_kvh * p.c.kv.head_stride + (int64_t)(key0 - column * p.c.kv.page_size) / q4::kBlock * L::kBlockBytes;
           found.key0 = key0;
-          found.exist = there ? min(q4::kBlock, my.held - key0) : 0;
+          const int exist = there ? min(q4::kBlock, my.held - key0) : 0;
+          // keys of [all_lo, all_hi), and those below min(sinks, all_hi), are seen by every row
+          const bool all = exist == q4::kBlock && key0 + q4::kBlock <= my.all_hi && (key0 >= my.all_lo || key0 + q4::kBlock <= p.c.sinks);
+          found.exist = exist | (all ? 0 : kPartly);
           __syncwarp();
           my.places[lane] = found;
           place = 0;
@@ -444,13 +465,13 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
           open_unit();
         }
       }
-      const int stage = fetched % 2;
+      const int stage = fetched % kStages;
 #pragma unroll
       for (int x = 0; x < kItem; ++x) {
         const Place found = my.places[place + x];
         const uint32_t to = zb::smem_addr(own + stage * L::kStage + x * L::kBlockBytes) + lane * 16;
         if (lane == 0) my.info[stage][x] = make_int2(found.key0, found.exist);
-        if (found.exist > 0)
+        if (found.exist & (kPartly - 1))
 #pragma unroll
           for (int i = 0; i < L::kBlockBytes; i += 512)
             if (i + 512 <= L::kBlockBytes || lane * 16 < L::kBlockBytes - i) copy16(to + i, found.at + i + lane * 16);
@@ -459,13 +480,10 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
       place += kItem;
       ++fetched;
     };
-    // Masks that the compiler does not see through stay in registers, and a code takes one instruction with the constant it is
-    // joined to; with both as immediates it takes two.
-    uint32_t low4 = 0x000f000fu, high4 = 0x00f000f0u;
-    asm("" : "+r"(low4), "+r"(high4));
+    const uint32_t low4 = 0x000f000fu, high4 = 0x00f000f0u, halves = gid < 4 ? 0x5410u : 0x7632u;
 
-    fetch();
-    fetch();
+#pragma unroll 1
+    for (int k = 0; k < kStages; ++k) fetch();
 #pragma unroll 1
     while (true) {
       if (opened == done) open_unit();
@@ -473,118 +491,159 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
       const Desc d = my.desc[done % 2];
       // The copies of the item to be computed, and with them those of its unit's queries.
       auto arrived = [&]() {
-        if (fetched - computed > 1) wait_copies<1>();
+        const int behind = fetched - computed - 1;
+        if (behind > 1) wait_copies<2>();
+        else if (behind > 0) wait_copies<1>();
         else wait_copies<0>();
         __syncwarp();
       };
       if (fetched == computed) fetch();
       arrived();
-      // ---- queries: B fragments; and of what a group's pair multiplies, -128 and 1 times the sum of its elements of the query, as
-      // three bf16 each: (c . q) comes with 128 instead of 0 for every code's zero
+      // ---- queries, scaled by a power of 2 to a largest element of 2^14 to 2^15: B fragments in fp16, and what a group's m multiplies,
+      // the sum of its elements of the query, as three bf16. (c . q) comes with 2^-24 for every code's 1, or with 2^-20 for those 4
+      // bits higher, whose elements of the query have 2^-4 less.
       const unsigned char* q_rows = own + L::kOffQ;
-      auto fragment = [&](int nt, int g) {
-        return 8 * nt + gid < d.rows ? *reinterpret_cast<const uint4*>(q_rows + (8 * nt + gid) * hd * 2 + (32 * g + 8 * t4) * 2)
-                                     : make_uint4(0, 0, 0, 0);
-      };
-      uint4 q[L::kKeep ? GROUPS : 1];
+      uint4 q[NT][L::kKeep ? GROUPS : 1];
       uint32_t qs[NT][3];
+      float scale[NT][2];  // of the scores of rows 2 t4, + 1
+      auto fragment = [&](int nt, int g, float by, float& sum) {
+        const uint4 w = 8 * nt + gid < d.rows ? *reinterpret_cast<const uint4*>(q_rows + (8 * nt + gid) * hd * 2 + (32 * g + 8 * t4) * 2)
+                                              : make_uint4(0, 0, 0, 0);
+        const float high = by * 0x1p-4f;
+        sum = (low_of(w.x) + high_of(w.x) + (low_of(w.y) + high_of(w.y)) + (low_of(w.z) + high_of(w.z) + (low_of(w.w) + high_of(w.w)))) * by;
+        return make_uint4(pack<true>(low_of(w.x) * by, high_of(w.x) * by), pack<true>(low_of(w.y) * high, high_of(w.y) * high),
+                          pack<true>(low_of(w.z) * by, high_of(w.z) * by), pack<true>(low_of(w.w) * high, high_of(w.w) * high));
+      };
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g)
+          if (8 * nt + gid < d.rows) {
+            const uint4 w = *reinterpret_cast<const uint4*>(q_rows + (8 * nt + gid) * hd * 2 + (32 * g + 8 * t4) * 2);
+            top = __vmaxu2(__vmaxu2(top, w.x & 0x7fff7fffu), __vmaxu2(w.y & 0x7fff7fffu, __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+          }
+        top = max(top >> 16, top & 0xffffu) >> 7;  // the largest exponent
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(max(top, __shfl_xor_sync(0xffffffffu, top, 2)), 16u);
+        const bool none = top >= 244;  // not finite, or at the end of the range: the row's scores become NaN
+        const float by = __uint_as_float((268u - min(top, 244u)) << 23);
         float of_group = 0.f;  // t4
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
-          const uint4 w = fragment(nt, g);
-          float sum = low_of(w.x) + high_of(w.x) + (low_of(w.y) + high_of(w.y)) + (low_of(w.z) + high_of(w.z)) + (low_of(w.w) + high_of(w.w));
+          float sum;
+          const uint4 f = fragment(nt, g, by, sum);
           sum += __shfl_xor_sync(0xffffffffu, sum, 1);
           sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          if (g == t4) of_group = sum;
-          if (L::kKeep) q[g] = w;
+          if (g == t4) of_group = none ? NAN : sum * 0x1p-24f;
+          if (L::kKeep) q[nt][g] = f;
         }
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
           const float kept = zb::bf16_round(of_group);
-          qs[nt][i] = pack<false>(-128.f * kept, kept);
+          qs[nt][i] = pack<false>(0.f, kept);
           of_group -= kept;
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const uint32_t its = __shfl_sync(0xffffffffu, top, 8 * t4 + 4 * r);
+          scale[nt][r] = p.c.scale_log2 * __uint_as_float((min(its, 244u) + 10u) << 23);
+        }
+        if (!L::kKeep) {  // the fragments over the queries
+          __syncwarp();
+          uint4 f[GROUPS];
+          float ignored;
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g) f[g] = fragment(nt, g, by, ignored);
+          __syncwarp();
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g)
+            *reinterpret_cast<uint4*>(own + L::kOffQ + (8 * nt + gid) * hd * 2 + (32 * g + 8 * t4) * 2) = f[g];
+          __syncwarp();
         }
       }
       __syncwarp();
       loaded = true;
-      float m[NT][2], l[NT][2], o[NT][2 * GROUPS][4];  // of rows 2 t4 and 2 t4 + 1 (and 8 on)
+      // Of rows 2 t4 and 2 t4 + 1 (and 8 on): m; sum of p s c 2^-24, or 2^-20, of 16 elements of a group at a time; and, on lanes
+      // 4 g + t4, the sum of 2^8 p m of group g, on lanes 16 + t4 that of p.
+      float m[NT][2], o[NT][2 * GROUPS][4], om[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         m[nt][0] = m[nt][1] = kNone;
-        l[nt][0] = l[nt][1] = 0.f;
+        om[nt][0] = om[nt][1] = om[nt][2] = om[nt][3] = 0.f;
 #pragma unroll
         for (int i = 0; i < 2 * GROUPS; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
       }
-      uint32_t* pairs_out = reinterpret_cast<uint32_t*>(own + L::kOffPairs);
+      uint32_t* s_out = reinterpret_cast<uint32_t*>(own + L::kOffPairs);  // [item's block][t4][rows 2 t4, + 1, or 8 on][group]
+      uint32_t* m_out = s_out + kItem * 8 * GROUPS;                         // [item's block][group][t4][rows 2 t4, + 1, or 8 on]
+      // Items from `item` on; returns the first that fp16 does not hold, which and those after it bf16 then takes. (Two loops: with
+      // the choice inside one, the accumulators changed places between its branches.)
+      auto run = [&](auto type, int item) {
+        constexpr bool HALF = decltype(type)::value;
 #pragma unroll 1
-      for (int item = 0; item < d.items; ++item) {
-        while (fetched - computed < 2) {
-          const int before = fetched;
-          fetch();
-          if (fetched == before) break;
-        }
-        const int stage = computed % 2;
+        for (; item < d.items; ++item) {
+#pragma unroll 1
+        for (int k = fetched - computed; k < kStages; ++k) fetch();
+        const int stage = computed % kStages;
         arrived();
-        const int4 info = *reinterpret_cast<const int4*>(my.info[stage]);
-        unsigned char* blocks = own + stage * L::kStage;
-        auto k_pairs = [&](int x) { return reinterpret_cast<uint32_t*>(blocks + x * L::kBlockBytes + 16 * hd); };
-        auto v_pairs = [&](int x) { return reinterpret_cast<uint32_t*>(blocks + x * L::kBlockBytes + 18 * hd); };
-        // keys that some rows do not see
+        int2 info[kItem];
         bool partly = false;
 #pragma unroll
         for (int x = 0; x < kItem; ++x) {
-          const int key0 = x ? info.z : info.x, exist = x ? info.w : info.y;
-          partly |= exist < q4::kBlock || key0 + q4::kBlock > d.all_hi || (key0 < d.all_lo && key0 + q4::kBlock > p.c.sinks);
+          info[x] = my.info[stage][x];
+          partly |= (info[x].y & kPartly) != 0;
         }
+        unsigned char* blocks = own + stage * L::kStage;
+        auto k_pairs = [&](int x) { return reinterpret_cast<uint32_t*>(blocks + x * L::kBlockBytes + 16 * hd); };
+        auto v_pairs = [&](int x) { return reinterpret_cast<uint32_t*>(blocks + x * L::kBlockBytes + 18 * hd); };
         if (partly) {  // rows that are no keys hold anything, and what no row sees shall not choose the values' type either
-          for (int i = lane; i < kItem * 16 * GROUPS; i += 32) {
-            const int x = i / (16 * GROUPS), j = i / GROUPS % 16, key = (x ? info.z : info.x) + j;
-            if (j >= (x ? info.w : info.y) || (key >= p.c.sinks && key < d.from))
-              k_pairs(x)[i % (16 * GROUPS)] = v_pairs(x)[i % (16 * GROUPS)] = 0;
-          }
+#pragma unroll
+          for (int x = 0; x < kItem; ++x)
+#pragma unroll 1
+            for (int i = lane; i < 16 * GROUPS; i += 32) {
+              const int j = i / GROUPS, key = info[x].x + j;
+              if (j >= (info[x].y & (kPartly - 1)) || (key >= p.c.sinks && key < d.from)) k_pairs(x)[i] = v_pairs(x)[i] = 0;
+            }
           __syncwarp();
         }
         // Pairs: none of the keys' may count as one that is not finite; the values' go to where the lanes that need them read
         // them, two keys' s and m beside each other.
-        bool half = true;
         {
           const int g = lane / 8 % GROUPS, t = lane % 4, h = lane / 4 % 2;  // a group, and the keys of scores' rows 2 t + 8 h, + 1
           const int row = 2 * t + (t & 1) + 8 * h;
-          bool k_none = false;
-          uint32_t a[kItem], b[kItem];
+          uint32_t none = 0, over = 0, a[kItem][2];
+          bool holds = true;
 #pragma unroll
           for (int x = 0; x < kItem; ++x) {
             const uint2 k2 = GROUPS == 4 ? reinterpret_cast<const uint2*>(k_pairs(x))[lane] : make_uint2(k_pairs(x)[lane], 0);
-            k_none |= q4::pair_is_none(k2.x) || q4::pair_is_none(k2.y);
-            a[x] = v_pairs(x)[row * GROUPS + g];
-            b[x] = v_pairs(x)[(row ^ 1) * GROUPS + g];
-            half &= half_holds(a[x]) && half_holds(b[x]);
+            none |= ((k2.x & 0x7fff7fffu) + 0x0e800e80u) | ((k2.y & 0x7fff7fffu) + 0x0e800e80u);  // as pair_is_none()
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              a[x][k] = v_pairs(x)[(row ^ k) * GROUPS + g];
+              half_holds(a[x][k], over, holds);
+            }
           }
-          half = __all_sync(0xffffffffu, half);
+          if (HALF && !__all_sync(0xffffffffu, holds && (over & 0x80008000u) == 0)) return item;
 #pragma unroll
           for (int x = 0; x < kItem; ++x) {
-            uint2 w;
-            if (half) {
-              w = make_uint2(pack<true>(low_of(a[x]), low_of(b[x])), pack<true>(high_of(a[x]), high_of(b[x])));
-            } else {
-              if (q4::pair_is_none(a[x])) a[x] = 0;
-              if (q4::pair_is_none(b[x])) b[x] = 0;
-              w = make_uint2(__byte_perm(a[x], b[x], 0x5410), __byte_perm(a[x], b[x], 0x7632));
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              if (!HALF && q4::pair_is_none(a[x][k])) a[x][k] = 0;
+            const float by = HALF ? 1.f : 0x1p-24f;
+            if (lane < 8 * GROUPS) {
+              s_out[x * 8 * GROUPS + (t * 2 + h) * GROUPS + g] = pack<HALF>(low_of(a[x][0]) * by, low_of(a[x][1]) * by);
+              m_out[x * 8 * GROUPS + (g * 4 + t) * 2 + h] = pack<HALF>(high_of(a[x][0]) * 0x1p8f, high_of(a[x][1]) * 0x1p8f);
             }
-            if (lane < 8 * GROUPS) *reinterpret_cast<uint2*>(pairs_out + ((x * GROUPS + g) * 4 + t) * 4 + 2 * h) = w;
           }
-          if (__any_sync(0xffffffffu, k_none)) {
+          if (__any_sync(0xffffffffu, (none & 0x80008000u) != 0)) {
 #pragma unroll
             for (int x = 0; x < kItem; ++x)
               for (int i = lane; i < 16 * GROUPS; i += 32)
                 if (q4::pair_is_none(k_pairs(x)[i])) k_pairs(x)[i] = 0;
-            }
+          }
           __syncwarp();
         }
-        auto body = [&](auto type) {
-          constexpr bool HALF = decltype(type)::value;
+        {
           // ---- scores
           float s[kItem][NT][4];
 #pragma unroll
@@ -605,23 +664,26 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
             }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {  // the pairs with the queries' sums
-              mma_new(s[x][nt], mine[0], mine[1], mine[0], mine[1], qs[nt][0], qs[nt][1]);
-              mma<false>(s[x][nt], mine[0], mine[1], 0u, 0u, qs[nt][2], 0u);
+              mma8_new(s[x][nt], mine[0], mine[1], qs[nt][0]);
+              mma8(s[x][nt], mine[0], mine[1], qs[nt][1]);
+              mma8(s[x][nt], mine[0], mine[1], qs[nt][2]);
             }
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
-              uint32_t a[2][4];  // 128 + c
+              // a code in the lowest 4 bits of an fp16 is c 2^-24, one 4 bits higher c 2^-20: no constant to join it to
+              uint32_t a[2][4];
 #pragma unroll
-              for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) a[h][i] = masked_or(w[h][g] >> (4 * i), low4, 0x43004300u);
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t upper = w[h][g] >> 8;
+                a[h][0] = w[h][g] & low4, a[h][1] = w[h][g] & high4, a[h][2] = upper & low4, a[h][3] = upper & high4;
+              }
               const float s0 = low_of(pr[0][g]), s1 = low_of(pr[1][g]);
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 float dot[4];
-                const uint4 f = L::kKeep ? q[g] : fragment(nt, g);
+                const uint4 f = L::kKeep ? q[nt][g] : *reinterpret_cast<const uint4*>(q_rows + (8 * nt + gid) * hd * 2 + (32 * g + 8 * t4) * 2);
                 mma_new(dot, a[0][0], a[1][0], a[0][1], a[1][1], f.x, f.y);
-                mma<false>(dot, a[0][2], a[1][2], a[0][3], a[1][3], f.z, f.w);
+                mma<true>(dot, a[0][2], a[1][2], a[0][3], a[1][3], f.z, f.w);
                 s[x][nt][0] = fmaf(s0, dot[0], s[x][nt][0]);
                 s[x][nt][1] = fmaf(s0, dot[1], s[x][nt][1]);
                 s[x][nt][2] = fmaf(s1, dot[2], s[x][nt][2]);
@@ -641,8 +703,8 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
                 for (int x = 0; x < kItem; ++x)
 #pragma unroll
                   for (int h = 0; h < 2; ++h) {
-                    const int j = key_row + 8 * h, key = (x ? info.z : info.x) + j;
-                    if (j >= (x ? info.w : info.y) || key >= hi || (key < lo && key >= p.c.sinks)) s[x][nt][2 * h + e] = -INFINITY;
+                    const int j = key_row + 8 * h, key = info[x].x + j;
+                    if (j >= (info[x].y & (kPartly - 1)) || key >= hi || (key < lo && key >= p.c.sinks)) s[x][nt][2 * h + e] = -INFINITY;
                   }
               }
           }
@@ -655,7 +717,7 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
             for (int i = 0; i < 4; ++i)
 #pragma unroll
               for (int x = 0; x < kItem; ++x) {
-                e[x][nt][i] = fmaf(s[x][nt][i], p.c.scale_log2, kShift - m[nt][i % 2]);
+                e[x][nt][i] = fmaf(s[x][nt][i], scale[nt][i % 2], kShift - m[nt][i % 2]);
                 above |= e[x][nt][i] > kShift;
               }
           if (__any_sync(0xffffffffu, above)) {
@@ -663,13 +725,16 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int r = 0; r < 2; ++r) {
-                float top = fmaxf(fmaxf(s[0][nt][r], s[0][nt][2 + r]), fmaxf(s[1][nt][r], s[1][nt][2 + r])) * p.c.scale_log2;
+                float top = fmaxf(s[0][nt][r], s[0][nt][2 + r]);
+#pragma unroll
+                for (int x = 1; x < kItem; ++x) top = fmaxf(top, fmaxf(s[x][nt][r], s[x][nt][2 + r]));
+                top *= scale[nt][r];
 #pragma unroll
                 for (int w = 4; w < 32; w *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
                 if (top > m[nt][r]) {  // of a row: all its lanes
                   const float corr = ex2(m[nt][r] - (top + kAbove));
                   m[nt][r] = top + kAbove;
-                  l[nt][r] *= corr;
+                  om[nt][r] *= corr;
 #pragma unroll
                   for (int i = 0; i < 2 * GROUPS; ++i) {
                     o[nt][i][r] *= corr;
@@ -679,7 +744,7 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
 #pragma unroll
                 for (int x = 0; x < kItem; ++x)
 #pragma unroll
-                  for (int h = 0; h < 2; ++h) e[x][nt][2 * h + r] = fmaf(s[x][nt][2 * h + r], p.c.scale_log2, kShift - m[nt][r]);
+                  for (int h = 0; h < 2; ++h) e[x][nt][2 * h + r] = fmaf(s[x][nt][2 * h + r], scale[nt][r], kShift - m[nt][r]);
               }
           }
           uint32_t pb[kItem][NT][2];
@@ -689,207 +754,189 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) e[x][nt][i] = ex2(e[x][nt][i]);
-              l[nt][0] += e[x][nt][0] + e[x][nt][2];
-              l[nt][1] += e[x][nt][1] + e[x][nt][3];
               pb[x][nt][0] = transpose8(pack<HALF>(e[x][nt][0], e[x][nt][1]));
               pb[x][nt][1] = transpose8(pack<HALF>(e[x][nt][2], e[x][nt][3]));
             }
-          // ---- values
+          // ---- values: a product's 16 rows are elements of one group, so that s goes onto the weights, two at a time, and the
+          // codes are the operand as they are. Lanes of gid 0-3 take nibbles 0-3 of word gid of the group, those of gid 4-7 nibbles
+          // 4-7 of word gid - 4.
 #pragma unroll
           for (int x = 0; x < kItem; ++x) {
-            constexpr int W = GROUPS / 2;  // words of a key here
-            uint32_t w[4][W];
-            uint4 sm[W];  // s and m of the keys of rows 2 t4, + 1, and of those 8 on
+            uint32_t w[4][GROUPS], s2[2][GROUPS], ma[2];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const int row = (k % 2 ? vb : va) + 8 * (k / 2);
-              const unsigned char* from = blocks + x * L::kBlockBytes + 8 * hd + row * (hd / 2) + gid * W * 4;
-              if constexpr (W == 2) *reinterpret_cast<uint2*>(w[k]) = *reinterpret_cast<const uint2*>(from);
-              else w[k][0] = *reinterpret_cast<const uint32_t*>(from);
+              const unsigned char* from = blocks + x * L::kBlockBytes + 8 * hd + row * (hd / 2) + gid % 4 * GROUPS * 4;
+              if constexpr (GROUPS == 4) *reinterpret_cast<uint4*>(w[k]) = *reinterpret_cast<const uint4*>(from);
+              else *reinterpret_cast<uint2*>(w[k]) = *reinterpret_cast<const uint2*>(from);
             }
 #pragma unroll
-            for (int i = 0; i < W; ++i)
-              sm[i] = *reinterpret_cast<const uint4*>(pairs_out + ((x * GROUPS + (gid * W) % GROUPS + i) * 4 + t4) * 4);
-            // codes of two keys beside each other: nibbles 0-3 and 4-7 of each word
-            uint32_t part[2][W][2];
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t* from = s_out + x * 8 * GROUPS + (t4 * 2 + h) * GROUPS;
+              if constexpr (GROUPS == 4) *reinterpret_cast<uint4*>(s2[h]) = *reinterpret_cast<const uint4*>(from);
+              else *reinterpret_cast<uint2*>(s2[h]) = *reinterpret_cast<const uint2*>(from);
+            }
+            {
+              const uint2 both = *reinterpret_cast<const uint2*>(m_out + x * 8 * GROUPS + (gid % GROUPS * 4 + t4) * 2);
+              const uint32_t one = HALF ? 0x3c003c00u : 0x3f803f80u;
+              ma[0] = gid < GROUPS ? both.x : gid == 4 ? one : 0u;
+              ma[1] = gid < GROUPS ? both.y : gid == 4 ? one : 0u;
+            }
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int nt = 0; nt < NT; ++nt) mma<HALF>(om[nt], ma[0], 0u, ma[1], 0u, pb[x][nt][0], pb[x][nt][1]);
 #pragma unroll
-              for (int i = 0; i < W; ++i) {
-                part[h][i][0] = __byte_perm(w[2 * h][i], w[2 * h + 1][i], 0x5410);
-                part[h][i][1] = __byte_perm(w[2 * h][i], w[2 * h + 1][i], 0x7632);
+            for (int g = 0; g < GROUPS; ++g) {
+              uint32_t a[2][4];  // codes of rows' keys 2 t4, + 1 (and 8 on), of a lane's four nibbles
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t y = __byte_perm(w[2 * h][g], w[2 * h + 1][g], halves);
+                if constexpr (HALF) {
+                  const uint32_t upper = y >> 8;
+                  a[h][0] = y & low4, a[h][1] = y & high4, a[h][2] = upper & low4, a[h][3] = upper & high4;
+                } else {
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {  // s c 2^-24, or 2^-20
+                    const uint32_t c = ((y >> (4 * i)) & 0x000f000fu) | 0x43004300u, k128 = 0x43004300u, k16 = 0x41804180u;
+                    __nv_bfloat162 v = __hmul2(__hsub2(q4::as_bf162(c), q4::as_bf162(k128)), q4::as_bf162(s2[h][g]));
+                    a[h][i] = q4::as_word(i % 2 ? __hmul2(v, q4::as_bf162(k16)) : v);
+                  }
+                }
               }
-            auto value = [&](uint32_t codes, int nibble, uint32_t sc, uint32_t mn) {
-              if constexpr (HALF) {
-                // the even nibbles as 1024 + c, the odd ones, 4 bits higher in the significand, as 64 + c
-                const uint32_t y = nibble >= 2 ? codes >> 8 : codes, zero = nibble % 2 ? 0x54005400u : 0x64006400u;
-                const uint32_t c = masked_or(y, nibble % 2 ? high4 : low4, zero);
-                const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), *reinterpret_cast<const __half2*>(&zero)),
-                                          *reinterpret_cast<const __half2*>(&sc), *reinterpret_cast<const __half2*>(&mn));
-                return *reinterpret_cast<const uint32_t*>(&v);
-              } else {
-                return q4::stands_for(((codes >> (4 * nibble)) & 0x000f000fu) | 0x43004300u, sc, mn);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                uint32_t b[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  b[h] = pb[x][nt][h];
+                  if constexpr (HALF) {
+                    const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&b[h]), *reinterpret_cast<const __half2*>(&s2[h][g]));
+                    b[h] = *reinterpret_cast<const uint32_t*>(&v);
+                  }
+                }
+                mma<HALF>(o[nt][2 * g], a[0][0], a[0][1], a[1][0], a[1][1], b[0], b[1]);
+                mma<HALF>(o[nt][2 * g + 1], a[0][2], a[0][3], a[1][2], a[1][3], b[0], b[1]);
               }
-            };
-#pragma unroll
-            for (int i = 0; i < 2 * GROUPS; ++i) {
-              // rows gid and gid + 8 of the product: nibble i of the lane's two words, or nibbles i and i + 4 of its one
-              const int x1 = W - 1, n1 = W == 2 ? i : i + 4;
-              const uint32_t a0 = value(part[0][0][i / 4], i % 4, sm[0].x, sm[0].y);
-              const uint32_t a1 = value(part[0][x1][n1 / 4], n1 % 4, sm[x1].x, sm[x1].y);
-              const uint32_t a2 = value(part[1][0][i / 4], i % 4, sm[0].z, sm[0].w);
-              const uint32_t a3 = value(part[1][x1][n1 / 4], n1 % 4, sm[x1].z, sm[x1].w);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma<HALF>(o[nt][i], a0, a1, a2, a3, pb[x][nt][0], pb[x][nt][1]);
             }
           }
-        };
-        if (half) body(std::true_type{});
-        else body(std::false_type{});
+        }
         __syncwarp();
         ++computed;
-      }
-      // ---- the unit's part: a lane has words' 8 elements of rows 2 t4, + 1: of two words, or one
-      constexpr int W = GROUPS / 2;
-      auto element = [&](int nt, int word, int r, int e) -> float& {  // element e lies in nibble e / 2 + 4 (e % 2)
-        const int nibble = e / 2 + 4 * (e % 2);
-        return W == 2 ? o[nt][nibble][2 * word + r] : o[nt][nibble % 4][2 * (nibble / 4) + r];
+        }
+        return item;
       };
+      const int held_items = run(std::true_type{}, 0);
+      if (held_items < d.items) run(std::false_type{}, held_items);
+      // ---- the unit's part: every second element of a word is on lane gid, the others on lane gid ^ 4; each takes 4 in a row
+      const bool upper_half = gid >= 4;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          float sum = l[nt][r];
+          const float sum = __shfl_sync(0xffffffffu, om[nt][r], 16 + t4);
+          float y[GROUPS][4];
 #pragma unroll
-          for (int w = 4; w < 32; w *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+          for (int g = 0; g < GROUPS; ++g) {
+            const float mg = __shfl_sync(0xffffffffu, om[nt][r], 4 * g + t4) * 0x1p-8f;
+            float x[4] = {fmaf(o[nt][2 * g][r], 0x1p24f, mg), fmaf(o[nt][2 * g][2 + r], 0x1p20f, mg),
+                          fmaf(o[nt][2 * g + 1][r], 0x1p24f, mg), fmaf(o[nt][2 * g + 1][2 + r], 0x1p20f, mg)};
+            const float z0 = __shfl_xor_sync(0xffffffffu, upper_half ? x[0] : x[2], 16);
+            const float z1 = __shfl_xor_sync(0xffffffffu, upper_half ? x[1] : x[3], 16);
+            y[g][0] = upper_half ? z0 : x[0], y[g][1] = upper_half ? x[2] : z0;
+            y[g][2] = upper_half ? z1 : x[1], y[g][3] = upper_half ? x[3] : z1;
+          }
           const int row = 8 * nt + 2 * t4 + r;
           if (row >= d.rows) continue;
+          const int dim = 8 * (gid % 4) + 4 * (gid / 4);  // of a group
           if (d.parts == 1) {
             const int64_t token = d.token0 + row / p.G;
             const int head = d.kvh * p.G + row % p.G;
             float f = sum == 0.f ? 0.f : 1.f / sum;
             if (p.c.gate && sum != 0.f) f *= sigmoid(p.c.gate[token * p.c.gate_stride + head]);
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-              const int word = gid * W + i;  // of dims 32 (word % GROUPS) + 8 (word / GROUPS) on
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = sum == 0.f ? 0u : pack<false>(element(nt, i, r, 2 * e) * f, element(nt, i, r, 2 * e + 1) * f);
-              *reinterpret_cast<uint4*>(p.c.out + token * p.c.out_stride + (int64_t)head * hd + 32 * (word % GROUPS) +
-                                        8 * (word / GROUPS)) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            for (int g = 0; g < GROUPS; ++g)
+              *reinterpret_cast<uint2*>(p.c.out + token * p.c.out_stride + (int64_t)head * hd + 32 * g + dim) =
+                  sum == 0.f ? make_uint2(0u, 0u) : make_uint2(pack<false>(y[g][0] * f, y[g][1] * f), pack<false>(y[g][2] * f, y[g][3] * f));
             if (p.c.lse && gid == 0)
               p.c.lse[token * p.c.Hq + head] = sum == 0.f ? -INFINITY : (m[nt][r] - kShift + log2f(sum)) * 0.6931471805599453f;
           } else {
-            const int64_t part = part_slot(d.first, d.index);
+            const unsigned at = part_slot(d.first, d.index) * L::kRows + row;  // parts of a call fit 2^31 floats
+            float* to = p.acc + at * hd + dim;
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-              const int word = gid * W + i;
-              float* to = p.acc + (part * p.c.rows + row) * hd + 32 * (word % GROUPS) + 8 * (word / GROUPS);
-              __stcg(reinterpret_cast<float4*>(to), make_float4(element(nt, i, r, 0), element(nt, i, r, 1), element(nt, i, r, 2), element(nt, i, r, 3)));
-              __stcg(reinterpret_cast<float4*>(to) + 1, make_float4(element(nt, i, r, 4), element(nt, i, r, 5), element(nt, i, r, 6), element(nt, i, r, 7)));
-            }
-            if (gid == 0) {
-              __stcg(p.ml + part * 2 * p.c.rows + row, sum == 0.f ? kNone : m[nt][r]);
-              __stcg(p.ml + (part * 2 + 1) * p.c.rows + row, sum);
-            }
+            for (int g = 0; g < GROUPS; ++g)
+              __stcg(reinterpret_cast<float4*>(to + 32 * g), make_float4(y[g][0], y[g][1], y[g][2], y[g][3]));
+            if (gid == 0) __stcg(p.ml + at, make_float2(sum == 0.f ? kNone : m[nt][r], sum));
           }
         }
       // ---- parts that are all there are joined, 16 neighbours at a time: into the first one's slot, or to the output
       int index = d.index, parts = d.parts, stride = 1, level = 0;
 #pragma unroll 1
       while (parts > 1) {
-        __threadfence();
         __syncwarp();
         const int leader = index / kJoin * kJoin, count = min(kJoin, parts - leader);  // in units of `stride` parts
         int last = 0;
         if (lane == 0) {
           // the warps between two first ones are inside the unit: theirs are free for the joins of joined parts
           unsigned* counter = p.counters + ((int64_t)(d.first + leader * stride + level) * 2 + (leader != 0));
-          unsigned old = *reinterpret_cast<volatile unsigned*>(counter), seen, arrived;
-          do {
-            seen = old;
-            arrived = (seen >> 12 == p.tag ? seen & 0xfffu : 0u) + 1;
-            old = atomicCAS(counter, seen, arrived == (unsigned)count ? 0u : p.tag << 12 | arrived);
-          } while (old != seen);
-          last = arrived == (unsigned)count;
-          __threadfence();
+          fence_gpu();  // the warp's part, behind the barrier above, comes before its arrival
+          last = atomicAdd(counter, 1u) + 1 == (unsigned)count;
+          if (last) *counter = 0;
+          if (last) fence_gpu();
         }
         last = __shfl_sync(0xffffffffu, last, 0);
         if (!last) break;
         const bool final = parts <= kJoin;
-        constexpr int kQuads = hd / 4, kTogether = 4, kAtOnce = 2;  // of a lane: rows' pieces, parts whose loads are in flight
-        const int64_t to = part_slot(d.first, leader * stride);
+        // A lane takes 4 elements of a row at a time, 8 parts' loads in flight together.
+        constexpr int kQuads = hd / 4, kTogether = 8;
+        const unsigned first_at = part_slot(d.first, leader * stride) * L::kRows;
+        const unsigned step = (unsigned)stride * 2 * L::kRows, back = leader == 0 ? L::kRows : 0;  // a unit's first part is in a second slot
 #pragma unroll 1
-        for (int x0 = lane; x0 < d.rows * kQuads; x0 += 32 * kAtOnce) {
-          float top[kAtOnce], sum[kAtOnce], y[kAtOnce][4];
-#pragma unroll
-          for (int a = 0; a < kAtOnce; ++a) {
-            top[a] = kNone;
-            sum[a] = y[a][0] = y[a][1] = y[a][2] = y[a][3] = 0.f;
-          }
+        for (int x0 = 0; x0 < d.rows * kQuads; x0 += 32) {
+          const int x = x0 + lane, row = x / kQuads, quad = x % kQuads;
+          const bool live = row < d.rows;
+          const unsigned at = first_at + (live ? row : 0);
+          float top = kNone, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
           for (int i0 = 0; i0 < count; i0 += kTogether) {
-            float pm[kAtOnce][kTogether], pl[kAtOnce][kTogether];
-            float4 v[kAtOnce][kTogether];
+            float2 ml[kTogether];
+            float4 v[kTogether];
 #pragma unroll
-            for (int a = 0; a < kAtOnce; ++a)
+            for (int k = 0; k < kTogether; ++k) {
+              const int i = i0 + k;
+              const unsigned from = i < count ? at + i * step - (i > 0 ? back : 0) : at;
+              ml[k] = __ldcg(p.ml + from);
+              v[k] = __ldcg(reinterpret_cast<const float4*>(p.acc + from * hd) + quad);
+              if (i >= count) ml[k] = make_float2(kNone, 0.f);
+            }
+            float high = top;
 #pragma unroll
-              for (int k = 0; k < kTogether; ++k) {
-                const int x = x0 + 32 * a, row = x / kQuads, quad = x % kQuads;
-                const bool there = i0 + k < count && row < d.rows;
-                const int64_t part = part_slot(d.first, (leader + (there ? i0 + k : 0)) * stride);
-                pm[a][k] = there ? __ldcg(p.ml + part * 2 * p.c.rows + row) : kNone;
-                pl[a][k] = there ? __ldcg(p.ml + (part * 2 + 1) * p.c.rows + row) : 0.f;
-                v[a][k] = there ? __ldcg(reinterpret_cast<const float4*>(p.acc + (part * p.c.rows + row) * hd + quad * 4))
-                                : make_float4(0.f, 0.f, 0.f, 0.f);
-              }
+            for (int k = 0; k < kTogether; ++k) high = fmaxf(high, ml[k].x);
+            const float before = ex2(top - high);
+            top = high;
+            sum *= before;
 #pragma unroll
-            for (int a = 0; a < kAtOnce; ++a) {
-              float high = top[a];
+            for (int e = 0; e < 4; ++e) y[e] *= before;
 #pragma unroll
-              for (int k = 0; k < kTogether; ++k) high = fmaxf(high, pm[a][k]);
-              const float before = ex2(top[a] - high);
-              top[a] = high;
-              sum[a] *= before;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) y[a][e] *= before;
-#pragma unroll
-              for (int k = 0; k < kTogether; ++k) {
-                const float f = ex2(pm[a][k] - high);
-                sum[a] = fmaf(pl[a][k], f, sum[a]);
-                y[a][0] = fmaf(v[a][k].x, f, y[a][0]), y[a][1] = fmaf(v[a][k].y, f, y[a][1]);
-                y[a][2] = fmaf(v[a][k].z, f, y[a][2]), y[a][3] = fmaf(v[a][k].w, f, y[a][3]);
-              }
+            for (int k = 0; k < kTogether; ++k) {
+              const float f = i0 + k < count ? ex2(ml[k].x - high) : 0.f;
+              sum = fmaf(ml[k].y, f, sum);
+              y[0] = fmaf(v[k].x, f, y[0]), y[1] = fmaf(v[k].y, f, y[1]);
+              y[2] = fmaf(v[k].z, f, y[2]), y[3] = fmaf(v[k].w, f, y[3]);
             }
           }
-          // (the first part's m and sum are rewritten only when every lane has read them)
-          if (!final) __syncwarp();
-#pragma unroll
-          for (int a = 0; a < kAtOnce; ++a) {
-            const int x = x0 + 32 * a, row = x / kQuads, quad = x % kQuads;
-            if (row >= d.rows) continue;
-            if (final) {
-              const int64_t token = d.token0 + row / p.G;
-              const int head = d.kvh * p.G + row % p.G;
-              float f = sum[a] == 0.f ? 0.f : 1.f / sum[a];
-              if (p.c.gate && sum[a] != 0.f) f *= sigmoid(p.c.gate[token * p.c.gate_stride + head]);
-              uint2 w;
-              w.x = sum[a] == 0.f ? 0u : pack<false>(y[a][0] * f, y[a][1] * f);
-              w.y = sum[a] == 0.f ? 0u : pack<false>(y[a][2] * f, y[a][3] * f);
-              *reinterpret_cast<uint2*>(p.c.out + token * p.c.out_stride + (int64_t)head * hd + quad * 4) = w;
-              if (p.c.lse && quad == 0)
-                p.c.lse[token * p.c.Hq + head] = sum[a] == 0.f ? -INFINITY : (top[a] - kShift + log2f(sum[a])) * 0.6931471805599453f;
-            } else {
-              __stcg(reinterpret_cast<float4*>(p.acc + (to * p.c.rows + row) * hd + quad * 4), make_float4(y[a][0], y[a][1], y[a][2], y[a][3]));
-              if (quad == 0) {
-                __stcg(p.ml + to * 2 * p.c.rows + row, top[a]);
-                __stcg(p.ml + (to * 2 + 1) * p.c.rows + row, sum[a]);
-              }
-            }
+          if (!final) __syncwarp();  // a row's first m and sum are rewritten when every lane has read them
+          if (live && final) {
+            const int64_t token = d.token0 + row / p.G;
+            const int head = d.kvh * p.G + row % p.G;
+            float f = sum == 0.f ? 0.f : 1.f / sum;
+            if (p.c.gate && sum != 0.f) f *= sigmoid(p.c.gate[token * p.c.gate_stride + head]);
+            *reinterpret_cast<uint2*>(p.c.out + token * p.c.out_stride + (int64_t)head * hd + quad * 4) =
+                sum == 0.f ? make_uint2(0u, 0u) : make_uint2(pack<false>(y[0] * f, y[1] * f), pack<false>(y[2] * f, y[3] * f));
+            if (p.c.lse && quad == 0)
+              p.c.lse[token * p.c.Hq + head] = sum == 0.f ? -INFINITY : (top - kShift + log2f(sum)) * 0.6931471805599453f;
+          } else if (live) {
+            __stcg(reinterpret_cast<float4*>(p.acc + at * hd) + quad, make_float4(y[0], y[1], y[2], y[3]));
+            if (quad == 0) __stcg(p.ml + at, make_float2(top, sum));
           }
-          if (!final) __syncwarp();
         }
         index = leader / kJoin;
         parts = (parts + kJoin - 1) / kJoin;
@@ -930,6 +977,7 @@ int launch(FewParams& p, int ctas, cudaStream_t stream) {
   using L = Shape<GROUPS, NT>;
   auto kernel = gqa_few_q4_kernel<GROUPS, NT>;
   constexpr int kSmem = L::kWarps * L::kPerWarp + (int)sizeof(Tail);
+  static_assert(sizeof(Round) <= L::kOffQ && L::kThreads <= 256, "a round of requests");
   static_assert((kSmem + 1024) * L::kCtas <= 228 * 1024, "shared memory");
   static bool configured[64] = {false};  // the shared-memory attribute, set once per device
   int dev = 0;
@@ -943,7 +991,7 @@ int launch(FewParams& p, int ctas, cudaStream_t stream) {
   return zb::check_launch("gqa_chunk_q4");
 }
 
-int warps_of(int rows) { return rows <= 8 ? 8 : 6; }
+int warps_of(int rows) { return rows <= 8 ? Shape<4, 1>::kWarps : Shape<4, 2>::kWarps; }
 
 }  // namespace
 
@@ -973,12 +1021,9 @@ int launch_few(const FewCall& call, cudaStream_t stream) {
   p.page_mul = (unsigned)((((uint64_t)1 << p.page_shift) + call.kv.page_size - 1) / call.kv.page_size);
   const int warps = warps_of(call.rows);
   const int ctas = ctas_of(call.kv.B, call.kv.N, call.kv.Hkv, (int64_t)call.kv.page_size * call.kv.max_pages, warps);
-  static std::atomic<unsigned> calls{0};
-  do p.tag = (calls.fetch_add(1, std::memory_order_relaxed) + 1) & 0xfffffu;
-  while (p.tag == 0);
   p.counters = reinterpret_cast<unsigned*>(call.workspace);
   p.acc = reinterpret_cast<float*>(call.workspace + kFewFlagBytes);
-  p.ml = p.acc + (int64_t)ctas * warps * 2 * call.rows * call.kv.hd;
+  p.ml = reinterpret_cast<float2*>(p.acc + (int64_t)ctas * warps * 2 * call.rows * call.kv.hd);
   p.status = device_status_ptr();
   if (call.kv.hd == 128) return call.rows == 8 ? launch<4, 1>(p, ctas, stream) : launch<4, 2>(p, ctas, stream);
   return call.rows == 8 ? launch<2, 1>(p, ctas, stream) : launch<2, 2>(p, ctas, stream);
