@@ -20,6 +20,10 @@ whatever its requests bring (prompts, chunks of prompts, single tokens), over a 
                                                              the pages of their requests)
     o = zb_gqa_chunk(q, caches, page_table, gate)           (causal attention over the pages, the gate in its store)
 
+Over a ``QuantKVPool``, pages that hold 4 bits an element, the same two as ``zb_gqa_append_q4`` and ``zb_gqa_chunk_q4``. With
+``config.attention_window`` > 0 (and ``attention_sinks`` first tokens that stay visible) the paged operators see that window; the
+other paths have none and refuse.
+
 The host reads no length there, so such a forward neither waits for the device nor loops over requests. A decode batch
 over a ``SlotKVPool`` that has ``positions`` and ``out_loc`` keeps the decode kernels, whatever its ``cu_seqlens_q`` is: at
 page size 1 they are the faster ones (256 requests of 1628 keys, 16 / 4 heads of 128: 155 us against 234).
@@ -76,6 +80,23 @@ class PagedKVPool:
         return self.v_buffer[self._index[layer_id]]
 
 
+class QuantKVPool:
+    """K and V of every global-attention layer in 4 bits, in pages of ``page_size`` tokens (a multiple of 16): ``[pages,
+    kv_heads, page_size / 16, 20 head_dim]`` bytes a layer (``ops.kv_q4_cache``; head dims 32, 64, 96 and 128), 0.31 of what
+    a ``PagedKVPool`` takes. A request's key position j lies in page ``page_table[b, j // page_size]``. Read and written by the
+    4-bit operators (batches whose ``cu_seqlens_q`` is a device tensor)."""
+
+    def __init__(self, layer_ids, pages: int, page_size: int, kv_heads: int, head_dim: int, device):
+        self.layer_ids = list(layer_ids)
+        self._index = {layer: i for i, layer in enumerate(self.layer_ids)}
+        layers = len(self.layer_ids)
+        self.buffer = ops.kv_q4_cache(layers * pages, page_size, kv_heads, head_dim, device).unflatten(0, (layers, pages))
+        self.pages, self.page_size = pages, page_size
+
+    def kv(self, layer_id: int) -> torch.Tensor:
+        return self.buffer[self._index[layer_id]]
+
+
 def rope_interleaved(x: torch.Tensor, positions: torch.Tensor, theta: float) -> torch.Tensor:
     """Interleaved-pair rotary embedding (is_neox=False): pair (2i, 2i+1) rotated by position * theta^(-2i/hd),
     in fp32, rounded to x's dtype."""
@@ -97,6 +118,8 @@ class Attention(BaseOP):
         self.head_dim = config.head_dim
         self._layer_id = layer_id
         self._theta = float(getattr(config, "rope_theta", 10000.0))
+        self._window = int(getattr(config, "attention_window", 0))
+        self._sinks = int(getattr(config, "attention_sinks", 0))
         D = config.hidden_size
         self.wq = Weight((self.num_heads * self.head_dim, D))
         self.wkv = Weight((2, self.num_kv_heads * self.head_dim, D))
@@ -124,18 +147,29 @@ class Attention(BaseOP):
                 raise RuntimeError("Attention.prepare() must run before graph capture")
             self.prepare()
         n, H, Hkv, hd = x.shape[0], self.num_heads, self.num_kv_heads, self.head_dim
-        kc, vc = pool.k(self._layer_id), pool.v(self._layer_id)
-        p = F.linear(x, self._proj)  # q | k | v | gate
-        gate = p[:, (H + 2 * Hkv) * hd:]
-        slots = kc.dim() == 3
         cu = meta.cu_seqlens_q
         on_device = isinstance(cu, torch.Tensor) and cu.is_cuda and cu.dtype == torch.int32
-        decode = slots and batch.is_decode and meta.positions is not None and meta.out_loc is not None
+        four_bits = isinstance(pool, QuantKVPool)
+        if (four_bits or self._window) and not on_device:
+            raise RuntimeError(("a 4-bit KV pool" if four_bits else "attention_window")
+                               + " needs attn_metadata.cu_seqlens_q as a device tensor (int32)")
+        p = F.linear(x, self._proj)  # q | k | v | gate
+        gate = p[:, (H + 2 * Hkv) * hd:]
+        if four_bits:
+            paged = (pool.kv(self._layer_id), meta.page_table, meta.cache_seqlens, cu)
+            q = ops.gqa_append_q4(p, *paged, heads=H, kv_heads=Hkv, temp=self._temp, eps=QK_NORM_EPS, rope_theta=self._theta,
+                                  positions=meta.positions)
+            o = ops.gqa_chunk_q4(q, *paged, softmax_scale=hd ** -0.5, window=self._window, sinks=self._sinks, gate=gate,
+                                 max_new=1 if batch.is_decode else None)
+            return F.linear(o.reshape(n, H * hd), self.wo.weight)
+        kc, vc = pool.k(self._layer_id), pool.v(self._layer_id)
+        slots = kc.dim() == 3
+        decode = slots and batch.is_decode and not self._window and meta.positions is not None and meta.out_loc is not None
         if on_device and not decode:  # a ragged batch described on the device
             paged = (kc, vc, meta.page_table, meta.cache_seqlens, meta.cu_seqlens_q)
             q = ops.gqa_append(p, *paged, heads=H, kv_heads=Hkv, temp=self._temp, eps=QK_NORM_EPS, rope_theta=self._theta,
                                positions=meta.positions)
-            o = ops.gqa_chunk(q, *paged, softmax_scale=hd ** -0.5, gate=gate)
+            o = ops.gqa_chunk(q, *paged, softmax_scale=hd ** -0.5, window=self._window, sinks=self._sinks, gate=gate)
         elif not slots:
             raise RuntimeError("a paged KV pool needs attn_metadata.cu_seqlens_q as a device tensor (int32)")
         elif batch.is_decode:  # the output gate rides in the attention kernel's store

@@ -33,6 +33,10 @@ class ModelConfig:
     num_kv_heads: int = 4
     head_dim: int = 128
     rope_theta: float = 10000.0
+    # of the global-attention layers: 0, or how many of the last keys a token sees, and how many of the first beside them
+    # (batches described on the device); the reference's layers see all
+    attention_window: int = 0
+    attention_sinks: int = 0
     intermediate_size: int = 0  # dense FFN width of the layers before moe_start_from_layer
     n_codebooks: int = 9
     codebook_size: int = 1024

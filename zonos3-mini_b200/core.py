@@ -62,7 +62,7 @@ class Batch:
 @dataclass
 class Context:
     batch: Batch | None = None
-    attn_backend: object = None  # attention.SlotKVPool of the model being run
+    attn_backend: object = None  # attention.SlotKVPool, PagedKVPool or QuantKVPool of the model being run
     extra: dict = field(default_factory=dict)
 
 

@@ -22,7 +22,7 @@
 // each), of which a warp takes an equal share (the split is as in gqa_chunk.cu, to warps instead of CTAs): it looks up the places of
 // its blocks, has the copies of the next item under way while it computes one, and keeps m, the sum and the accumulator of a unit in
 // its registers, where a lane has 8 consecutive elements of up to four rows' outputs. A unit that spans warps leaves a part of each
-// in the workspace; the warp that finishes the last of up to 16 neighbouring parts joins them in the order of their keys, and so on
+// in the workspace; the warp that finishes the last of up to 8 neighbouring parts joins them in the order of their keys, and so on
 // for the joined ones. No warp waits for another, and results do not depend on timing.
 //
 // Measured ways that were slower (256 tokens of 16 / 4 heads of 128 over 1628 keys): seven warps a CTA that share a unit's items, an eighth
@@ -40,7 +40,7 @@ constexpr int kItem = 2;      // blocks of an item
 constexpr int kStages = 2;    // items of a warp: one that is computed, and copies under way
 constexpr int kUnitCost = 4;  // of a unit, in items
 constexpr int kMinShare = 3;  // items of a warp, its units' cost among them
-constexpr int kJoin = 16;     // parts that are joined at once
+constexpr int kJoin = 8;      // parts that are joined at once
 constexpr float kAbove = 8.f, kShift = 15.f;
 constexpr float kNone = -3.0e38f;  // m of a row that has seen no key
 
@@ -91,8 +91,9 @@ struct Shape {
   static constexpr int kOffPairs = kOffQ + kRows * kHd * 2;  // pairs of values, as the lanes need them
   static constexpr int kOffOwn = kOffPairs + kItem * GROUPS * 64;
   static constexpr int kPerWarp = (kOffOwn + (int)sizeof(Own) + 127) / 128 * 128;
-  // 16 warps an SM have 128 registers a thread; with 16 rows the accumulators alone are 64, so 12 have 168
-  static constexpr int kWarps = NT == 1 ? 8 : 6, kCtas = 2, kThreads = 32 * kWarps;
+  // 12 warps an SM have 168 registers a thread. 16 with 128 keep some in memory: 71 us against 72 for 256 tokens over 1628 keys,
+  // but 40 against 36 for 2 over 65001.
+  static constexpr int kWarps = 6, kCtas = 2, kThreads = 32 * kWarps;
   // The queries' fragments stay in registers, or are read again for every block where the accumulators take those.
   static constexpr bool kKeep = NT == 1;
 };
@@ -488,7 +489,7 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
     while (true) {
       if (opened == done) open_unit();
       if (opened == done) break;
-      const Desc d = my.desc[done % 2];
+      const Desc& d = my.desc[done % 2];  // not held in registers through the items
       // The copies of the item to be computed, and with them those of its unit's queries.
       auto arrived = [&]() {
         const int behind = fetched - computed - 1;
@@ -580,8 +581,9 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
       // the choice inside one, the accumulators changed places between its branches.)
       auto run = [&](auto type, int item) {
         constexpr bool HALF = decltype(type)::value;
+        const int items = d.items;
 #pragma unroll 1
-        for (; item < d.items; ++item) {
+        for (; item < items; ++item) {
 #pragma unroll 1
         for (int k = fetched - computed; k < kStages; ++k) fetch();
         const int stage = computed % kStages;
@@ -867,7 +869,7 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
             if (gid == 0) __stcg(p.ml + at, make_float2(sum == 0.f ? kNone : m[nt][r], sum));
           }
         }
-      // ---- parts that are all there are joined, 16 neighbours at a time: into the first one's slot, or to the output
+      // ---- parts that are all there are joined, 8 neighbours at a time: into the first one's slot, or to the output
       int index = d.index, parts = d.parts, stride = 1, level = 0;
 #pragma unroll 1
       while (parts > 1) {
@@ -885,58 +887,75 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
         last = __shfl_sync(0xffffffffu, last, 0);
         if (!last) break;
         const bool final = parts <= kJoin;
-        // A lane takes 4 elements of a row at a time, 8 parts' loads in flight together.
-        constexpr int kQuads = hd / 4, kTogether = 8;
+        // What it takes is round trips to L2, of about a microsecond: 4 pieces of 4 elements a lane (4 rows of 128) of 4 parts are
+        // loaded together.
+        constexpr int kQuads = hd / 4, kPieces = 4, kTogether = 4;
         const unsigned first_at = part_slot(d.first, leader * stride) * L::kRows;
         const unsigned step = (unsigned)stride * 2 * L::kRows, back = leader == 0 ? L::kRows : 0;  // a unit's first part is in a second slot
 #pragma unroll 1
-        for (int x0 = 0; x0 < d.rows * kQuads; x0 += 32) {
-          const int x = x0 + lane, row = x / kQuads, quad = x % kQuads;
-          const bool live = row < d.rows;
-          const unsigned at = first_at + (live ? row : 0);
-          float top = kNone, sum = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int x0 = lane; x0 < d.rows * kQuads; x0 += 32 * kPieces) {
+          float top[kPieces], sum[kPieces], y[kPieces][4];
+          unsigned at[kPieces];
+#pragma unroll
+          for (int a = 0; a < kPieces; ++a) {
+            const int row = (x0 + 32 * a) / kQuads;
+            at[a] = first_at + (row < d.rows ? row : 0);
+            top[a] = kNone;
+            sum[a] = y[a][0] = y[a][1] = y[a][2] = y[a][3] = 0.f;
+          }
 #pragma unroll 1
           for (int i0 = 0; i0 < count; i0 += kTogether) {
-            float2 ml[kTogether];
-            float4 v[kTogether];
+            float2 ml[kPieces][kTogether];
+            float4 v[kPieces][kTogether];
 #pragma unroll
             for (int k = 0; k < kTogether; ++k) {
-              const int i = i0 + k;
-              const unsigned from = i < count ? at + i * step - (i > 0 ? back : 0) : at;
-              ml[k] = __ldcg(p.ml + from);
-              v[k] = __ldcg(reinterpret_cast<const float4*>(p.acc + from * hd) + quad);
-              if (i >= count) ml[k] = make_float2(kNone, 0.f);
+              const int i = min(i0 + k, count - 1);
+              const unsigned further = i * step - (i > 0 ? back : 0);
+#pragma unroll
+              for (int a = 0; a < kPieces; ++a) {
+                ml[a][k] = __ldcg(p.ml + at[a] + further);
+                v[a][k] = __ldcg(reinterpret_cast<const float4*>(p.acc + (at[a] + further) * hd) + x0 % kQuads);
+              }
             }
-            float high = top;
 #pragma unroll
-            for (int k = 0; k < kTogether; ++k) high = fmaxf(high, ml[k].x);
-            const float before = ex2(top - high);
-            top = high;
-            sum *= before;
+            for (int a = 0; a < kPieces; ++a) {
+              float high = top[a];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] *= before;
+              for (int k = 0; k < kTogether; ++k) high = fmaxf(high, ml[a][k].x);  // the last part again where there are none left
+              const float before = ex2(top[a] - high);
+              top[a] = high;
+              sum[a] *= before;
 #pragma unroll
-            for (int k = 0; k < kTogether; ++k) {
-              const float f = i0 + k < count ? ex2(ml[k].x - high) : 0.f;
-              sum = fmaf(ml[k].y, f, sum);
-              y[0] = fmaf(v[k].x, f, y[0]), y[1] = fmaf(v[k].y, f, y[1]);
-              y[2] = fmaf(v[k].z, f, y[2]), y[3] = fmaf(v[k].w, f, y[3]);
+              for (int e = 0; e < 4; ++e) y[a][e] *= before;
+#pragma unroll
+              for (int k = 0; k < kTogether; ++k) {
+                const float f = i0 + k < count ? ex2(ml[a][k].x - high) : 0.f;
+                sum[a] = fmaf(ml[a][k].y, f, sum[a]);
+                y[a][0] = fmaf(v[a][k].x, f, y[a][0]), y[a][1] = fmaf(v[a][k].y, f, y[a][1]);
+                y[a][2] = fmaf(v[a][k].z, f, y[a][2]), y[a][3] = fmaf(v[a][k].w, f, y[a][3]);
+              }
             }
           }
           if (!final) __syncwarp();  // a row's first m and sum are rewritten when every lane has read them
-          if (live && final) {
-            const int64_t token = d.token0 + row / p.G;
-            const int head = d.kvh * p.G + row % p.G;
-            float f = sum == 0.f ? 0.f : 1.f / sum;
-            if (p.c.gate && sum != 0.f) f *= sigmoid(p.c.gate[token * p.c.gate_stride + head]);
-            *reinterpret_cast<uint2*>(p.c.out + token * p.c.out_stride + (int64_t)head * hd + quad * 4) =
-                sum == 0.f ? make_uint2(0u, 0u) : make_uint2(pack<false>(y[0] * f, y[1] * f), pack<false>(y[2] * f, y[3] * f));
-            if (p.c.lse && quad == 0)
-              p.c.lse[token * p.c.Hq + head] = sum == 0.f ? -INFINITY : (top - kShift + log2f(sum)) * 0.6931471805599453f;
-          } else if (live) {
-            __stcg(reinterpret_cast<float4*>(p.acc + at * hd) + quad, make_float4(y[0], y[1], y[2], y[3]));
-            if (quad == 0) __stcg(p.ml + at, make_float2(top, sum));
+#pragma unroll
+          for (int a = 0; a < kPieces; ++a) {
+            const int x = x0 + 32 * a, row = x / kQuads, quad = x % kQuads;
+            if (row >= d.rows) continue;
+            if (final) {
+              const int64_t token = d.token0 + row / p.G;
+              const int head = d.kvh * p.G + row % p.G;
+              float f = sum[a] == 0.f ? 0.f : 1.f / sum[a];
+              if (p.c.gate && sum[a] != 0.f) f *= sigmoid(p.c.gate[token * p.c.gate_stride + head]);
+              *reinterpret_cast<uint2*>(p.c.out + token * p.c.out_stride + (int64_t)head * hd + quad * 4) =
+                  sum[a] == 0.f ? make_uint2(0u, 0u) : make_uint2(pack<false>(y[a][0] * f, y[a][1] * f), pack<false>(y[a][2] * f, y[a][3] * f));
+              if (p.c.lse && quad == 0)
+                p.c.lse[token * p.c.Hq + head] = sum[a] == 0.f ? -INFINITY : (top[a] - kShift + log2f(sum[a])) * 0.6931471805599453f;
+            } else {
+              __stcg(reinterpret_cast<float4*>(p.acc + at[a] * hd) + quad, make_float4(y[a][0], y[a][1], y[a][2], y[a][3]));
+              if (quad == 0) __stcg(p.ml + at[a], make_float2(top[a], sum[a]));
+            }
           }
+          if (!final) __syncwarp();
         }
         index = leader / kJoin;
         parts = (parts + kJoin - 1) / kJoin;

@@ -27,7 +27,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib, ops
-from .attention import Attention, PagedKVPool, SlotKVPool
+from .attention import Attention, PagedKVPool, QuantKVPool, SlotKVPool
 from .attnres import FusedBlockAttnResContext, forward_layers_full
 from .base import BaseOP, OPList, Weight
 from .core import AttnMetadata, Batch, Req, forward_batch, get_global_ctx
@@ -126,13 +126,20 @@ class Zonos3ForCausalLM(BaseOP):
         """Columns of the padded head output (the logits row stride)."""
         return (self.n_codebooks * self.audio_vocab + 7) // 8 * 8
 
-    def allocate_caches(self, capacity: int, kv_slots: int, device, page_size: int | None = None):
+    def allocate_caches(self, capacity: int, kv_slots: int, device, page_size: int | None = None, kv_bits: int = 16):
         """Per-slot DeltaNet state pools of ``capacity`` streams and the KV pool: a ``SlotKVPool`` of ``kv_slots`` token
-        slots, or with ``page_size`` a ``PagedKVPool`` of as many tokens in pages (for batches described on the device;
-        ``DecodeGraph`` takes the former)."""
+        slots, or with ``page_size`` a ``PagedKVPool`` of as many tokens in pages (for batches described on the device), or with
+        ``kv_bits=4`` a ``QuantKVPool`` of them in 4 bits (pages of a multiple of 16, 16 unless ``page_size`` says otherwise).
+        ``DecodeGraph`` takes the first and the last."""
+        if kv_bits not in (4, 16):
+            raise ValueError(f"kv_bits must be 16 or 4, got {kv_bits}")
         for gdn in self.gdn_layers():
             gdn.allocate_cache(capacity, device, torch.bfloat16)
         c = self._config
+        if kv_bits == 4:
+            page_size = page_size or 16
+            return QuantKVPool(self.attention_layer_ids(), -(-kv_slots // page_size), page_size, c.num_kv_heads, c.head_dim,
+                               device)
         if page_size is not None:
             return PagedKVPool(self.attention_layer_ids(), -(-kv_slots // page_size), page_size, c.num_kv_heads, c.head_dim,
                                device)
@@ -194,13 +201,16 @@ class DecodeGraph:
     stream's page table, the codes appended to the repetition window, the sampler's draw counter + 1. So replays
     alone run an autoregressive decode; ``step()`` instead loads host ids / metadata first (the server's path).
 
-    The pool has page size 1 (``SlotKVPool``): the step's bookkeeping moves every stream from slot to slot.
+    The pool has page size 1 (``SlotKVPool``): the step's bookkeeping moves every stream from slot to slot. Or it holds 4 bits
+    (``QuantKVPool``): ``page_table`` then has the pool's pages and ``out_loc`` is not used; cache lengths stop at the tokens that
+    a row of the table has pages for.
     """
 
-    def __init__(self, model: Zonos3ForCausalLM, pool: SlotKVPool, batch_size: int, page_table: torch.Tensor,
+    def __init__(self, model: Zonos3ForCausalLM, pool: SlotKVPool | QuantKVPool, batch_size: int, page_table: torch.Tensor,
                  slots: torch.Tensor | None = None, sampling: SamplingConfig | None = None, stop_id: int | None = None):
-        if any(pool.k(layer).dim() != 3 for layer in model.attention_layer_ids()):
-            raise ValueError("DecodeGraph needs a pool of page size 1 (allocate_caches without page_size)")
+        four_bits = isinstance(pool, QuantKVPool)
+        if not four_bits and any(pool.k(layer).dim() != 3 for layer in model.attention_layer_ids()):
+            raise ValueError("DecodeGraph needs a pool of page size 1 (allocate_caches without page_size) or of 4 bits")
         c = model.config
         dev = page_table.device
         self.model, self.pool, self.bs = model, pool, batch_size
@@ -215,6 +225,10 @@ class DecodeGraph:
         if page_table.shape[0] != B or page_table.dtype != torch.int32:
             raise ValueError(f"page_table must be a [{B}, max_len] int32 tensor")
         self.page_table = page_table.contiguous()
+        # what the bookkeeping takes slots from: the table itself, or as wide as its pages' tokens where no slots are used
+        self._slot_table = self.page_table if not four_bits else torch.zeros(B, page_table.shape[1] * pool.page_size, **i32)
+        # every stream's row, for the paged operators
+        self.bounds = torch.arange(B + 1, **i32) if four_bits or c.attention_window else None
         self.input_ids = torch.zeros(B, self.C + (c.text_vocab is not None), **i32)
         self.codes = torch.zeros(B, self.C + 1, **i32)
         self.positions = torch.zeros(B, **i32)
@@ -234,7 +248,8 @@ class DecodeGraph:
         self.penalties = torch.full((B,), float(self.sampling.repetition_penalty), device=dev, dtype=torch.float32)
         self.batch = Batch(reqs=[Req(i, 1, cached_len=1) for i in range(B)], is_decode=True, padded_size=B,
                            input_ids=self.input_ids,
-                           attn_metadata=AttnMetadata(self.positions, self.out_loc, self.page_table, self.cache_seqlens))
+                           attn_metadata=AttnMetadata(self.positions, self.out_loc, self.page_table, self.cache_seqlens,
+                                                      self.bounds))
         self.graph: torch.cuda.CUDAGraph | None = None
         self.launches_per_step = 0  # this library's kernels in the captured step
         for gdn in model.gdn_layers():
@@ -256,7 +271,7 @@ class DecodeGraph:
                        softcap=self.softcap)
         # the next step's inputs, on the device (one kernel)
         ops.decode_advance(self.codes, self.input_ids, self.positions, self.cache_seqlens, self.out_loc,
-                           self.page_table, self.counter, history=self.history if self.W else None,
+                           self._slot_table, self.counter, history=self.history if self.W else None,
                            ring=self.ring if self.W else None)
 
     def _context(self):
