@@ -84,6 +84,8 @@ constexpr int kFewRows = 32;     // up to here the row warps share a unit's rows
 constexpr int kFineRows = 16;
 constexpr int kSoftWarps = 8, kMmaWarp = 8, kLoadWarp = 9, kLoadWarps = 3;
 constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
+// 4 bits: three warps write out the keys and three the values, which with the products' and the copies' warp are two warpgroups.
+constexpr int kOutWarps = 3, kThreadsQ4 = 32 * (kLoadWarp + 1 + 2 * kOutWarps);
 constexpr int kMaxSlots = 10, kDescs = 4;
 // 4 bits: stages of 64 keys (their values too) as they lie in the cache, which two warps write out as bf16 tiles.
 constexpr int kRawStages = 3, kRawBlocks = 4;
@@ -162,7 +164,6 @@ struct Tail {
   uint64_t desc_full[kDescs], desc_empty[kDescs];
   alignas(16) unsigned mask[kMasks][4];  // keys of a tile that exist
   Desc desc[kDescs];
-  int sums[2][kThreads / 32];
   int idle[2];        // rows of no request: those before the first, those from the second on
   int start[5];       // this CTA's first unit: request, its row, tokens and keys, and the pair of streams
   int64_t start_off;  // how far into the pair's work, all KV heads, the CTA begins
@@ -185,6 +186,7 @@ struct Shape {
   static constexpr uint32_t kOffRaw = kOffQ + 2 * kItem;
   static constexpr uint32_t kOffTail = kOffRaw + kRawStages * kRaw;
   static constexpr size_t kSmem = kOffTail + sizeof(Tail);
+  static constexpr int kThreads = Q4 ? kThreadsQ4 : ::kThreads;
   static_assert(kSlots * kItem >= kMaxRequests * 4 + kThreads * 16, "the plan's tables fit the ring");
   static_assert(kSmem <= 232448, "shared memory");
   static constexpr uint32_t kColS = 0, kColO = 2 * kTile;  // stream s: S at s * 128, O at 256 + s * HD
@@ -455,6 +457,7 @@ __device__ __forceinline__ int tile_behind(const ChunkParams& p, const Desc& d, 
 }
 
 // Exclusive prefix of v over the block's threads; `total` the sum. `buffer` alternates from call to call.
+template <int THREADS>
 __device__ __forceinline__ int block_scan(int v, Tail& tl, int buffer, int& total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int in = v;
@@ -463,13 +466,14 @@ __device__ __forceinline__ int block_scan(int v, Tail& tl, int buffer, int& tota
     const int u = __shfl_up_sync(0xffffffffu, in, o);
     if (lane >= o) in += u;
   }
-  if (lane == 31) tl.sums[buffer][warp] = in;
+  int* sums = reinterpret_cast<int*>(tl.ml) + buffer * (THREADS / 32);  // the rows' maxima come later
+  if (lane == 31) sums[warp] = in;
   __syncthreads();
   int before = 0;
   total = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    const int s = tl.sums[buffer][w];
+  for (int w = 0; w < THREADS / 32; ++w) {
+    const int s = sums[w];
     if (w < warp) before += s;
     total += s;
   }
@@ -565,9 +569,10 @@ __device__ __forceinline__ void join_few(const ChunkParams& p, const Desc& u, in
 // Q4: the cache holds 4 bits (and may leave requests of few rows to another kernel). SINKS: there are first keys that stay
 // visible; a kernel of its own, as the few registers it takes would be spilled ones for the rest.
 template <int HD, bool Q4, bool SINKS>
-__global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_constant__ ChunkParams p,
+__global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(const __grid_constant__ ChunkParams p,
                                                                 const __grid_constant__ Maps maps) {
   using L = Shape<HD, Q4>;
+  constexpr int kThreads = L::kThreads;
   extern __shared__ __align__(1024) unsigned char gbase[];
   const uint32_t base = zb::smem_addr(gbase);
   if (base % 1024 != 0) {  // the swizzled tiles ask for it; there is no static shared memory before them
@@ -583,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
 
   if (tid == 0) {
     for (int s = 0; s < L::kSlots; ++s) {
-      zb::mbar_init(zb::smem_addr(&tl.full[s]), p.box ? 1 : kLoadWarps * 32 + 1);
+      zb::mbar_init(zb::smem_addr(&tl.full[s]), Q4 ? kOutWarps : p.box ? 1 : kLoadWarps * 32 + 1);
       zb::mbar_init(zb::smem_addr(&tl.empty[s]), 1);
     }
     for (int s = 0; s < 2; ++s) {
@@ -596,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     }
     for (int s = 0; s < kMasks; ++s) {
       zb::mbar_init(zb::smem_addr(&tl.armed[s]), 1);
-      zb::mbar_init(zb::smem_addr(&tl.scanned[s]), kLoadWarps - 1);
+      zb::mbar_init(zb::smem_addr(&tl.scanned[s]), Q4 ? 2 * kOutWarps : kLoadWarps - 1);
     }
     zb::mbar_init(zb::smem_addr(&tl.drained), 1);
     zb::mbar_init(zb::smem_addr(&tl.halves), 32 * kSoftWarps);
@@ -632,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     const int n = b < B ? stream_pairs(p, b0 == 0 ? mine.tokens : request(p, b).tokens) : 0;
     if (b < B) out_of_order |= p.kv.cu[b + 1] < p.kv.cu[b] || p.kv.cu[b] < 0 || p.kv.cu[b + 1] > p.kv.N;
     int total;
-    const int before = block_scan(n, tl, buffer, total);
+    const int before = block_scan<kThreads>(n, tl, buffer, total);
     if (b < B) pairs_before[b] = (int)(all_pairs + before);
     all_pairs += total;
   }
@@ -658,13 +663,13 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   };
   const Pair first_pair = pair_of(tid);
   int first_total = 0;
-  const int first_before = block_scan(first_pair.work, tl, buffer, first_total);
+  const int first_before = block_scan<kThreads>(first_pair.work, tl, buffer, first_total);
   int64_t work = first_total;
 #pragma unroll 1
   for (int j0 = kThreads; j0 < pairs; j0 += kThreads) {
     int total;
     buffer ^= 1;
-    block_scan(pair_of(j0 + tid).work, tl, buffer, total);
+    block_scan<kThreads>(pair_of(j0 + tid).work, tl, buffer, total);
     work += total;
   }
   work *= Hkv;
@@ -680,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
       if (j0 > 0) {
         q = pair_of(j0 + tid);
         buffer ^= 1;
-        before = block_scan(q.work, tl, buffer, total);
+        before = block_scan<kThreads>(q.work, tl, buffer, total);
       }
       const int64_t at = (seen + before) * Hkv;
       if (q.work > 0 && begin >= at && begin < at + (int64_t)q.work * Hkv) {
@@ -712,7 +717,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     // nothing for this CTA
   } else if (warp >= kLoadWarp) {
     // =============================================================================================== loaders
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+    if constexpr (Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     const int lw = warp - kLoadWarp;
     constexpr int kChunks = HD / 8;          // 16-byte pieces of a row
     constexpr int kPass = 32 / kChunks;      // rows of a warp's copy instruction
@@ -884,11 +890,12 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                                zb::smem_addr(&tl.armed[slot]));
               }
             }
-          } else {  // the keys (warp 10) and values (warp 11) of a tile as bf16, absent ones as zeros
-            const int kv = lw - 1, part = lane % 4, groups = hd / zb::q4::kGroup;
+          } else {  // the keys (warps 10-12) and values (13-15) of a tile as bf16, absent ones as zeros
+            const int kv = (lw - 1) / kOutWarps, share = (lw - 1) % kOutWarps, part = lane % 4, groups = hd / zb::q4::kGroup;
             // The 8 rows that a warp takes at a time, ordered so that two rows of a quarter of its lanes read and write other
             // banks: 64 bytes of codes and, in the swizzled tile, 4 pieces of 16 bytes each.
             const int row8 = (0x63724150u >> (4 * (lane / 4))) & 7;
+            const uint32_t low4 = 0x000f000fu;
 #pragma unroll 1
             for (int t = 0; t < u.tiles && going; ++t, ++tile_no, item += 2) {
               const int slot = (item + kv) % L::kSlots;
@@ -903,8 +910,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                 }
                 const unsigned char* raw = gbase + L::kOffRaw + stage * L::kRaw;
                 const unsigned lower = half ? exist.z : exist.x, upper = half ? exist.w : exist.y;
-#pragma unroll 4
-                for (int i = 0; i < 8; ++i) {
+#pragma unroll 1
+                for (int i = share; i < 8; i += kOutWarps) {
                   const int r = 8 * i + row8, in = r % zb::q4::kBlock;  // of the stage, of the block
                   const unsigned char* from = raw + r / zb::q4::kBlock * block;
                   const bool exists = ((i < 4 ? lower : upper) >> (r % 32)) & 1u;
@@ -932,6 +939,7 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
                           zb::q4::read_word(words[g], pair);
                   }
                 }
+                (void)low4;
                 __syncwarp();
                 if (lane == 0) arrive(tl.scanned[stage]);
               }
@@ -1050,7 +1058,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
     if (warp == kLoadWarp + 1) landed(tl.q_full, 2, q_item);
   } else if (warp == kMmaWarp) {
     // =============================================================================================== tensor cores
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
+    if constexpr (Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     constexpr uint32_t kIdS = tc::idesc_bf16(0, kTile), kIdO = tc::idesc_bf16(0, HD, false, /*b_mn=*/true);
     uint32_t height = 0;  // the rest of the descriptors: the unit's rows
     // This warp's own time between two products is time the tensor cores stand still once their short queue is empty: ring
@@ -1191,7 +1200,8 @@ __global__ void __launch_bounds__(kThreads, 1) gqa_chunk_kernel(const __grid_con
   } else {
     // =============================================================================================== rows
     // 8 x 32 x 192 + 4 x 32 x 120 registers are the 384 x 168 that the CTA was launched with
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    if constexpr (Q4) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");  // with 8 x 32 x 72 of the others, the 512 x 128 of the launch
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     const int s = warp / 4;  // stream
     const uint32_t tlane = tmem + ((uint32_t)(32 * (warp % 4)) << 16);
     const uint32_t col_s = tlane + L::kColS + s * kTile, col_o = tlane + L::kColO + s * HD;
@@ -1805,7 +1815,7 @@ int launch_chunk(ChunkParams& p, const Launch& l, cudaStream_t stream) {
     ZB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<HD, Q4>::kSmem));
     if (dev >= 0 && dev < 64) configured[dev] = true;
   }
-  ZB_CUDA(zb::launch(kernel, dim3((unsigned)l.ctas), dim3(kThreads), Shape<HD, Q4>::kSmem, stream, 1, p, maps));
+  ZB_CUDA(zb::launch(kernel, dim3((unsigned)l.ctas), dim3(Shape<HD, Q4>::kThreads), Shape<HD, Q4>::kSmem, stream, 1, p, maps));
   return zb::check_launch("gqa_chunk");
 }
 

@@ -52,10 +52,16 @@ __device__ __forceinline__ bool pair_is_none(uint32_t pair) { return (((pair & 0
 __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
 __device__ __forceinline__ uint32_t as_word(__nv_bfloat162 h) { return *reinterpret_cast<const uint32_t*>(&h); }
 
+// (x & mask) | bits, in one instruction: of two constants the compiler makes two.
+__device__ __forceinline__ uint32_t masked_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(d) : "r"(x), "r"(mask), "r"(bits));
+  return d;
+}
 // 128 + c of codes 2 i, 2 i + 1 of a word, as bf16: 128 has its last bit at 1, so a code is the lower bits of the significand.
 template <int I>
 __device__ __forceinline__ uint32_t codes_128(uint32_t word) {
-  return ((word >> (4 * I)) & 0x000f000fu) | 0x43004300u;
+  return masked_or(word >> (4 * I), 0x000f000fu, 0x43004300u);
 }
 // m + s c of two codes, rounded once: s2, m2 hold s and m twice (or those of two tokens).
 __device__ __forceinline__ uint32_t stands_for(uint32_t c128, uint32_t s2, uint32_t m2) {
