@@ -381,11 +381,11 @@ int zb_gqa_chunk_sinks(const uint16_t* q, int64_t q_stride, const uint16_t* k_ca
  * pairs of their keys, 16 rows of hd / 32; [18 hd, 20 hd) those of their values. 32 consecutive elements of a row are a group
  * with a pair (s, m) of bf16 (a 32-bit word, s in its lower half), and stand for m + s c, c their codes 0 .. 15. A row's codes
  * are 32-bit words: word t * (hd / 32) + g holds elements 32 g + 8 t + e, e = 0 .. 7, element e in bits 4 (e / 2 + 4 (e % 2))
- * and up. A pair with a magnitude of 2^100 or more or a NaN (never written) stands for zeros. Replaces no part of the
+ * and up. A pair with a magnitude of 2^64 or more or a NaN (never written) stands for zeros. Replaces no part of the
  * reference, whose cache is bf16.
  *
  * zb_gqa_append_q4: as zb_gqa_append; k, rounded to bf16, and v go into the cache with m the smallest element of a group, s =
- * bf16((largest - m) / 15), 0 below 2^-100, c = floor((x - m) / s + 1/2). NaN is stored as 0, magnitudes above 2^99 as that.
+ * bf16((largest - m) / 15), 0 below 2^-100, c = floor((x - m) / s + 1/2). NaN is stored as 0, magnitudes above 2^63 as that.
  * Hq may be 0 (proj holds k | v; q_out is not used). */
 int zb_gqa_append_q4(const uint16_t* proj, int64_t proj_stride, const uint16_t* temp, const int32_t* positions, float eps,
                      int normalize, double rope_theta, int rotary_dim, int interleaved, uint16_t* q_out, int64_t q_stride,

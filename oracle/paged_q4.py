@@ -13,7 +13,7 @@ GROUP, BLOCK = 32, 16
 def quantise(x):
     """Codes [..., hd] (int64), s and m [..., hd / 32] (float64, values of bf16) of bf16 rows x [..., hd]."""
     x = x.double()
-    x = torch.where(x.isnan(), torch.zeros_like(x), x.clamp(-(2.0 ** 99), 2.0 ** 99)).unflatten(-1, (-1, GROUP))
+    x = torch.where(x.isnan(), torch.zeros_like(x), x.clamp(-(2.0 ** 63), 2.0 ** 63)).unflatten(-1, (-1, GROUP))
     m, high = x.amin(-1), x.amax(-1)
     s = ((high - m) / 15).float().bfloat16().double()
     s = torch.where(s < 2.0 ** -100, torch.zeros_like(s), s)
@@ -23,9 +23,9 @@ def quantise(x):
 
 
 def stands_for(codes, s, m):
-    """Values [..., hd] (float64); a pair that is not finite, or of 2^100 and more, counts as zeros."""
+    """Values [..., hd] (float64); a pair that is not finite, or of 2^64 and more, counts as zeros."""
     s, m = s.repeat_interleave(GROUP, -1), m.repeat_interleave(GROUP, -1)
-    none = ~((s.abs() < 2.0 ** 100) & (m.abs() < 2.0 ** 100))
+    none = ~((s.abs() < 2.0 ** 64) & (m.abs() < 2.0 ** 64))
     return torch.where(none, torch.zeros_like(s), m + s * codes.double())
 
 

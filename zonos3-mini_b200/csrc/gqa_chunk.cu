@@ -91,6 +91,9 @@ constexpr int kMaxSlots = 10, kDescs = 4;
 constexpr int kRawStages = 3, kRawBlocks = 4;
 constexpr int kMasks = 8;  // of key masks and of looked-through tiles: the loaders run at most 5 tiles ahead of the rows
 constexpr float kAbove = 24.f;  // how far (log2) the m that is subtracted may lie above a row's largest score
+// 4 bits: the weights come 2^15 larger, so that fp16, whose rounding is an eighth of bf16's, holds them: from there down to 2^-39,
+// the largest not below 2^-9.
+constexpr float kShiftQ4 = 15.f;
 constexpr int kMaxRequests = 16384;
 // The flags' part of a workspace, of every call's alike: calls of different grids take turns on one workspace, and what one
 // leaves in its parts must not lie where another has its flags.
@@ -160,7 +163,7 @@ struct Tail {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t q_full[2], q_empty[2];
   uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
-  uint64_t armed[kMasks], scanned[kMasks], drained, halves;  // with 4 bits, armed: a stage is there; scanned: it is free
+  uint64_t armed[kMasks], scanned[kMasks], drained, halves, agreed;  // with 4 bits, armed: a stage is there; scanned: it is free
   uint64_t desc_full[kDescs], desc_empty[kDescs];
   alignas(16) unsigned mask[kMasks][4];  // keys of a tile that exist
   Desc desc[kDescs];
@@ -170,7 +173,7 @@ struct Tail {
   float ml[2][kStreamRows][2];  // maximum and sum of the rows' two halves, when the streams share rows
   uint32_t tmem;
   int abort;
-  int found[kMasks][2];  // either half of the tile's values holds some that are not finite
+  int found[kMasks][2];  // either half of the tile's values holds some that are not finite; with 4 bits, that fp16 does not hold
 };
 
 template <int HD, bool Q4 = false>
@@ -355,6 +358,11 @@ __device__ __forceinline__ uint32_t to_bf16x2(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ uint32_t to_fp16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
 // Sign bits set where the bf16 values are not finite (all exponent bits set: one more carries into the sign).
 __device__ __forceinline__ unsigned not_finite(unsigned pair) { return (pair & 0x7f807f80u) + 0x00800080u; }
 __device__ __forceinline__ unsigned not_finite(const uint4& v) {
@@ -517,7 +525,7 @@ __device__ __forceinline__ int64_t part_slot(int cta, int i) { return (int64_t)(
 // Joins the parts of a unit of few rows, in the order of their keys: a thread of the row warps takes 8 dims of a row, the
 // loads of 8 parts in flight together.
 template <int HD>
-__device__ __forceinline__ void join_few(const ChunkParams& p, const Desc& u, int cta, int tid) {
+__device__ __forceinline__ void join_few(const ChunkParams& p, const Desc& u, int cta, int tid, float shift) {
   constexpr int kTogether = 8;
   const int sharers = 32 * kSoftWarps / u.rows, r = tid % u.rows;  // threads of a row
   if (tid / u.rows >= sharers) return;
@@ -562,7 +570,7 @@ __device__ __forceinline__ void join_few(const ChunkParams& p, const Desc& u, in
       *reinterpret_cast<uint4*>(p.out + token * p.out_stride + (int64_t)h * p.kv.hd + piece * 8) =
           make_uint4(to_bf16x2(y[0] * f, y[1] * f), to_bf16x2(y[2] * f, y[3] * f), to_bf16x2(y[4] * f, y[5] * f),
                      to_bf16x2(y[6] * f, y[7] * f));
-    if (p.lse && piece == 0) p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+    if (p.lse && piece == 0) p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (top - shift + log2f(l)) * 0.6931471805599453f;
   }
 }
 
@@ -573,6 +581,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
                                                                 const __grid_constant__ Maps maps) {
   using L = Shape<HD, Q4>;
   constexpr int kThreads = L::kThreads;
+  constexpr float kShift = Q4 ? kShiftQ4 : 0.f;
   extern __shared__ __align__(1024) unsigned char gbase[];
   const uint32_t base = zb::smem_addr(gbase);
   if (base % 1024 != 0) {  // the swizzled tiles ask for it; there is no static shared memory before them
@@ -605,12 +614,15 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
     }
     zb::mbar_init(zb::smem_addr(&tl.drained), 1);
     zb::mbar_init(zb::smem_addr(&tl.halves), 32 * kSoftWarps);
+    zb::mbar_init(zb::smem_addr(&tl.agreed), kOutWarps);
     for (int s = 0; s < kDescs; ++s) {
       zb::mbar_init(zb::smem_addr(&tl.desc_full[s]), 1);
       zb::mbar_init(zb::smem_addr(&tl.desc_empty[s]), kSoftWarps + 1);
     }
     zb::fence_mbar_init();
     tl.abort = 0;
+    if (Q4)
+      for (int i = 0; i < kMasks; ++i) tl.found[i][0] = tl.found[i][1] = 0;
   }
   if (warp == kMmaWarp) tc::alloc(zb::smem_addr(&tl.tmem), 512);
   if (warp == kLoadWarp && lane < 3)
@@ -871,7 +883,8 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 const int r = 32 * k + lane;
-                bits[k] = __ballot_sync(0xffffffffu, first + r < held && (live >> (r / zb::q4::kBlock) & 1u));
+                const bool hidden = first + r >= p.sinks && first + r < d.from;  // from every row
+                bits[k] = __ballot_sync(0xffffffffu, first + r < held && !hidden && (live >> (r / zb::q4::kBlock) & 1u));
               }
               if (t + 1 < u.tiles) next = look_box(t + 1);
 #pragma unroll 1
@@ -891,11 +904,11 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
               }
             }
           } else {  // the keys (warps 10-12) and values (13-15) of a tile as bf16, absent ones as zeros
-            const int kv = (lw - 1) / kOutWarps, share = (lw - 1) % kOutWarps, part = lane % 4, groups = hd / zb::q4::kGroup;
-            // The 8 rows that a warp takes at a time, ordered so that two rows of a quarter of its lanes read and write other
-            // banks: 64 bytes of codes and, in the swizzled tile, 4 pieces of 16 bytes each.
-            const int row8 = (0x63724150u >> (4 * (lane / 4))) & 7;
-            const uint32_t low4 = 0x000f000fu;
+            // A lane takes one group of a row, so its pair is looked at once for four words; it takes those in an order that the row
+            // shifts, so that a warp's rows, 64 (or 32) bytes of codes each, are in different banks.
+            constexpr int kLanes = HD / 32, kRows = 32 / kLanes;  // of a row, of a pass
+            const int kv = (lw - 1) / kOutWarps, share = (lw - 1) % kOutWarps, groups = hd / zb::q4::kGroup;
+            const int g = lane % kLanes, sub = lane / kLanes, turn = sub * kLanes / 8;
 #pragma unroll 1
             for (int t = 0; t < u.tiles && going; ++t, ++tile_no, item += 2) {
               const int slot = (item + kv) % L::kSlots;
@@ -910,36 +923,53 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
                 }
                 const unsigned char* raw = gbase + L::kOffRaw + stage * L::kRaw;
                 const unsigned lower = half ? exist.z : exist.x, upper = half ? exist.w : exist.y;
+                // Values are written as fp16, whose rounding is an eighth of bf16's, and looked at on the way. What one of the three
+                // warps finds that fp16 does not hold makes all of them write the half again, as bf16; they agree on it before the
+                // stage is given back. (Each looking through the whole stage beforehand took 184 us for 4 x 512 tokens behind 8192.)
+                auto write = [&](auto type) {
+                  constexpr bool HALF = decltype(type)::value;
+                  uint32_t over = 0;
+                  bool holds = true;
 #pragma unroll 1
-                for (int i = share; i < 8; i += kOutWarps) {
-                  const int r = 8 * i + row8, in = r % zb::q4::kBlock;  // of the stage, of the block
-                  const unsigned char* from = raw + r / zb::q4::kBlock * block;
-                  const bool exists = ((i < 4 ? lower : upper) >> (r % 32)) & 1u;
-                  uint32_t words[HD / 32], pairs[HD / 32];
-                  const uint32_t* w = reinterpret_cast<const uint32_t*>(from + 8 * kv * hd + in * (hd / 2)) + part * groups;
-                  const uint32_t* q = reinterpret_cast<const uint32_t*>(from + (16 + 2 * kv) * hd) + in * groups;
-                  if (HD == 128 && hd == HD) {
-                    *reinterpret_cast<uint4*>(words) = *reinterpret_cast<const uint4*>(w);
-                    *reinterpret_cast<uint4*>(pairs) = *reinterpret_cast<const uint4*>(q);
-                  } else if (HD == 64 && hd == HD) {
-                    *reinterpret_cast<uint2*>(words) = *reinterpret_cast<const uint2*>(w);
-                    *reinterpret_cast<uint2*>(pairs) = *reinterpret_cast<const uint2*>(q);
-                  } else {
+                  for (int i = share; i < 64 / kRows; i += kOutWarps) {
+                    const int r = kRows * i + sub, in = r % zb::q4::kBlock;  // of the stage, of the block
+                    const unsigned char* from = raw + r / zb::q4::kBlock * block;
+                    const bool exists = ((r < 32 ? lower : upper) >> (r % 32)) & 1u;
+                    if (g < groups) {
+                      const uint32_t* w = reinterpret_cast<const uint32_t*>(from + 8 * kv * hd + in * (hd / 2)) + g;
+                      uint32_t pair = reinterpret_cast<const uint32_t*>(from + (16 + 2 * kv) * hd)[in * groups + g], words[4];
 #pragma unroll
-                    for (int g = 0; g < HD / 32; ++g) {
-                      words[g] = g < groups ? w[g] : 0;
-                      pairs[g] = g < groups ? q[g] : 0;
+                      for (int k = 0; k < 4; ++k) words[k] = w[((k + turn) & 3) * groups];
+                      if (!exists || zb::q4::pair_is_none(pair)) pair = 0;
+                      auto to = [&](int k) {
+                        return reinterpret_cast<uint4*>(gbase + slot * L::kItem + piece<HD>(64 * half + r, 4 * g + ((k + turn) & 3)));
+                      };
+                      if constexpr (HALF) {
+                        zb::q4::fp16_holds(pair, over, holds);
+                        const zb::q4::HalfPair halves(pair);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) *to(k) = halves.read_word(words[k]);
+                      } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) *to(k) = zb::q4::read_word(words[k], pair);
+                      }
                     }
                   }
-#pragma unroll
-                  for (int g = 0; g < HD / 32; ++g) {
-                    const uint32_t pair = exists && !zb::q4::pair_is_none(pairs[g]) ? pairs[g] : 0u;
-                    if (g < groups)
-                      *reinterpret_cast<uint4*>(gbase + slot * L::kItem + piece<HD>(64 * half + r, 4 * g + part)) =
-                          zb::q4::read_word(words[g], pair);
+                  return __all_sync(0xffffffffu, holds && (over & 0x80008000u) == 0);
+                };
+                if (kv) {
+                  int* found = tl.found[tile_no % kMasks];
+                  if (share == 0 && half == 0 && lane < 2) tl.found[(tile_no + 1) % kMasks][lane] = 0;  // of 7 tiles ago, which is done
+                  const bool held = write(std::true_type{});
+                  if (lane == 0) {
+                    if (!held) found[half] = 1;
+                    arrive(tl.agreed);
                   }
+                  wait(tl.agreed, raws & 1, abort);
+                  if (*reinterpret_cast<volatile int*>(found + half) != 0) write(std::false_type{});
+                } else {
+                  write(std::false_type{});
                 }
-                (void)low4;
                 __syncwarp();
                 if (lane == 0) arrive(tl.scanned[stage]);
               }
@@ -1061,6 +1091,8 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
     if constexpr (Q4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     constexpr uint32_t kIdS = tc::idesc_bf16(0, kTile), kIdO = tc::idesc_bf16(0, HD, false, /*b_mn=*/true);
+    constexpr uint32_t kFp16 = (1u << 7) | (1u << 10);  // bits that make the operands bf16; off where values are fp16
+    uint32_t types[2] = {0, 0};                         // what to take off for either half of a tile
     uint32_t height = 0;  // the rest of the descriptors: the unit's rows
     // This warp's own time between two products is time the tensor cores stand still once their short queue is empty: ring
     // positions are kept instead of divided out, and one lane issues a stream's products and commits in one go.
@@ -1073,7 +1105,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
       }
     };
     Ring at{0, 0};  // of the unit's next tile's keys; its values lie one further
-    int q_item = 0, scans = 0;
+    int q_item = 0, scans = 0, tile_no = 0;
     uint32_t parity = 0;  // bit s: of stream s's weights
     auto full = [&](const Ring& i) { wait(tl.full[i.slot], i.phase, abort); };
     auto commit = [&](const uint64_t& bar) { tc::commit(zb::smem_addr(&bar)); };
@@ -1095,8 +1127,8 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
 #pragma unroll
       for (int k0 = 0; k0 < kTile / 32; ++k0) {
         const int ks = k0 + half * (kTile / 32);
-        mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, vd + ks * 2 * L::kGroup / 16, kIdO | height,
-               accumulate || ks > 0);
+        mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, vd + ks * 2 * L::kGroup / 16,
+               (kIdO | height) & ~types[half], accumulate || ks > 0);
       }
       if (fine)
 #pragma unroll
@@ -1114,7 +1146,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
       if (u.mode == kStop || gave_up(abort)) break;
       if (u.tiles == 0) continue;
       const bool two = u.rows > p.tokens * G;  // two streams of rows share each tile, or one's two halves take turns
-      const bool fine = u.rows <= kFineRows;
+      const bool fine = !Q4 && u.rows <= kFineRows;
       height = tc::idesc_bf16(fine ? 64 : kStreamRows, 0) & ~tc::idesc_bf16(0, 0);
       const int stride = two ? 1 : 2;          // tiles from one of a stream to its next
       const int held = held_keys(p, u.keys);
@@ -1129,6 +1161,12 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
         bool found = false;
         if (t >= 0) {
           full(v);
+          if constexpr (Q4) {
+            const int* found = tl.found[tile_no % kMasks];
+            types[0] = uniform(found[0]) ? 0 : kFp16;
+            types[1] = uniform(found[1]) ? 0 : kFp16;
+            ++tile_no;
+          }
           // rows of the last page past the request's keys came along with a tensor copy: no key, so no value either
           if (!Q4 && p.box && first + kTile > held && held % p.box != 0) {
             const int r0 = held - first, r1 = (r0 + p.box - 1) / p.box * p.box;
@@ -1220,7 +1258,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
       const int stream_rows = p.tokens * G;
       const bool two = u.rows > stream_rows;
       const int first_row = two ? s * stream_rows : 0, rows = min(stream_rows, u.rows - first_row);
-      const bool fine = u.rows <= kFineRows;
+      const bool fine = !Q4 && u.rows <= kFineRows;
       const bool idle = 32 * (warp % 4) >= rows;  // no lane of the warp has a row
       const int stride = two ? 1 : 2;
       float m = kAbove, l = 0.f;
@@ -1259,6 +1297,12 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
               arrive(tl.p_full[s]);
             }
             continue;
+          }
+          bool half_types = true;  // fp16 holds the values of both halves of the tile
+          if constexpr (Q4) {
+            const int v_item = 2 * (tile_no + t) + 1;
+            wait(tl.full[v_item % L::kSlots], (v_item / L::kSlots) & 1, abort);  // this stream's last product has waited for the one before
+            half_types = !(tl.found[(tile_no + t) % kMasks][0] | tl.found[(tile_no + t) % kMasks][1]);
           }
           const unsigned* there = tl.mask[(tile_no + t) % kMasks];
           const uint4 all4 = *reinterpret_cast<const uint4*>(there);
@@ -1391,7 +1435,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
             }
             sum2[0] = sum2[1] = 0;
             if (!scan) hand_over(tl.p_half[s]);
-          } else if (partly) {  // 32 keys at a time, without those that no row of the warp sees; first their largest score
+          } else if (partly || (Q4 && !half_types)) {  // 32 keys at a time, without those that no row of the warp sees; first their largest score
             float top = -INFINITY;
             auto scores = [&](int c, uint32_t (&y)[32]) {  // those that the row does not see as -infinity; whether any row sees one
               const unsigned word = seen(c);
@@ -1419,7 +1463,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
             }
             // The first keys of a unit's row set m by their largest score, whose weight is a power of 2 then, and exact.
             holds(top, t < stride);
-            minus = pack2(-m, -m);
+            minus = pack2(kShift - m, kShift - m);
             sum2[0] = sum2[1] = 0;
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {  // the weights take half of the scores' columns: those of scores already read
@@ -1432,7 +1476,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
                   a = ex2(a);
                   z = ex2(z);
                   sum2[j % 2] = add2(sum2[j % 2], pack2(a, z));
-                  packed[j] = to_bf16x2(a, z);
+                  packed[j] = Q4 && !tl.found[(tile_no + t) % kMasks][c / 2] ? to_fp16x2(a, z) : to_bf16x2(a, z);
                 }
               }
               tc::st16(col_s + 16 * c, packed);
@@ -1476,7 +1520,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
                   if (g > 0) {
                     const float a = e[(g + 1) % 2][2 * i], z = e[(g + 1) % 2][2 * i + 1];
                     sum2[i % 2] = add2(sum2[i % 2], pack2(a, z));
-                    packed[(g - 1) * kPairs + i] = to_bf16x2(a, z);
+                    packed[(g - 1) * kPairs + i] = Q4 ? to_fp16x2(a, z) : to_bf16x2(a, z);
                   }
                 }
               }
@@ -1486,7 +1530,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
             do {
 #pragma unroll
               for (int c = 0; c < 4; ++c) ld32(col_s + 32 * c, x + 32 * c);
-              minus = pack2(-m, -m);
+              minus = pack2(kShift - m, kShift - m);
               sum2[0] = sum2[1] = 0;
               tc::ld_wait();
               weigh(0, packed);
@@ -1690,7 +1734,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
             p.ml[part * 2 * p.rows_max + r] = m;
             p.ml[(part * 2 + 1) * p.rows_max + r] = l;
           } else if (p.lse) {
-            p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+            p.lse[token * p.Hq + h] = l == 0.f ? -INFINITY : (m - kShift + log2f(l)) * 0.6931471805599453f;
           }
         }
       }
@@ -1701,7 +1745,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
         if (u.mode == kPart0) {
           if (tid == 0) raise_flag(p.flags + cta, p.raised);
         } else {
-          if (few && wait_parts(p, u, cta, lane)) join_few<HD>(p, u, cta, tid);
+          if (few && wait_parts(p, u, cta, lane)) join_few<HD>(p, u, cta, tid, kShift);
           meet();  // every thread is done with the parts
           if (tid < u.parts - 1) p.flags[cta + 1 + tid] = 0;
         }

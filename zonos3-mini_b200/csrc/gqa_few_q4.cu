@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
 #pragma unroll
           for (int x = 0; x < kItem; ++x) {
             const uint2 k2 = GROUPS == 4 ? reinterpret_cast<const uint2*>(k_pairs(x))[lane] : make_uint2(k_pairs(x)[lane], 0);
-            none |= ((k2.x & 0x7fff7fffu) + 0x0e800e80u) | ((k2.y & 0x7fff7fffu) + 0x0e800e80u);  // as pair_is_none()
+            none |= q4::none_bits(k2.x) | q4::none_bits(k2.y);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               a[x][k] = v_pairs(x)[(row ^ k) * GROUPS + g];

@@ -1,11 +1,12 @@
 // A paged KV cache in 4 bits: its layout, and the arithmetic of its groups.
 //
 // 32 consecutive elements of a token's key or value of one KV head are a group; it is kept as 4-bit codes c and a pair (s, m)
-// of bf16, and stands for x = m + s c. From x (bf16; NaN counts as 0, and what is beyond +-2^99 as that):
+// of bf16, and stands for x = m + s c. From x (bf16; NaN counts as 0, and what is beyond +-2^63 as that):
 //   m = min x,  s = bf16((max x - min x) / 15) (0 where that is below 2^-100),  c = floor((x - m) / s + 1/2), 0 .. 15 (0 where s = 0)
 // m is one of the elements, so storing it rounds nothing; s is rounded before it divides, so c allows for it. A pair with a
-// magnitude of 2^100 or more, or a NaN, is never written and stands for zeros: rows that no token wrote hold anything, and
-// 0 x inf would be NaN in a matrix product that counts them with weight 0.
+// magnitude of 2^64 or more, or a NaN, is never written and stands for zeros: rows that no token wrote hold anything, and 0 x
+// inf would be NaN in a matrix product that counts them with weight 0; and sums of 2^26 values, times weights of up to 2^15, stay
+// in fp32's range.
 //
 // 16 consecutive keys of a head are a block of 20 hd bytes, a page of a head is page_size / 16 blocks one after the other:
 //   [0, 8 hd) codes of the keys, 16 rows of hd / 2 bytes; [8 hd, 16 hd) codes of the values;
@@ -16,6 +17,8 @@
 // group; and the words of a t are consecutive, which are what one lane of a fragment of 16 keys needs of a row.
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include "paged.cuh"
 
 namespace zb {
@@ -23,7 +26,7 @@ namespace q4 {
 
 constexpr int kBlock = 16;   // keys of a block
 constexpr int kGroup = 32;   // elements of a group
-constexpr float kLargest = 0x1p99f, kSmallestStep = 0x1p-100f;
+constexpr float kLargest = 0x1p63f, kSmallestStep = 0x1p-100f;
 
 __host__ __device__ constexpr int block_bytes(int hd) { return 20 * hd; }
 
@@ -45,9 +48,10 @@ inline int check_cache(const PagedBatch& p, const char* who) {
   return kOk;
 }
 
-// A pair as the rule above has it: 0 where one of its numbers is not finite or has a magnitude of 2^100 or more (its exponent
-// field is 227 or more: added to 0x8000 - 0x7180 it carries into the sign).
-__device__ __forceinline__ bool pair_is_none(uint32_t pair) { return (((pair & 0x7fff7fffu) + 0x0e800e80u) & 0x80008000u) != 0; }
+// Whether a pair stands for zeros by the rule above: a number that is not finite or has a magnitude of 2^64 or more has an exponent
+// field of 191 or more, and with 0x8000 - 0x5f80 added carries into its sign (which `none_bits` leaves, among other bits).
+__device__ __forceinline__ uint32_t none_bits(uint32_t pair) { return (pair & 0x7fff7fffu) + 0x20802080u; }
+__device__ __forceinline__ bool pair_is_none(uint32_t pair) { return (none_bits(pair) & 0x80008000u) != 0; }
 
 __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
 __device__ __forceinline__ uint32_t as_word(__nv_bfloat162 h) { return *reinterpret_cast<const uint32_t*>(&h); }
@@ -73,6 +77,35 @@ __device__ __forceinline__ uint4 read_word(uint32_t word, uint32_t pair) {
   return make_uint4(stands_for(codes_128<0>(word), s2, m2), stands_for(codes_128<1>(word), s2, m2),
                     stands_for(codes_128<2>(word), s2, m2), stands_for(codes_128<3>(word), s2, m2));
 }
+
+// Whether fp16 holds what a pair stands for as well as bf16 and better: |m| is below 2^14 and s below 2^10 (a sign bit of `over`
+// else), and s is 2^-14 or more, so that fp16's smallest step is little beside it, or the pair is 0 (`holds`).
+__device__ __forceinline__ void fp16_holds(uint32_t pair, uint32_t& over, bool& holds) {
+  const uint32_t a = pair & 0x7fff7fffu;
+  over |= a + (((0x8000u - 0x4680u) << 16) | (0x8000u - 0x4480u));
+  holds &= pair << 16 >= 0x3880u << 16 || a == 0;
+}
+// A pair in fp16, s and m twice; and the 8 elements of a word of codes, m + s c rounded once.
+struct HalfPair {
+  uint32_t s2, m2;
+  __device__ __forceinline__ explicit HalfPair(uint32_t pair) {
+    const float s = __uint_as_float(pair << 16), m = __uint_as_float(pair & 0xffff0000u);
+    asm("cvt.rn.f16x2.f32 %0, %1, %1;" : "=r"(s2) : "f"(s));
+    asm("cvt.rn.f16x2.f32 %0, %1, %1;" : "=r"(m2) : "f"(m));
+  }
+  template <int I>
+  __device__ __forceinline__ uint32_t two(uint32_t word) const {
+    // 1024 + c, or 64 + c from 4 bits higher in the significand
+    const uint32_t zero = I % 2 ? 0x54005400u : 0x64006400u;
+    const uint32_t c = masked_or(I >= 2 ? word >> 8 : word, I % 2 ? 0x00f000f0u : 0x000f000fu, zero);
+    const __half2 v = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), *reinterpret_cast<const __half2*>(&zero)),
+                              *reinterpret_cast<const __half2*>(&s2), *reinterpret_cast<const __half2*>(&m2));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  __device__ __forceinline__ uint4 read_word(uint32_t word) const {
+    return make_uint4(two<0>(word), two<1>(word), two<2>(word), two<3>(word));
+  }
+};
 
 // 8 bf16 elements of a group whose other elements are on the lanes' neighbours (4 lanes of a group, lane % 4 = t): their
 // word of codes and the group's pair. Every lane of the warp takes part.

@@ -1291,7 +1291,7 @@ def gqa_append_q4(proj, kv_cache, page_table, cache_seqlens, cu_seqlens_q, *, he
 
     k after its norm and rotation, rounded to bf16, and v are kept in groups of 32 elements: x = m + s c, m the group's
     smallest element, s = bf16((largest - smallest) / 15) (0 below 2^-100), c = floor((x - m) / s + 1/2) in 4 bits. So an
-    element is kept to s / 2 (and 2^-9 of the group's range for the rounding of s). NaN is kept as 0, magnitudes beyond 2^99
+    element is kept to s / 2 (and 2^-9 of the group's range for the rounding of s). NaN is kept as 0, magnitudes beyond 2^63
     as that."""
     paged, index, Hkv, hd = _paged_q4(proj, kv_cache, page_table, cache_seqlens, cu_seqlens_q, kv_heads)
     shape = proj.shape
