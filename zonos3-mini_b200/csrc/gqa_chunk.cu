@@ -163,7 +163,7 @@ struct Tail {
   uint64_t full[kMaxSlots], empty[kMaxSlots];
   uint64_t q_full[2], q_empty[2];
   uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
-  uint64_t armed[kMasks], scanned[kMasks], drained, halves, agreed;  // with 4 bits, armed: a stage is there; scanned: it is free
+  uint64_t armed[kMasks], scanned[kMasks], drained, halves;  // with 4 bits, armed: a stage is there; scanned: it is free
   uint64_t desc_full[kDescs], desc_empty[kDescs];
   alignas(16) unsigned mask[kMasks][4];  // keys of a tile that exist
   Desc desc[kDescs];
@@ -173,7 +173,7 @@ struct Tail {
   float ml[2][kStreamRows][2];  // maximum and sum of the rows' two halves, when the streams share rows
   uint32_t tmem;
   int abort;
-  int found[kMasks][2];  // either half of the tile's values holds some that are not finite; with 4 bits, that fp16 does not hold
+  int found[kMasks][2];  // either half of the tile's values holds some that are not finite; with 4 bits a byte for each block, 1: bf16
 };
 
 template <int HD, bool Q4 = false>
@@ -614,15 +614,12 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
     }
     zb::mbar_init(zb::smem_addr(&tl.drained), 1);
     zb::mbar_init(zb::smem_addr(&tl.halves), 32 * kSoftWarps);
-    zb::mbar_init(zb::smem_addr(&tl.agreed), kOutWarps);
     for (int s = 0; s < kDescs; ++s) {
       zb::mbar_init(zb::smem_addr(&tl.desc_full[s]), 1);
       zb::mbar_init(zb::smem_addr(&tl.desc_empty[s]), kSoftWarps + 1);
     }
     zb::fence_mbar_init();
     tl.abort = 0;
-    if (Q4)
-      for (int i = 0; i < kMasks; ++i) tl.found[i][0] = tl.found[i][1] = 0;
   }
   if (warp == kMmaWarp) tc::alloc(zb::smem_addr(&tl.tmem), 512);
   if (warp == kLoadWarp && lane < 3)
@@ -906,7 +903,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
           } else {  // the keys (warps 10-12) and values (13-15) of a tile as bf16, absent ones as zeros
             // A lane takes one group of a row, so its pair is looked at once for four words; it takes those in an order that the row
             // shifts, so that a warp's rows, 64 (or 32) bytes of codes each, are in different banks.
-            constexpr int kLanes = HD / 32, kRows = 32 / kLanes;  // of a row, of a pass
+            constexpr int kLanes = HD / 32, kRows = 32 / kLanes, kPasses = zb::q4::kBlock / kRows;  // of a row, of a pass, of a block
             const int kv = (lw - 1) / kOutWarps, share = (lw - 1) % kOutWarps, groups = hd / zb::q4::kGroup;
             const int g = lane % kLanes, sub = lane / kLanes, turn = sub * kLanes / 8;
 #pragma unroll 1
@@ -923,52 +920,48 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
                 }
                 const unsigned char* raw = gbase + L::kOffRaw + stage * L::kRaw;
                 const unsigned lower = half ? exist.z : exist.x, upper = half ? exist.w : exist.y;
-                // Values are written as fp16, whose rounding is an eighth of bf16's, and looked at on the way. What one of the three
-                // warps finds that fp16 does not hold makes all of them write the half again, as bf16; they agree on it before the
-                // stage is given back. (Each looking through the whole stage beforehand took 184 us for 4 x 512 tokens behind 8192.)
-                auto write = [&](auto type) {
-                  constexpr bool HALF = decltype(type)::value;
-                  uint32_t over = 0;
-                  bool holds = true;
+                // A warp takes whole blocks. Values are written as fp16, whose rounding is an eighth of bf16's, in blocks that fp16
+                // holds: one product of the tensor cores takes the 16 keys of a block, so each block has a type of its own and the
+                // warps need not agree on it (on one type for a stage: 181 us for 4 x 512 tokens behind 8192, now 177).
 #pragma unroll 1
-                  for (int i = share; i < 64 / kRows; i += kOutWarps) {
-                    const int r = kRows * i + sub, in = r % zb::q4::kBlock;  // of the stage, of the block
-                    const unsigned char* from = raw + r / zb::q4::kBlock * block;
-                    const bool exists = ((r < 32 ? lower : upper) >> (r % 32)) & 1u;
-                    if (g < groups) {
+                for (int blk = (share + kOutWarps - raws % kOutWarps) % kOutWarps; blk < kRawBlocks; blk += kOutWarps) {
+                  const unsigned char* from = raw + blk * block;
+                  const unsigned exists = (blk & 2 ? upper : lower) >> (blk & 1) * zb::q4::kBlock;
+                  uint32_t pair[kPasses], over = 0;
+                  bool holds = kv != 0;
+                  if (g < groups) {
+#pragma unroll
+                    for (int i = 0; i < kPasses; ++i) {
+                      const int in = kRows * i + sub;
+                      pair[i] = reinterpret_cast<const uint32_t*>(from + (16 + 2 * kv) * hd)[in * groups + g];
+                      if (!(exists >> in & 1u) || zb::q4::pair_is_none(pair[i])) pair[i] = 0;
+                      zb::q4::fp16_holds(pair[i], over, holds);
+                    }
+                  }
+                  const bool half_type = __all_sync(0xffffffffu, holds && (over & 0x80008000u) == 0);
+                  if (kv && lane == 0) reinterpret_cast<unsigned char*>(tl.found[tile_no % kMasks])[kRawBlocks * half + blk] = !half_type;
+                  if (g < groups) {
+#pragma unroll
+                    for (int i = 0; i < kPasses; ++i) {
+                      const int in = kRows * i + sub;
                       const uint32_t* w = reinterpret_cast<const uint32_t*>(from + 8 * kv * hd + in * (hd / 2)) + g;
-                      uint32_t pair = reinterpret_cast<const uint32_t*>(from + (16 + 2 * kv) * hd)[in * groups + g], words[4];
+                      uint32_t words[4];
 #pragma unroll
                       for (int k = 0; k < 4; ++k) words[k] = w[((k + turn) & 3) * groups];
-                      if (!exists || zb::q4::pair_is_none(pair)) pair = 0;
                       auto to = [&](int k) {
-                        return reinterpret_cast<uint4*>(gbase + slot * L::kItem + piece<HD>(64 * half + r, 4 * g + ((k + turn) & 3)));
+                        return reinterpret_cast<uint4*>(gbase + slot * L::kItem +
+                                                        piece<HD>(64 * half + zb::q4::kBlock * blk + in, 4 * g + ((k + turn) & 3)));
                       };
-                      if constexpr (HALF) {
-                        zb::q4::fp16_holds(pair, over, holds);
-                        const zb::q4::HalfPair halves(pair);
+                      if (half_type) {
+                        const zb::q4::HalfPair halves(pair[i]);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) *to(k) = halves.read_word(words[k]);
                       } else {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) *to(k) = zb::q4::read_word(words[k], pair);
+                        for (int k = 0; k < 4; ++k) *to(k) = zb::q4::read_word(words[k], pair[i]);
                       }
                     }
                   }
-                  return __all_sync(0xffffffffu, holds && (over & 0x80008000u) == 0);
-                };
-                if (kv) {
-                  int* found = tl.found[tile_no % kMasks];
-                  if (share == 0 && half == 0 && lane < 2) tl.found[(tile_no + 1) % kMasks][lane] = 0;  // of 7 tiles ago, which is done
-                  const bool held = write(std::true_type{});
-                  if (lane == 0) {
-                    if (!held) found[half] = 1;
-                    arrive(tl.agreed);
-                  }
-                  wait(tl.agreed, raws & 1, abort);
-                  if (*reinterpret_cast<volatile int*>(found + half) != 0) write(std::false_type{});
-                } else {
-                  write(std::false_type{});
                 }
                 __syncwarp();
                 if (lane == 0) arrive(tl.scanned[stage]);
@@ -1092,7 +1085,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 120;");
     constexpr uint32_t kIdS = tc::idesc_bf16(0, kTile), kIdO = tc::idesc_bf16(0, HD, false, /*b_mn=*/true);
     constexpr uint32_t kFp16 = (1u << 7) | (1u << 10);  // bits that make the operands bf16; off where values are fp16
-    uint32_t types[2] = {0, 0};                         // what to take off for either half of a tile
+    int types[2] = {0, 0};  // 4 bits: whether the blocks of either half of a tile are bf16, a byte each
     uint32_t height = 0;  // the rest of the descriptors: the unit's rows
     // This warp's own time between two products is time the tensor cores stand still once their short queue is empty: ring
     // positions are kept instead of divided out, and one lane issues a stream's products and commits in one go.
@@ -1128,7 +1121,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
       for (int k0 = 0; k0 < kTile / 32; ++k0) {
         const int ks = k0 + half * (kTile / 32);
         mma_ts(tmem + L::kColO + s * HD, tmem + L::kColS + s * kTile + 8 * ks, vd + ks * 2 * L::kGroup / 16,
-               (kIdO | height) & ~types[half], accumulate || ks > 0);
+               Q4 && !(types[half] >> 8 * k0 & 1) ? (kIdO | height) & ~kFp16 : kIdO | height, accumulate || ks > 0);
       }
       if (fine)
 #pragma unroll
@@ -1163,8 +1156,8 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
           full(v);
           if constexpr (Q4) {
             const int* found = tl.found[tile_no % kMasks];
-            types[0] = uniform(found[0]) ? 0 : kFp16;
-            types[1] = uniform(found[1]) ? 0 : kFp16;
+            types[0] = uniform(found[0]);
+            types[1] = uniform(found[1]);
             ++tile_no;
           }
           // rows of the last page past the request's keys came along with a tensor copy: no key, so no value either
@@ -1298,7 +1291,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
             }
             continue;
           }
-          bool half_types = true;  // fp16 holds the values of both halves of the tile
+          bool half_types = true;  // all values of the tile are fp16
           if constexpr (Q4) {
             const int v_item = 2 * (tile_no + t) + 1;
             wait(tl.full[v_item % L::kSlots], (v_item / L::kSlots) & 1, abort);  // this stream's last product has waited for the one before
@@ -1469,6 +1462,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
             for (int c = 0; c < 4; ++c) {  // the weights take half of the scores' columns: those of scores already read
               uint32_t y[32], packed[16] = {};
               if (scores(c, y)) {
+                const int bf16 = Q4 ? tl.found[(tile_no + t) % kMasks][c / 2] >> 16 * (c & 1) : 0;
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                   float a, z;
@@ -1476,7 +1470,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
                   a = ex2(a);
                   z = ex2(z);
                   sum2[j % 2] = add2(sum2[j % 2], pack2(a, z));
-                  packed[j] = Q4 && !tl.found[(tile_no + t) % kMasks][c / 2] ? to_fp16x2(a, z) : to_bf16x2(a, z);
+                  packed[j] = Q4 && !(bf16 & (j < 8 ? 1 : 256)) ? to_fp16x2(a, z) : to_bf16x2(a, z);
                 }
               }
               tc::st16(col_s + 16 * c, packed);
