@@ -147,36 +147,39 @@ __global__ void __launch_bounds__(kWarps * 32) gqa_append_kernel(const __grid_co
           *reinterpret_cast<uint4*>(p.kv.v + slot + (int64_t)(h - p.Hq - p.kv.Hkv) * p.kv.head_stride + gl * 8) = raw[i];
         continue;
       }
-      float x[8], factor = 1.f;
-      widen(raw[i], x);
-      if (p.normalize) {
-        float ss = 0.f;
+      uint4 packed = raw[i];
+      if (!Q4 || h - lane / GL < p.Hq + p.kv.Hkv) {  // not values only
+        float x[8], factor = 1.f;
+        widen(raw[i], x);
+        if (p.normalize) {
+          float ss = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+          for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
 #pragma unroll
-        for (int o = GL / 2; o > 0; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        factor = rsqrtf(fmaf(ss, p.inv_hd, p.eps));
-      }
-      if (is_q && p.temp) factor *= fabsf(__bfloat162float(p.temp[h]));
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] *= factor;
-      if (p.interleaved) {
-#pragma unroll
-        for (int j = 0; j < 8; j += 2) {
-          if (!turned) break;
-          const float a = x[j], c = x[j + 1];
-          x[j] = a * cs[j] - c * sn[j];
-          x[j + 1] = a * sn[j] + c * cs[j];
+          for (int o = GL / 2; o > 0; o /= 2) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          factor = rsqrtf(fmaf(ss, p.inv_hd, p.eps));
         }
-      } else {
-        const int partner = lane + (upper ? -(half / 8) : half / 8);
+        if (is_q && p.temp) factor *= fabsf(__bfloat162float(p.temp[h]));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float other = __shfl_sync(0xffffffffu, x[j], turned ? partner : lane);
-          if (turned) x[j] = upper ? other * sn[j] + x[j] * cs[j] : x[j] * cs[j] - other * sn[j];
+        for (int j = 0; j < 8; ++j) x[j] *= factor;
+        if (p.interleaved) {
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            if (!turned) break;
+            const float a = x[j], c = x[j + 1];
+            x[j] = a * cs[j] - c * sn[j];
+            x[j + 1] = a * sn[j] + c * cs[j];
+          }
+        } else {
+          const int partner = lane + (upper ? -(half / 8) : half / 8);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float other = __shfl_sync(0xffffffffu, x[j], turned ? partner : lane);
+            if (turned) x[j] = upper ? other * sn[j] + x[j] * cs[j] : x[j] * cs[j] - other * sn[j];
+          }
         }
+        if (!is_v) packed = zb::pack_bf16x8(x);
       }
-      const uint4 packed = is_v ? raw[i] : zb::pack_bf16x8(x);
       uint32_t word = 0, pair = 0;
       if (Q4 && h - lane / GL + kHeads > p.Hq) word = zb::q4::write_word(packed, pair);  // the warp has keys or values
       if (!carries || h >= heads) continue;

@@ -142,21 +142,21 @@ __device__ __forceinline__ uint32_t write_word(uint4 x, uint32_t& pair) {
   float s = bf16_round(__fdiv_rn(high - low, 15.f));
   if (s < kSmallestStep) s = 0.f;
   pair = (__float_as_uint(s) >> 16) | (__float_as_uint(low) & 0xffff0000u);
-  const float r = s > 0.f ? __frcp_rn(s) : 0.f, half = 0.5f * s;
+  // floor(d / s + 1/2) is d r rounded to an integer, or one more: r is below 1 / s by more than its and the product's roundings,
+  // and what is left of d after that many steps, which fp32 holds exactly, tells which.
+  // It is not above 15, as s is within 2^-8 of a fifteenth of the largest d. With s = 0 all codes are 0.
+  const float r = s > 0.f ? __frcp_rn(s) * (1.f - 0x1p-20f) : 0.f, half = s > 0.f ? 0.5f * s : INFINITY;
   constexpr float kMagic = 12582912.f;  // 1.5 x 2^23: a sum with it has the nearest integer in its lower bits
-  uint32_t word = 0;
+  constexpr uint32_t kMagicBits = 0x4b400000u;
+  uint32_t word = 0u - kMagicBits * 0x11111111u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const float d = __uint_as_float(e ? w[i] & 0xffff0000u : w[i] << 16) - low;
-      float c = fmaf(d, r, kMagic) - kMagic;
-      // d r may be an ulp off, and rounds halves to even: what is left of d after c steps tells which code it is
-      const float left = fmaf(-c, s, d);
-      if (left >= half) c += 1.f;
-      if (left < -half) c -= 1.f;
-      c = s > 0.f ? fminf(c, 15.f) : 0.f;
-      word |= (__float_as_uint(c + kMagic) & 15u) << (4 * (i + 4 * e));
+      float c = fmaf(d, r, kMagic);
+      if (fmaf(kMagic - c, s, d) >= half) c += 1.f;
+      word += __float_as_uint(c) << (4 * (i + 4 * e));
     }
   }
   return word;
