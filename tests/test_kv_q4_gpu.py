@@ -331,6 +331,23 @@ def test_chunk_values_of_all_magnitudes(zb, news, scale):
         _check_chunk(zb, q, cache, table, seqlens, cu)
 
 
+@pytest.mark.parametrize("news", [[1, 2], [40, 3], [130, 17]])
+@pytest.mark.parametrize("hd,page", [(128, 16), (64, 48), (96, 32), (32, 64)])
+def test_chunk_blocks_of_different_magnitudes(zb, news, hd, page):
+    """Blocks of 16 keys whose values fp16 holds beside blocks that it does not hold: for their size, and for a group's step of 0."""
+    gen = torch.Generator().manual_seed(hd + news[0])
+    for window, sinks in ((0, 0), (90, 5)):
+        table, seqlens, cu, pages = _batch(gen, news, [300, 700], page)
+        k, v = (torch.randn(pages, page, 2, hd, generator=gen) for _ in range(2))
+        kind = torch.randint(0, 4, (pages, page // 16, 1, 2, 1), generator=gen)
+        v = v.unflatten(1, (-1, 16))
+        v = torch.where(kind == 0, v * 2.0 ** 14, torch.where(kind == 1, v.clone().mul_(2.0 ** 11), v * 2.0 ** 12))
+        v[..., :32] = torch.where(kind == 3, torch.tensor(2.0 ** 13), v[..., :32])
+        cache = paged_q4.store_all(k.bfloat16(), v.flatten(1, 2).bfloat16())
+        q = torch.randn(int(cu[-1]), 8, hd, generator=gen).bfloat16()
+        _check_chunk(zb, q, cache, table, seqlens, cu, window=window, sinks=sinks)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 1), (2, 0), (128, 128), (500, 4), (3, 300), (130, 17), (1 << 40, 1 << 40)])
 def test_chunk_windows_and_sinks(zb, window, sinks):
     gen = torch.Generator().manual_seed(sinks)

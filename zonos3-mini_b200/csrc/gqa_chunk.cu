@@ -1,7 +1,7 @@
 // Attention of every request's new tokens over its pages of a KV cache.
 //
 // Token t of request b at key position p (paged.cuh) sees the keys j <= p (causal; every key of the request otherwise)
-// with j > p - window when there is a window, and whose page is in the cache. With s_j = scale q . k_j over them,
+// with j > p - window (or j < sinks) when there is a window, and whose page is in the cache. With s_j = scale q . k_j over them,
 //   out = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  lse = m + log sum_j e^(s_j - m),  m = max_j s_j;
 // a token that sees no key, or belongs to no request, gives 0 (lse -inf). Query head h reads KV head h / (Hq / Hkv).
 // The layer's output gate multiplies head h's row by sigmoid(gate[t, h]) before the one rounding to bf16.
@@ -30,7 +30,7 @@
 // lengths, and the result does not depend on timing.
 //
 // Warps: 0-3 and 4-7 the rows of stream 0 and 1; 8 issues the tensor-core work; 9-11 look up pages and copy K, V and Q
-// rows (any page size, any strides) into shared memory, several tiles ahead and across units.
+// rows (any page size, any strides) into shared memory, several tiles ahead and across units (9-15 for 4 bits, below).
 //
 // A key hidden from some rows of a tile must not reach them even when its value is not finite, and 0 x inf is NaN in a
 // matrix product. So where a tile's keys are visible to some of its rows only, warps 10 and 11 look through the V tile while
@@ -59,6 +59,20 @@
 // against 158 with heads of 128, 120 against 120 with heads of 64. The 16-byte copies cost most on pages of one row: the 4 x 512
 // tokens take 199 us, the prompts 84; and where a head dim is padded: 96 dims 192 us for the 4 x 512 tokens, 32 dims 180 us for
 // 256 single tokens, more than 64 dims do (115, 127).
+//
+// First keys that stay visible (SINKS): with a window, keys j < sinks are seen too. A unit's tiles are then those of the sinks
+// and those from its first row's window on; nothing between them is read. Kernels without it keep their registers: one kernel
+// for both spilled. A prompt of 8192 with a window of 1024 and 4 first keys (65 GFLOP) takes 106 us, the whole
+// prompt without a window 270; 64 single tokens behind 16383 keys 41 us.
+//
+// A cache in 4 bits (Q4, kv_q4.cuh): the same two products, so keys and values have to lie as 16-bit numbers where the tensor
+// cores read them. Warp 9 copies blocks of 16 keys as they are, 64 keys a stage, three stages ahead (a bulk copy each); warps
+// 10-12 write out a tile's keys and 13-15 its values. The row warps and these share the registers 184 to 72 a thread. Keys are
+// bf16 as the queries are; values and weights are fp16 in every block of 16 keys that fp16 holds (else bf16): errors on
+// 4 x 512 tokens behind 8192 are 0.0023 of the outputs' norm, with bf16 0.0032, the plain form's 0.0017. The rows wait for a tile's
+// values before they form its weights, which costs 177 us for 160 there; with 12 warps a CTA, three for all of this, it was 277.
+// What is left above the bf16 cache's 149 us is the row warps' slots, of which six more warps take half, and that wait.
+// Requests of few rows are gqa_few_q4.cu's: a product of 64 rows for the 4 of a token would cost what reading less gains.
 #include <algorithm>
 
 #include "few_q4.cuh"

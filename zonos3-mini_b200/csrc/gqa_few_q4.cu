@@ -25,6 +25,10 @@
 // in the workspace; the warp that finishes the last of up to 8 neighbouring parts joins them in the order of their keys, and so on
 // for the joined ones. No warp waits for another, and results do not depend on timing.
 //
+// Measured (B200, 16 / 4 heads of 128): 256 tokens over 1628 keys (268 MB) 72 us, 3.7 TB/s, 0.57 of a copy's; the copies alone
+// take 48, the unpacking and products 17 beside them, the joins 4. Issue slots 51 %, the logic pipe 46 %, matrix pipe 23 %: a warp's
+// chain of wait, unpack, products, weights leaves slots that more warps (12 to 16 an SM) or stages did not fill. 2 tokens over 65001
+// keys (83 MB) 36 us, 12 of them the three levels of joins; one over 878 keys 16, launch and chain.
 // Measured ways that were slower (256 tokens of 16 / 4 heads of 128 over 1628 keys): seven warps a CTA that share a unit's items, an eighth
 // that starts the copies, the accumulators joined in shared memory: 105-112 us. Each warp waited for copies and at every
 // unit's end for the slowest; half of the cycles issued nothing.

@@ -1148,8 +1148,8 @@ def gqa_chunk(q, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens_q, *, s
 
     q [N, Hq, hd] bf16 (row stride allowed); the caches, page_table, cache_seqlens and cu_seqlens_q as for
     :func:`gqa_append`. Query head h reads KV head h // (Hq / Hkv). A token at key position p sees keys 0 .. p (with
-    ``window`` > 0 the last ``window`` of them, and the first ``sinks``; with ``causal=False`` every key of its request); a page outside
-    [0, pages) masks its keys. softmax_scale (> 0) defaults to hd ** -0.5. gate: optional [N, Hq] bf16 logits (row
+    ``window`` > 0 the last ``window`` of them, and the first ``sinks``; with ``causal=False`` every key of its request);
+    a page outside [0, pages) masks its keys. softmax_scale (> 0) defaults to hd ** -0.5. gate: optional [N, Hq] bf16 logits (row
     stride allowed); head h's output is multiplied by sigmoid(gate[t, h]) before its one rounding. lse: optional
     contiguous [N, Hq] fp32 tensor that receives the natural logarithm of the softmax denominators. A token that sees
     no key, or belongs to no request, gets zeros and an lse of -inf. The lengths are read on the device: a captured
@@ -1202,14 +1202,16 @@ def _chunk_workspace_bytes(B, N, Hq, Hkv, hd, max_keys) -> int:
     return _lib.load().zb_gqa_chunk_workspace_bytes(B, N, Hq, Hkv, hd, max_keys)
 
 
-_CHUNK_WS: dict = {}  # (device, stream, bytes of flags) -> the workspace of eager calls on that stream (flags another call left do not count)
+# (device, stream, bytes of flags) -> the workspace of eager calls on that stream (flags another call left do not count)
+_CHUNK_WS: dict = {}
 _CHUNK_FLAG_BYTES = 4096  # the flags lie at the workspace's start
 _CHUNK_Q4_FLAG_BYTES = 36864
 
 
 def _chunk_workspace(q: torch.Tensor, stream: int, nbytes: int, flag_bytes: int = _CHUNK_FLAG_BYTES) -> torch.Tensor:
-    """A workspace with its flags zero (one for each size of them: what one operator has for flags is another's partial results). Eager calls on a stream share one, in stream order; under capture every call gets
-    its own (from the graph's pool, its flags zeroed by the graph), as a replay may run beside eager calls."""
+    """A workspace with its flags zero (one for each size of them: what one operator has for flags is another's partial
+    results). Eager calls on a stream share one, in stream order; under capture every call gets its own (from the graph's
+    pool, its flags zeroed by the graph), as a replay may run beside eager calls."""
     key = q.get_device(), stream, flag_bytes
     capturing = torch.cuda.is_current_stream_capturing()
     ws = None if capturing else _CHUNK_WS.get(key)
