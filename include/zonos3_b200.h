@@ -403,7 +403,8 @@ int zb_kv_read_q4(const uint8_t* kv_cache, int64_t page_stride, int64_t head_str
 
 /* zb_gqa_chunk_q4: as zb_gqa_chunk_sinks, over the values the cache stands for. max_new (0: not known): no request brings more
  * new tokens than so many; a request that does sets status bit 256 and its rows may be left unwritten. The workspace is that of
- * zb_gqa_chunk_q4_workspace_bytes with the same max_new; its first 36864 bytes are the flags. */
+ * zb_gqa_chunk_q4_workspace_bytes with the same max_new; its first 36864 bytes are the flags, so it is not one that
+ * zb_gqa_chunk's calls use. */
 int64_t zb_gqa_chunk_q4_workspace_bytes(int B, int N, int Hq, int Hkv, int hd, int64_t max_keys, int max_new);
 int zb_gqa_chunk_q4(const uint16_t* q, int64_t q_stride, const uint8_t* kv_cache, int64_t page_stride, int64_t head_stride,
                     int64_t num_pages, int page_size, const int32_t* page_table, int64_t table_stride, int max_pages,

@@ -1362,8 +1362,8 @@ def gqa_chunk_q4(q, kv_cache, page_table, cache_seqlens, cu_seqlens_q, *, softma
     kv_cache as for :func:`gqa_append_q4`; the other arguments as for :func:`gqa_chunk`. ``max_new``: no request brings more new
     tokens than so many, when the caller knows (1 for a decode batch); a small one saves the launch for requests of many rows.
     A request that brings more all the same sets :func:`device_status` bit 256 and its rows may be left unwritten.
-    workspace: at least :func:`gqa_chunk_q4_workspace_bytes` bytes, its first 36864 zero before the first call. Returns out
-    [N, Hq, hd] bf16."""
+    workspace: at least :func:`gqa_chunk_q4_workspace_bytes` bytes, its first 36864 zero before the first call (not
+    one that :func:`gqa_chunk` is given too). Returns out [N, Hq, hd] bf16."""
     paged, index, Hkv, hd = _paged_q4(q, kv_cache, page_table, cache_seqlens, cu_seqlens_q, None)
     N, Hq = q.shape[0], q.shape[1]
     q_stride = _token_rows("q", q, index, N, Hq, hd)
