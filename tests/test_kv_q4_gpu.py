@@ -363,6 +363,14 @@ def test_chunk_few_rows_over_a_long_cache(zb, keys, Hq, hd, max_new):
     _check_chunk(zb, *_chunk_inputs(gen, [1, 3], [keys - 1, keys // 3], Hq, Hq // 4, hd, 64), max_new=max_new)
 
 
+@pytest.mark.parametrize("Hq,Hkv,hd", [(8, 8, 64), (14, 2, 64), (6, 2, 64), (8, 8, 128), (6, 2, 128)])
+@pytest.mark.parametrize("max_new", [None, 1])
+def test_chunk_odd_rows_over_a_long_cache(zb, Hq, Hkv, hd, max_new):
+    """An odd number of rows, whose parts are joined in more than one step: a warp's lanes do not all have an element of them."""
+    gen = torch.Generator().manual_seed(Hq + hd)
+    _check_chunk(zb, *_chunk_inputs(gen, [1, 1, 1], [9000, 700, 5001], Hq, Hkv, hd, 48), max_new=max_new)
+
+
 @pytest.mark.parametrize("max_new", [None, 3])
 def test_chunk_many_requests(zb, max_new):
     """More requests than CTAs, with and without new tokens; requests of few and of many rows."""

@@ -897,7 +897,8 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
         const unsigned first_at = part_slot(d.first, leader * stride) * L::kRows;
         const unsigned step = (unsigned)stride * 2 * L::kRows, back = leader == 0 ? L::kRows : 0;  // a unit's first part is in a second slot
 #pragma unroll 1
-        for (int x0 = lane; x0 < d.rows * kQuads; x0 += 32 * kPieces) {
+        for (int base = 0; base < d.rows * kQuads; base += 32 * kPieces) {  // as often for every lane: the warp meets in it
+          const int x0 = base + lane;
           float top[kPieces], sum[kPieces], y[kPieces][4];
           unsigned at[kPieces];
 #pragma unroll
