@@ -104,10 +104,13 @@ constexpr int kMaxSlots = 10, kDescs = 4;
 // 4 bits: stages of 64 keys (their values too) as they lie in the cache, which two warps write out as bf16 tiles.
 constexpr int kRawStages = 3, kRawBlocks = 4;
 constexpr int kMasks = 8;  // of key masks and of looked-through tiles: the loaders run at most 5 tiles ahead of the rows
-constexpr float kAbove = 24.f;  // how far (log2) the m that is subtracted may lie above a row's largest score
-// 4 bits: the weights come 2^15 larger, so that fp16, whose rounding is an eighth of bf16's, holds them: from there down to 2^-39,
-// the largest not below 2^-9.
-constexpr float kShiftQ4 = 15.f;
+// How far (log2) the m that is subtracted may lie above a row's largest score, and how far a unit's first m has to lie above it.
+constexpr float kAbove = 24.f, kRoom = 12.f;
+// 4 bits: the weights come 2^15 larger, so that fp16, whose rounding is an eighth of bf16's, holds them. m lies at most 8 above the
+// largest score, so a row's largest weight is 2^7 to 2^15, weights are rounded as fp16 does down to 2^-21 of it (2^-14), and what
+// they lack below that is 2^-32 of it a key: 2^-12 at a million keys. With 24, keys 11 nats below a first one that stands out were gone.
+// They are summed before they are rounded: that takes no instruction, and the roundings above 2^-21 have either sign.
+constexpr float kAboveQ4 = 8.f, kRoomQ4 = 2.f, kShiftQ4 = 15.f;
 constexpr int kMaxRequests = 16384;
 // The flags' part of a workspace, of every call's alike: calls of different grids take turns on one workspace, and what one
 // leaves in its parts must not lie where another has its flags.
@@ -595,7 +598,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
                                                                 const __grid_constant__ Maps maps) {
   using L = Shape<HD, Q4>;
   constexpr int kThreads = L::kThreads;
-  constexpr float kShift = Q4 ? kShiftQ4 : 0.f;
+  constexpr float kShift = Q4 ? kShiftQ4 : 0.f, kAbove = Q4 ? kAboveQ4 : ::kAbove, kRoom = Q4 ? kRoomQ4 : ::kRoom;
   extern __shared__ __align__(1024) unsigned char gbase[];
   const uint32_t base = zb::smem_addr(gbase);
   if (base % 1024 != 0) {  // the swizzled tiles ask for it; there is no static shared memory before them
@@ -1345,7 +1348,7 @@ __global__ void __launch_bounds__(Shape<HD, Q4>::kThreads, 1) gqa_chunk_kernel(c
           // lanes without a row. `set`: first keys set m whatever it is.
           auto holds = [&](float top, bool set) {
             top *= p.scale_log2;
-            const bool off = l != 0.f ? top > m : (set || top > m - kAbove / 2 || top < m - kAbove) && top > -INFINITY;
+            const bool off = l != 0.f ? top > m : (set || top > m - kRoom || top < m - kAbove) && top > -INFINITY;
             if (!__any_sync(0xffffffffu, off)) return true;
             top += kAbove;
             const float corr = off && l != 0.f ? ex2(m - top) : 1.f;  // without a key so far both are 0
