@@ -462,8 +462,9 @@ __device__ __forceinline__ void unit_tiles(const ChunkParams& p, const Request& 
   d.tiles = hi1 > lo0 ? (hi1 + kTile - 1) / kTile - d.tile0 : 0;
   d.sink_tiles = d.gap = 0;
   const int seen_first = min(p.sinks, hi1);
-  if (lo0 > 0 && seen_first > 0) {  // the sinks' tiles come before the window's
-    d.sink_tiles = min((seen_first + kTile - 1) / kTile, d.tile0);
+  if (lo0 > 0 && seen_first > 0) {  // the sinks' tiles come before the window's, the last of them may be its first
+    const int tiles = (seen_first + kTile - 1) / kTile;
+    d.sink_tiles = d.tiles > 0 ? min(tiles, d.tile0) : tiles;  // no window: the table ends before it
     d.gap = d.tile0 - d.sink_tiles;
     d.tiles += d.sink_tiles;
     d.tile0 = 0;
