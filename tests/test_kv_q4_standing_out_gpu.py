@@ -74,3 +74,20 @@ def test_a_first_tile_anywhere(zb, low):
     k, v = paged_q4.read(cache)
     k[..., :32] += low  # 8 bits hold the sums
     _check(zb, q, paged_q4.store_all(k.bfloat16(), v.bfloat16()), table, seqlens, cu)
+
+
+@pytest.mark.parametrize("sigma,nats", [(2.0 ** -10, 14.0), (2.0 ** -9, 14.0), (2.0 ** -7, 16.0), (2.0 ** -5, 16.0), (2.0 ** -60, 12.0)])
+@pytest.mark.parametrize("Hq,hd", [(4, 128), (12, 128), (4, 64)])
+def test_small_values_behind_a_key_that_stands_out(zb, sigma, nats, Hq, hd):
+    """Single tokens, each unit's keys summed by one or two warps (many requests, over the same pages): small values with weights of
+    2^-20 and less of the largest. Bound, where weights and s c are bf16's: 2^-8 for the output, 2 x 2^-8 for the weights above and below
+    the fraction bar, 2^-8 of a group's range (4 mean |v|, of random signs: counted as 2)."""
+    gen = torch.Generator().manual_seed(Hq + hd)
+    keys, requests = 65536, 2400
+    q, cache, table, seqlens, cu = _outstanding(gen, [1], [keys - 1], Hq, 1, hd, 256, nats, 0.5, values=sigma)
+    many = [q.expand(requests, Hq, hd), cache, table.expand(requests, -1), seqlens.expand(requests)]
+    many = [t.contiguous().to(DEV) for t in many]
+    out = zb.ops.gqa_chunk_q4(*many, torch.arange(requests + 1, dtype=torch.int32, device=DEV), softmax_scale=1.0, max_new=1)
+    ref, spread, *_ = paged.chunk(q, *paged_q4.read(cache), table, seqlens, cu, scale=1.0)
+    _close(out, ref.expand_as(out), (5 * 2.0 ** -8 * spread).expand_as(out))
+    assert zb.ops.device_status() == 0
