@@ -28,9 +28,10 @@
 // for the joined ones. No warp waits for another, and results do not depend on timing.
 //
 // Measured (B200, 16 / 4 heads of 128): 256 tokens over 1628 keys (268 MB) 73 us, 3.7 TB/s, 0.56 of a copy's (1.6 of them the
-// look for small steps); 77 with a cold L2 and 89 where all values are bf16's (|v| below 2^-7 or so); the copies alone take 48, the unpacking and products 17 beside them, the joins 4. Issue slots 51 %, the logic pipe 46 %, matrix pipe 23 %: a warp's
-// chain of wait, unpack, products, weights leaves slots that more warps (12 to 16 an SM) or stages did not fill. 2 tokens over 65001
-// keys (83 MB) 37 us, 12 of them the three levels of joins; one over 878 keys 16, launch and chain.
+// look for small steps); 77 with a cold L2 and 89 where all values are bf16's (|v| below 2^-7 or so); the copies alone take 48,
+// the unpacking and products 17 beside them, the joins 4. Issue slots 51 %, the logic pipe 46 %, matrix pipe 23 %: a warp's chain of
+// wait, unpack, products, weights leaves slots that more warps (12 to 16 an SM) or stages did not fill. 2 tokens over 65001 keys
+// (83 MB) 37 us, 12 of them the three levels of joins; one over 878 keys 16, launch and chain.
 // Measured ways that were slower (256 tokens of 16 / 4 heads of 128 over 1628 keys): seven warps a CTA that share a unit's items, an eighth
 // that starts the copies, the accumulators joined in shared memory: 105-112 us. Each warp waited for copies and at every
 // unit's end for the slowest; half of the cycles issued nothing.
@@ -899,6 +900,7 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
         }
         last = __shfl_sync(0xffffffffu, last, 0);
         if (!last) break;
+        __syncwarp();  // what lane 0 acquired is before every lane's reads: a shuffle alone orders no memory
         const bool final = parts <= kJoin;
         // What it takes is round trips to L2, of about a microsecond: 4 pieces of 4 elements a lane (4 rows of 128) of 4 parts are
         // loaded together.
