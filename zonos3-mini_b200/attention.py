@@ -160,7 +160,7 @@ class Attention(BaseOP):
             q = ops.gqa_append_q4(p, *paged, heads=H, kv_heads=Hkv, temp=self._temp, eps=QK_NORM_EPS, rope_theta=self._theta,
                                   positions=meta.positions)
             o = ops.gqa_chunk_q4(q, *paged, softmax_scale=hd ** -0.5, window=self._window, sinks=self._sinks, gate=gate,
-                                 max_new=1 if batch.is_decode else None)
+                                 max_new=getattr(meta, "max_new", None))
             return F.linear(o.reshape(n, H * hd), self.wo.weight)
         kc, vc = pool.k(self._layer_id), pool.v(self._layer_id)
         slots = kc.dim() == 3

@@ -43,6 +43,9 @@ class AttnMetadata:
     cache_seqlens: "torch.Tensor"  # [B] int32
     # request b's new rows are [cu[b], cu[b+1]): a host list or tensor for a prefill, an int32 device tensor for any batch
     cu_seqlens_q: "list[int] | torch.Tensor | None" = None
+    # no request brings more new rows than so many, where whoever made the batch knows (a 4-bit pool's decode step: 1); a promise
+    # that cu_seqlens_q has to keep
+    max_new: "int | None" = None
 
 
 @dataclass

@@ -249,7 +249,7 @@ class DecodeGraph:
         self.batch = Batch(reqs=[Req(i, 1, cached_len=1) for i in range(B)], is_decode=True, padded_size=B,
                            input_ids=self.input_ids,
                            attn_metadata=AttnMetadata(self.positions, self.out_loc, self.page_table, self.cache_seqlens,
-                                                      self.bounds))
+                                                      self.bounds, max_new=1))
         self.graph: torch.cuda.CUDAGraph | None = None
         self.launches_per_step = 0  # this library's kernels in the captured step
         for gdn in model.gdn_layers():
