@@ -33,10 +33,6 @@ class ModelConfig:
     num_kv_heads: int = 4
     head_dim: int = 128
     rope_theta: float = 10000.0
-    # of the global-attention layers: 0, or how many of the last keys a token sees, and how many of the first beside them
-    # (batches described on the device); the reference's layers see all
-    attention_window: int = 0
-    attention_sinks: int = 0
     intermediate_size: int = 0  # dense FFN width of the layers before moe_start_from_layer
     n_codebooks: int = 9
     codebook_size: int = 1024
@@ -44,6 +40,10 @@ class ModelConfig:
     text_extra_tokens: int = 0
     audio_pad_id: int = 1025
     loss_softcap: float = 15.0
+    # of the global-attention layers: 0, or how many of the last keys a token sees, and how many of the first beside them
+    # (batches described on the device); the reference's layers see all
+    attention_window: int = 0
+    attention_sinks: int = 0
 
     def get_num_experts_per_tok(self, layer_id: int) -> int:
         return self.moe_topk
