@@ -22,3 +22,22 @@ def test_positional_arguments_keep_their_places(zb):
     values[order.index("intermediate_size")] = 4096
     config = zb.config.ModelConfig(*values)
     assert config.intermediate_size == 4096 and config.attention_window == config.attention_sinks == 0
+
+
+def _graph(zb, config, pool):
+    """A decode graph that is not captured: its buffers, on the CPU."""
+    model = zb.model.Zonos3ForCausalLM(zb.config.ModelConfig(512, num_layers=4, moe_n_experts=4, moe_topk=2, moe_intermediate_size=64,
+                                                             num_qo_heads=4, num_kv_heads=2))
+    model._config = config
+    return zb.model.DecodeGraph(model, pool, 3, torch.zeros(3, 8, dtype=torch.int32))
+
+
+def test_a_config_without_the_fields_decodes(zb):
+    whole = zb.config.ModelConfig(512, num_layers=4, num_qo_heads=4, num_kv_heads=2)
+    known = {f.name: getattr(whole, f.name) for f in dataclasses.fields(whole) if not f.name.startswith("attention_window")}
+    known.pop("attention_sinks")
+    config = types.SimpleNamespace(**known, audio_vocab_size=whole.audio_vocab_size)
+    pool = zb.attention.SlotKVPool([3], 64, 2, 128, "cpu")
+    assert _graph(zb, config, pool).bounds is None
+    config.attention_window = 9
+    assert _graph(zb, config, pool).bounds.tolist() == [0, 1, 2, 3]

@@ -228,7 +228,7 @@ class DecodeGraph:
         # what the bookkeeping takes slots from: the table itself, or as wide as its pages' tokens where no slots are used
         self._slot_table = self.page_table if not four_bits else torch.zeros(B, page_table.shape[1] * pool.page_size, **i32)
         # every stream's row, for the paged operators
-        self.bounds = torch.arange(B + 1, **i32) if four_bits or c.attention_window else None
+        self.bounds = torch.arange(B + 1, **i32) if four_bits or getattr(c, "attention_window", 0) else None
         self.input_ids = torch.zeros(B, self.C + (c.text_vocab is not None), **i32)
         self.codes = torch.zeros(B, self.C + 1, **i32)
         self.positions = torch.zeros(B, **i32)
