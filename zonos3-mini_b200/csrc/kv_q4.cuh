@@ -3,6 +3,7 @@
 // 32 consecutive elements of a token's key or value of one KV head are a group; it is kept as 4-bit codes c and a pair (s, m)
 // of bf16, and stands for x = m + s c. From x (bf16; NaN counts as 0, and what is beyond +-2^63 as that):
 //   m = min x,  s = bf16((max x - min x) / 15) (0 where that is below 2^-100),  c = floor((x - m) / s + 1/2), 0 .. 15 (0 where s = 0)
+// with the difference and the quotient in s rounded to fp32 before, and c exact.
 // m is one of the elements, so storing it rounds nothing; s is rounded before it divides, so c allows for it. A pair with a
 // magnitude of 2^64 or more, or a NaN, is never written and stands for zeros: rows that no token wrote hold anything, and 0 x
 // inf would be NaN in a matrix product that counts them with weight 0; and sums of 2^26 values, times weights of up to 2^15, stay
@@ -144,6 +145,7 @@ __device__ __forceinline__ uint32_t write_word(uint4 x, uint32_t& pair) {
   pair = (__float_as_uint(s) >> 16) | (__float_as_uint(low) & 0xffff0000u);
   // floor(d / s + 1/2) is d r rounded to an integer, or one more: r is below 1 / s by more than its and the product's roundings,
   // and what is left of d after that many steps, which fp32 holds exactly, tells which.
+  // d is rounded down where fp32 does not hold it: a border, (c + 1/2) s, has few bits, so what is below it stays below.
   // It is not above 15, as s is within 2^-8 of a fifteenth of the largest d. With s = 0 all codes are 0.
   const float r = s > 0.f ? __frcp_rn(s) * (1.f - 0x1p-20f) : 0.f, half = s > 0.f ? 0.5f * s : INFINITY;
   constexpr float kMagic = 12582912.f;  // 1.5 x 2^23: a sum with it has the nearest integer in its lower bits
@@ -153,7 +155,7 @@ __device__ __forceinline__ uint32_t write_word(uint4 x, uint32_t& pair) {
   for (int i = 0; i < 4; ++i) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float d = __uint_as_float(e ? w[i] & 0xffff0000u : w[i] << 16) - low;
+      const float d = __fsub_rd(__uint_as_float(e ? w[i] & 0xffff0000u : w[i] << 16), low);
       float c = fmaf(d, r, kMagic);
       if (fmaf(kMagic - c, s, d) >= half) c += 1.f;
       word += __float_as_uint(c) << (4 * (i + 4 * e));
