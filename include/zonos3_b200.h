@@ -457,7 +457,7 @@ int zb_embed_norm(const int32_t* ids, int64_t ids_stride, int ncols, const uint1
 /* The bookkeeping between two captured decode steps, in one single-block launch: ids[b, :ids_cols] = codes[b, ...]
  * (the sampled codes, then the text column, become the next input row), history[b, c, *ring] = codes[b, c] for the
  * first C codebooks (history NULL: none; W columns, *ring the next one), positions[b] += 1, seqlens[b] =
- * min(seqlens[b] + 1, max_len), out_loc[b] = page_table[b, seqlens[b] - 1]; then *ring = (*ring + 1) % W and
+ * min(seqlens[b] + 1, max_len), out_loc[b] = page_table[b, seqlens[b] - 1] (table_stride 0: one row for all); then *ring = (*ring + 1) % W and
  * *counter += 1 (the sampler's draw counter). The engine does this on the host between steps (the scheduler builds
  * the next batch's ids and attention metadata); here it stays on the device so that replays alone decode. No
  * reference counterpart as a kernel. */

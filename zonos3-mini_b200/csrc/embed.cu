@@ -192,7 +192,7 @@ ZB_API int zb_decode_advance(const int32_t* codes, int codes_cols, int32_t* ids,
                              int32_t* out_loc, const int32_t* page_table, int64_t table_stride, int max_len, int B,
                              cudaStream_t stream) {
   ZB_REQUIRE(B >= 0 && codes_cols > 0 && ids_cols > 0 && ids_cols <= codes_cols && C >= 0 && C <= codes_cols &&
-                 W >= 0 && max_len > 0 && table_stride >= max_len,
+                 W >= 0 && max_len > 0 && (table_stride >= max_len || table_stride == 0),
              "decode_advance: bad sizes B=%d codes_cols=%d ids_cols=%d C=%d W=%d max_len=%d", B, codes_cols, ids_cols,
              C, W, max_len);
   if (B == 0) return zb::kOk;

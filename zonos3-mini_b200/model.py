@@ -225,8 +225,8 @@ class DecodeGraph:
         if page_table.shape[0] != B or page_table.dtype != torch.int32:
             raise ValueError(f"page_table must be a [{B}, max_len] int32 tensor")
         self.page_table = page_table.contiguous()
-        # what the bookkeeping takes slots from: the table itself, or as wide as its pages' tokens where no slots are used
-        self._slot_table = self.page_table if not four_bits else torch.zeros(B, page_table.shape[1] * pool.page_size, **i32)
+        # what the bookkeeping takes slots from: the table itself, or where no slots are used one row, as wide as a stream's pages' tokens
+        self._slot_table = self.page_table if not four_bits else torch.zeros(1, page_table.shape[1] * pool.page_size, **i32).expand(B, -1)
         # every stream's row, for the paged operators
         self.bounds = torch.arange(B + 1, **i32) if four_bits or getattr(c, "attention_window", 0) else None
         self.input_ids = torch.zeros(B, self.C + (c.text_vocab is not None), **i32)

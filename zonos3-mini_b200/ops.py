@@ -1008,7 +1008,7 @@ def decode_advance(codes, ids, positions, cache_seqlens, out_loc, page_table, co
     """The bookkeeping between two decode steps in one kernel (zb_decode_advance): the sampled codes [B, >= cols]
     become the next ids [B, cols]; the first C codes enter the repetition window history [B, C, W] at column
     ring[0]; positions and cache_seqlens advance by one (lengths capped at the page table's width); out_loc takes
-    each stream's next page-table slot; ring and the sampler's draw counter (int64 [1]) advance."""
+    each stream's next page-table slot (rows may be one expanded row); ring and the sampler's draw counter (int64 [1]) advance."""
     dev = codes.device
     for name, t in (("codes", codes), ("ids", ids), ("positions", positions), ("cache_seqlens", cache_seqlens),
                     ("out_loc", out_loc), ("page_table", page_table)):
