@@ -76,7 +76,8 @@ def test_a_first_tile_anywhere(zb, low):
     _check(zb, q, paged_q4.store_all(k.bfloat16(), v.bfloat16()), table, seqlens, cu)
 
 
-@pytest.mark.parametrize("sigma,nats", [(2.0 ** -10, 14.0), (2.0 ** -9, 14.0), (2.0 ** -7, 16.0), (2.0 ** -5, 16.0), (2.0 ** -60, 12.0)])
+@pytest.mark.parametrize("sigma,nats", [(2.0 ** -10, 14.0), (2.0 ** -9, 14.0), (2.0 ** -10, 16.0), (2.0 ** -7, 16.0), (2.0 ** -5, 16.0), (2.0 ** -5, 20.0),
+                                        (2.0 ** -60, 12.0)])
 @pytest.mark.parametrize("Hq,hd", [(4, 128), (12, 128), (4, 64)])
 def test_small_values_behind_a_key_that_stands_out(zb, sigma, nats, Hq, hd):
     """Single tokens, each unit's keys summed by one or two warps (many requests, over the same pages): small values with weights of

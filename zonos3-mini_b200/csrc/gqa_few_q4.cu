@@ -11,12 +11,13 @@
 //     sums, split into three bf16. So the scores are as good as fp32's, down to 2^-35 of a row's largest element;
 //   out^T [16 dims of a group, 8 rows] += c (s_g p^T), and p^T m_g and the sum of p by a product more. Weights are fp16, 2^-12 of
 //     each: bf16's 2^-9 would be the largest error here. fp16 has less range, so an item whose pairs are not all within it
-//     (half_holds()), or one that has a group with small steps only, and those after it take bf16.
-// A weight is 2^(score - m + 15) with m a row's reference, its largest score or up to 4 (log2) above it when it is set; it is set
-// anew by a score above it, hardly ever after the first block. So weights lie in fp16's range: up to 2^15, the largest not below 2^11
-// when m is set, and those below 2^-40 of m count as 0. m and the sum cancel in the end. s p is as good down to 2^-14: with
-// a step of 2^-8 in each group of an item, for keys 17 (log2) and more below the largest, and it is lost another 11 below that.
-// (With 8 above and steps of 2^-12 alone, many keys 20 below a first one that stands out lost their s c.)
+//     (half_holds()) and those after it take bf16.
+// A weight is 2^(score - m + 15) with m a row's reference, its largest score or up to 2 (log2) above it when it is set; it is set
+// anew by a score above it, rarely after the first items. So weights lie in fp16's range: up to 2^15, the largest not below 2^13
+// when m is set, and those below 2^-40 of m count as 0. m and the sum cancel in the end. s p is formed in fp16 too and has its
+// range: with the smallest step, 2^-12, it is rounded as fp16 does for weights down to 2^-15 of the largest and gone at 2^-26; with
+// steps of 2^-4 at 2^-23 and 2^-34. (With m up to 8 above, 65536 keys 2^-20 to 2^-23 of a first one that stands out were off by a
+// tenth to a third. 0 above costs 256 tokens over 1628 keys 74.3 us for setting m more often, 1 72.8, 2 72.2, 4 and 8 71.9.)
 // The keys of a 16-key block stand in the scores' rows in the order 0 1 3 2 4 5 7 6 and 8 on: the two rows of a quarter of the lanes then
 // read other banks, and the four rows that a quarter's values come from too, as far as 64-byte rows allow.
 //
@@ -27,11 +28,11 @@
 // in the workspace; the warp that finishes the last of up to 8 neighbouring parts joins them in the order of their keys, and so on
 // for the joined ones. No warp waits for another, and results do not depend on timing.
 //
-// Measured (B200, 16 / 4 heads of 128): 256 tokens over 1628 keys (268 MB) 73 us, 3.7 TB/s, 0.56 of a copy's (1.6 of them the
-// look for small steps); 77 with a cold L2 and 89 where all values are bf16's (|v| below 2^-7 or so); the copies alone take 48,
-// the unpacking and products 17 beside them, the joins 4. Issue slots 51 %, the logic pipe 46 %, matrix pipe 23 %: a warp's chain of
-// wait, unpack, products, weights leaves slots that more warps (12 to 16 an SM) or stages did not fill. 2 tokens over 65001 keys
-// (83 MB) 37 us, 12 of them the three levels of joins; one over 878 keys 16, launch and chain.
+// Measured (B200, 16 / 4 heads of 128): 256 tokens over 1628 keys (268 MB) 72 us, 3.7 TB/s, 0.57 of a copy's (90 where values take
+// bf16, all steps below 2^-12); the copies alone take 48, the unpacking and products 17 beside them, the joins 4. Issue slots 51 %, the
+// logic pipe 46 %, matrix pipe 23 %: a warp's chain of wait, unpack, products, weights leaves slots that more warps (12 to 16 an SM) or
+// stages did not fill. 2 tokens over 65001 keys (83 MB) 36 us, 12 of them the three levels of joins; one over 878 keys 16, launch
+// and chain.
 // Measured ways that were slower (256 tokens of 16 / 4 heads of 128 over 1628 keys): seven warps a CTA that share a unit's items, an eighth
 // that starts the copies, the accumulators joined in shared memory: 105-112 us. Each warp waited for copies and at every
 // unit's end for the slowest; half of the cycles issued nothing.
@@ -48,7 +49,7 @@ constexpr int kStages = 2;    // items of a warp: one that is computed, and copi
 constexpr int kUnitCost = 4;  // of a unit, in items
 constexpr int kMinShare = 3;  // items of a warp, its units' cost among them
 constexpr int kJoin = 8;      // parts that are joined at once
-constexpr float kAbove = 4.f, kShift = 15.f;
+constexpr float kAbove = 2.f, kShift = 15.f;
 constexpr float kNone = -3.0e38f;  // m of a row that has seen no key
 
 struct FewParams {
@@ -156,12 +157,10 @@ __device__ __forceinline__ float high_of(uint32_t pair) { return __uint_as_float
 
 // Whether fp16 keeps a pair's s and 2^8 m well: s is below 2 and |m| below 2^7 (a sign bit of `over` else), and s is 2^-12 or
 // more, or the pair is 0 (`holds`). And whether it is not 0 (`some`), and s 2^-8 or more (`big`).
-__device__ __forceinline__ void half_holds(uint32_t pair, uint32_t& over, bool& holds, bool& some, bool& big) {
+__device__ __forceinline__ void half_holds(uint32_t pair, uint32_t& over, bool& holds) {
   const uint32_t a = pair & 0x7fff7fffu;
   over |= a + (((0x8000u - 0x4300u) << 16) | (0x8000u - 0x4000u));
   holds &= a << 16 >= 0x3980u << 16 || a == 0;
-  some |= a != 0;
-  big |= a << 16 >= 0x3b80u << 16;
 }
 // Bit 7 of the bytes that are not 0.
 __device__ __forceinline__ uint32_t bytes_set(uint32_t x) { return (((x & 0x7f7f7f7fu) + 0x7f7f7f7fu) | x) & 0x80808080u; }
@@ -625,7 +624,7 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
           const int g = lane / 8 % GROUPS, t = lane % 4, h = lane / 4 % 2;  // a group, and the keys of scores' rows 2 t + 8 h, + 1
           const int row = 2 * t + (t & 1) + 8 * h;
           uint32_t none = 0, over = 0, a[kItem][2];
-          bool holds = true, some = false, big = false;
+          bool holds = true;
 #pragma unroll
           for (int x = 0; x < kItem; ++x) {
             const uint2 k2 = GROUPS == 4 ? reinterpret_cast<const uint2*>(k_pairs(x))[lane] : make_uint2(k_pairs(x)[lane], 0);
@@ -633,13 +632,10 @@ __global__ void __launch_bounds__(Shape<GROUPS, NT>::kThreads, Shape<GROUPS, NT>
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               a[x][k] = v_pairs(x)[(row ^ k) * GROUPS + g];
-              half_holds(a[x][k], over, holds, some, big);
+              half_holds(a[x][k], over, holds);
             }
           }
-          if constexpr (HALF) {  // 8 lanes have a group
-            const uint32_t groups = bytes_set(__ballot_sync(0xffffffffu, some)), well = bytes_set(__ballot_sync(0xffffffffu, big));
-            if (!__all_sync(0xffffffffu, holds && (over & 0x80008000u) == 0) || (groups & ~well) != 0) return item;
-          }
+          if (HALF && !__all_sync(0xffffffffu, holds && (over & 0x80008000u) == 0)) return item;
 #pragma unroll
           for (int x = 0; x < kItem; ++x) {
 #pragma unroll
