@@ -41,9 +41,11 @@ __global__ void __launch_bounds__(kWarps * 32) kv_read_q4_kernel(const __grid_co
   {
     int b = zb::request_of(p.kv.cu, p.kv.B, (int)t0, lane);
     const int t = (int)t0 + lane;
-    if (b < 0) b = 0;  // before the first request, or behind the last one, where there is nothing to look for
-    if (p.kv.B > 0 && t >= p.kv.cu[p.kv.B]) b = p.kv.B;
-    while (b < p.kv.B && p.kv.cu[b + 1] <= t) ++b;
+    if (b < 0) b = 0;  // before the first request, or behind the last one
+    if (b < p.kv.B && p.kv.cu[b + 1] <= t) {
+      if (p.kv.cu[p.kv.B] <= t) b = p.kv.B;  // nothing to look for, through whatever requests without rows
+      while (b < p.kv.B && p.kv.cu[b + 1] <= t) ++b;
+    }
     if (lane < tokens && b < p.kv.B && p.kv.cu[b] <= t) {
       const int64_t pos = (int64_t)p.kv.keys[b] - ((int64_t)p.kv.cu[b + 1] - t);
       if (pos >= 0 && pos / p.kv.page_size < p.kv.max_pages) {
