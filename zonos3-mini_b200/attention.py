@@ -20,7 +20,8 @@ whatever its requests bring (prompts, chunks of prompts, single tokens), over a 
                                                              the pages of their requests)
     o = zb_gqa_chunk(q, caches, page_table, gate)           (causal attention over the pages, the gate in its store)
 
-Over a ``QuantKVPool``, pages that hold 4 bits an element, the same two as ``zb_gqa_append_q4`` and ``zb_gqa_chunk_q4``. With
+Over a ``QuantKVPool``, pages that hold 4 bits an element, the same two as ``zb_gqa_append_q4`` and ``zb_gqa_chunk_q4``; there
+``attn_metadata.max_new = 1`` saves a decode step the launch for requests of many rows. With
 ``config.attention_window`` > 0 (and ``attention_sinks`` first tokens that stay visible) the paged operators see that window; the
 other paths have none and refuse.
 

@@ -35,7 +35,8 @@ class AttnMetadata:
     With ``cu_seqlens_q`` as a [B + 1] int32 device tensor the layers run the paged operators: ``page_table`` then holds
     pages of the pool's page size, a new row's slot and rotary position follow from the lengths, and ``positions`` (else
     None) overrides the latter; ``out_loc`` is not read. A decode batch over a pool of page size 1 that has ``positions``
-    and ``out_loc`` runs the decode kernels all the same."""
+    and ``out_loc`` runs the decode kernels all the same, unless the layers have a window. A pool of 4 bits and layers with a
+    window take the device tensor only."""
 
     positions: "torch.Tensor | None"  # [N] int32
     out_loc: "torch.Tensor | None"  # [N] int32

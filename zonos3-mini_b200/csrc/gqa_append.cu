@@ -24,7 +24,7 @@
 //
 // With Q4 the cache is one of 4 bits (kv_q4.cuh): k rounded to bf16 as above, and v, go to their groups' codes and pairs. A
 // lane's 8 elements are one word of codes, the 4 lanes of a group find its bounds with two exchanges. The 16210 tokens (176 MB)
-// take 56 us, 3.1 TB/s: issue slots 72 %. Two comparisons an element instead of one, and values through the norm and the turn,
+// take 56 us, 3.1 TB/s: issue slots 71 %. Two comparisons an element instead of one, and values through the norm and the turn,
 // made it 61.
 #include <cmath>
 

@@ -71,7 +71,10 @@
 // bf16 as the queries are; values and weights are fp16 in every block of 16 keys that fp16 holds (else bf16): errors on
 // 4 x 512 tokens behind 8192 are 0.0023 of the outputs' norm, with bf16 0.0032, the plain form's 0.0017. The rows wait for a tile's
 // values before they form its weights, which costs 177 us for 160 there; with 12 warps a CTA, three for all of this, it was 277.
-// What is left above the bf16 cache's 149 us is the row warps' slots, of which six more warps take half, and that wait.
+// What is left above the bf16 cache's 146 us is the row warps' slots, of which six more warps take half, and that wait.
+// fp16's range asks for an m nearer to the largest score than bf16's (kAboveQ4), so wider scores set it anew more often: 4 x 512
+// tokens over 8704 keys 192 us with scores that spread by 1 nat, 215 by 4, 223 by 16 (193, 195 and 219 with bf16's distance). Scores
+// beyond 2^22 (log2) are past what fp32 resolves within it.
 // Requests of few rows are gqa_few_q4.cu's: a product of 64 rows for the 4 of a token would cost what reading less gains.
 #include <algorithm>
 
@@ -101,7 +104,7 @@ constexpr int kThreads = 32 * (kLoadWarp + kLoadWarps);
 // 4 bits: three warps write out the keys and three the values, which with the products' and the copies' warp are two warpgroups.
 constexpr int kOutWarps = 3, kThreadsQ4 = 32 * (kLoadWarp + 1 + 2 * kOutWarps);
 constexpr int kMaxSlots = 10, kDescs = 4;
-// 4 bits: stages of 64 keys (their values too) as they lie in the cache, which two warps write out as bf16 tiles.
+// 4 bits: stages of 64 keys (their values too) as they lie in the cache, which six warps write out as tiles of 16-bit numbers.
 constexpr int kRawStages = 3, kRawBlocks = 4;
 constexpr int kMasks = 8;  // of key masks and of looked-through tiles: the loaders run at most 5 tiles ahead of the rows
 // How far (log2) the m that is subtracted may lie above a row's largest score, and how far a unit's first m has to lie above it.
