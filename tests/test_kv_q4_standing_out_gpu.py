@@ -92,3 +92,11 @@ def test_small_values_behind_a_key_that_stands_out(zb, sigma, nats, Hq, hd):
     ref, spread, *_ = paged.chunk(q, *paged_q4.read(cache), table, seqlens, cu, scale=1.0)
     _close(out, ref.expand_as(out), (5 * 2.0 ** -8 * spread).expand_as(out))
     assert zb.ops.device_status() == 0
+
+
+@pytest.mark.parametrize("hd,Hq", [(128, 3), (96, 2), (64, 2), (32, 2)])
+@pytest.mark.parametrize("nats", [10.0, 11.0, 11.5, 12.0])
+def test_many_rows_over_a_long_flat_tail(zb, hd, Hq, nats):
+    """Units that several CTAs hold parts of: only the first part sees the key that stands out."""
+    gen = torch.Generator().manual_seed(int(nats * 2) + hd)
+    _check(zb, *_outstanding(gen, [40], [17000], Hq, 1, hd, 64, nats, 0.0))
